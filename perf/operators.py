@@ -1,0 +1,639 @@
+"""The gated-delta-net layer operators whose speed is measured, with their plain forms.
+
+What a layer does around the encoded state: tables of a ragged batch built from
+its request lengths; the gated delta rule over whole sequences, for serving
+(states kept in a slot pool) and for training (with every gradient), and for one
+token of each request; the norm before the block, fused with the scaled residual
+sum, and the norm after it, fused with the block's gate, both with gradients.
+
+``run`` computes the plain forms with elementary torch operations in fp32 where
+``own`` is false, and calls the package's operators where it is true.  ``exact``
+evaluates the definitions in float64, token by token.
+"""
+
+from __future__ import annotations
+
+import math
+import random
+import sys
+from pathlib import Path
+
+import torch
+
+own = False
+
+DIM = 128
+CHUNK = 64
+L2_EPS = 1e-6
+NORM_EPS = 1e-6
+SCALE = DIM ** -0.5
+
+
+def listed() -> list[dict]:
+    return [
+        # A small batch's tables: 24 requests of one prefill step.
+        {"name": "tables_24", "kind": "tables", "requests": 24, "longest": 512},
+        # The tables of a very large ragged batch.
+        {"name": "tables_4096", "kind": "tables", "requests": 4096, "longest": 2048},
+        # One decode token of a single request: 32 heads, fp32 state pool.
+        {"name": "step_1", "kind": "step", "batch": 1, "heads": 32, "key_heads": 16,
+         "pool": "f32", "padded": 0},
+        # One decode token of 256 requests, 5% of the entries padding, at the
+        # layer's 32 value heads.
+        {"name": "step_256", "kind": "step", "batch": 256, "heads": 32, "key_heads": 16,
+         "pool": "f32", "padded": 13},
+        # Prefill of a ragged batch of 24 requests, some of them resumed, with
+        # empty and one-token requests among them, into a bf16 pool.
+        {"name": "prefill_ragged", "kind": "prefill", "requests": 24, "longest": 1500,
+         "heads": 32, "key_heads": 16, "pool": "bf16"},
+        # Prefill of one long prompt.
+        {"name": "prefill_long", "kind": "prefill", "requests": 1, "longest": 32768,
+         "heads": 32, "key_heads": 16, "pool": "f32"},
+        # A training step of the rule on few heads (one rank of a sharded layer).
+        {"name": "train_small", "kind": "train", "requests": 3, "longest": 333, "heads": 8,
+         "key_heads": 4},
+        # A training step on four packed sequences at all heads.
+        {"name": "train_large", "kind": "train", "requests": 4, "longest": 2048, "heads": 32,
+         "key_heads": 16, "packed": True},
+        # The gated norm after the rule: 256 decode tokens, then a training step.
+        {"name": "gated_norm_decode", "kind": "gated_norm", "tokens": 256, "heads": 32,
+         "train": False, "dtype": "bf16"},
+        {"name": "gated_norm_train", "kind": "gated_norm", "tokens": 8192, "heads": 32,
+         "train": True, "dtype": "bf16"},
+        # The norm before the block with the scaled residual sum.
+        {"name": "residual_norm_decode", "kind": "residual_norm", "tokens": 256, "width": 2048,
+         "train": False, "dtype": "bf16", "stream": "bf16"},
+        {"name": "residual_norm_train", "kind": "residual_norm", "tokens": 8192, "width": 4096,
+         "train": True, "dtype": "bf16", "stream": "f32"},
+    ]
+
+
+def draw(rng) -> dict:
+    def size(low, high):
+        return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+    kind = rng.choice(["tables", "step", "prefill", "train", "gated_norm", "residual_norm"])
+    if kind == "tables":
+        return {"kind": kind, "requests": size(1, 4096), "longest": size(1, 2048),
+                "draw": rng.randrange(1 << 20)}
+    key_heads = rng.choice([1, 2, 4, 8, 16])
+    heads = key_heads * rng.choice([1, 2, 2, 4] if key_heads < 16 else [1, 2])
+    if kind == "step":
+        batch = size(1, 256)
+        return {"kind": kind, "batch": batch, "heads": heads, "key_heads": key_heads,
+                "pool": rng.choice(["f32", "bf16"]), "padded": rng.randint(0, batch // 8)}
+    if kind == "prefill":
+        longest = size(1, 32768)
+        return {"kind": kind, "requests": size(1, max(1, min(64, 32768 // longest))),
+                "longest": longest, "heads": heads, "key_heads": key_heads,
+                "pool": rng.choice(["f32", "bf16"]), "draw": rng.randrange(1 << 20)}
+    if kind == "train":
+        longest = size(1, 2048)
+        return {"kind": kind, "requests": size(1, max(1, min(32, 8192 // longest))),
+                "longest": longest, "heads": heads, "key_heads": key_heads,
+                "packed": rng.random() < 0.5, "draw": rng.randrange(1 << 20)}
+    if kind == "gated_norm":
+        return {"kind": kind, "tokens": size(1, 8192), "heads": heads,
+                "train": rng.random() < 0.6, "dtype": rng.choice(["bf16", "bf16", "f32"])}
+    return {"kind": kind, "tokens": size(1, 8192), "width": 8 * size(8, 512),
+            "train": rng.random() < 0.6, "dtype": rng.choice(["bf16", "bf16", "f32"]),
+            "stream": rng.choice(["bf16", "f32"])}
+
+
+# ------------------------------------------------------------------- inputs
+
+def _generator(seed: int, device) -> torch.Generator:
+    return torch.Generator(device=device).manual_seed(seed)
+
+
+def _device() -> torch.device:
+    return torch.device("cuda", torch.cuda.current_device())
+
+
+def _dtype(name: str) -> torch.dtype:
+    return {"f32": torch.float32, "bf16": torch.bfloat16}[name]
+
+
+def _lengths(case: dict) -> list[int]:
+    """The requests' token counts: the longest first in an order of the case's
+    own; where there are several, an empty and a one-token request too."""
+    rng = random.Random(case.get("draw", 7) * 8191 + case["requests"])
+    n, longest = case["requests"], case["longest"]
+    lengths = [longest] + [int(round(math.exp(rng.uniform(0.0, math.log(longest + 1)))))
+                           for _ in range(n - 1)]
+    lengths = [min(x, longest) for x in lengths]
+    if case.get("packed"):  # sequences cut to fill a training batch: half full at least
+        lengths = [longest] + [rng.randint((longest + 1) // 2, longest) for _ in range(n - 1)]
+    if n > 3 and not case.get("packed"):
+        lengths[1], lengths[2] = 0, 1
+    rng.shuffle(lengths)
+    return lengths
+
+
+def _plain_tables(lengths: torch.Tensor, slot_ids: torch.Tensor, max_tokens: int, rows: int):
+    """offsets [N+1], chunk_offsets [N+1], chunks [rows,4], order [N] (int32)."""
+    n = lengths.numel()
+    zero = torch.zeros(1, dtype=torch.int64, device=lengths.device)
+    sums = torch.cumsum(lengths.clamp(min=0).to(torch.int64), 0).clamp(max=max_tokens)
+    offsets = torch.cat([zero, sums])
+    tokens = offsets[1:] - offsets[:-1]
+    counts = (tokens + CHUNK - 1) // CHUNK
+    chunk_offsets = torch.cat([zero, torch.cumsum(counts, 0)])
+    row = torch.arange(rows, device=lengths.device)
+    request = torch.searchsorted(chunk_offsets[1:], row, right=True).clamp(max=n - 1)
+    used = row < chunk_offsets[-1]
+    local = row - chunk_offsets[request]
+    first = offsets[request] + local * CHUNK
+    count = (tokens[request] - local * CHUNK).clamp(max=CHUNK)
+    chunks = torch.stack([torch.where(used, request, -1), torch.where(used, first, 0),
+                          torch.where(used, count, 0),
+                          torch.where(used, slot_ids[request].to(torch.int64), -1)], 1)
+    order = torch.argsort(counts, descending=True, stable=True)
+    return (offsets.to(torch.int32), chunk_offsets.to(torch.int32), chunks.to(torch.int32),
+            order.to(torch.int32))
+
+
+def _rows(max_tokens: int, requests: int) -> int:
+    """Chunk rows that any split of max_tokens over the requests fits in."""
+    return max_tokens // CHUNK + requests
+
+
+def _tokens_of_a_layer(tokens, heads, key_heads, gen, dev):
+    """Queries, keys and values as slices of one fused projection, the log
+    decays and the write strengths of one layer."""
+    mixed = torch.randn((tokens, (2 * key_heads + heads) * DIM), generator=gen,
+                        device=dev).to(torch.bfloat16)
+    q = mixed[:, :key_heads * DIM].view(tokens, key_heads, DIM)
+    k = mixed[:, key_heads * DIM:2 * key_heads * DIM].view(tokens, key_heads, DIM)
+    v = mixed[:, 2 * key_heads * DIM:].view(tokens, heads, DIM)
+    rate = torch.exp(torch.rand((1, heads), generator=gen, device=dev) * 6.0 - 6.0)
+    noise = torch.randn((tokens, heads), generator=gen, device=dev)
+    log_decay = -rate * torch.nn.functional.softplus(noise)
+    beta = torch.sigmoid(torch.randn((tokens, heads), generator=gen, device=dev))
+    return q, k, v, log_decay, beta.to(torch.bfloat16)
+
+
+def prepare(case: dict, seed: int) -> dict:
+    dev = _device()
+    gen = _generator(seed, dev)
+    kind = case["kind"]
+    if kind == "tables":
+        n = case["requests"]
+        base = torch.tensor(_lengths(case), dtype=torch.int32, device=dev)
+        lengths = base[torch.randperm(n, generator=gen, device=dev)].contiguous()
+        slots = torch.randperm(n + 3, generator=gen, device=dev)[:n].to(torch.int32)
+        most = int(sum(_lengths(case))) + 5
+        return {"kind": kind, "lengths": lengths, "slots": slots, "max_tokens": most,
+                "rows": _rows(most, n)}
+    if kind == "step":
+        b, h, hk = case["batch"], case["heads"], case["key_heads"]
+        q, k, v, log_decay, beta = _tokens_of_a_layer(b, h, hk, gen, dev)
+        pool = (torch.randn((b + 3, h, DIM, DIM), generator=gen, device=dev) * 0.1).to(
+            _dtype(case["pool"]))
+        slots = torch.randperm(b + 3, generator=gen, device=dev)[:b].to(torch.int32)
+        if case["padded"]:
+            at = torch.randperm(b, generator=gen, device=dev)[:case["padded"]]
+            slots[at] = -1
+        out = torch.zeros((b, h, DIM), dtype=torch.bfloat16, device=dev)
+        return {"kind": kind, "q": q, "k": k, "v": v, "log_decay": log_decay, "beta": beta,
+                "pool": pool, "slots": slots, "out": out}
+    if kind in ("prefill", "train"):
+        lens = _lengths(case)
+        n, h, hk, total = len(lens), case["heads"], case["key_heads"], sum(lens)
+        q, k, v, log_decay, beta = _tokens_of_a_layer(total, h, hk, gen, dev)
+        lengths = torch.tensor(lens, dtype=torch.int32, device=dev)
+        slots = torch.randperm(n + 2, generator=gen, device=dev)[:n].to(torch.int32)
+        tables = _plain_tables(lengths, slots, total, _rows(total, n))
+        s = {"kind": kind, "lens": lens, "q": q, "k": k, "v": v, "log_decay": log_decay,
+             "beta": beta, "tables": tables, "slots": slots}
+        if kind == "prefill":
+            s["pool"] = (torch.randn((n + 2, h, DIM, DIM), generator=gen, device=dev) * 0.1).to(
+                _dtype(case["pool"]))
+            s["resume"] = (torch.arange(n, device=dev) % 2).to(torch.int32)
+            s["out"] = torch.zeros((total, h, DIM), dtype=torch.bfloat16, device=dev)
+        else:
+            s["initial"] = torch.randn((n, h, DIM, DIM), generator=gen, device=dev) * 0.1
+            s["d_out"] = torch.randn((total, h, DIM), generator=gen, device=dev).to(
+                torch.bfloat16)
+            s["d_final"] = torch.randn((n, h, DIM, DIM), generator=gen, device=dev) * 0.1
+            for name in ("q", "k", "v", "log_decay", "beta", "initial"):
+                s[name] = s[name].detach().requires_grad_(True)
+        return s
+    dtype = _dtype(case["dtype"])
+    if kind == "gated_norm":
+        shape = (case["tokens"], case["heads"], DIM)
+        x = torch.randn(shape, generator=gen, device=dev).to(dtype)
+        gate = torch.randn(shape, generator=gen, device=dev).to(dtype)
+        weight = 1.0 + 0.1 * torch.randn(DIM, generator=gen, device=dev)
+        s = {"kind": kind, "train": case["train"], "x": x, "gate": gate, "weight": weight}
+        names = ("x", "gate", "weight")
+    else:
+        shape = (case["tokens"], case["width"])
+        x = torch.randn(shape, generator=gen, device=dev).to(dtype)
+        residual = (2.0 * torch.randn(shape, generator=gen, device=dev)).to(
+            _dtype(case["stream"]))
+        weight = 1.0 + 0.1 * torch.randn(case["width"], generator=gen, device=dev)
+        s = {"kind": kind, "train": case["train"], "x": x, "residual": residual,
+             "weight": weight, "scale": 0.5}
+        names = ("x", "residual", "weight")
+    if case["train"]:
+        s["d_out"] = torch.randn(shape, generator=gen, device=dev).to(dtype)
+        if kind == "residual_norm":
+            s["d_sum"] = torch.randn(shape, generator=gen, device=dev).to(residual.dtype)
+        for name in names:
+            s[name] = s[name].detach().requires_grad_(True)
+    return s
+
+
+# ----------------------------------------------------------- the plain forms
+
+def _unit(x: torch.Tensor) -> torch.Tensor:
+    return x * torch.rsqrt((x * x).sum(-1, keepdim=True) + L2_EPS)
+
+
+def _plain_step(s: dict):
+    live = torch.nonzero(s["slots"] >= 0).reshape(-1)
+    slots = s["slots"][live].long()
+    group = s["v"].shape[1] // s["q"].shape[1]
+    q = (_unit(s["q"][live].float()) * SCALE).repeat_interleave(group, 1)
+    k = _unit(s["k"][live].float()).repeat_interleave(group, 1)
+    v, beta = s["v"][live].float(), s["beta"][live].float()
+    state = s["pool"][slots].float() * torch.exp(s["log_decay"][live])[..., None, None]
+    delta = beta[..., None] * (v - torch.matmul(state, k[..., None])[..., 0])
+    state = state + delta[..., :, None] * k[..., None, :]
+    s["out"][live] = torch.matmul(state, q[..., None])[..., 0].to(s["out"].dtype)
+    s["pool"][slots] = state.to(s["pool"].dtype)
+    return {"out": s["out"], "pool": s["pool"]}
+
+
+def _index(lens: list[int], dev) -> torch.Tensor:
+    """[N, whole chunks of the longest]: each request's token rows, -1 past its end."""
+    length = torch.tensor(lens, device=dev)
+    width = max(1, (max(lens) + CHUNK - 1) // CHUNK) * CHUNK
+    at = torch.arange(width, device=dev)[None, :]
+    start = torch.cumsum(length, 0) - length
+    return torch.where(at < length[:, None], start[:, None] + at, -1)
+
+
+def _plain_rule(q, k, v, log_decay, beta, lens, initial):
+    """The chunked form, requests side by side: fp32 out [T,H,128] and final
+    states [N,H,128(v),128(k)]."""
+    index = _index(lens, q.device)
+    n, width = index.shape
+    h, group, nc = v.shape[1], v.shape[1] // q.shape[1], width // CHUNK
+    live = (index >= 0)[..., None]
+    at = index.clamp(min=0)
+
+    def blocks(x):  # [T,H,D] -> [N,H,nc,CHUNK,D], zeros past each request's end
+        x = torch.where(live[..., None], x[at], torch.zeros((), device=x.device))
+        return x.reshape(n, nc, CHUNK, h, -1).permute(0, 3, 1, 2, 4).contiguous()
+
+    qs = blocks((_unit(q.float()) * SCALE).repeat_interleave(group, 1))
+    ks = blocks(_unit(k.float()).repeat_interleave(group, 1))
+    vs, b, g = blocks(v.float()), blocks(beta.float()[..., None]), blocks(log_decay[..., None])
+    total = torch.cumsum(g, 3)
+    lower = torch.ones((CHUNK, CHUNK), dtype=torch.bool, device=q.device).tril()
+    decay = torch.exp((total - total.transpose(-1, -2)).masked_fill(~lower, -math.inf))
+    write = ks * b
+    read = decay * torch.matmul(qs, write.transpose(-1, -2).contiguous())
+    step = -(decay * torch.matmul(ks, write.transpose(-1, -2).contiguous())).tril(-1)
+    solve = step + torch.eye(CHUNK, device=q.device)
+    for _ in range(5):  # (1 + A)(1 + A^2)(1 + A^4)..., A nilpotent
+        step = torch.matmul(step, step)
+        solve = solve + torch.matmul(solve, step)
+    fresh = torch.matmul(solve, vs)
+    seen = torch.matmul(solve, ks * torch.exp(total))
+    end = total[:, :, :, -1:]
+    kept = (write * torch.exp(end - total)).transpose(-1, -2).contiguous()
+    whole = torch.exp(end)
+    state = initial.transpose(-1, -2).contiguous()  # [N,H,key,value]
+    states, errors = [], []
+    for c in range(nc):
+        states.append(state)
+        errors.append(fresh[:, :, c] - torch.matmul(seen[:, :, c], state))
+        state = state * whole[:, :, c] + torch.matmul(kept[:, :, c], errors[-1])
+    out = (torch.matmul(qs * torch.exp(total), torch.stack(states, 2))
+           + torch.matmul(read, torch.stack(errors, 2)))
+    out = out.permute(0, 2, 3, 1, 4).reshape(n, width, h, DIM)
+    return out[index >= 0], state.transpose(-1, -2)
+
+
+def _plain_prefill(s: dict):
+    slots = s["slots"].long()
+    initial = s["pool"][slots].float() * s["resume"][:, None, None, None]
+    out, final = _plain_rule(s["q"], s["k"], s["v"], s["log_decay"], s["beta"], s["lens"],
+                             initial)
+    s["out"].copy_(out)
+    s["pool"][slots] = final.to(s["pool"].dtype)
+    return {"out": s["out"], "pool": s["pool"]}
+
+
+TRAINED = ("q", "k", "v", "log_decay", "beta", "initial")
+
+
+def _named(out, final, grads) -> dict:
+    return {"out": out, "final": final, **{f"d_{n}": g for n, g in zip(TRAINED, grads)}}
+
+
+def _plain_train(s: dict):
+    with torch.enable_grad():
+        out, final = _plain_rule(*(s[x] for x in TRAINED[:5]), s["lens"], s["initial"])
+    grads = torch.autograd.grad([out, final], [s[x] for x in TRAINED],
+                                [s["d_out"].float(), s["d_final"]])
+    return _named(out.detach().to(torch.bfloat16), final.detach(), grads)
+
+
+def _plain_gated_norm(x, gate, weight):
+    x, gate = x.float(), gate.float()
+    unit = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + NORM_EPS)
+    return unit * weight * (gate * torch.sigmoid(gate))
+
+
+def _plain_residual_norm(x, residual, weight, scale):
+    """The new residual stream, in its own type, and the norm of what it holds."""
+    total = residual.float() + scale * x.float()
+    if residual.dtype != torch.float32:  # the stream is what the next layer reads
+        total = total + (total.to(residual.dtype).float() - total).detach()
+    return total * torch.rsqrt((total * total).mean(-1, keepdim=True) + NORM_EPS) * weight, total
+
+
+def _plain_norms(s: dict):
+    if s["kind"] == "gated_norm":
+        names, dtypes = ("x", "gate", "weight"), (s["x"].dtype,)
+        call = lambda: (_plain_gated_norm(s["x"], s["gate"], s["weight"]),)  # noqa: E731
+    else:
+        names, dtypes = ("x", "residual", "weight"), (s["x"].dtype, s["residual"].dtype)
+        call = lambda: _plain_residual_norm(s["x"], s["residual"], s["weight"],  # noqa: E731
+                                            s["scale"])
+    with torch.set_grad_enabled(s["train"]):
+        outs = call()
+    got = {n: o.detach().to(d) for n, o, d in zip(("out", "sum"), outs, dtypes)}
+    if s["train"]:
+        grads = torch.autograd.grad(
+            outs, [s[n] for n in names],
+            [s[n].float() for n in ("d_out", "d_sum")[:len(outs)]])
+        got.update({f"d_{n}": g for n, g in zip(names, grads)})
+    return got
+
+
+# ------------------------------------------------------------ the operators
+
+def _package():
+    path = str(Path(__file__).resolve().parents[1] / "gdn-state-codec_amd")
+    if path not in sys.path:
+        sys.path.insert(0, path)
+    import gdn_state_codec
+
+    return gdn_state_codec
+
+
+def _own(s: dict):
+    package = _package()
+    kind = s["kind"]
+    if kind == "tables":
+        t = package.request_tables(s["lengths"], s["slots"], s["max_tokens"])
+        return {"offsets": t.offsets, "chunk_offsets": t.chunk_offsets, "chunks": t.chunks,
+                "order": t.order}
+    if kind == "step":
+        package.gated_delta_step(s["q"], s["k"], s["v"], s["log_decay"], s["beta"], s["pool"],
+                                 s["slots"], out=s["out"])
+        return {"out": s["out"], "pool": s["pool"]}
+    if kind == "prefill":
+        tables = package.RequestTables(*s["tables"])
+        package.gated_delta_prefill(s["q"], s["k"], s["v"], s["log_decay"], s["beta"], tables,
+                                    s["pool"], resume=s["resume"], out=s["out"])
+        return {"out": s["out"], "pool": s["pool"]}
+    if kind == "train":
+        tables = package.RequestTables(*s["tables"])
+        with torch.enable_grad():
+            out, final = package.gated_delta_rule(*(s[x] for x in TRAINED[:5]), tables,
+                                                  s["initial"])
+        grads = torch.autograd.grad([out, final], [s[x] for x in TRAINED],
+                                    [s["d_out"], s["d_final"]])
+        return _named(out.detach(), final.detach(), grads)
+    with torch.set_grad_enabled(s["train"]):
+        if kind == "gated_norm":
+            names = ("x", "gate", "weight")
+            outs = (package.gated_norm(s["x"], s["gate"], s["weight"], eps=NORM_EPS),)
+        else:
+            names = ("x", "residual", "weight")
+            outs = package.residual_norm(s["x"], s["residual"], s["weight"], scale=s["scale"],
+                                         eps=NORM_EPS)
+    got = {n: o.detach() for n, o in zip(("out", "sum"), outs)}
+    if s["train"]:
+        grads = torch.autograd.grad(outs, [s[n] for n in names],
+                                    [s[n] for n in ("d_out", "d_sum")[:len(outs)]])
+        got.update({f"d_{n}": g for n, g in zip(names, grads)})
+    return got
+
+
+def run(state: dict):
+    if own:
+        return _own(state)
+    kind = state["kind"]
+    if kind == "tables":
+        t = _plain_tables(state["lengths"], state["slots"], state["max_tokens"], state["rows"])
+        return dict(zip(("offsets", "chunk_offsets", "chunks", "order"), t))
+    if kind == "step":
+        return _plain_step(state)
+    if kind == "prefill":
+        return _plain_prefill(state)
+    if kind == "train":
+        return _plain_train(state)
+    return _plain_norms(state)
+
+
+# -------------------------------------------------------------- 64-bit values
+
+def _unit64(x: torch.Tensor):
+    r = ((x * x).sum(-1, keepdim=True) + L2_EPS) ** -0.5
+    return x * r, r
+
+
+def _unit64_gradient(x, r, d):
+    return r * d - x * r ** 3 * (x * d).sum(-1, keepdim=True)
+
+
+def _exact_rule(s: dict, initial: torch.Tensor, backward: bool):
+    """The recurrence token by token, every request at once (a finished one
+    decays by 1 and writes nothing): S' = a S; e = v - S' k; S = S' + b e k^T;
+    o = S q, with S [value][key]; and its gradients, in float64."""
+    with torch.no_grad():
+        return _exact_recurrence(s, initial, backward)
+
+
+def _exact_recurrence(s: dict, initial: torch.Tensor, backward: bool):
+    lens, dev = s["lens"], s["q"].device
+    total, hk = s["q"].shape[:2]
+    h = s["v"].shape[1]
+    n, group, longest = len(lens), h // hk, max(lens)
+    starts = torch.tensor([sum(lens[:i]) for i in range(n)], device=dev)
+    length = torch.tensor(lens, device=dev)
+    q_raw, k_raw = s["q"].detach().double(), s["k"].detach().double()
+    q_unit, rq = _unit64(q_raw)
+    k_unit, rk = _unit64(k_raw)
+    q = (q_unit * SCALE).repeat_interleave(group, 1)
+    k = k_unit.repeat_interleave(group, 1)
+    v, a = s["v"].detach().double(), torch.exp(s["log_decay"].detach().double())
+    b = s["beta"].detach().double()
+    out = torch.zeros((total + 1, h, DIM), dtype=torch.float64, device=dev)
+    state = initial.detach().double()
+    kept = (torch.empty((longest, n, h, DIM, DIM), dtype=torch.float64, device=dev)
+            if backward else None)
+    errors = torch.zeros((longest, n, h, DIM), dtype=torch.float64, device=dev) if backward else None
+    for t in range(longest):
+        live = t < length
+        at = torch.where(live, starts + t, 0)
+        kt, mask = k[at], live[:, None]
+        decay = torch.where(mask, a[at], 1.0)
+        state = state * decay[..., None, None]
+        error = v[at] - torch.matmul(state, kt[..., None])[..., 0]
+        strength = torch.where(mask, b[at], 0.0)
+        state = state + (strength[..., None] * error)[..., :, None] * kt[..., None, :]
+        out[torch.where(live, at, total)] = torch.matmul(state, q[at][..., None])[..., 0]
+        if backward:
+            kept[t], errors[t] = state, error
+    if not backward:
+        return out[:total], state
+    d_q, d_k = torch.zeros_like(q), torch.zeros_like(k)
+    d_v, d_a, d_b = torch.zeros_like(v), torch.zeros_like(a), torch.zeros_like(b)
+    d_out = s["d_out"].double()
+    ds = s["d_final"].double()
+    for t in range(longest - 1, -1, -1):
+        live = t < length
+        at = torch.where(live, starts + t, 0)
+        mask = live[:, None]
+        kt, qt = k[at], q[at]
+        do = torch.where(mask[..., None], d_out[at], 0.0)
+        strength = torch.where(mask, b[at], 0.0)
+        decay = torch.where(mask, a[at], 1.0)
+        d_qt = torch.matmul(kept[t].transpose(-1, -2), do[..., None])[..., 0]
+        ds = ds + do[..., :, None] * qt[..., None, :]
+        m = torch.matmul(ds, kt[..., None])[..., 0]  # by value
+        d_error = strength[..., None] * m
+        error = torch.where(mask[..., None], errors[t], 0.0)
+        before = kept[t] - (strength[..., None] * error)[..., :, None] * kt[..., None, :]
+        d_kt = (strength[..., None] * torch.matmul(ds.transpose(-1, -2), error[..., None])[..., 0]
+                - torch.matmul(before.transpose(-1, -2), d_error[..., None])[..., 0])
+        ds = ds - d_error[..., :, None] * kt[..., None, :]
+        row = torch.where(live, at, -1)
+        pick, rows = live.nonzero()[:, 0], row[live]
+        d_q[rows], d_k[rows], d_v[rows] = d_qt[pick], d_kt[pick], d_error[pick]
+        d_b[rows] = (m * error).sum(-1)[pick]
+        d_a[rows] = (ds * before).sum((-1, -2))[pick]
+        ds = ds * decay[..., None, None]
+    d_q = d_q.reshape(total, hk, group, DIM).sum(2) * SCALE
+    d_k = d_k.reshape(total, hk, group, DIM).sum(2)
+    grads = (_unit64_gradient(q_raw, rq, d_q), _unit64_gradient(k_raw, rk, d_k), d_v, d_a, d_b,
+             ds)
+    return _named(out[:total], state, grads)
+
+
+def _exact_tables(s: dict) -> dict:
+    lens, slots = s["lengths"].tolist(), s["slots"].tolist()
+    offsets, first, rows = [0], [0], []
+    for r, length in enumerate(lens):
+        begin, end = offsets[-1], min(offsets[-1] + max(length, 0), s["max_tokens"])
+        rows += [(r, t, min(CHUNK, end - t), slots[r]) for t in range(begin, end, CHUNK)]
+        offsets.append(end)
+        first.append(len(rows))
+    order = sorted(range(len(lens)), key=lambda r: first[r] - first[r + 1])
+    rows += [(-1, 0, 0, -1)] * (s["rows"] - len(rows))
+    made = {"offsets": offsets, "chunk_offsets": first, "chunks": rows, "order": order}
+    return {n: torch.tensor(x, dtype=torch.int32) for n, x in made.items()}
+
+
+def exact(case: dict, seed: int):
+    s = prepare(case, seed)
+    kind = s["kind"]
+    if kind == "tables":
+        return _exact_tables(s)
+    if kind == "step":
+        b = s["slots"].numel()
+        live = [i for i, slot in enumerate(s["slots"].tolist()) if slot >= 0]
+        slots = s["slots"][live].long()
+        one = {**{n: s[n][live] for n in ("q", "k", "v", "log_decay", "beta")},
+               "lens": [1] * len(live)}
+        got, final = _exact_rule(one, s["pool"][slots], False)
+        out = torch.zeros((b,) + tuple(got.shape[1:]), dtype=torch.float64, device=got.device)
+        out[live] = got
+        pool = s["pool"].double()
+        pool[slots] = final
+        return {"out": out, "pool": pool}
+    if kind == "prefill":
+        slots = s["slots"].long()
+        initial = s["pool"][slots].double() * s["resume"][:, None, None, None]
+        out, final = _exact_rule(s, initial, False)
+        pool = s["pool"].double()
+        pool[slots] = final
+        return {"out": out, "pool": pool}
+    if kind == "train":
+        return _exact_rule(s, s["initial"], True)
+    x, weight = s["x"].detach().double(), s["weight"].detach().double()
+    width = x.shape[-1]
+    if kind == "gated_norm":
+        total, gate = x, s["gate"].detach().double()
+        half = 1.0 / (1.0 + torch.exp(-gate))
+        through, slope = gate * half, half * (1.0 + gate * (1.0 - half))
+    else:
+        total = s["residual"].detach().double() + s["scale"] * x
+        if s["residual"].dtype != torch.float32:
+            total = total.to(s["residual"].dtype).double()
+        through = slope = 1.0
+    r = ((total * total).sum(-1, keepdim=True) / width + NORM_EPS) ** -0.5
+    unit = total * r
+    got = {"out": unit * weight * through}
+    if kind == "residual_norm":
+        got["sum"] = total
+    if s["train"]:
+        d = s["d_out"].double()
+        d_unit = d * weight * through
+        d_total = r * (d_unit - unit * (d_unit * unit).sum(-1, keepdim=True) / width)
+        d_weight = (d * unit * through).reshape(-1, width).sum(0)
+        if kind == "gated_norm":
+            got.update({"d_x": d_total, "d_gate": d * unit * weight * slope,
+                        "d_weight": d_weight})
+        else:
+            d_total = d_total + s["d_sum"].double()
+            got.update({"d_x": s["scale"] * d_total, "d_residual": d_total,
+                        "d_weight": d_weight})
+    return got
+
+
+# ------------------------------------------------------------------ the floor
+
+def work(case: dict) -> dict:
+    kind = case["kind"]
+    if kind == "tables":
+        rows = _rows(sum(_lengths(case)) + 5, case["requests"])
+        return {"bytes": 4 * (2 * case["requests"] + 3 * case["requests"] + 2) + 16 * rows,
+                "flops": 0}
+    if kind in ("step", "prefill", "train"):
+        h, hk = case["heads"], case["key_heads"]
+        if kind == "step":
+            tokens = requests = resumed = case["batch"] - case["padded"]
+        else:
+            lens = _lengths(case)
+            tokens, requests = sum(lens), len(lens)
+            resumed = requests // 2 if kind == "prefill" else requests
+        cell = 2 if case.get("pool") == "bf16" else 4
+        inputs = tokens * (2 * 2 * hk * DIM + 2 * h * DIM + 6 * h)
+        outputs = tokens * 2 * h * DIM
+        read, written = resumed * h * DIM * DIM * cell, requests * h * DIM * DIM * cell
+        # a token reads the state twice and adds to it once: 3 products of 128 x 128
+        flops = 6 * tokens * h * DIM * DIM
+        if kind != "train":
+            return {"bytes": inputs + outputs + read + written, "flops": flops}
+        # the backward pass reads the inputs and the output's gradient again and
+        # writes a gradient of each input; its products are twice the forward's
+        # and its state's, the forward's states once more
+        return {"bytes": 3 * inputs + 2 * outputs + 2 * (read + written), "flops": 4 * flops}
+    width = DIM * case["heads"] if kind == "gated_norm" else case["width"]
+    cells, cell = case["tokens"] * width, 2 if case["dtype"] == "bf16" else 4
+    if kind == "gated_norm":
+        each = 8 * cell if case["train"] else 3 * cell
+    else:
+        stream = 2 if case["stream"] == "bf16" else 4
+        # x, residual -> out, sum; and with gradients d_out, d_sum, sum -> d_x, d_residual
+        each = 2 * (cell + stream) + (2 * cell + 3 * stream if case["train"] else 0)
+    return {"bytes": cells * each, "flops": cells * (30 if case["train"] else 10)}
