@@ -401,7 +401,7 @@ def _own(s: dict):
     if kind == "prefill":
         tables = package.RequestTables(*s["tables"])
         package.gated_delta_prefill(s["q"], s["k"], s["v"], s["log_decay"], s["beta"], tables,
-                                    s["pool"], resume=s["resume"], out=s["out"])
+                                    s["slots"], s["pool"], resume=s["resume"], out=s["out"])
         return {"out": s["out"], "pool": s["pool"]}
     if kind == "train":
         tables = package.RequestTables(*s["tables"])
