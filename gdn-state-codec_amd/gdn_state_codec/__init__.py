@@ -15,6 +15,13 @@ from .codec import (
     project_decode,
 )
 from .capsule import CapsuleIdentity
+from .layer import (
+    RequestTables,
+    gated_delta_step,
+    gated_norm,
+    request_tables,
+    residual_norm,
+)
 from .runtime import GdnStateCodecExperiment, GdnStateCodecRuntime
 from .window import DecodeRuntime, WindowSlot
 
@@ -23,12 +30,15 @@ __all__ = [
     "LAYOUT_KEY_VALUE",
     "LAYOUT_VALUE_KEY",
     "DecodeRuntime",
+    "RequestTables",
     "GdnStateCodecExperiment",
     "GdnStateCodecRuntime",
     "WindowSlot",
     "NativeLibrary",
     "decode",
     "encode",
+    "gated_delta_step",
+    "gated_norm",
     "library_dir",
     "library_path",
     "native",
@@ -36,4 +46,6 @@ __all__ = [
     "pool_encode",
     "project_chunked",
     "project_decode",
+    "request_tables",
+    "residual_norm",
 ]

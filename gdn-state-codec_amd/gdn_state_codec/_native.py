@@ -79,6 +79,17 @@ SIGNATURES: dict[str, list] = {
         [_P] * 10 + [_U32, _C, _U64, _U64, _P, _P, _U64, _P, _U32],
     "statecentric_gdn_state_codec_capsule_restore_launch_v1":
         [_P] * 4 + [_U64, _C, _U64, _U64, _P, _U32] + [_P] * 10 + [_U32],
+    # include/gdn_state_codec_layer.h
+    "statecentric_gdn_state_codec_request_tables_launch_v1":
+        [_P, _P, _P, _U32, _U32, _U32] + [_P] * 4,
+    "statecentric_gdn_state_codec_gated_delta_step_launch_v1":
+        [_P] * 9 + [_U32] * 4 + [_U64] * 3 + [_U32, _F, _U32],
+    "statecentric_gdn_state_codec_gated_norm_launch_v1": [_P] * 5 + [_U64, _U32, _F],
+    "statecentric_gdn_state_codec_gated_norm_backward_launch_v1": [_P] * 9 + [_U64, _U32, _F],
+    "statecentric_gdn_state_codec_residual_norm_launch_v1":
+        [_P] * 6 + [_U64, _U32, _U32, _U32, _F, _F],
+    "statecentric_gdn_state_codec_residual_norm_backward_launch_v1":
+        [_P] * 9 + [_U64, _U32, _U32, _U32, _F, _F],
 }
 
 # Entry points that do not return a status: name -> (argtypes, restype).
@@ -88,6 +99,7 @@ OTHER_SIGNATURES: dict[str, tuple] = {
     "statecentric_gdn_state_codec_boundary_runtime_create_v1": ([_U32], _P),
     "statecentric_gdn_state_codec_boundary_runtime_destroy_v1": ([_P], None),
     "statecentric_gdn_state_codec_capsule_bytes_v1": ([_U32], _U64),
+    "statecentric_gdn_state_codec_norm_partials_v1": ([_U64, _U32], _U32),
 }
 
 

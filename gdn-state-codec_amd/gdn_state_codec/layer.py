@@ -1,0 +1,288 @@
+"""torch-facing dense operators of a gated-delta-net layer
+(include/gdn_state_codec_layer.h): the tables of a ragged batch, the gated delta
+rule for one token, for prefill and for training, and the norms around it.
+
+Each function checks shapes, dtypes, devices and strides on the host (raising
+``RuntimeError``, as the codec's do), launches the gfx950 kernels on torch's
+current stream and raises ``RuntimeError`` on a nonzero status.  Nothing here
+waits for the GPU: lengths, slot ids and tables stay on the device.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from ._native import native
+
+DIM = 128
+CHUNK = 64             # tokens of a row of RequestTables.chunks
+MAX_REQUESTS = 4096
+QUERY_SCALE = DIM ** -0.5
+_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+
+
+def _stream() -> int:
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _require(condition: bool, message: str) -> None:
+    if not condition:
+        raise RuntimeError(f"GDN State Codec {message}")
+
+
+def _launched(status: int, what: str) -> None:
+    if status != 0:
+        raise RuntimeError(f"GDN State Codec {what} launch failed: {status}")
+
+
+def _on_device(t: torch.Tensor, name: str) -> None:
+    _require(t.is_cuda and t.get_device() == torch.cuda.current_device(),
+             f"{name} must be on the current GPU")
+
+
+def _dense(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype) -> None:
+    """A contiguous tensor of exactly this shape and type, on the current GPU."""
+    _require(t.dtype == dtype and t.shape == shape and t.is_contiguous(),
+             f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}, got "
+             f"{t.dtype} {tuple(t.shape)} with strides {tuple(t.stride())}")
+    _on_device(t, name)
+
+
+class RequestTables(NamedTuple):
+    """The device tables of a ragged batch of N requests (all int32)."""
+
+    offsets: torch.Tensor        # [N+1] first token of each request, then their total
+    chunk_offsets: torch.Tensor  # [N+1] first row of each request in `chunks`
+    chunks: torch.Tensor         # [rows,4] request, first token, tokens, slot
+    order: torch.Tensor          # [N] requests by falling chunk count
+
+
+def table_rows(max_tokens: int, requests: int) -> int:
+    """Rows of ``RequestTables.chunks``: what any lengths need at most."""
+    return max_tokens // CHUNK + requests
+
+
+def request_tables(lengths: torch.Tensor, slot_ids: torch.Tensor,
+                   max_tokens: int) -> RequestTables:
+    """The tables of a batch whose requests' tokens are packed in one
+    ``max_tokens``-row buffer, from device int32 ``lengths`` and ``slot_ids`` [N]
+    (N in 1..4096; slot -1: padding).  A negative length counts as 0, and tokens
+    past ``max_tokens`` are cut off."""
+    _require(lengths.dim() == 1 and 1 <= lengths.numel() <= MAX_REQUESTS,
+             f"request lengths must be [1..{MAX_REQUESTS}]")
+    n = lengths.numel()
+    _dense(lengths, "request lengths", (n,), torch.int32)
+    _dense(slot_ids, "request slot ids", (n,), torch.int32)
+    _require(0 <= max_tokens < 2 ** 31, "request tables' max_tokens must be in 0..2^31-1")
+    rows = table_rows(max_tokens, n)
+    # One allocation; each table starts on a 16-byte boundary.
+    step = (n + 4) // 4 * 4
+    buffer = torch.empty(4 * rows + 3 * step, dtype=torch.int32, device=lengths.device)
+    chunks, offsets, chunk_offsets, order = buffer.split((4 * rows, step, step, step))
+    tables = RequestTables(offsets[:n + 1], chunk_offsets[:n + 1], chunks.view(rows, 4),
+                           order[:n])
+    _launched(native().request_tables_launch_v1(
+        _stream(), lengths.data_ptr(), slot_ids.data_ptr(), n, max_tokens, rows,
+        tables.offsets.data_ptr(), tables.chunk_offsets.data_ptr(), tables.chunks.data_ptr(),
+        tables.order.data_ptr()), "request tables")
+    return tables
+
+
+# ------------------------------------------------------- the gated delta rule
+
+def _token_rows(t: torch.Tensor, name: str, tokens: int) -> int:
+    """Checks bf16 [tokens,heads,128] whose heads are packed; the distance between
+    tokens may be any multiple of 8 elements (a slice of a fused projection).
+    Returns that distance."""
+    _require(t.dtype == torch.bfloat16 and t.dim() == 3 and t.shape[0] == tokens
+             and t.shape[1] > 0 and t.shape[2] == DIM,
+             f"{name} must be bf16 [{tokens},heads,128], got {t.dtype} {tuple(t.shape)}")
+    _on_device(t, name)
+    stride = t.stride(0) if tokens > 1 else t.shape[1] * DIM
+    _require(t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == DIM) and stride % 8 == 0
+             and stride >= t.shape[1] * DIM,
+             f"{name} must hold whole [heads,128] rows a multiple of 8 elements apart, got "
+             f"strides {tuple(t.stride())}")
+    return stride
+
+
+def _rule_inputs(queries, keys, values, log_decay, beta):
+    """Checks one batch of tokens; returns (tokens, value heads, key heads, strides)."""
+    tokens = queries.shape[0]
+    strides = (_token_rows(queries, "queries", tokens), _token_rows(keys, "keys", tokens),
+               _token_rows(values, "values", tokens))
+    heads, key_heads = values.shape[1], keys.shape[1]
+    _require(queries.shape[1] == key_heads and heads % key_heads == 0,
+             "queries and keys must have as many heads, and values a multiple of them")
+    _dense(log_decay, "log decay", (tokens, heads), torch.float32)
+    _dense(beta, "beta", (tokens, heads), torch.bfloat16)
+    return tokens, heads, key_heads, strides
+
+
+def _pool(pool: torch.Tensor, heads: int) -> int:
+    _require(pool.dtype in _TYPES and pool.dim() == 4 and pool.shape[0] > 0
+             and tuple(pool.shape[1:]) == (heads, DIM, DIM) and pool.is_contiguous(),
+             f"state pool must be contiguous fp32 or bf16 [slots,{heads},128 value,128 key]")
+    _on_device(pool, "state pool")
+    return _TYPES[pool.dtype]
+
+
+def gated_delta_step(queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
+                     log_decay: torch.Tensor, beta: torch.Tensor, pool: torch.Tensor,
+                     slot_ids: torch.Tensor, scale: float = QUERY_SCALE,
+                     normalize: bool = True, out: torch.Tensor | None = None) -> torch.Tensor:
+    """One token of the gated delta rule for each of B requests, on the dense
+    states ``pool`` [slots,H,128 value,128 key] (fp32 or bf16, one layer), updated
+    in place at ``slot_ids`` int32 [B] (distinct; outside the pool, as -1: padding,
+    skipped, its output row left as it was).
+
+    queries, keys bf16 [B,Hk,128], values bf16 [B,H,128] (rows of a fused
+    projection are fine), log_decay fp32 and beta bf16 [B,H]; returns bf16
+    [B,H,128].  ``normalize`` divides queries and keys by their 2-norm."""
+    batch, heads, key_heads, strides = _rule_inputs(queries, keys, values, log_decay, beta)
+    pool_dtype = _pool(pool, heads)
+    _dense(slot_ids, "slot ids", (batch,), torch.int32)
+    if out is None:
+        out = torch.zeros((batch, heads, DIM), dtype=torch.bfloat16, device=values.device)
+    else:
+        _dense(out, "output", (batch, heads, DIM), torch.bfloat16)
+    if batch:
+        _launched(native().gated_delta_step_launch_v1(
+            _stream(), queries.data_ptr(), keys.data_ptr(), values.data_ptr(),
+            log_decay.data_ptr(), beta.data_ptr(), pool.data_ptr(), slot_ids.data_ptr(),
+            out.data_ptr(), batch, pool.shape[0], heads, key_heads, *strides, pool_dtype,
+            scale, normalize), "gated delta step")
+    return out
+
+
+# ------------------------------------------------------------------ the norms
+
+def _rows_of(t: torch.Tensor, name: str, width: int) -> int:
+    _require(t.dtype in _TYPES and t.dim() >= 1 and t.shape[-1] == width and t.is_contiguous(),
+             f"{name} must be contiguous fp32 or bf16 [...,{width}], got {t.dtype} "
+             f"{tuple(t.shape)}")
+    _on_device(t, name)
+    return t.numel() // width
+
+
+def _partials(rows: int, width: int, device) -> torch.Tensor:
+    return torch.empty((native().norm_partials_v1(rows, width), width), dtype=torch.float32,
+                       device=device)
+
+
+def _gated_norm(x, gate, weight, eps: float) -> torch.Tensor:
+    out = torch.empty_like(x)
+    if x.numel():
+        _launched(native().gated_norm_launch_v1(
+            _stream(), x.data_ptr(), gate.data_ptr(), weight.data_ptr(), out.data_ptr(),
+            x.numel() // DIM, _TYPES[x.dtype], eps), "gated norm")
+    return out
+
+
+class _GatedNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, weight, eps):
+        ctx.save_for_backward(x, gate, weight)
+        ctx.eps = eps
+        return _gated_norm(x, gate, weight, eps)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_out):
+        x, gate, weight = ctx.saved_tensors
+        rows = x.numel() // DIM
+        d_out = d_out.to(x.dtype).contiguous()
+        d_x, d_gate, d_weight = torch.empty_like(x), torch.empty_like(x), torch.zeros_like(weight)
+        if rows:
+            _launched(native().gated_norm_backward_launch_v1(
+                _stream(), x.data_ptr(), gate.data_ptr(), weight.data_ptr(), d_out.data_ptr(),
+                d_x.data_ptr(), d_gate.data_ptr(), d_weight.data_ptr(),
+                _partials(rows, DIM, x.device).data_ptr(), rows, _TYPES[x.dtype], ctx.eps),
+                "gated norm backward")
+        return d_x, d_gate, d_weight, None
+
+
+def gated_norm(x: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor,
+               eps: float = 1e-6) -> torch.Tensor:
+    """``x / sqrt(mean(x^2) + eps) * weight * gate * sigmoid(gate)`` over the last
+    dimension (128): the norm after the rule, fused with the block's gate.
+
+    x and gate [...,128] of one type (bf16 or fp32), weight fp32 [128]; the result
+    has x's type.  Differentiable in all three."""
+    _rows_of(x, "gated norm input", DIM)
+    _rows_of(gate, "gate", DIM)
+    _require(gate.shape == x.shape and gate.dtype == x.dtype,
+             "gate must have the input's shape and type")
+    _dense(weight, "gated norm weight", (DIM,), torch.float32)
+    if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad
+                                    or weight.requires_grad):
+        return _GatedNorm.apply(x, gate, weight, eps)
+    return _gated_norm(x, gate, weight, eps)
+
+
+def _residual_norm(x, residual, weight, scale: float, eps: float):
+    out, total = torch.empty_like(x), torch.empty_like(residual)
+    if x.numel():
+        width = x.shape[-1]
+        _launched(native().residual_norm_launch_v1(
+            _stream(), x.data_ptr(), residual.data_ptr(), weight.data_ptr(), out.data_ptr(),
+            total.data_ptr(), x.numel() // width, width, _TYPES[x.dtype],
+            _TYPES[residual.dtype], scale, eps), "residual norm")
+    return out, total
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, weight, scale, eps):
+        out, total = _residual_norm(x, residual, weight, scale, eps)
+        ctx.save_for_backward(total, weight)
+        ctx.dtype, ctx.scale, ctx.eps = x.dtype, scale, eps
+        ctx.set_materialize_grads(False)
+        return out, total
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_out, d_total):
+        total, weight = ctx.saved_tensors
+        width = total.shape[-1]
+        rows = total.numel() // width
+        d_out = (torch.zeros_like(total, dtype=ctx.dtype) if d_out is None
+                 else d_out.to(ctx.dtype).contiguous())
+        if d_total is not None:
+            d_total = d_total.to(total.dtype).contiguous()
+        d_x, d_residual = torch.empty_like(d_out), torch.empty_like(total)
+        d_weight = torch.zeros_like(weight)
+        if rows:
+            _launched(native().residual_norm_backward_launch_v1(
+                _stream(), total.data_ptr(), weight.data_ptr(), d_out.data_ptr(),
+                0 if d_total is None else d_total.data_ptr(), d_x.data_ptr(),
+                d_residual.data_ptr(), d_weight.data_ptr(),
+                _partials(rows, width, total.device).data_ptr(), rows, width,
+                _TYPES[ctx.dtype], _TYPES[total.dtype], ctx.scale, ctx.eps),
+                "residual norm backward")
+        return d_x, d_residual, d_weight, None, None
+
+
+def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
+                  scale: float = 1.0, eps: float = 1e-6):
+    """``(out, sum)`` with ``sum = residual + scale * x`` in the residual stream's
+    type and ``out = sum / sqrt(mean(sum^2) + eps) * weight`` in x's: the norm
+    before a block, fused with the scaled residual sum of the block before.
+
+    x [...,D] and residual [...,D] bf16 or fp32 (each its own), weight fp32 [D], D
+    a multiple of 8 up to 16384.  The norm is of the stored (rounded) sum.
+    Differentiable in x, residual and weight."""
+    _require(x.dim() >= 1, "residual norm input must have a last dimension")
+    width = x.shape[-1]
+    _require(width % 8 == 0 and 0 < width <= 16384,
+             "residual norm width must be a multiple of 8 up to 16384")
+    _rows_of(x, "residual norm input", width)
+    _rows_of(residual, "residual stream", width)
+    _require(residual.shape == x.shape, "the residual stream must have the input's shape")
+    _dense(weight, "residual norm weight", (width,), torch.float32)
+    if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad
+                                    or weight.requires_grad):
+        return _ResidualNorm.apply(x, residual, weight, scale, eps)
+    return _residual_norm(x, residual, weight, scale, eps)
