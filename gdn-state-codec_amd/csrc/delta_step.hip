@@ -16,6 +16,7 @@
 #include <stdint.h>
 
 #include "activations.h"
+#include "delta_chunk.h"
 #include "gdn_state_codec_layer.h"
 #include "lane_exchange.h"
 #include "launch.h"
@@ -25,7 +26,7 @@ namespace gdn {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr float kUnitEps = 1e-6f;  // inside the square root of q's and k's norms
+
 
 struct StepArgs {
   const bf16_bits* queries;

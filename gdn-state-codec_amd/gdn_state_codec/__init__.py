@@ -17,6 +17,7 @@ from .codec import (
 from .capsule import CapsuleIdentity
 from .layer import (
     RequestTables,
+    gated_delta_prefill,
     gated_delta_step,
     gated_norm,
     request_tables,
@@ -37,6 +38,7 @@ __all__ = [
     "NativeLibrary",
     "decode",
     "encode",
+    "gated_delta_prefill",
     "gated_delta_step",
     "gated_norm",
     "library_dir",

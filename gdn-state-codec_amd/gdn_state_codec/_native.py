@@ -23,6 +23,18 @@ _F = ctypes.c_float
 _I32 = ctypes.c_int32
 _C = ctypes.c_char_p
 
+class RuleStruct(ctypes.Structure):
+    """``gdn_state_codec_rule`` (include/gdn_state_codec_layer.h)."""
+
+    _fields_ = (
+        [(name, _P) for name in ("queries", "keys", "values", "log_decay", "beta")]
+        + [(name, _U64) for name in ("query_stride", "key_stride", "value_stride")]
+        + [(name, _P) for name in ("offsets", "chunk_offsets", "chunks", "order", "workspace")]
+        + [("workspace_bytes", _U64)]
+        + [(name, _U32) for name in ("requests", "rows", "tokens", "value_heads", "key_heads")]
+        + [("scale", _F), ("normalize", _U32)])
+
+
 # name -> argtypes (all return int32 status)
 SIGNATURES: dict[str, list] = {
     # codec, reference entry points
@@ -84,6 +96,9 @@ SIGNATURES: dict[str, list] = {
         [_P, _P, _P, _U32, _U32, _U32] + [_P] * 4,
     "statecentric_gdn_state_codec_gated_delta_step_launch_v1":
         [_P] * 9 + [_U32] * 4 + [_U64] * 3 + [_U32, _F, _U32],
+    "statecentric_gdn_state_codec_gated_delta_prefill_launch_v1":
+        [_P] * 5 + [_U32, _U32, _P],
+    "statecentric_gdn_state_codec_gated_delta_forward_launch_v1": [_P] * 5,
     "statecentric_gdn_state_codec_gated_norm_launch_v1": [_P] * 5 + [_U64, _U32, _F],
     "statecentric_gdn_state_codec_gated_norm_backward_launch_v1": [_P] * 9 + [_U64, _U32, _F],
     "statecentric_gdn_state_codec_residual_norm_launch_v1":
@@ -99,6 +114,7 @@ OTHER_SIGNATURES: dict[str, tuple] = {
     "statecentric_gdn_state_codec_boundary_runtime_create_v1": ([_U32], _P),
     "statecentric_gdn_state_codec_boundary_runtime_destroy_v1": ([_P], None),
     "statecentric_gdn_state_codec_capsule_bytes_v1": ([_U32], _U64),
+    "statecentric_gdn_state_codec_gated_delta_workspace_v1": ([_U32] * 4, _U64),
     "statecentric_gdn_state_codec_norm_partials_v1": ([_U64, _U32], _U32),
 }
 

@@ -10,11 +10,12 @@ waits for the GPU: lengths, slot ids and tables stay on the device.
 
 from __future__ import annotations
 
+import ctypes
 from typing import NamedTuple
 
 import torch
 
-from ._native import native
+from ._native import RuleStruct, native
 
 DIM = 128
 CHUNK = 64             # tokens of a row of RequestTables.chunks
@@ -154,6 +155,81 @@ def gated_delta_step(queries: torch.Tensor, keys: torch.Tensor, values: torch.Te
             log_decay.data_ptr(), beta.data_ptr(), pool.data_ptr(), slot_ids.data_ptr(),
             out.data_ptr(), batch, pool.shape[0], heads, key_heads, *strides, pool_dtype,
             scale, normalize), "gated delta step")
+    return out
+
+
+def _check_tables(tables: RequestTables, tokens: int) -> int:
+    """Checks that the tables are a batch's of `tokens` token rows; returns N."""
+    requests = tables.order.numel()
+    _require(1 <= requests <= MAX_REQUESTS, f"tables must hold 1..{MAX_REQUESTS} requests")
+    for t, name, shape in ((tables.offsets, "offsets", (requests + 1,)),
+                           (tables.chunk_offsets, "chunk_offsets", (requests + 1,)),
+                           (tables.chunks, "chunks", (table_rows(tokens, requests), 4)),
+                           (tables.order, "order", (requests,))):
+        _dense(t, f"tables.{name}", shape, torch.int32)
+    return requests
+
+
+def workspace_bytes(tokens: int, requests: int, heads: int, key_heads: int,
+                    train: bool = False) -> int:
+    """Bytes of scratch that a prefill (or a forward and backward pass) takes."""
+    return native().gated_delta_workspace_v1(table_rows(tokens, requests), heads, key_heads,
+                                             train)
+
+
+def _rule(queries, keys, values, log_decay, beta, tables, scale, normalize, workspace, train):
+    """The checked argument struct of a whole-sequence call and its workspace."""
+    tokens, heads, key_heads, strides = _rule_inputs(queries, keys, values, log_decay, beta)
+    requests = _check_tables(tables, tokens)
+    needed = workspace_bytes(tokens, requests, heads, key_heads, train)
+    if workspace is None:
+        workspace = torch.empty(needed, dtype=torch.uint8, device=values.device)
+    else:
+        _require(workspace.dtype == torch.uint8 and workspace.is_contiguous()
+                 and workspace.numel() >= needed,
+                 f"workspace must be contiguous uint8 of at least {needed} bytes")
+        _on_device(workspace, "workspace")
+    rule = RuleStruct(queries.data_ptr(), keys.data_ptr(), values.data_ptr(),
+                      log_decay.data_ptr(), beta.data_ptr(), *strides,
+                      tables.offsets.data_ptr(), tables.chunk_offsets.data_ptr(),
+                      tables.chunks.data_ptr(), tables.order.data_ptr(), workspace.data_ptr(),
+                      workspace.numel(), requests, tables.chunks.shape[0], tokens, heads,
+                      key_heads, scale, normalize)
+    return rule, workspace
+
+
+def gated_delta_prefill(queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
+                        log_decay: torch.Tensor, beta: torch.Tensor, tables: RequestTables,
+                        slot_ids: torch.Tensor, pool: torch.Tensor,
+                        resume: torch.Tensor | None = None, scale: float = QUERY_SCALE,
+                        normalize: bool = True, workspace: torch.Tensor | None = None,
+                        out: torch.Tensor | None = None) -> torch.Tensor:
+    """The gated delta rule over the packed sequences of N requests, on the dense
+    states ``pool`` [slots,H,128 value,128 key] (fp32 or bf16, one layer): request
+    r starts from the state at ``slot_ids[r]`` (int32 [N], distinct; outside the
+    pool, as -1: padding, skipped) where ``resume`` (int32 [N]) is nonzero or not
+    given, from zeros where it is 0, and leaves its final state there.
+
+    queries, keys bf16 [T,Hk,128], values bf16 [T,H,128] (rows of a fused
+    projection are fine), log_decay fp32 and beta bf16 [T,H]; ``tables`` are
+    :func:`request_tables`' for ``max_tokens`` T and the same slot ids.  Returns
+    bf16 [T,H,128]; rows of no request, and padding's, stay as they were.
+    ``workspace`` (uint8, :func:`workspace_bytes`) may be kept between calls."""
+    rule, workspace = _rule(queries, keys, values, log_decay, beta, tables, scale, normalize,
+                            workspace, False)
+    heads = values.shape[1]
+    pool_dtype = _pool(pool, heads)
+    _dense(slot_ids, "slot ids", (rule.requests,), torch.int32)
+    if resume is not None:
+        _dense(resume, "resume", (rule.requests,), torch.int32)
+    if out is None:
+        out = torch.zeros((rule.tokens, heads, DIM), dtype=torch.bfloat16, device=values.device)
+    else:
+        _dense(out, "output", (rule.tokens, heads, DIM), torch.bfloat16)
+    _launched(native().gated_delta_prefill_launch_v1(
+        _stream(), ctypes.byref(rule), slot_ids.data_ptr(),
+        0 if resume is None else resume.data_ptr(), pool.data_ptr(), pool.shape[0], pool_dtype,
+        out.data_ptr()), "gated delta prefill")
     return out
 
 

@@ -71,6 +71,54 @@ int32_t statecentric_gdn_state_codec_gated_delta_step_launch_v1(
     uint64_t query_stride, uint64_t key_stride, uint64_t value_stride,
     uint32_t pool_dtype, float scale, uint32_t normalize);
 
+/* A packed ragged batch and the scratch its whole-sequence form works in. */
+typedef struct gdn_state_codec_rule {
+  const uint16_t* queries;      /* bf16 [tokens][key_heads][128] */
+  const uint16_t* keys;         /* bf16 [tokens][key_heads][128] */
+  const uint16_t* values;       /* bf16 [tokens][value_heads][128] */
+  const float* log_decay;       /* [tokens][value_heads] */
+  const uint16_t* beta;         /* bf16 [tokens][value_heads] */
+  uint64_t query_stride;        /* elements between tokens, multiples of 8 */
+  uint64_t key_stride;
+  uint64_t value_stride;
+  const int32_t* offsets;       /* request_tables' outputs for max_tokens = tokens */
+  const int32_t* chunk_offsets;
+  const int32_t* chunks;
+  const int32_t* order;
+  void* workspace;              /* gated_delta_workspace(...) bytes at least */
+  uint64_t workspace_bytes;
+  uint32_t requests;            /* 1..4096 */
+  uint32_t rows;                /* tokens / 64 + requests */
+  uint32_t tokens;
+  uint32_t value_heads;
+  uint32_t key_heads;
+  float scale;
+  uint32_t normalize;
+} gdn_state_codec_rule;
+
+/* Bytes of the workspace: for prefill (train 0), or for a forward and backward
+ * pass (train 1; the backward pass reads what the forward pass left there). */
+uint64_t statecentric_gdn_state_codec_gated_delta_workspace_v1(
+    uint32_t rows, uint32_t value_heads, uint32_t key_heads, uint32_t train);
+
+/* Whole sequences on a slot-indexed pool [slots][value_heads][128 value]
+ * [128 key] of pool_dtype: request r starts from its slot's state (resume NULL or
+ * resume[r] != 0) or from zeros, and leaves its final state there.  slot_ids int32
+ * [requests] (distinct); a request whose slot is outside 0..slots-1 (padding, -1)
+ * is skipped, its outputs left as they were.  An empty request leaves its state, or
+ * zeros where it does not resume.  outputs bf16 [tokens][value_heads][128]. */
+int32_t statecentric_gdn_state_codec_gated_delta_prefill_launch_v1(
+    void* stream, const gdn_state_codec_rule* rule, const int32_t* slot_ids,
+    const int32_t* resume, void* pool, uint32_t slots, uint32_t pool_dtype,
+    uint16_t* outputs);
+
+/* Whole packed sequences for training: initial (or NULL: zeros) and final_states
+ * fp32 [requests][value_heads][128 value][128 key].  The slots in `chunks` must be
+ * 0 or more.  Leaves in the workspace what the backward pass reads. */
+int32_t statecentric_gdn_state_codec_gated_delta_forward_launch_v1(
+    void* stream, const gdn_state_codec_rule* rule, const float* initial,
+    float* final_states, uint16_t* outputs);
+
 /* out = x / sqrt(mean(x^2) + eps) * weight * gate * sigmoid(gate) over rows of
  * 128.  x, gate, out [rows][128] of `dtype`, weight fp32 [128]. */
 int32_t statecentric_gdn_state_codec_gated_norm_launch_v1(
