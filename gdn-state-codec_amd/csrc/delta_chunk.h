@@ -63,21 +63,22 @@ __device__ __forceinline__ constexpr int upper_first(int row) { return row < 2 ?
 constexpr int kSolveParts = 3;  // parts of N (an fp32 operand)
 constexpr int kReadParts = 2;   // parts of P b: the outputs it makes are bf16
 
-// Factors of a chunk's tokens for one value head, fp32 [6][64].
+// Factors of a chunk's tokens for one value head, fp32 [7][64].
 enum : int {
   kReadKey = 0,    // exp(G_i) / |k_i|
   kReadQuery = 1,  // exp(G_i) scale / |q_i|
   kStrength = 2,   // b_i, 0 past the request's end
   kWrite = 3,      // exp(G_63 - G_j) / |k_j|
-  kSum = 4,        // G_i
-  kWhole = 5,      // exp(G_63), in every place
-  kFactors = 6
+  kWhole = 4,      // exp(G_63), in every place
+  kSum = 5,        // G_i, and below it what fp32 left of it
+  kSumRest = 6,
+  kFactors = 7
 };
 
 // Bytes of the workspace's parts.
 constexpr uint64_t kHeadFactors = kFactors * kChunk * 4;
 __host__ __device__ constexpr uint64_t key_block_bytes(bool train) {
-  return (train ? 4 : 3) * kKeyTiles * kTileBytes + 2 * kChunk * 4;  // + 1/|k|, scale/|q|
+  return train ? 4 * kKeyTiles * kTileBytes + 3 * kChunk * 4 : 3 * kKeyTiles * kTileBytes;
 }
 __host__ __device__ constexpr uint64_t value_block_bytes(bool train) {
   const uint64_t serving = (kSolveParts + kReadParts) * kTriangle * kTileBytes + kHeadFactors;
@@ -130,8 +131,8 @@ struct ChunkSpace {
 constexpr int kKeyRows = 0;
 constexpr int kQueryRows = kKeyTiles * kTileBytes;
 constexpr int kKeyColumns = 2 * kKeyTiles * kTileBytes;
-__host__ __device__ constexpr int norms_at(bool train) { return (train ? 4 : 3) * kKeyTiles * kTileBytes; }
 constexpr int kQueryColumns = 3 * kKeyTiles * kTileBytes;  // training
+constexpr int kNorms = 4 * kKeyTiles * kTileBytes;  // training: fp32 1/|k|, scale/|q|, 1/|q|
 // Places inside a value block: factors, N, P b, then N^T and P^T (training).
 constexpr int kSolve = kHeadFactors;
 constexpr int kReadOut = kSolve + kSolveParts * kTriangle * kTileBytes;
@@ -212,6 +213,35 @@ __device__ __forceinline__ f32x4 mfma3(const uint4 (&a)[3], const uint4& b, f32x
 
 __device__ __forceinline__ f32x4 load4(const float* p) {
   return *reinterpret_cast<const f32x4*>(p);
+}
+
+// Four neighbouring cells of a state.
+__device__ __forceinline__ f32x4 load_cells(const float* p) { return load4(p); }
+__device__ __forceinline__ f32x4 load_cells(const bf16_bits* p) {
+  const uint2 w = *reinterpret_cast<const uint2*>(p);
+  return f32x4{widen_low(w.x), widen_high(w.x), widen_low(w.y), widen_high(w.y)};
+}
+__device__ __forceinline__ void store_cells(float* p, const f32x4& x) {
+  *reinterpret_cast<f32x4*>(p) = x;
+}
+__device__ __forceinline__ void store_cells(bf16_bits* p, const f32x4& x) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]));
+}
+
+// One tile, 16 bytes a lane, from global memory into LDS at `to` (bytes, the same
+// for the wavefront) without passing the registers.  The caller waits
+// (stage_ready) before any lane reads it.
+__device__ __forceinline__ void stage_tile(const char* tile, int lane, uint32_t to) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
+               :
+               : "v"(16 * lane), "s"(tile), "s"(to)
+               : "memory");
+}
+
+// Every staged tile of the workgroup is in LDS, and the stage read before may be
+// overwritten, after this.
+__device__ __forceinline__ void stage_ready() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 }  // namespace gdn

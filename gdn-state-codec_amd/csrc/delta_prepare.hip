@@ -36,6 +36,7 @@ struct Staged {
   float strength[2][kChunk];
   float k_unit[kChunk];     // 1 / |k|
   float q_unit[kChunk];     // scale / |q|
+  float q_norm[kChunk];     // 1 / |q|
 };
 
 // LDS written by other lanes of the same wavefront is read after this.
@@ -159,15 +160,28 @@ __device__ __forceinline__ void read_out_head(const Staged& s, int slot, int lan
   }
 }
 
+// The outputs of tokens of no request: zeros, for one key head's value heads.
+__device__ __forceinline__ void clear_rest(const RuleArgs& a, uint32_t head,
+                                           bf16_bits* outputs) {
+  const uint32_t from = min(static_cast<uint32_t>(a.offsets[a.requests]), a.tokens);
+  const uint32_t width = a.group * kDim;
+  for (uint64_t i = threadIdx.x; i < static_cast<uint64_t>(a.tokens - from) * width;
+       i += kThreads) {
+    outputs[(from + i / width) * a.space.value_heads * kDim + head * width + i % width] = 0;
+  }
+}
+
 template <bool kTrain>
-__global__ __launch_bounds__(kThreads) void delta_prepare_kernel(RuleArgs a) {
+__global__ __launch_bounds__(kThreads) void delta_prepare_kernel(RuleArgs a,
+                                                                bf16_bits* outputs) {
   __shared__ Staged s;
   const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
   const uint32_t row = blockIdx.x / a.space.key_heads;
   const uint32_t head = blockIdx.x % a.space.key_heads;
   const int4 chunk = a.chunks[row];
   const int count = chunk_tokens(a, chunk);
-  if (count == 0 || chunk.w < 0) return;  // past the last chunk, or padding
+  if (kTrain && row == 0) clear_rest(a, head, outputs);
+  if (count == 0 || (!kTrain && chunk.w < 0)) return;  // past the last chunk, or padding
   const uint64_t first = chunk.y;
 
   {  // stage the rows, 32 columns a thread, zeros past the request's end
@@ -197,7 +211,8 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(RuleArgs a) {
     qq = add_partner<2>(add_partner<1>(qq));
     if (part == 0) {
       s.k_unit[token] = a.normalize ? 1.0f / sqrtf(kk + kUnitEps) : 1.0f;
-      s.q_unit[token] = a.scale * (a.normalize ? 1.0f / sqrtf(qq + kUnitEps) : 1.0f);
+      s.q_norm[token] = a.normalize ? 1.0f / sqrtf(qq + kUnitEps) : 1.0f;
+      s.q_unit[token] = a.scale * s.q_norm[token];
     }
   }
   __syncthreads();
@@ -262,10 +277,11 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(RuleArgs a) {
         }
       }
     }
-    if (t < kChunk) {
-      float* norms = reinterpret_cast<float*>(key_block + norms_at(kTrain));
+    if (kTrain && t < kChunk) {
+      float* norms = reinterpret_cast<float*>(key_block + kNorms);
       norms[t] = s.k_unit[t];
       norms[kChunk + t] = s.q_unit[t];
+      norms[2 * kChunk + t] = s.q_norm[t];
     }
   }
 
@@ -297,6 +313,8 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(RuleArgs a) {
       factors[kWrite * kChunk + lane] =
           expf(static_cast<float>(end - sum)) * s.k_unit[lane];
       factors[kSum * kChunk + lane] = static_cast<float>(sum);
+      factors[kSumRest * kChunk + lane] =
+          static_cast<float>(sum - static_cast<double>(static_cast<float>(sum)));
       factors[kWhole * kChunk + lane] = expf(static_cast<float>(end));
     }
     __syncthreads();
@@ -309,10 +327,11 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(RuleArgs a) {
 
 }  // namespace
 
-int32_t launch_delta_prepare(void* stream, const RuleArgs& args) {
+int32_t launch_delta_prepare(void* stream, const RuleArgs& args, bf16_bits* outputs) {
   const dim3 grid(args.space.rows * args.space.key_heads), block(kThreads);
-  return args.space.train ? launch(delta_prepare_kernel<true>, grid, block, stream, args)
-                          : launch(delta_prepare_kernel<false>, grid, block, stream, args);
+  return args.space.train
+             ? launch(delta_prepare_kernel<true>, grid, block, stream, args, outputs)
+             : launch(delta_prepare_kernel<false>, grid, block, stream, args, outputs);
 }
 
 }  // namespace gdn

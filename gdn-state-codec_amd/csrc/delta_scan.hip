@@ -16,6 +16,8 @@
 
 namespace gdn {
 
+int32_t launch_delta_prepare(void* stream, const RuleArgs& args, bf16_bits* outputs);
+
 struct ScanArgs {
   RuleArgs rule;
   const void* initial;       // states [..][value head][value][key], or null: zeros
@@ -28,19 +30,6 @@ struct ScanArgs {
 
 namespace {
 
-// One float4 of a pool row: 4 keys of one value.
-__device__ __forceinline__ f32x4 load_cells(const float* p) { return load4(p); }
-__device__ __forceinline__ f32x4 load_cells(const bf16_bits* p) {
-  const uint2 w = *reinterpret_cast<const uint2*>(p);
-  return f32x4{widen_low(w.x), widen_high(w.x), widen_low(w.y), widen_high(w.y)};
-}
-__device__ __forceinline__ void store_cells(float* p, const f32x4& x) {
-  *reinterpret_cast<f32x4*>(p) = x;
-}
-__device__ __forceinline__ void store_cells(bf16_bits* p, const f32x4& x) {
-  *reinterpret_cast<uint2*>(p) = make_uint2(bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]));
-}
-
 // A chunk's operands in LDS: K, Q and K^T of the key head, then the first 32 KiB
 // of the value head's block (factors, N, P b; 512 bytes of it are not used).
 constexpr int kKeyStage = 3 * kKeyTiles * kTileBytes;
@@ -48,16 +37,6 @@ constexpr int kValueStage = 32 * kTileBytes;
 constexpr int kStage = kKeyStage + kValueStage;
 static_assert(value_block_bytes(false) <= kValueStage, "the stage holds a value block");
 static_assert(2 * kStage <= static_cast<int>(kLdsPerCu), "two stages fill the LDS");
-
-// One tile, 16 bytes a lane, from global memory into LDS at `to` (bytes, the same
-// for the wavefront) without passing the registers.  The caller waits
-// (stage_ready) before any lane reads it.
-__device__ __forceinline__ void stage_tile(const char* tile, int lane, uint32_t to) {
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
-               :
-               : "v"(16 * lane), "s"(tile), "s"(to)
-               : "memory");
-}
 
 template <int kWaves>
 __device__ __forceinline__ void stage_chunk(const char* keys, const char* block, int wave,
@@ -68,12 +47,6 @@ __device__ __forceinline__ void stage_chunk(const char* keys, const char* block,
     const char* from = tile < 48 ? keys + tile * kTileBytes : block + (tile - 48) * kTileBytes;
     stage_tile(from, lane, to + tile * kTileBytes);
   }
-}
-
-// Every staged tile of the workgroup is in LDS, and the stage read before may be
-// overwritten, after this.
-__device__ __forceinline__ void stage_ready() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 template <typename Pool, int kWaves, bool kTrain>
@@ -139,6 +112,14 @@ __global__ __launch_bounds__(64 * kWaves, 1) void delta_scan_kernel(ScanArgs arg
 
   f32x4 error[4], out[4];
   const auto store_outputs = [&](uint32_t c, int tokens) {
+    if constexpr (kTrain) {
+      float* e = space.errors(first_row + c, head) + value;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) e[(16 * t + 4 * g + i) * kDim] = error[t][i];
+      }
+    }
     bf16_bits* o = args.outputs + (begin + c * kChunk) * token_step + head * kDim + value;
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -279,14 +260,6 @@ __global__ __launch_bounds__(64 * kWaves, 1) void delta_scan_kernel(ScanArgs arg
         out[t] = mfma(high, plain[0], out[t]);
       }
     }
-    if constexpr (kTrain) {
-      float* e = space.errors(row, head) + value;
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) e[(16 * t + 4 * g + i) * kDim] = error[t][i];
-      }
-    }
   }
   if (chunks != 0) store_outputs(chunks - 1, length - (chunks - 1) * kChunk);
 
@@ -312,8 +285,6 @@ int32_t launch_delta_scan(void* stream, const ScanArgs& args, uint32_t dtype) {
   return dtype == kDtypeF32 ? launch_scan<float, 4, false>(stream, args)
                             : launch_scan<bf16_bits, 4, false>(stream, args);
 }
-
-int32_t launch_delta_prepare(void* stream, const RuleArgs& args);
 
 // Checks the caller's arguments and fills the kernels'; false: a bad argument.
 bool rule_args(const gdn_state_codec_rule* rule, bool train, RuleArgs& a) {
@@ -358,7 +329,7 @@ extern "C" int32_t statecentric_gdn_state_codec_gated_delta_prefill_launch_v1(
   }
   args.initial = pool, args.final_states = pool, args.slot_ids = slot_ids, args.resume = resume;
   args.slots = slots, args.outputs = outputs;
-  const int32_t status = gdn::launch_delta_prepare(stream, args.rule);
+  const int32_t status = gdn::launch_delta_prepare(stream, args.rule, outputs);
   return status != gdn::kStatusOk ? status : gdn::launch_delta_scan(stream, args, pool_dtype);
 }
 
@@ -372,7 +343,7 @@ extern "C" int32_t statecentric_gdn_state_codec_gated_delta_forward_launch_v1(
   }
   args.initial = initial, args.final_states = final_states, args.slots = rule->requests;
   args.outputs = outputs;
-  const int32_t status = gdn::launch_delta_prepare(stream, args.rule);
+  const int32_t status = gdn::launch_delta_prepare(stream, args.rule, outputs);
   return status != gdn::kStatusOk ? status
                                   : gdn::launch_delta_scan(stream, args, gdn::kDtypeF32);
 }

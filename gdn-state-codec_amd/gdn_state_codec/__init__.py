@@ -18,6 +18,7 @@ from .capsule import CapsuleIdentity
 from .layer import (
     RequestTables,
     gated_delta_prefill,
+    gated_delta_rule,
     gated_delta_step,
     gated_norm,
     request_tables,
@@ -39,6 +40,7 @@ __all__ = [
     "decode",
     "encode",
     "gated_delta_prefill",
+    "gated_delta_rule",
     "gated_delta_step",
     "gated_norm",
     "library_dir",

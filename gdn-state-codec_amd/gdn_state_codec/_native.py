@@ -99,6 +99,7 @@ SIGNATURES: dict[str, list] = {
     "statecentric_gdn_state_codec_gated_delta_prefill_launch_v1":
         [_P] * 5 + [_U32, _U32, _P],
     "statecentric_gdn_state_codec_gated_delta_forward_launch_v1": [_P] * 5,
+    "statecentric_gdn_state_codec_gated_delta_backward_launch_v1": [_P] * 10,
     "statecentric_gdn_state_codec_gated_norm_launch_v1": [_P] * 5 + [_U64, _U32, _F],
     "statecentric_gdn_state_codec_gated_norm_backward_launch_v1": [_P] * 9 + [_U64, _U32, _F],
     "statecentric_gdn_state_codec_residual_norm_launch_v1":

@@ -233,6 +233,63 @@ def gated_delta_prefill(queries: torch.Tensor, keys: torch.Tensor, values: torch
     return out
 
 
+class _GatedDeltaRule(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, queries, keys, values, log_decay, beta, initial, tables, scale, normalize):
+        rule, workspace = _rule(queries, keys, values, log_decay, beta, tables, scale, normalize,
+                                None, True)
+        heads = values.shape[1]
+        out = torch.empty((rule.tokens, heads, DIM), dtype=torch.bfloat16, device=values.device)
+        final = torch.empty((rule.requests, heads, DIM, DIM), dtype=torch.float32,
+                            device=values.device)
+        _launched(native().gated_delta_forward_launch_v1(
+            _stream(), ctypes.byref(rule), 0 if initial is None else initial.data_ptr(),
+            final.data_ptr(), out.data_ptr()), "gated delta forward")
+        # The struct's pointers stay good as long as these tensors are kept.
+        ctx.save_for_backward(queries, keys, values, log_decay, beta, *tables, workspace)
+        ctx.rule, ctx.resumed = rule, initial is not None
+        ctx.set_materialize_grads(False)
+        return out, final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_out, d_final):
+        queries, keys, values, log_decay, beta = ctx.saved_tensors[:5]
+        rule = ctx.rule
+        shape = (rule.requests, rule.value_heads, DIM, DIM)
+        if d_out is None:
+            d_out = torch.zeros(values.shape, dtype=torch.bfloat16, device=values.device)
+        d_out = d_out.to(torch.bfloat16).contiguous()
+        if d_final is not None:
+            d_final = d_final.to(torch.float32).contiguous()
+        new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
+        grads = [new(t) for t in (queries, keys, values, log_decay, beta)]
+        d_initial = (torch.empty(shape, dtype=torch.float32, device=values.device)
+                     if ctx.resumed else None)
+        _launched(native().gated_delta_backward_launch_v1(
+            _stream(), ctypes.byref(rule), d_out.data_ptr(),
+            0 if d_final is None else d_final.data_ptr(), *(t.data_ptr() for t in grads),
+            0 if d_initial is None else d_initial.data_ptr()), "gated delta backward")
+        return *grads, d_initial, None, None, None
+
+
+def gated_delta_rule(queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
+                     log_decay: torch.Tensor, beta: torch.Tensor, tables: RequestTables,
+                     initial: torch.Tensor | None = None, scale: float = QUERY_SCALE,
+                     normalize: bool = True):
+    """``(out, final)`` of the gated delta rule over the packed sequences of N
+    requests, differentiable in every tensor: the inputs of
+    :func:`gated_delta_prefill` with ``initial`` fp32 [N,H,128 value,128 key] (or
+    None: zeros) in the pool's place.  out is bf16 [T,H,128] (zeros in rows of no
+    request), final fp32 like initial.  The graph keeps a workspace of
+    ``workspace_bytes(T, N, H, Hk, train=True)`` until its backward pass."""
+    if initial is not None:
+        _dense(initial, "initial states", (tables.order.numel(), values.shape[1], DIM, DIM),
+               torch.float32)
+    return _GatedDeltaRule.apply(queries, keys, values, log_decay, beta, initial, tables, scale,
+                                 normalize)
+
+
 # ------------------------------------------------------------------ the norms
 
 def _rows_of(t: torch.Tensor, name: str, width: int) -> int:

@@ -113,11 +113,23 @@ int32_t statecentric_gdn_state_codec_gated_delta_prefill_launch_v1(
     uint16_t* outputs);
 
 /* Whole packed sequences for training: initial (or NULL: zeros) and final_states
- * fp32 [requests][value_heads][128 value][128 key].  The slots in `chunks` must be
- * 0 or more.  Leaves in the workspace what the backward pass reads. */
+ * fp32 [requests][value_heads][128 value][128 key]; the tables' slots are not
+ * read.  Outputs of tokens of no request are zeros.  Leaves in the workspace what
+ * the backward pass reads. */
 int32_t statecentric_gdn_state_codec_gated_delta_forward_launch_v1(
     void* stream, const gdn_state_codec_rule* rule, const float* initial,
     float* final_states, uint16_t* outputs);
+
+/* Gradients of gated_delta_forward, from d_outputs (bf16, contiguous) and d_final
+ * (or NULL: zeros), with the same `rule` and its workspace as that call left it:
+ * d_queries, d_keys bf16 [tokens][key_heads][128], d_values bf16
+ * [tokens][value_heads][128], d_log_decay fp32 and d_beta bf16
+ * [tokens][value_heads], d_initial (or NULL) like initial.  Gradients of tokens of
+ * no request are zeros.  May be called again. */
+int32_t statecentric_gdn_state_codec_gated_delta_backward_launch_v1(
+    void* stream, const gdn_state_codec_rule* rule, const uint16_t* d_outputs,
+    const float* d_final, uint16_t* d_queries, uint16_t* d_keys, uint16_t* d_values,
+    float* d_log_decay, uint16_t* d_beta, float* d_initial);
 
 /* out = x / sqrt(mean(x^2) + eps) * weight * gate * sigmoid(gate) over rows of
  * 128.  x, gate, out [rows][128] of `dtype`, weight fp32 [128]. */
