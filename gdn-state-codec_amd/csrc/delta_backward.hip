@@ -41,23 +41,22 @@ struct BackArgs {
   bf16_bits* d_beta;
 };
 
-// A chunk's operands in LDS: K (16 tiles), K^T and Q^T (32), the factors (2 tiles,
-// the second's end not used) and N^T (18).  P^T stays in registers: with it, two
-// stages would not fit.
-constexpr int kStageRows = 0;
-constexpr int kStageColumns = kKeyTiles * kTileBytes;
-constexpr int kStageFactors = 3 * kKeyTiles * kTileBytes;
-constexpr int kStageSolve = kStageFactors + 2 * kTileBytes;
-constexpr int kStageTiles = 3 * kKeyTiles + 2 + kSolveParts * kTriangle;
-constexpr int kStage = kStageTiles * kTileBytes;
+// A chunk's operands in LDS, in two halves, each fetched while the other is at work:
+// the factors (2 KiB), N^T and K rows; then K^T, Q^T and the first two parts of the
+// next chunk's P^T.  80 KiB, so that two workgroups share a compute unit; P^T's third
+// part goes to registers instead.
+constexpr int kStageSolve = 2 * kTileBytes;
+constexpr int kStageKeys = kStageSolve + kTriangleBytes;
+constexpr int kStageColumns = kStageKeys + kKeyTiles * kTileBytes;
+constexpr int kStageRead = kStageColumns + 2 * kKeyTiles * kTileBytes;
+constexpr int kStage = kStageRead + 2 * kTriangle * kTileBytes;
 static_assert(kHeadFactors <= 2 * kTileBytes, "the factors' tiles");
-static_assert(2 * kStage <= static_cast<int>(kLdsPerCu), "two stages fit the LDS");
+static_assert(workgroups_by_lds(kStage) == 2, "two workgroups share a compute unit");
 constexpr int kWaves = 4;
-static_assert(kStageTiles % kWaves == 0, "tiles deal out evenly");
+constexpr int kSlices = kDim / (16 * kWaves);
 
-__global__ __launch_bounds__(64 * kWaves, 1) void delta_back_scan_kernel(BackArgs args) {
-  constexpr int kSlices = kDim / (16 * kWaves);
-  __shared__ __align__(16) char stages[2][kStage];
+__global__ __launch_bounds__(64 * kWaves, 2) void delta_back_scan_kernel(BackArgs args) {
+  __shared__ __align__(16) char stage[kStage];
   const RuleArgs& a = args.rule;
   const ChunkSpace& space = a.space;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -66,16 +65,18 @@ __global__ __launch_bounds__(64 * kWaves, 1) void delta_back_scan_kernel(BackArg
   const uint64_t item = static_cast<uint64_t>(turn / kSlices) * 8 + (blockIdx.x & 7);
   if (item >= static_cast<uint64_t>(a.requests) * space.value_heads) return;
   const uint32_t head = static_cast<uint32_t>(item % space.value_heads);
-  const int32_t request = a.order[item / space.value_heads];
-  if (request < 0 || static_cast<uint32_t>(request) >= a.requests) return;
-  const int value = (turn % kSlices) * 16 * kWaves + 16 * wave + r;
+  const uint32_t key_head = head / a.group;
+  const uint32_t request = static_cast<uint32_t>(a.order[item / space.value_heads]);
+  if (request >= a.requests) return;
+  const int first_value = 16 * (kWaves * (turn % kSlices) + wave), value = first_value + r;
   const uint64_t tile = (static_cast<uint64_t>(request) * space.value_heads + head) * kTile +
-                        value * kDim + 4 * g;
+                        value * kDim;
 
-  f32x4 state[8];  // the state's gradient, keys 16 t + 4 g + i
+  f32x4 state[8];  // the state's gradient, rows as in the forward scan
 #pragma unroll
   for (int t = 0; t < 8; ++t) {
-    state[t] = args.d_final ? load4(args.d_final + tile + 16 * t) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    state[t] = args.d_final ? load4(args.d_final + tile + state_key(t, 4 * g))
+                            : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
 
   const uint32_t first_row = min(static_cast<uint32_t>(a.chunk_offsets[request]), space.rows);
@@ -85,111 +86,142 @@ __global__ __launch_bounds__(64 * kWaves, 1) void delta_back_scan_kernel(BackArg
   const uint32_t length = min(static_cast<uint32_t>(a.offsets[request + 1]), a.tokens) - begin;
   const uint32_t chunks = min(rows, (length + kChunk - 1) / kChunk);
   const uint32_t stage_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
-      (__attribute__((address_space(3))) char*)&stages[0][0]));
-  const uint64_t token_step = static_cast<uint64_t>(space.value_heads) * kDim;
+      (__attribute__((address_space(3))) char*)&stage[0]));
+  const uint32_t key_step = static_cast<uint32_t>(a.key_stride) * 2;
+  const uint32_t out_step = space.value_heads * kDim * 2;
+  const uint32_t linear = 16 * lane;
 
-  bf16_bits outs[4][4];            // dO of the tokens 16 t + 4 g + i
-  uint4 back[kSolveParts * kTriangle];  // P^T
-  const auto fetch = [&](uint32_t c) {
-    const char* const keys = space.key_block(first_row + c, head / a.group);
-    const char* const block = space.value_block(first_row + c, head);
+  const auto fetch_first = [&](uint32_t c) {
+    const uint64_t token = begin + c * kChunk;
+    const uint32_t last = min(length - c * kChunk, static_cast<uint32_t>(kChunk)) - 1;
+    const char* k = reinterpret_cast<const char*>(a.keys + token * a.key_stride +
+                                                  key_head * kDim);
+    const char* block = space.value_block(first_row + c, head);
 #pragma unroll
-    for (int i = 0; i < kStageTiles / kWaves; ++i) {
-      const int t = i * kWaves + wave;
-      const char* from = t < 16   ? keys + kKeyRows + t * kTileBytes
-                         : t < 48 ? keys + kKeyColumns + (t - 16) * kTileBytes
-                         : t < 50 ? block + (t - 48) * kTileBytes
-                                  : block + kSolveBack + (t - 50) * kTileBytes;
-      stage_tile(from, lane, stage_at + (c & 1) * kStage + t * kTileBytes);
+    for (int t = 0; t < 4; ++t) {  // rows 16 t.., keys 32 wave..
+      const uint32_t row = min(static_cast<uint32_t>(16 * t + r), last);
+      stage_tile(k + 64 * wave, row * key_step + 16 * g,
+                 stage_at + kStageKeys + (4 * t + wave) * kTileBytes);
     }
-    const uint4* const p = reinterpret_cast<const uint4*>(block + kReadBack) + lane;
 #pragma unroll
-    for (int i = 0; i < kSolveParts * kTriangle; ++i) back[i] = p[i * 64];
-    const int last = min(static_cast<int>(length - c * kChunk), kChunk) - 1;
-    const bf16_bits* d = args.d_outputs + (begin + c * kChunk) * token_step + head * kDim + value;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) outs[t][i] = d[min(16 * t + 4 * g + i, last) * token_step];
+    for (int i = 0; i < 5; ++i) {
+      const int at = kWaves * i + wave;
+      const char* from = at < 2 ? block + at * kTileBytes
+                                : block + kSolveBack + (at - 2) * kTileBytes;
+      stage_tile(from, linear, stage_at + at * kTileBytes);
     }
   };
-  if (chunks != 0) fetch(chunks - 1);
-
-  f32x4 x[4], y[4];
-  const auto store_rows = [&](uint32_t c, int tokens) {
-    float* e = space.error_gradient(first_row + c, head) + value;
-    bf16_bits* d = args.d_values + (begin + c * kChunk) * token_step + head * kDim + value;
+  // The gradient of the outputs: columns 4 (r / 4).. of tokens 16 t + 4 g + (r & 3).
+  uint2 next_out[4];
+  uint4 read_low[kTriangle];  // P^T's third part
+  const auto fetch_read = [&](uint32_t c) {
+    const char* block = space.value_block(first_row + c, head) + kReadBack;
+#pragma unroll
+    for (int i = 0; i < 2 * kTriangle / kWaves; ++i) {
+      const int at = kWaves * i + wave;
+      stage_tile(block + at * kTileBytes, linear, stage_at + kStageRead + at * kTileBytes);
+    }
+#pragma unroll
+    for (int i = 0; i < kTriangle; ++i) {
+      read_low[i] = reinterpret_cast<const uint4*>(block + (2 * kTriangle + i) * kTileBytes)[lane];
+    }
+    const uint32_t last = min(length - c * kChunk, static_cast<uint32_t>(kChunk)) - 1;
+    const char* d = reinterpret_cast<const char*>(args.d_outputs) +
+                    (begin + static_cast<uint64_t>(c) * kChunk) * out_step +
+                    2 * (head * kDim + first_value);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int token = 16 * t + 4 * g + i;
-        e[token * kDim] = x[t][i];
-        if (token < tokens) {
-          d[token * token_step] = static_cast<bf16_bits>(bf16_pair(y[t][i], 0.0f));
-        }
-      }
+      const uint32_t row = min(static_cast<uint32_t>(16 * t + 4 * g + (r & 3)), last);
+      next_out[t] = *reinterpret_cast<const uint2*>(d + (row * out_step + 2 * (r & 12)));
     }
   };
+  const auto fetch_columns = [&](uint32_t c) {
+    const char* columns = space.key_block(first_row + c, key_head);
+#pragma unroll
+    for (int i = 0; i < 2 * kKeyTiles / kWaves; ++i) {
+      const int at = kWaves * i + wave;
+      stage_tile(columns + at * kTileBytes, linear, stage_at + kStageColumns + at * kTileBytes);
+    }
+  };
+  const uint4* const k_rows = reinterpret_cast<const uint4*>(stage + kStageKeys) + lane;
+  const uint4* const k_columns = reinterpret_cast<const uint4*>(stage + kStageColumns) + lane;
+  const uint4* const q_columns = k_columns + kKeyTiles * 64;
+  const uint4* const solve = reinterpret_cast<const uint4*>(stage + kStageSolve) + lane;
+  const uint4* const read_back = reinterpret_cast<const uint4*>(stage + kStageRead) + lane;
 
-  for (uint32_t c = chunks; c-- > 0;) {
-    stage_ready();
-    const uint32_t row = first_row + c;
-    const char* const stage = stages[c & 1];
-    const uint4* const k_rows = reinterpret_cast<const uint4*>(stage + kStageRows) + lane;
-    const uint4* const k_columns = reinterpret_cast<const uint4*>(stage + kStageColumns) + lane;
-    const uint4* const q_columns = k_columns + kKeyTiles * 64;
-    const uint4* const solve = reinterpret_cast<const uint4*>(stage + kStageSolve) + lane;
-    const float* const factors = reinterpret_cast<const float*>(stage + kStageFactors) + 4 * g;
+  // dO of a chunk as an operand over its tokens (rows past its end are zeros), and
+  // P^T dO, which needs no state: both a chunk ahead of the state.
+  uint4 d_part[2];
+  f32x4 v[4];
+  const auto take_outputs = [&](uint32_t c) {
     const int tokens = min(static_cast<int>(length - c * kChunk), kChunk);
-    // Used before the next loads are issued, so that no wait for these covers them.
-    uint32_t d_out[4][4];
-    uint4 read_back[kSolveParts * kTriangle];
+    uint2 x[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        d_out[t][i] = 16 * t + 4 * g + i < tokens ? outs[t][i] : 0;
-        asm volatile("" : "+v"(d_out[t][i]));
-      }
+      const bool live = 16 * t + 4 * g + (r & 3) < tokens;
+      x[t] = transpose_quad(make_uint2(live ? next_out[t].x : 0, live ? next_out[t].y : 0), lane);
     }
-#pragma unroll
-    for (int i = 0; i < kSolveParts * kTriangle; ++i) {
-      read_back[i] = back[i];
-      asm volatile("" : "+v"(read_back[i].x), "+v"(read_back[i].y), "+v"(read_back[i].z),
-                   "+v"(read_back[i].w));
-    }
-    // V' of P^T dO, which needs no state; then P^T's registers take the next chunk's.
-    f32x4 v[4];
-    uint4 d_part[2];
-#pragma unroll
-    for (int step = 0; step < 2; ++step) {
-      d_part[step] = make_uint4(d_out[2 * step][0] | d_out[2 * step][1] << 16,
-                                d_out[2 * step][2] | d_out[2 * step][3] << 16,
-                                d_out[2 * step + 1][0] | d_out[2 * step + 1][1] << 16,
-                                d_out[2 * step + 1][2] | d_out[2 * step + 1][3] << 16);
-    }
+    d_part[0] = make_uint4(x[0].x, x[0].y, x[1].x, x[1].y);
+    d_part[1] = make_uint4(x[2].x, x[2].y, x[3].x, x[3].y);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       v[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int step = upper_first(t); step < 2; ++step) {
-        uint4 p[3];
-#pragma unroll
-        for (int i = 0; i < 3; ++i) p[i] = read_back[i * kTriangle + upper_tile(t, step)];
-        v[t] = mfma3(p, d_part[step], v[t]);
+        const int at = upper_tile(t, step);
+        v[t] = mfma(read_low[at], d_part[step], v[t]);
+        v[t] = mfma(read_back[(kTriangle + at) * 64], d_part[step], v[t]);
+        v[t] = mfma(read_back[at * 64], d_part[step], v[t]);
       }
     }
-    if (c != 0) fetch(c - 1);
+  };
+
+  if (chunks != 0) {
+    fetch_read(chunks - 1);
+    fetch_first(chunks - 1);
+    stage_ready();
+    take_outputs(chunks - 1);
+  }
+
+  f32x4 x[4];
+  uint2 y[4];
+  const auto store_rows = [&](uint32_t c, int tokens) {
+    float* e = space.error_gradient(first_row + c, head) + value;
+    char* d = reinterpret_cast<char*>(args.d_values) +
+              (begin + static_cast<uint64_t>(c) * kChunk) * out_step +
+              2 * (head * kDim + first_value);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[(16 * t + 4 * g + i) * kDim] = x[t][i];
+      const int token = 16 * t + 4 * g + (r & 3);
+      const uint2 run = transpose_quad(y[t], lane);
+      if (token < tokens) *reinterpret_cast<uint2*>(d + (token * out_step + 2 * (r & 12))) = run;
+    }
+  };
+
+  for (uint32_t c = chunks; c-- > 0;) {
+    stage_ready();  // the first half is there, the second has been read
+    f32x4 factors[4];  // of tokens 16 t + 4 g + (r & 3)
+    float queries[4], carries[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int token = 16 * t + 4 * g + (r & 3);
+      factors[t] = reinterpret_cast<const f32x4*>(stage)[token];
+      queries[t] = reinterpret_cast<const float*>(stage)[kReadQuery + token];
+      carries[t] = reinterpret_cast<const float*>(stage)[kCarry + token];
+    }
+    fetch_columns(c);
+    if (c != 0) fetch_read(c - 1);
     if (c + 1 != chunks) {
       store_rows(c + 1, min(static_cast<int>(length - (c + 1) * kChunk), kChunk));
     }
     {
-      float* p = space.state_gradient(row, head) + value;
+      float* p = space.state_gradient(first_row + c, head) + value;
 #pragma unroll
       for (int t = 0; t < 8; ++t) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[(16 * t + 4 * g + i) * kDim] = state[t][i];
+        for (int i = 0; i < 4; ++i) p[state_key(t, 4 * g + i) * kDim] = state[t][i];
       }
     }
     {
@@ -200,17 +232,19 @@ __global__ __launch_bounds__(64 * kWaves, 1) void delta_back_scan_kernel(BackArg
       }
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        f32x4 seen = {0.0f, 0.0f, 0.0f, 0.0f};
+        f32x4 seen[2] = {};
 #pragma unroll
         for (int step = 0; step < 4; ++step) {
-          seen = mfma3(k_rows[(4 * t + step) * 64], part[step], seen);
-        }
-        const f32x4 factor = load4(factors + kWrite * kChunk + 16 * t);
+          const uint4 k = k_rows[(4 * t + step) * 64];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[t][i] = fmaf(factor[i], seen[i], v[t][i]);
+          for (int p = 2; p >= 0; --p) seen[p & 1] = mfma(k, part[step][p], seen[p & 1]);
+        }
+        const f32x4 carry = of_rows(carries[t]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[t][i] = fmaf(carry[i], seen[0][i] + seen[1][i], v[t][i]);
       }
     }
-    // X = V' + N^T (b V')
+    // X = V' + N^T (b V'), Y = b X
     {
       uint4 part[2][3];
 #pragma unroll
@@ -218,7 +252,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void delta_back_scan_kernel(BackArg
         f32x4 w[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const f32x4 b = load4(factors + kStrength * kChunk + 32 * step + 16 * u);
+          const f32x4 b = of_rows(factors[2 * step + u][kStrength]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) w[u][i] = b[i] * v[2 * step + u][i];
         }
@@ -234,31 +268,45 @@ __global__ __launch_bounds__(64 * kWaves, 1) void delta_back_scan_kernel(BackArg
           for (int p = 0; p < 3; ++p) n[p] = solve[(p * kTriangle + upper_tile(t, step)) * 64];
           x[t] = mfma6(n, part[step], x[t]);
         }
-        const f32x4 b = load4(factors + kStrength * kChunk + 16 * t);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) y[t][i] = b[i] * x[t][i];
       }
     }
+    stage_ready();  // the second half is there, the first has been read
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      // Used before the next loads are issued, so that no wait for it covers them.
+      asm volatile("" : "+v"(next_out[t].x), "+v"(next_out[t].y));
+    }
+#pragma unroll
+    for (int i = 0; i < kTriangle; ++i) {
+      asm volatile("" : "+v"(read_low[i].x), "+v"(read_low[i].y), "+v"(read_low[i].z),
+                   "+v"(read_low[i].w));
+    }
+    if (c != 0) fetch_first(c - 1);
     // dS0
-    const float whole = factors[kWhole * kChunk];
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) state[t][i] *= whole;
+      for (int i = 0; i < 4; ++i) state[t][i] *= factors[0][kWhole];
     }
 #pragma unroll
     for (int step = 0; step < 2; ++step) {
       uint4 by_query[3], by_key[3];
       f32x4 p[2], m[2];
+      float d[8];
+      widen8(d_part[step], d);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const f32x4 q = load4(factors + kReadQuery * kChunk + 32 * step + 16 * u);
-        const f32x4 k = load4(factors + kReadKey * kChunk + 32 * step + 16 * u);
+        const int t = 2 * step + u;
+        const f32x4 b = of_rows(factors[t][kStrength]);
+        const f32x4 k = of_rows(factors[t][kReadKey]), q = of_rows(queries[t]);
+        f32x4 row;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          p[u][i] = q[i] * widen_low(d_out[2 * step + u][i]);
-          m[u][i] = -k[i] * y[2 * step + u][i];
+          row[i] = b[i] * x[t][i];
+          p[u][i] = q[i] * d[4 * u + i];
+          m[u][i] = -k[i] * row[i];
         }
+        y[t] = make_uint2(bf16_pair(row[0], row[1]), bf16_pair(row[2], row[3]));
       }
       split3(p[0], p[1], by_query);
       split3(m[0], m[1], by_key);
@@ -268,23 +316,27 @@ __global__ __launch_bounds__(64 * kWaves, 1) void delta_back_scan_kernel(BackArg
         state[t] = mfma3(k_columns[(2 * t + step) * 64], by_key, state[t]);
       }
     }
+    if (c != 0) take_outputs(c - 1);
   }
   if (chunks != 0) store_rows(0, min(static_cast<int>(length), kChunk));
 
   if (args.d_initial) {
 #pragma unroll
-    for (int t = 0; t < 8; ++t) store_cells(args.d_initial + tile + 16 * t, state[t]);
+    for (int t = 0; t < 8; ++t) {
+      store_cells(args.d_initial + tile + state_key(t, 4 * g), state[t]);
+    }
   }
 }
 
 // ------------------------------------------------------- q, k, g and b
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 512;
 constexpr int kWide = 68;  // fp32 a row of a 64 x 64 matrix
+constexpr int kRowTiles = 16;  // operand tiles of 64 rows over the 128 values
 
 // Eight neighbouring values of a row, as an operand's places of natural order.
-__device__ __forceinline__ void split_row(const float* p, uint4 (&part)[3]) {
-  split3(load4(p), load4(p + 4), part);
+__device__ __forceinline__ void split_row(const f32x4 (&x)[2], uint4 (&part)[3]) {
+  split3(x[0], x[1], part);
 }
 
 __device__ __forceinline__ float sum16(float x) {  // over the 16 lanes of a DPP row
@@ -294,18 +346,34 @@ __device__ __forceinline__ float sum16(float x) {  // over the 16 lanes of a DPP
   return add_partner<8>(x);
 }
 
-// One workgroup per chunk row and key head; wavefront w takes keys 32 w..32 w + 31
-// of all 64 tokens, and token rows 16 w.. of F and H.
-__global__ __launch_bounds__(kThreads, 1) void delta_gradient_kernel(BackArgs args) {
-  __shared__ __align__(16) float f[kChunk][kWide];
-  __shared__ __align__(16) float h[kChunk][kWide];
-  __shared__ __align__(16) float factors[kFactors][kChunk];
-  __shared__ __align__(16) float norms[3][kChunk];  // 1/|k|, scale/|q|, 1/|q|
-  __shared__ float sums[3][4][kChunk];
-  __shared__ float ends[4];
+struct Gradient {
+  // X and E cut into parts, 16 tiles a part; then the four kinds of F and H, 6 tiles
+  // a part.
+  union {
+    uint4 rows[2][3][kRowTiles][64];
+    uint4 kinds[4][3][kTriangle][64];
+  };
+  uint4 outs[kRowTiles][64];  // dO
+  float f[kChunk][kWide];
+  float h[kChunk][kWide];
+  float factors[kFactors];
+  float norms[3][kChunk];  // 1/|k|, scale/|q|, 1/|q|
+  float along[4][kChunk];  // X.E by step
+  float sums[2][4][kChunk];
+  float ends[8];
+};
+static_assert(sizeof(Gradient) <= kLdsPerCu, "one workgroup a compute unit");
+
+// One workgroup per chunk row and key head.  Wavefront w takes keys of state tiles
+// 2 (w / 2) and the next and token tiles 2 (w & 1) and the next, so that an operand
+// read from LDS meets two others.  X and E are cut into parts once, by the wavefront
+// that loads them, and so are F and H.
+__global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args) {
+  __shared__ __align__(16) Gradient s;
   const RuleArgs& a = args.rule;
   const ChunkSpace& space = a.space;
-  const int t = threadIdx.x, wave = t >> 6, lane = t & 63, r = lane & 15, g = lane >> 4;
+  const int t = threadIdx.x, lane = t & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const uint32_t row = blockIdx.x / space.key_heads;
   const uint32_t head = blockIdx.x % space.key_heads;
   const uint64_t token_step = static_cast<uint64_t>(space.value_heads) * kDim;
@@ -330,162 +398,211 @@ __global__ __launch_bounds__(kThreads, 1) void delta_gradient_kernel(BackArgs ar
   if (count == 0) return;
   const uint64_t first = chunk.y;
   const char* const keys = space.key_block(row, head);
-  const int key = 32 * wave + r;  // and 16 more
-
-  // This wavefront's columns of q and k, as operands over tokens and as they meet
-  // an accumulator (token 16 i + 4 g + j).
-  uint4 k_columns[2][2], q_columns[2][2];
-  float k_cells[2][4][4], q_cells[2][4][4];
-#pragma unroll
-  for (int c = 0; c < 2; ++c) {
-#pragma unroll
-    for (int step = 0; step < 2; ++step) {
-      const int at = (2 * (2 * wave + c) + step) * kTileBytes + 16 * lane;
-      const uint4 k = *reinterpret_cast<const uint4*>(keys + kKeyColumns + at);
-      const uint4 q = *reinterpret_cast<const uint4*>(keys + kQueryColumns + at);
-      k_columns[c][step] = k, q_columns[c][step] = q;
-      float kx[8], qx[8];
-      widen8(k, kx);
-      widen8(q, qx);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        k_cells[c][2 * step + j / 4][j % 4] = kx[j];
-        q_cells[c][2 * step + j / 4][j % 4] = qx[j];
-      }
-    }
-  }
+  const int pair = wave >> 1, half = wave & 1;
+  const uint32_t outs_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+      (__attribute__((address_space(3))) char*)&s.outs[0][0]));
   if (t < 3 * kChunk) {
-    norms[t / kChunk][t % kChunk] = reinterpret_cast<const float*>(keys + kNorms)[t];
+    s.norms[t / kChunk][t % kChunk] = reinterpret_cast<const float*>(keys + kNorms)[t];
   }
 
-  f32x4 d_q[2][4] = {}, d_k[2][4] = {};
+  f32x4 d_q[2][2] = {}, d_k[2][2] = {};  // [state tile 2 pair + c][token tile 2 half + i]
   for (uint32_t member = 0; member < a.group; ++member) {
     const uint32_t value_head = head * a.group + member;
     const float* const s0 = space.state(row, value_head);
     const float* const s1 = space.state_gradient(row, value_head);
     const float* const errors = space.errors(row, value_head);
     const float* const xs = space.error_gradient(row, value_head);
-    const bf16_bits* const d_out = args.d_outputs + first * token_step + value_head * kDim;
-    const auto d_row = [&](int token, int step) {  // dO as an operand over values
-      return token < count ? *reinterpret_cast<const uint4*>(d_out + token * token_step +
-                                                             32 * step + 8 * g)
-                           : make_uint4(0, 0, 0, 0);
+    // X and E of units (token tile, step) `wave` and `wave` + 8.
+    f32x4 x[2][2], e[2][2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int unit = wave + 8 * u;
+      const int at = (16 * (unit >> 2) + r) * kDim + 32 * (unit & 3) + 8 * g;
+      x[u][0] = load4(xs + at), x[u][1] = load4(xs + at + 4);
+      e[u][0] = load4(errors + at), e[u][1] = load4(errors + at + 4);
+    }
+    f32x4 start[4][2], grad[4][2];  // S0's and dS1's rows of a tile of keys
+    const auto load_rows = [&](const float* state, int c, f32x4 (&rows)[4][2]) {
+      const float* p = state + state_key(2 * pair + c, r) * kDim + 8 * g;
+#pragma unroll
+      for (int step = 0; step < 4; ++step) {
+        rows[step][0] = load4(p + 32 * step);
+        rows[step][1] = load4(p + 32 * step + 4);
+      }
     };
-    __syncthreads();  // the last head's f, h, factors and sums have been read
-    for (int i = t; i < kFactors * kChunk; i += kThreads) {
-      factors[i / kChunk][i % kChunk] =
-          reinterpret_cast<const float*>(space.value_block(row, value_head))[i];
+    load_rows(s0, 0, start);
+    load_rows(s1, 0, grad);
+    if (member != 0) __syncthreads();  // the last head's values have been read
+    {  // dO as an operand over the values: rows past the end repeat the last, and
+       // meet rows of K and Q that are zeros
+      const char* d = reinterpret_cast<const char*>(args.d_outputs + first * token_step +
+                                                    value_head * kDim);
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int unit = wave + 8 * u;
+        const uint32_t token = min(16 * (unit >> 2) + r, count - 1);
+        stage_tile(d + 64 * (unit & 3), token * static_cast<uint32_t>(token_step) * 2 + 16 * g,
+                   outs_at + unit * kTileBytes);
+      }
+    }
+    for (int i = t; i < kFactors; i += kThreads) {
+      s.factors[i] = reinterpret_cast<const float*>(space.value_block(row, value_head))[i];
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int unit = wave + 8 * u;
+      uint4 part[3];
+      float along = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        along = fmaf(x[u][0][i], e[u][0][i], fmaf(x[u][1][i], e[u][1][i], along));
+      }
+      along = add_partner<32>(add_partner<16>(along));
+      if (g == 0) s.along[unit & 3][16 * (unit >> 2) + r] = along;
+      split_row(x[u], part);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) s.rows[0][p][unit][lane] = part[p];
+      split_row(e[u], part);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) s.rows[1][p][unit][lane] = part[p];
+    }
+    stage_ready();
+
+    // F and H, ten blocks (i, j), j <= i, of 16 x 16; the two beside them that an
+    // operand tile holds are zeros.
+    for (int block = wave; block < 12; block += 8) {
+      const int i = block < 1 ? 0 : block < 3 ? 1 : block < 6 ? 2 : block < 10 ? 3
+                    : block == 10 ? 0 : 2;
+      const int j = block < 10 ? block - i * (i + 1) / 2 : i + 1;
+      f32x4 fx = {0.0f, 0.0f, 0.0f, 0.0f}, hx = fx;
+      if (block < 10) {
+#pragma unroll
+        for (int step = 0; step < 4; ++step) {
+          const int at = 4 * i + step, to = 4 * j + step;
+          uint4 x_part[3], e_part[3];
+#pragma unroll
+          for (int p = 0; p < 3; ++p) {
+            x_part[p] = s.rows[0][p][at][lane];
+            e_part[p] = s.rows[1][p][to][lane];
+          }
+          fx = mfma3(s.outs[at][lane], e_part, fx);
+          hx = mfma6(x_part, e_part, hx);
+        }
+      }
+      const int column = 16 * j + r;
+      const float b_column = s.factors[4 * column + kStrength];
+      const float sum = s.factors[kSum + column], rest = s.factors[kSumRest + column];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int line = 16 * i + 4 * g + c;
+        const float decay =
+            decay_between(s.factors[kSum + line], s.factors[kSumRest + line], sum, rest);
+        s.f[line][column] = column <= line ? decay * (fx[c] * b_column) : 0.0f;
+        s.h[line][column] =
+            column < line ? decay * (s.factors[4 * line + kStrength] * hx[c] * b_column) : 0.0f;
+      }
+    }
+
+    // S0 dO, S0 X and dS1 E of this wavefront's keys and tokens.
+    f32x4 read_q[2][2] = {}, read_k[2][2] = {}, written[2][2] = {};
+    float end = 0.0f;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      uint4 part[4][3];
+#pragma unroll
+      for (int step = 0; step < 4; ++step) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          end = fmaf(start[step][0][j], grad[step][0][j],
+                     fmaf(start[step][1][j], grad[step][1][j], end));
+        }
+        split_row(start[step], part[step]);
+      }
+      if (c == 0) load_rows(s0, 1, start);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int step = 0; step < 4; ++step) {
+          const int at = 4 * (2 * half + i) + step;
+          uint4 x_part[3];
+#pragma unroll
+          for (int p = 0; p < 3; ++p) x_part[p] = s.rows[0][p][at][lane];
+          read_q[c][i] = mfma3(s.outs[at][lane], part[step], read_q[c][i]);
+          read_k[c][i] = mfma6(x_part, part[step], read_k[c][i]);
+        }
+      }
+#pragma unroll
+      for (int step = 0; step < 4; ++step) split_row(grad[step], part[step]);
+      if (c == 0) load_rows(s1, 1, grad);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int step = 0; step < 4; ++step) {
+          const int at = 4 * (2 * half + i) + step;
+          uint4 e_part[3];
+#pragma unroll
+          for (int p = 0; p < 3; ++p) e_part[p] = s.rows[1][p][at][lane];
+          written[c][i] = mfma6(e_part, part[step], written[c][i]);
+        }
+      }
+    }
+    // Both halves of the tokens hold these keys; one of them counts.
+    end = half == 0 ? end * s.factors[kWhole] : 0.0f;
+    __syncthreads();  // f and h are whole, X's and E's parts have been read
+
+    // The four kinds, six units each: F and H by rows (over the tokens before), their
+    // transposes (over the tokens after), with the norms of what they meet.
+#pragma unroll
+    for (int u = 0; u < 3; ++u) {
+      const int unit = wave + 8 * u, kind = unit / 6, at = unit % 6;
+      const float(&m)[kChunk][kWide] = (kind & 1) ? s.h : s.f;
+      f32x4 y[2];
+      if (kind < 2) {
+        const int tile = at < 2 ? at : 2 + ((at - 2) >> 1), step = at < 2 ? 0 : (at & 1);
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          const int from = 32 * step + 16 * v + 4 * g;
+          const f32x4 cells = load4(&m[16 * tile + r][from]), unit_k = load4(&s.norms[0][from]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[v][i] = cells[i] * unit_k[i];
+        }
+      } else {
+        const int tile = at < 4 ? at >> 1 : at - 2, step = at < 4 ? (at & 1) : 1;
+        const float sign = kind == 3 ? -1.0f : 1.0f;
+#pragma unroll
+        for (int v = 0; v < 2; ++v) {
+          const int from = 32 * step + 16 * v + 4 * g;
+          const f32x4 unit_q = load4(&s.norms[kind == 3 ? 0 : 1][from]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) y[v][i] = m[from + i][16 * tile + r] * (sign * unit_q[i]);
+        }
+      }
+      uint4 part[3];
+      split_row(y, part);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) s.kinds[kind][p][at][lane] = part[p];
+    }
+    uint4 k_columns[2][2], q_columns[2][2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int step = 0; step < 2; ++step) {
+        const int at = (2 * (2 * pair + c) + step) * kTileBytes + 16 * lane;
+        k_columns[c][step] = *reinterpret_cast<const uint4*>(keys + kKeyColumns + at);
+        q_columns[c][step] = *reinterpret_cast<const uint4*>(keys + kQueryColumns + at);
+      }
     }
     __syncthreads();
 
-    {  // F and H, rows 16 wave + 4 g + j
-      uint4 x_part[4][3], o_part[4];
-      const int token = 16 * wave + r;
+    float cells_k[2][8], cells_q[2][8];  // of the token tiles: 4 i + j
 #pragma unroll
-      for (int step = 0; step < 4; ++step) {
-        split_row(xs + token * kDim + 32 * step + 8 * g, x_part[step]);
-        o_part[step] = d_row(token, step);
-      }
-      for (int c = 0; c < 4; ++c) {
-        f32x4 fx = {0.0f, 0.0f, 0.0f, 0.0f}, hx = fx;
-        if (c <= wave) {
-          float along = 0.0f;
-#pragma unroll
-          for (int step = 0; step < 4; ++step) {
-            const float* e = errors + (16 * c + r) * kDim + 32 * step + 8 * g;
-            uint4 e_part[3];
-            split_row(e, e_part);
-            fx = mfma3(o_part[step], e_part, fx);
-            hx = mfma6(x_part[step], e_part, hx);
-            if (c == wave) {
-              const float* x = xs + token * kDim + 32 * step + 8 * g;
-#pragma unroll
-              for (int j = 0; j < 8; ++j) along = fmaf(x[j], e[j], along);
-            }
-          }
-          if (c == wave) {  // X.E of the token, over the four lane groups
-            along = add_partner<32>(add_partner<16>(along));
-            if (g == 0 && token < count) {
-              args.d_beta[(first + token) * space.value_heads + value_head] =
-                  static_cast<bf16_bits>(bf16_pair(along, 0.0f));
-            }
-          }
-        }
-        const int column = 16 * c + r;
-        const float b_column = factors[kStrength][column];
-        const float sum = factors[kSum][column], rest = factors[kSumRest][column];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = 16 * wave + 4 * g + j;
-          const float decay = expf((factors[kSum][i] - sum) + (factors[kSumRest][i] - rest));
-          f[i][column] = column <= i ? decay * (fx[j] * b_column) : 0.0f;
-          h[i][column] = column < i ? decay * (factors[kStrength][i] * hx[j] * b_column) : 0.0f;
-        }
-      }
+    for (int c = 0; c < 2; ++c) {
+      widen8(half == 0 ? k_columns[c][0] : k_columns[c][1], cells_k[c]);
+      widen8(half == 0 ? q_columns[c][0] : q_columns[c][1], cells_q[c]);
     }
-
-    // S0 dO, S0 X and dS1 E of this wavefront's keys.
-    f32x4 read_q[2][4] = {}, read_k[2][4] = {}, written[2][4] = {};
-    float end = 0.0f;
-    {
-      uint4 part[2][4][3];
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-#pragma unroll
-        for (int step = 0; step < 4; ++step) {
-          split_row(s0 + (key + 16 * c) * kDim + 32 * step + 8 * g, part[c][step]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int step = 0; step < 4; ++step) {
-          uint4 x_part[3];
-          split_row(xs + (16 * i + r) * kDim + 32 * step + 8 * g, x_part);
-          const uint4 o = d_row(16 * i + r, step);
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            read_q[c][i] = mfma3(o, part[c][step], read_q[c][i]);
-            read_k[c][i] = mfma6(x_part, part[c][step], read_k[c][i]);
-          }
-        }
-      }
-    }
-    {
-      uint4 part[2][4][3];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-#pragma unroll
-        for (int step = 0; step < 4; ++step) {
-          const uint64_t at = (key + 16 * c) * kDim + 32 * step + 8 * g;
-          const f32x4 x = load4(s1 + at), y = load4(s1 + at + 4);
-          const f32x4 u = load4(s0 + at), v = load4(s0 + at + 4);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) end = fmaf(x[j], u[j], fmaf(y[j], v[j], end));
-          split3(x, y, part[c][step]);
-        }
-      }
-      end *= factors[kWhole][0];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int step = 0; step < 4; ++step) {
-          uint4 e_part[3];
-          split_row(errors + (16 * i + r) * kDim + 32 * step + 8 * g, e_part);
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            written[c][i] = mfma6(e_part, part[c][step], written[c][i]);
-          }
-        }
-      }
-    }
-    __syncthreads();  // f and h are whole
-
-    // The products with F and H and their transposes, row tile by row tile.
-    float flux[4][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const f32x4 b = load4(&factors[kStrength][16 * i + 4 * g]);
+    for (int i = 0; i < 2; ++i) {
+      const int tile = 2 * half + i;
       f32x4 by_query[2], by_read[2], by_write[2];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -493,138 +610,149 @@ __global__ __launch_bounds__(kThreads, 1) void delta_gradient_kernel(BackArgs ar
       }
 #pragma unroll
       for (int step = 0; step < 2; ++step) {
-        const int at = 32 * step + 4 * g;  // places at.. and at + 16..
-        if (step < lower_steps(i)) {  // row token 16 i + r, over the tokens before it
-          const f32x4 u = load4(&norms[0][at]), v = load4(&norms[0][at + 16]);
-          f32x4 x = load4(&f[16 * i + r][at]), y = load4(&f[16 * i + r][at + 16]);
-          uint4 part[3];
+        uint4 part[3];
+        if (step <= half) {  // the tokens before
+          const int at = half == 0 ? i : 2 * tile - 2 + step;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] *= u[j], y[j] *= v[j];
-          split3(x, y, part);
+          for (int p = 0; p < 3; ++p) part[p] = s.kinds[0][p][at][lane];
 #pragma unroll
           for (int c = 0; c < 2; ++c) by_query[c] = mfma3(part, k_columns[c][step], by_query[c]);
-          x = load4(&h[16 * i + r][at]), y = load4(&h[16 * i + r][at + 16]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) x[j] *= u[j], y[j] *= v[j];
-          split3(x, y, part);
+          for (int p = 0; p < 3; ++p) part[p] = s.kinds[1][p][at][lane];
 #pragma unroll
           for (int c = 0; c < 2; ++c) by_read[c] = mfma3(part, k_columns[c][step], by_read[c]);
         }
-        if (step >= upper_first(i)) {  // row token 16 i + r, over the tokens after it
-          f32x4 x, y;
-          uint4 part[3];
+        if (step >= half) {  // the tokens after
+          const int at = half == 0 ? 2 * i + step : tile + 2;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            x[j] = f[at + j][16 * i + r] * norms[1][at + j];
-            y[j] = f[at + 16 + j][16 * i + r] * norms[1][at + 16 + j];
-          }
-          split3(x, y, part);
+          for (int p = 0; p < 3; ++p) part[p] = s.kinds[2][p][at][lane];
 #pragma unroll
           for (int c = 0; c < 2; ++c) by_write[c] = mfma3(part, q_columns[c][step], by_write[c]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            x[j] = -h[at + j][16 * i + r] * norms[0][at + j];
-            y[j] = -h[at + 16 + j][16 * i + r] * norms[0][at + 16 + j];
-          }
-          split3(x, y, part);
+          for (int p = 0; p < 3; ++p) part[p] = s.kinds[3][p][at][lane];
 #pragma unroll
           for (int c = 0; c < 2; ++c) by_write[c] = mfma3(part, k_columns[c][step], by_write[c]);
         }
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int token = 16 * i + 4 * g + j;
-        const float k_unit = norms[0][token], q_unit = norms[1][token];
-        const float decay = expf(factors[kSum][token]);
-        const float kept = expf((factors[kSum][kChunk - 1] - factors[kSum][token]) +
-                                (factors[kSumRest][kChunk - 1] - factors[kSumRest][token]));
+        const int token = 16 * tile + 4 * g + j;
+        const float k_unit = s.norms[0][token], q_unit = s.norms[1][token];
+        const float b = s.factors[4 * token + kStrength];
+        const float decay = __builtin_amdgcn_exp2f(s.factors[kSum + token]);
+        const float kept = decay_between(s.factors[kSum + kChunk - 1],
+                                         s.factors[kSumRest + kChunk - 1],
+                                         s.factors[kSum + token], s.factors[kSumRest + token]);
         float total = 0.0f;
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           const float dq = fmaf(decay, read_q[c][i][j], by_query[c][j]);
-          const float read = -fmaf(decay * b[j], read_k[c][i][j], by_read[c][j]);
-          const float carried = kept * b[j] * written[c][i][j];
+          const float read = -fmaf(decay * b, read_k[c][i][j], by_read[c][j]);
+          const float carried = kept * b * written[c][i][j];
           const float write = carried + by_write[c][j];
-          const float k = k_unit * k_cells[c][i][j], q = q_unit * q_cells[c][i][j];
+          const float k = k_unit * cells_k[c][4 * i + j], q = q_unit * cells_q[c][4 * i + j];
           total = fmaf(q, dq, fmaf(k, read - write, total));
           end = fmaf(k, carried, end);
           d_q[c][i][j] += dq;
           d_k[c][i][j] += read + write;
         }
-        flux[i][j] = sum16(total);
+        total = sum16(total);
+        if (r == 0) s.sums[0][pair][token] = total;
       }
     }
     end = wave_sum_valu(end);
-    if (lane == 0) ends[wave] = end;
-    if (r == 0) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) sums[0][wave][16 * i + 4 * g + j] = flux[i][j];
-      }
-    }
+    if (lane == 0) s.ends[wave] = end;
     __syncthreads();
     if (wave == 0) {
-      float total = (sums[0][0][lane] + sums[0][1][lane]) + (sums[0][2][lane] + sums[0][3][lane]);
-      if (lane == 63) total += (ends[0] + ends[1]) + (ends[2] + ends[3]);
+      float total = (s.sums[0][0][lane] + s.sums[0][1][lane]) +
+                    (s.sums[0][2][lane] + s.sums[0][3][lane]);
+      if (lane == 63) {
+        total += ((s.ends[0] + s.ends[1]) + (s.ends[2] + s.ends[3])) +
+                 ((s.ends[4] + s.ends[5]) + (s.ends[6] + s.ends[7]));
+      }
 #pragma unroll
       for (int step = 1; step < 64; step <<= 1) {  // from each token to the chunk's end
         const float after = __shfl_down(total, step);
         if (lane + step < 64) total += after;
       }
+      const float b = (s.along[0][lane] + s.along[1][lane]) + (s.along[2][lane] + s.along[3][lane]);
       if (lane < count) {
-        args.d_log_decay[(first + lane) * space.value_heads + value_head] = total;
+        const uint64_t at = (first + lane) * space.value_heads + value_head;
+        args.d_log_decay[at] = total;
+        args.d_beta[at] = static_cast<bf16_bits>(bf16_pair(b, 0.0f));
       }
     }
   }
 
   // Through the norms: with u = scale / |q|, d(raw) = u dq - q (u q.dq) / |q|^2, and
   // for keys the same with scale 1.
-  if (a.normalize) {
+  float cells_k[2][8], cells_q[2][8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+  for (int c = 0; c < 2; ++c) {
+    const int at = (2 * (2 * pair + c) + half) * kTileBytes + 16 * lane;
+    widen8(*reinterpret_cast<const uint4*>(keys + kKeyColumns + at), cells_k[c]);
+    widen8(*reinterpret_cast<const uint4*>(keys + kQueryColumns + at), cells_q[c]);
+  }
+  __syncthreads();  // the last head's sums have been read
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float q = 0.0f, k = 0.0f;
+  for (int i = 0; i < 2; ++i) {
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          q = fmaf(q_cells[c][i][j], d_q[c][i][j], q);
-          k = fmaf(k_cells[c][i][j], d_k[c][i][j], k);
-        }
-        q = sum16(q), k = sum16(k);
-        if (r == 0) {
-          sums[1][wave][16 * i + 4 * g + j] = q;
-          sums[2][wave][16 * i + 4 * g + j] = k;
-        }
+    for (int j = 0; j < 4; ++j) {
+      float q = 0.0f, k = 0.0f;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        q = fmaf(cells_q[c][4 * i + j], d_q[c][i][j], q);
+        k = fmaf(cells_k[c][4 * i + j], d_k[c][i][j], k);
+      }
+      q = sum16(q), k = sum16(k);
+      if (r == 0) {
+        s.sums[0][pair][16 * (2 * half + i) + 4 * g + j] = q;
+        s.sums[1][pair][16 * (2 * half + i) + 4 * g + j] = k;
       }
     }
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 2; ++i) {
+    const int tile = 2 * half + i;
+    f32x4 dq[2], dk[2];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int token = 16 * i + 4 * g + j;
-      const float k_unit = norms[0][token], q_unit = norms[1][token];
+      const int token = 16 * tile + 4 * g + j;
+      const float k_unit = s.norms[0][token], q_unit = s.norms[1][token];
       float q_along = 0.0f, k_along = 0.0f;
       if (a.normalize) {
-        q_along = ((sums[1][0][token] + sums[1][1][token]) +
-                   (sums[1][2][token] + sums[1][3][token])) *
-                  q_unit * norms[2][token] * norms[2][token];
-        k_along = ((sums[2][0][token] + sums[2][1][token]) +
-                   (sums[2][2][token] + sums[2][3][token])) *
+        q_along = ((s.sums[0][0][token] + s.sums[0][1][token]) +
+                   (s.sums[0][2][token] + s.sums[0][3][token])) *
+                  q_unit * s.norms[2][token] * s.norms[2][token];
+        k_along = ((s.sums[1][0][token] + s.sums[1][1][token]) +
+                   (s.sums[1][2][token] + s.sums[1][3][token])) *
                   k_unit * k_unit * k_unit;
       }
-      if (token < count) {
-        const uint64_t at = ((first + token) * space.key_heads + head) * kDim + key;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float dq = fmaf(-q_cells[c][i][j], q_along, q_unit * d_q[c][i][j]);
-          const float dk = fmaf(-k_cells[c][i][j], k_along, k_unit * d_k[c][i][j]);
-          args.d_queries[at + 16 * c] = static_cast<bf16_bits>(bf16_pair(dq, 0.0f));
-          args.d_keys[at + 16 * c] = static_cast<bf16_bits>(bf16_pair(dk, 0.0f));
-        }
+      for (int c = 0; c < 2; ++c) {
+        dq[c][j] = fmaf(-cells_q[c][4 * i + j], q_along, q_unit * d_q[c][i][j]);
+        dk[c][j] = fmaf(-cells_k[c][4 * i + j], k_along, k_unit * d_k[c][i][j]);
       }
+    }
+    // Four tokens by four keys of a quad, transposed: lane 4 m + j gets token j's keys
+    // 8 m.. of the pair's 32, four of each tile.
+    uint2 q_run[2], k_run[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      q_run[c] = transpose_quad(make_uint2(bf16_pair(dq[c][0], dq[c][1]),
+                                           bf16_pair(dq[c][2], dq[c][3])), lane);
+      k_run[c] = transpose_quad(make_uint2(bf16_pair(dk[c][0], dk[c][1]),
+                                           bf16_pair(dk[c][2], dk[c][3])), lane);
+    }
+    const int token = 16 * tile + 4 * g + (r & 3);
+    if (token < count) {
+      const uint64_t at = ((first + token) * space.key_heads + head) * kDim + 32 * pair +
+                          8 * (r >> 2);
+      *reinterpret_cast<uint4*>(args.d_queries + at) =
+          make_uint4(q_run[0].x, q_run[0].y, q_run[1].x, q_run[1].y);
+      *reinterpret_cast<uint4*>(args.d_keys + at) =
+          make_uint4(k_run[0].x, k_run[0].y, k_run[1].x, k_run[1].y);
     }
   }
 }
@@ -648,7 +776,7 @@ extern "C" int32_t statecentric_gdn_state_codec_gated_delta_backward_launch_v1(
   args.d_log_decay = d_log_decay, args.d_beta = d_beta;
   const gdn::ChunkSpace& space = args.rule.space;
   const uint64_t items = static_cast<uint64_t>(rule->requests) * rule->value_heads;
-  const uint64_t scans = (items + 7) / 8 * 8 * (gdn::kDim / (16 * gdn::kWaves));
+  const uint64_t scans = (items + 7) / 8 * 8 * gdn::kSlices;
   if (scans > gdn::kMaxGrid) return gdn::kStatusInvalidArgument;
   const int32_t status = gdn::launch(gdn::delta_back_scan_kernel,
                                      dim3(static_cast<uint32_t>(scans)),

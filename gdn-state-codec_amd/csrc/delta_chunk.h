@@ -21,13 +21,14 @@
 // Accumulators, states, sums and factors are fp32; the decays' running sums are
 // fp64, so that exp(G_i - G_j) of neighbours keeps its accuracy where G is large.
 //
-// Layouts.  An operand tile is 64 lanes x 16 bytes: lane l holds row (or column)
-// l & 15 and 8 places of the contraction.  Contractions over keys or tokens use
-// places of one order: the 8 places of lane group g = l >> 4 of a 32-wide step s
-// are 32 s + 4 g + {0..3} and 32 s + 16 + 4 g + {0..3}.  Those are exactly the
-// rows that group g holds of two accumulator tiles (rows 4 g + r), so a product's
-// accumulators, cut into parts, are the next product's operand with no exchange
-// between lanes.
+// Layouts.  An operand is 16 rows (or columns) by 32 places of a contraction: lane
+// l holds row l & 15 and the 8 places of lane group g = l >> 4.  An accumulator
+// tile gives lane l column l & 15 of rows 4 g .. 4 g + 3.  The places of group g in
+// step s of a contraction are the rows it holds of accumulator tiles 2 s and
+// 2 s + 1, so a product's accumulators, cut into parts, are the next product's
+// operand as they are.  For tokens that makes them 32 s + 4 g + {0..3} and
+// 32 s + 16 + 4 g + {0..3}; the rows of the state's tiles are keys in such an order
+// (state_key) that they are keys 32 s + 8 g + {0..7}, 16 bytes of a row of q or k.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -36,6 +37,7 @@
 #include "activations.h"
 #include "bf16_operands.h"
 #include "gdn_state_codec_layer.h"
+#include "lane_exchange.h"
 #include "launch.h"
 
 namespace gdn {
@@ -43,14 +45,18 @@ namespace gdn {
 constexpr int kChunk = GDN_STATE_CODEC_CHUNK;
 constexpr float kUnitEps = 1e-6f;  // inside the square root of q's and k's norms
 
-// Operand tiles of one chunk and key head: K and Q (rows = tokens, contraction
-// over keys; 4 row tiles x 4 steps), their transposes (rows = keys, contraction
-// over tokens; 8 row tiles x 2 steps; Q's for training only).
+// bf16 operand tiles (64 lanes x 16 bytes) of one chunk and key head: K^T (rows =
+// keys in state order, contraction over tokens; 8 row tiles x 2 steps), and for
+// training Q^T.
 constexpr int kTileBytes = 1024;
-constexpr int kKeyTiles = 16;      // tiles of each of the four
-// Triangular operands (rows = tokens, contraction over tokens): 6 of the 8 tiles
-// hold anything.
+constexpr int kKeyTiles = 16;
+// Triangular operands (rows and contraction = tokens): 6 of the 8 tiles hold
+// anything.  N, P and their transposes are three bf16 parts, 18 KiB (cut once
+// here instead of by every slice that reads them); P b is two, since the outputs it
+// makes are bf16.
 constexpr int kTriangle = 6;
+constexpr int kTriangleBytes = 3 * kTriangle * kTileBytes;
+constexpr int kReadOutBytes = 2 * kTriangle * kTileBytes;
 __device__ __forceinline__ constexpr int lower_tile(int row, int step) {
   return row < 2 ? row : 2 * row - 2 + step;  // (0,0) (1,0) (2,0) (2,1) (3,0) (3,1)
 }
@@ -60,30 +66,47 @@ __device__ __forceinline__ constexpr int upper_tile(int row, int step) {
 __device__ __forceinline__ constexpr int lower_steps(int row) { return row < 2 ? 1 : 2; }
 __device__ __forceinline__ constexpr int upper_first(int row) { return row < 2 ? 0 : 1; }
 
-constexpr int kSolveParts = 3;  // parts of N (an fp32 operand)
-constexpr int kReadParts = 2;   // parts of P b: the outputs it makes are bf16
+// Key of row `row` of the state's tile `tile`.
+__device__ __forceinline__ constexpr int state_key(int tile, int row) {
+  return 32 * (tile >> 1) + 8 * (row >> 2) + 4 * (tile & 1) + (row & 3);
+}
+// Token of place i of lane group g in step `step`.
+__device__ __forceinline__ constexpr int token_place(int step, int g, int i) {
+  return 32 * step + (i < 4 ? 4 * g + i : 12 + 4 * g + i);
+}
 
-// Factors of a chunk's tokens for one value head, fp32 [7][64].
+// Factors of a chunk's tokens for one value head (fp32): four of each token side by
+// side (the forward chain's), then four rows.
 enum : int {
   kReadKey = 0,    // exp(G_i) / |k_i|
-  kReadQuery = 1,  // exp(G_i) scale / |q_i|
-  kStrength = 2,   // b_i, 0 past the request's end
-  kWrite = 3,      // exp(G_63 - G_j) / |k_j|
-  kWhole = 4,      // exp(G_63), in every place
-  kSum = 5,        // G_i, and below it what fp32 left of it
-  kSumRest = 6,
-  kFactors = 7
+  kStrength = 1,   // b_i, 0 past the request's end
+  kWrite = 2,      // exp(G_63 - G_j) b_j / |k_j|
+  kWhole = 3,      // exp(G_63)
+  kReadQuery = 4 * kChunk,           // exp(G_i) scale / |q_i|
+  kSum = kReadQuery + kChunk,        // G_i / ln 2, and below it what fp32 left of it
+  kSumRest = kSum + kChunk,
+  kCarry = kSumRest + kChunk,        // exp(G_63 - G_j) / |k_j|
+  kFactors = kCarry + kChunk
 };
 
 // Bytes of the workspace's parts.
-constexpr uint64_t kHeadFactors = kFactors * kChunk * 4;
+constexpr int kHeadFactors = kFactors * 4;
 __host__ __device__ constexpr uint64_t key_block_bytes(bool train) {
-  return train ? 4 * kKeyTiles * kTileBytes + 3 * kChunk * 4 : 3 * kKeyTiles * kTileBytes;
+  return train ? 2 * kKeyTiles * kTileBytes + 3 * kChunk * 4 : kKeyTiles * kTileBytes;
 }
 __host__ __device__ constexpr uint64_t value_block_bytes(bool train) {
-  const uint64_t serving = (kSolveParts + kReadParts) * kTriangle * kTileBytes + kHeadFactors;
-  return train ? serving + 2 * kSolveParts * kTriangle * kTileBytes : serving;
+  return kHeadFactors + kReadOutBytes + (train ? 3 : 1) * kTriangleBytes;
 }
+// Places inside a key block: K^T, then for training Q^T and the norms (fp32 1/|k|,
+// scale/|q|, 1/|q|).
+constexpr int kKeyColumns = 0;
+constexpr int kQueryColumns = kKeyTiles * kTileBytes;
+constexpr int kNorms = 2 * kKeyTiles * kTileBytes;
+// Places inside a value block: factors, N, P b, then for training N^T and P^T.
+constexpr int kSolve = kHeadFactors;
+constexpr int kReadOut = kSolve + kTriangleBytes;
+constexpr int kSolveBack = kReadOut + kReadOutBytes;
+constexpr int kReadBack = kSolveBack + kTriangleBytes;
 
 // One chunk's key block, value block and, for training, states and rows.
 struct ChunkSpace {
@@ -99,12 +122,11 @@ struct ChunkSpace {
   }
   // Training: the start state and the end state's gradient of each chunk and
   // value head (fp32 [key][value]), then E and X (fp32 [64][128] each).
-  // (1 KiB more: a block is read in whole tiles.)
   __host__ __device__ uint64_t total() const {
     return states_at() + (train ? static_cast<uint64_t>(rows) * value_heads *
                                       (2 * kTile + 2 * kChunk * kDim) * 4
                                 : 0) +
-           kTileBytes;
+           kTileBytes;  // blocks are read in whole tiles
   }
   __device__ char* key_block(uint32_t row, uint32_t head) const {
     return base + (static_cast<uint64_t>(row) * key_heads + head) * key_block_bytes(train);
@@ -127,18 +149,6 @@ struct ChunkSpace {
     return state(row, head) + 2 * kTile + kChunk * kDim;
   }
 };
-// Places inside a key block.
-constexpr int kKeyRows = 0;
-constexpr int kQueryRows = kKeyTiles * kTileBytes;
-constexpr int kKeyColumns = 2 * kKeyTiles * kTileBytes;
-constexpr int kQueryColumns = 3 * kKeyTiles * kTileBytes;  // training
-constexpr int kNorms = 4 * kKeyTiles * kTileBytes;  // training: fp32 1/|k|, scale/|q|, 1/|q|
-// Places inside a value block: factors, N, P b, then N^T and P^T (training).
-constexpr int kSolve = kHeadFactors;
-constexpr int kReadOut = kSolve + kSolveParts * kTriangle * kTileBytes;
-constexpr int kSolveBack = kReadOut + kReadParts * kTriangle * kTileBytes;
-constexpr int kReadBack = kSolveBack + kSolveParts * kTriangle * kTileBytes;
-
 struct RuleArgs {
   const bf16_bits* queries;
   const bf16_bits* keys;
@@ -190,6 +200,12 @@ __device__ __forceinline__ void split3(const f32x4& x, const f32x4& y, uint4 (&p
   split3_pair(y[2], y[3], part[0].w, part[1].w, part[2].w);
 }
 
+// The same of one accumulator tile: half of an operand's places.
+__device__ __forceinline__ void split3_half(const f32x4& x, uint2 (&part)[3]) {
+  split3_pair(x[0], x[1], part[0].x, part[1].x, part[2].x);
+  split3_pair(x[2], x[3], part[0].y, part[1].y, part[2].y);
+}
+
 // c + a b of two fp32 operands in parts.
 __device__ __forceinline__ f32x4 mfma6(const uint4 (&a)[3], const uint4 (&b)[3], f32x4 c) {
   c = mfma(a[0], b[2], c);
@@ -228,13 +244,45 @@ __device__ __forceinline__ void store_cells(bf16_bits* p, const f32x4& x) {
   *reinterpret_cast<uint2*>(p) = make_uint2(bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]));
 }
 
-// One tile, 16 bytes a lane, from global memory into LDS at `to` (bytes, the same
-// for the wavefront) without passing the registers.  The caller waits
-// (stage_ready) before any lane reads it.
-__device__ __forceinline__ void stage_tile(const char* tile, int lane, uint32_t to) {
+// A lane's four rows of an accumulator tile, from the quad of lanes that holds one
+// each: lane 4 m + i has token i's factor.
+template <int kCtrl>
+__device__ __forceinline__ float quad(float x) {
+  return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), kCtrl, 0xF, 0xF, true));
+}
+__device__ __forceinline__ f32x4 of_rows(float x) {
+  return f32x4{quad<0x00>(x), quad<0x55>(x), quad<0xAA>(x), quad<0xFF>(x)};
+}
+
+// A 4 x 4 block of bf16 over a quad of lanes, transposed: from lane j's column j
+// (rows 0, 1 | 2, 3) to its row j (columns 0, 1 | 2, 3), and back.  It makes
+// accumulator columns whole 8-byte runs of a row.
+__device__ __forceinline__ uint2 transpose_quad(const uint2& x, int lane) {
+  const uint32_t near = (lane & 1) ? 0x03020706u : 0x05040100u;
+  const uint32_t px = __builtin_amdgcn_mov_dpp(x.x, kDppQuadSwap1, 0xF, 0xF, true);
+  const uint32_t py = __builtin_amdgcn_mov_dpp(x.y, kDppQuadSwap1, 0xF, 0xF, true);
+  const uint32_t u = __builtin_amdgcn_perm(px, x.x, near);
+  const uint32_t v = __builtin_amdgcn_perm(py, x.y, near);
+  const bool up = (lane & 2) != 0;
+  const uint32_t got = __builtin_amdgcn_mov_dpp(up ? u : v, kDppQuadSwap2, 0xF, 0xF, true);
+  return make_uint2(up ? got : u, up ? v : got);
+}
+
+// exp(G_i - G_j) from the sums in units of ln 2, on the transcendental unit (about
+// an ulp).
+__device__ __forceinline__ float decay_between(float sum_i, float rest_i, float sum_j,
+                                               float rest_j) {
+  return __builtin_amdgcn_exp2f((sum_i - sum_j) + (rest_i - rest_j));
+}
+
+// One tile into LDS at `to` (bytes, the same for the wavefront), 16 bytes a lane at
+// `from` plus its own byte offset, without passing the registers.  The caller waits
+// (stage_ready) before any lane reads it.  M0 holds the LDS address; nothing else in
+// the kernels that call this uses it.
+__device__ __forceinline__ void stage_tile(const char* from, uint32_t offset, uint32_t to) {
   asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                :
-               : "v"(16 * lane), "s"(tile), "s"(to)
+               : "v"(offset), "s"(from), "s"(to)
                : "memory");
 }
 
@@ -242,6 +290,12 @@ __device__ __forceinline__ void stage_tile(const char* tile, int lane, uint32_t 
 // overwritten, after this.
 __device__ __forceinline__ void stage_ready() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// LDS written before it may be read by the workgroup's other wavefronts after it.
+// Loads and stores to global memory stay in flight.
+__device__ __forceinline__ void exchange() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 }  // namespace gdn

@@ -1,14 +1,18 @@
 // The state-independent half of the gated delta rule's chunked form, for every
-// chunk and key head at once: the operands K, Q and their transposes, the norms,
-// and for each value head of the group the factors, N and P b (and for training
-// N^T and P^T); formulas and layouts in delta_chunk.h.
+// chunk and key head at once: the transposed operands, the norms, and for each
+// value head of the group the factors, N and P b (and for training N^T and P^T);
+// formulas and layouts in delta_chunk.h.
 //
 // One workgroup per chunk row and key head.  K K^T and Q K^T are formed once per
-// key head on the matrix cores (exact bf16 products).  N comes from forward
-// substitution, one column a lane: lane j keeps N_1j..N_63j in registers, and the
-// rows of A b come from LDS as broadcasts (every lane reads the same 16 bytes).
-// That is 2016 fp32 fmas a wavefront, the kernel's bound together with their
-// broadcasts; substitution is stable for any keys, which powers of A are not.
+// key head on the matrix cores (exact bf16 products), then each wavefront takes a
+// value head's N or its P b, with no barrier between them.
+//
+// N by blocks of 16 tokens.  The four diagonal blocks are solved at once by forward
+// substitution, one column a lane (120 fmas).  Below them
+//   N_ij = -(I + N_ii b_i) (A_ij + sum_(j<=m<i) A_im b_m N_mj)
+// is 16 products of 16 x 16 on the fp32 matrix cores, each block an accumulator
+// that is the next product's operand as it is.  Substitution and this recursion
+// are stable for any keys, which powers of A are not.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -21,6 +25,12 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kPitch = 136;  // bf16 a staged row: 128 and 16 bytes against bank conflicts
 constexpr int kWide = 68;    // fp32 a row of a 64 x 64 matrix
+constexpr double kInverseLn2 = 1.4426950408889634074;
+
+struct Head {  // one wavefront's value head
+  float sum[kChunk], rest[kChunk];  // G / ln 2
+  float strength[kChunk];
+};
 
 struct Staged {
   union {
@@ -28,15 +38,14 @@ struct Staged {
       uint16_t k[kChunk][kPitch];
       uint16_t q[kChunk][kPitch];
     };
-    float solve[2][kChunk][kWide];  // A b, then N, of two value heads
+    float solve[2][kChunk][kWide];  // A, then N, of two wavefronts
   };
   float kk[kChunk][kWide];
   float qk[kChunk][kWide];
-  double sum[2][kChunk];    // G
-  float strength[2][kChunk];
-  float k_unit[kChunk];     // 1 / |k|
-  float q_unit[kChunk];     // scale / |q|
-  float q_norm[kChunk];     // 1 / |q|
+  Head heads[4];
+  float k_unit[kChunk];  // 1 / |k|
+  float q_unit[kChunk];  // scale / |q|
+  float q_norm[kChunk];  // 1 / |q|
 };
 
 // LDS written by other lanes of the same wavefront is read after this.
@@ -46,72 +55,140 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
 }
 
-__device__ __forceinline__ int place(int step, int g, int i) {  // of a contraction
-  return 32 * step + (i < 4 ? 4 * g + i : 12 + 4 * g + i);
+// c + a b for 16 x 16 fp32 blocks: lane l has row l & 15, columns 4 g.. of a, and
+// rows 4 g.. of b's column l & 15 (an accumulator).
+__device__ __forceinline__ f32x4 block_product(const f32x4& a, const f32x4& b, f32x4 c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+  return c;
 }
 
-__device__ __forceinline__ void store_parts(char* tiles, int tile, int lane,
-                                            const uint4 (&part)[3], int parts) {
+__device__ __forceinline__ f32x4 times(const f32x4& a, const f32x4& b) {
+  return f32x4{a[0] * b[0], a[1] * b[1], a[2] * b[2], a[3] * b[3]};
+}
+
+__device__ __forceinline__ void store_tile(char* operand, int tile, int lane, const f32x4& x,
+                                           const f32x4& y) {
+  uint4 part[3];
+  split3(x, y, part);
 #pragma unroll
   for (int p = 0; p < 3; ++p) {
-    if (p < parts) {
-      reinterpret_cast<uint4*>(tiles + (p * kTriangle + tile) * kTileBytes)[lane] = part[p];
-    }
+    reinterpret_cast<uint4*>(operand + (p * kTriangle + tile) * kTileBytes)[lane] = part[p];
   }
 }
 
-// Forward substitution of one value head by one wavefront, and N's operands.
 template <bool kTrain>
-__device__ __forceinline__ void solve_head(Staged& s, int slot, int lane, char* block) {
-  float (&m)[kChunk][kWide] = s.solve[slot];
-  const double mine = s.sum[slot][lane];
-  const float k_mine = s.k_unit[lane], b_mine = s.strength[slot][lane];
-  float n[kChunk];  // column `lane`
+__device__ __forceinline__ void solve_head(Staged& s, const Head& head, float (&m)[kChunk][kWide],
+                                           int lane, char* block) {
+  const int r = lane & 15, g = lane >> 4;
+  // A, block by block as accumulators (row 4 g + i, column r), and in LDS.
+  f32x4 a[4][4];
 #pragma unroll
-  for (int i = 0; i < kChunk; ++i) {
-    const float decay = expf(static_cast<float>(s.sum[slot][i] - mine));
-    const float a = i > lane ? decay * (s.k_unit[i] * k_mine * s.kk[i][lane]) : 0.0f;
-    n[i] = -a;
-    m[i][lane] = a * b_mine;
-  }
-  wave_sync();
+  for (int i = 0; i < 4; ++i) {
+    const f32x4 sum = load4(&head.sum[16 * i + 4 * g]), rest = load4(&head.rest[16 * i + 4 * g]);
+    const f32x4 unit = load4(&s.k_unit[16 * i + 4 * g]);
 #pragma unroll
-  for (int i = 1; i < kChunk; ++i) {
-    float sum[4] = {n[i], 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int j = 0; j < i; j += 4) {
-      const f32x4 row = load4(&m[i][j]);  // zero from the diagonal on
+    for (int j = 0; j <= i; ++j) {
+      const int column = 16 * j + r;
+      const float sum_c = head.sum[column], rest_c = head.rest[column];
+      const float unit_c = s.k_unit[column];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        if (j + c < i) sum[c] = fmaf(-row[c], n[j + c], sum[c]);
+        const int row = 16 * i + 4 * g + c;
+        const float x = decay_between(sum[c], rest[c], sum_c, rest_c) *
+                        (unit[c] * unit_c * s.kk[row][column]);
+        a[i][j][c] = column < row ? x : 0.0f;
+        m[row][column] = a[i][j][c];
       }
     }
-    n[i] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
   }
-  wave_sync();  // A b has been read
-#pragma unroll
-  for (int i = 0; i < kChunk; ++i) m[i][lane] = n[i];
   wave_sync();
-  const int row = lane & 15, g = lane >> 4;
+  {  // the diagonal blocks: lane group g solves block g, column r
+    float n[16], scaled[16];
+    const float* const strength = &head.strength[16 * g];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const float* const row = &m[16 * g + i][16 * g];
+      float x = -row[r], y = 0.0f;
+#pragma unroll
+      for (int c = 0; c < i; c += 4) {
+        const f32x4 l = load4(row + c);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (c + u < i) {
+            if (u & 1) y = fmaf(-l[u], scaled[c + u], y);
+            else x = fmaf(-l[u], scaled[c + u], x);
+          }
+        }
+      }
+      n[i] = x + y;
+      scaled[i] = strength[i] * n[i];
+    }
+    wave_sync();  // A's diagonal blocks have been read
+#pragma unroll
+    for (int i = 0; i < 16; ++i) m[16 * g + i][16 * g + r] = n[i];
+  }
+  wave_sync();
+  f32x4 inverse[4];  // I + N_ii b_i, row r
+  f32x4 n[4][4], scaled[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32x4 row = load4(&m[16 * i + r][16 * i + 4 * g]);
+    const f32x4 b = load4(&head.strength[16 * i + 4 * g]);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      inverse[i][c] = fmaf(row[c], b[c], 4 * g + c == r ? 1.0f : 0.0f);
+      n[i][i][c] = m[16 * i + 4 * g + c][16 * i + r];
+    }
+    scaled[i][i] = times(b, n[i][i]);
+  }
+#pragma unroll
+  for (int i = 1; i < 4; ++i) {
+    const f32x4 b = load4(&head.strength[16 * i + 4 * g]);
+#pragma unroll
+    for (int j = 0; j < i; ++j) {
+      f32x4 x = a[i][j];
+#pragma unroll
+      for (int c = j; c < i; ++c) {
+        x = block_product(load4(&m[16 * i + r][16 * c + 4 * g]), scaled[c][j], x);
+      }
+      const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+      x = block_product(inverse[i], x, zero);
+      n[i][j] = -x;
+      scaled[i][j] = times(b, n[i][j]);
+    }
+  }
+  wave_sync();  // A has been read
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool empty = (i == 0 && j == 1) || (i == 2 && j == 3);  // above, in a tile
+      if (j < i || empty) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          m[16 * i + 4 * g + c][16 * j + r] = empty ? 0.0f : n[i][j][c];
+        }
+      }
+    }
+  }
+  wave_sync();
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
 #pragma unroll
     for (int step = 0; step < 2; ++step) {
-      uint4 part[3];
       if (step < lower_steps(t)) {
-        const float* p = &m[16 * t + row][32 * step + 4 * g];
-        split3(load4(p), load4(p + 16), part);
-        store_parts(block + kSolve, lower_tile(t, step), lane, part, kSolveParts);
+        const float* p = &m[16 * t + r][32 * step + 4 * g];
+        store_tile(block + kSolve, lower_tile(t, step), lane, load4(p), load4(p + 16));
       }
       if (kTrain && step >= upper_first(t)) {
         f32x4 x, y;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x[i] = m[place(step, g, i)][16 * t + row];
-          y[i] = m[place(step, g, i + 4)][16 * t + row];
+          x[i] = m[token_place(step, g, i)][16 * t + r];
+          y[i] = m[token_place(step, g, i + 4)][16 * t + r];
         }
-        split3(x, y, part);
-        store_parts(block + kSolveBack, upper_tile(t, step), lane, part, kSolveParts);
+        store_tile(block + kSolveBack, upper_tile(t, step), lane, x, y);
       }
     }
   }
@@ -119,42 +196,57 @@ __device__ __forceinline__ void solve_head(Staged& s, int slot, int lane, char* 
 
 // P b of one value head (and P^T) by one wavefront.
 template <bool kTrain>
-__device__ __forceinline__ void read_out_head(const Staged& s, int slot, int lane, char* block) {
-  const int row = lane & 15, g = lane >> 4;
+__device__ __forceinline__ void read_out_head(const Staged& s, const Head& head, int lane,
+                                              char* block) {
+  const int r = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
-    const int at = 16 * t + row;
-    const double mine = s.sum[slot][at];
+    const int at = 16 * t + r;
+    const float sum = head.sum[at], rest = head.rest[at];
 #pragma unroll
     for (int step = 0; step < 2; ++step) {
       f32x4 x[2];
-      uint4 part[3];
       if (step < lower_steps(t)) {  // row i = at, columns j
+        const float q_unit = s.q_unit[at];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int j = place(step, g, i);
-          const float decay = expf(static_cast<float>(mine - s.sum[slot][j]));
-          x[i / 4][i % 4] = j <= at ? decay * (s.q_unit[at] * s.k_unit[j] * s.qk[at][j]) *
-                                          s.strength[slot][j]
-                                    : 0.0f;
+        for (int u = 0; u < 2; ++u) {
+          const int from = 32 * step + 16 * u + 4 * g;
+          const f32x4 sums = load4(&head.sum[from]), rests = load4(&head.rest[from]);
+          const f32x4 units = load4(&s.k_unit[from]), b = load4(&head.strength[from]);
+          const f32x4 product = load4(&s.qk[at][from]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float y = decay_between(sum, rest, sums[i], rests[i]) *
+                            (q_unit * units[i] * product[i]) * b[i];
+            x[u][i] = from + i <= at ? y : 0.0f;
+          }
         }
         // Two parts, rounded: 2^-16 of a weight whose sums become bf16 outputs.
-        split2_pair(x[0][0], x[0][1], part[0].x, part[1].x);
-        split2_pair(x[0][2], x[0][3], part[0].y, part[1].y);
-        split2_pair(x[1][0], x[1][1], part[0].z, part[1].z);
-        split2_pair(x[1][2], x[1][3], part[0].w, part[1].w);
-        store_parts(block + kReadOut, lower_tile(t, step), lane, part, kReadParts);
+        uint4 high, low;
+        split2_pair(x[0][0], x[0][1], high.x, low.x);
+        split2_pair(x[0][2], x[0][3], high.y, low.y);
+        split2_pair(x[1][0], x[1][1], high.z, low.z);
+        split2_pair(x[1][2], x[1][3], high.w, low.w);
+        uint4* const p = reinterpret_cast<uint4*>(block + kReadOut +
+                                                  lower_tile(t, step) * kTileBytes) + lane;
+        p[0] = high;
+        p[kTriangle * 64] = low;
       }
       if (kTrain && step >= upper_first(t)) {  // row j = at, columns i
+        const float k_unit = s.k_unit[at];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int token = place(step, g, i);
-          const float decay = expf(static_cast<float>(s.sum[slot][token] - mine));
-          x[i / 4][i % 4] =
-              at <= token ? decay * (s.q_unit[token] * s.k_unit[at] * s.qk[token][at]) : 0.0f;
+        for (int u = 0; u < 2; ++u) {
+          const int from = 32 * step + 16 * u + 4 * g;
+          const f32x4 sums = load4(&head.sum[from]), rests = load4(&head.rest[from]);
+          const f32x4 units = load4(&s.q_unit[from]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float y = decay_between(sums[i], rests[i], sum, rest) *
+                            (units[i] * k_unit * s.qk[from + i][at]);
+            x[u][i] = at <= from + i ? y : 0.0f;
+          }
         }
-        split3(x[0], x[1], part);
-        store_parts(block + kReadBack, upper_tile(t, step), lane, part, kSolveParts);
+        store_tile(block + kReadBack, upper_tile(t, step), lane, x[0], x[1]);
       }
     }
   }
@@ -174,7 +266,7 @@ __device__ __forceinline__ void clear_rest(const RuleArgs& a, uint32_t head,
 template <bool kTrain>
 __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(RuleArgs a,
                                                                 bf16_bits* outputs) {
-  __shared__ Staged s;
+  __shared__ __align__(16) Staged s;
   const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
   const uint32_t row = blockIdx.x / a.space.key_heads;
   const uint32_t head = blockIdx.x % a.space.key_heads;
@@ -186,24 +278,29 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(RuleArgs a,
 
   {  // stage the rows, 32 columns a thread, zeros past the request's end
     const int token = t >> 2, part = t & 3;
+    uint4 k[4], q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      k[i] = q[i] = make_uint4(0, 0, 0, 0);
+      const int column = 32 * i + 8 * part;
+      if (token < count) {
+        k[i] = *reinterpret_cast<const uint4*>(a.keys + (first + token) * a.key_stride +
+                                               head * kDim + column);
+        q[i] = *reinterpret_cast<const uint4*>(a.queries + (first + token) * a.query_stride +
+                                               head * kDim + column);
+      }
+    }
     float kk = 0.0f, qq = 0.0f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      uint4 k = make_uint4(0, 0, 0, 0), q = k;
-      const int column = 32 * part + 8 * i;
-      if (token < count) {
-        k = *reinterpret_cast<const uint4*>(a.keys + (first + token) * a.key_stride +
-                                            head * kDim + column);
-        q = *reinterpret_cast<const uint4*>(a.queries + (first + token) * a.query_stride +
-                                            head * kDim + column);
-      }
-      *reinterpret_cast<uint4*>(&s.k[token][column]) = k;
-      *reinterpret_cast<uint4*>(&s.q[token][column]) = q;
+      const int column = 32 * i + 8 * part;
+      *reinterpret_cast<uint4*>(&s.k[token][column]) = k[i];
+      *reinterpret_cast<uint4*>(&s.q[token][column]) = q[i];
       float x[8];
-      widen8(k, x);
+      widen8(k[i], x);
 #pragma unroll
       for (int c = 0; c < 8; ++c) kk = fmaf(x[c], x[c], kk);
-      widen8(q, x);
+      widen8(q[i], x);
 #pragma unroll
       for (int c = 0; c < 8; ++c) qq = fmaf(x[c], x[c], qq);
     }
@@ -240,31 +337,16 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(RuleArgs a,
         s.qk[16 * wave + 4 * g + i][16 * c + r] = qk[i];
       }
     }
-    // Its rows as operands over the keys.
-#pragma unroll
-    for (int step = 0; step < 4; ++step) {
-      const uint16_t* k_row = &s.k[16 * wave + r][32 * step + 4 * g];
-      const uint16_t* q_row = &s.q[16 * wave + r][32 * step + 4 * g];
-      const uint2 k0 = *reinterpret_cast<const uint2*>(k_row);
-      const uint2 k1 = *reinterpret_cast<const uint2*>(k_row + 16);
-      const uint2 q0 = *reinterpret_cast<const uint2*>(q_row);
-      const uint2 q1 = *reinterpret_cast<const uint2*>(q_row + 16);
-      const int tile = (4 * wave + step) * kTileBytes;
-      reinterpret_cast<uint4*>(key_block + kKeyRows + tile)[lane] =
-          make_uint4(k0.x, k0.y, k1.x, k1.y);
-      reinterpret_cast<uint4*>(key_block + kQueryRows + tile)[lane] =
-          make_uint4(q0.x, q0.y, q1.x, q1.y);
-    }
-    // Two row tiles of the transposes: rows = keys, over the tokens.
+    // Two row tiles of the transposes: rows = keys in state order, over the tokens.
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const int key = 32 * wave + 16 * c + r;
+      const int key = state_key(2 * wave + c, r);
 #pragma unroll
       for (int step = 0; step < 2; ++step) {
         uint32_t kw[4], qw[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const int x = place(step, g, 2 * i), y = place(step, g, 2 * i + 1);
+          const int x = token_place(step, g, 2 * i), y = token_place(step, g, 2 * i + 1);
           kw[i] = s.k[x][key] | static_cast<uint32_t>(s.k[y][key]) << 16;
           if constexpr (kTrain) qw[i] = s.q[x][key] | static_cast<uint32_t>(s.q[y][key]) << 16;
         }
@@ -284,43 +366,45 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(RuleArgs a,
       norms[2 * kChunk + t] = s.q_norm[t];
     }
   }
+  __syncthreads();  // K and Q have been read; K K^T and Q K^T are whole
 
-  // Value heads two at a time: wavefronts 0 and 1 solve, 2 and 3 form P b.
-  for (uint32_t pair = 0; pair < a.group; pair += 2) {
-    __syncthreads();  // K and Q (or the last pair's N and factors) have been read
-    const int slot = wave & 1;
-    const uint32_t member = pair + slot;
-    const bool live = member < a.group;
-    const uint32_t value_head = head * a.group + (live ? member : 0);
+  // Wavefronts 0 and 2 solve, 1 and 3 form P b, each for every second value head.
+  Head& mine = s.heads[wave];
+  for (uint32_t member = wave >> 1; member < a.group; member += 2) {
+    const uint32_t value_head = head * a.group + member;
     char* const block = a.space.value_block(row, value_head);
-    if (wave < 2 && live) {
-      const uint64_t at = (first + lane) * a.space.value_heads + value_head;
-      double sum = lane < count ? static_cast<double>(a.log_decay[at]) : 0.0;
-      const float strength = lane < count ? widen(a.beta[at]) : 0.0f;
+    const uint64_t at = (first + lane) * a.space.value_heads + value_head;
+    double total = lane < count ? static_cast<double>(a.log_decay[at]) * kInverseLn2 : 0.0;
+    const float strength = lane < count ? widen(a.beta[at]) : 0.0f;
 #pragma unroll
-      for (int step = 1; step < 64; step <<= 1) {
-        const double before = __shfl_up(sum, step);
-        if (lane >= step) sum += before;
-      }
-      s.sum[slot][lane] = sum;
-      s.strength[slot][lane] = strength;
-      const double end = __shfl(sum, 63);
-      const float decay = expf(static_cast<float>(sum));
-      float* factors = reinterpret_cast<float*>(block);
-      factors[kReadKey * kChunk + lane] = decay * s.k_unit[lane];
-      factors[kReadQuery * kChunk + lane] = decay * s.q_unit[lane];
-      factors[kStrength * kChunk + lane] = strength;
-      factors[kWrite * kChunk + lane] =
-          expf(static_cast<float>(end - sum)) * s.k_unit[lane];
-      factors[kSum * kChunk + lane] = static_cast<float>(sum);
-      factors[kSumRest * kChunk + lane] =
-          static_cast<float>(sum - static_cast<double>(static_cast<float>(sum)));
-      factors[kWhole * kChunk + lane] = expf(static_cast<float>(end));
+    for (int step = 1; step < 64; step <<= 1) {
+      const double before = __shfl_up(total, step);
+      if (lane >= step) total += before;
     }
-    __syncthreads();
-    if (live) {
-      if (wave < 2) solve_head<kTrain>(s, slot, lane, block);
-      else read_out_head<kTrain>(s, slot, lane, block);
+    const float sum = static_cast<float>(total);
+    const float rest = static_cast<float>(total - static_cast<double>(sum));
+    wave_sync();  // the last head's values have been read
+    mine.sum[lane] = sum;
+    mine.rest[lane] = rest;
+    mine.strength[lane] = strength;
+    wave_sync();
+    if ((wave & 1) == 0) {
+      solve_head<kTrain>(s, mine, s.solve[wave >> 1], lane, block);
+    } else {
+      const double end = __shfl(total, 63);
+      const float decay = __builtin_amdgcn_exp2f(sum);
+      const float k_unit = lane < count ? s.k_unit[lane] : 0.0f;  // no rows past the end
+      float* factors = reinterpret_cast<float*>(block);
+      const float carry =
+          __builtin_amdgcn_exp2f(static_cast<float>(end - total)) * k_unit;
+      reinterpret_cast<f32x4*>(factors)[lane] =
+          f32x4{decay * k_unit, strength, carry * strength,
+                __builtin_amdgcn_exp2f(static_cast<float>(end))};
+      factors[kCarry + lane] = carry;
+      factors[kReadQuery + lane] = decay * s.q_unit[lane];
+      factors[kSum + lane] = sum;
+      factors[kSumRest + lane] = rest;
+      read_out_head<kTrain>(s, mine, lane, block);
     }
   }
 }

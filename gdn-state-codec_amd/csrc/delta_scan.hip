@@ -1,14 +1,23 @@
 // The sequential half of the gated delta rule's chunked form, forward
 // (formulas, layouts and precision in delta_chunk.h).
 //
-// Column v of a state [key][value] meets only column v of V, E and O, so one
-// wavefront takes 16 kColumns columns of one request's value head through all its
-// chunks, with the state in its accumulators: no LDS, no barrier, no exchange
-// between lanes.  Per chunk and 16 columns it issues
-//   K S0: 48, N (b R): 36, P (b E): 18, Q S0: 32, K^T U: 48   matrix instructions
-// (K S0's results are the operand of N, N's of both updates, so S0 to S1 is one
-// chain).  The operands come from the workspace in the order the lanes hold them,
-// 16 bytes a lane and load.
+// Column v of a state [key][value] meets only column v of V, E and O, so columns
+// go to wavefronts and workgroups as they like, but from S0 to S1 is one chain,
+//   S0 -> K S0 -> R -> N (b R) -> E -> K^T U -> S1,
+// chunk after chunk.  Per chunk and 16 columns it issues
+//   K S0: 48, N (b R): 36, K^T U: 48, and beside the chain Q S0: 32, (P b) E: 18
+// matrix instructions.  Two forms:
+//
+// delta_scan_wide_kernel, for throughput: a workgroup takes a whole head, each of its
+// eight wavefronts 16 columns with all 64 tokens, the state in its accumulators.
+// What one product hands to the next are accumulators cut into parts, in registers:
+// no exchange.  The operands, the same for all eight, come through LDS a chunk ahead.
+//
+// delta_scan_narrow_kernel, for few heads, where a long request's chain is all there
+// is: a workgroup takes 16 columns, and its wavefronts share each product by token
+// rows (or state rows), four on the chain and four on the outputs.  What a product
+// hands to the next goes through LDS, three exchanges a chunk; a wavefront's own
+// operands go from global memory to its registers a chunk ahead.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -30,177 +39,230 @@ struct ScanArgs {
 
 namespace {
 
-// A chunk's operands in LDS: K, Q and K^T of the key head, then the first 32 KiB
-// of the value head's block (factors, N, P b; 512 bytes of it are not used).
-constexpr int kKeyStage = 3 * kKeyTiles * kTileBytes;
-constexpr int kValueStage = 32 * kTileBytes;
-constexpr int kStage = kKeyStage + kValueStage;
-static_assert(value_block_bytes(false) <= kValueStage, "the stage holds a value block");
-static_assert(2 * kStage <= static_cast<int>(kLdsPerCu), "two stages fill the LDS");
+// Where one workgroup works: a request's value head, and its tokens and chunk rows as
+// far as the tables stay inside the batch.
+struct Work {
+  uint32_t head, request;
+  uint64_t tile;  // of the state
+  uint32_t first_row, begin, length, chunks;
+  bool resumed;
+};
 
-template <int kWaves>
-__device__ __forceinline__ void stage_chunk(const char* keys, const char* block, int wave,
-                                            int lane, uint32_t to) {
+// Item `item` of requests x value heads, longest requests first; false: none, or
+// padding.
+__device__ __forceinline__ bool find_work(const ScanArgs& args, uint64_t item, Work& w) {
+  const RuleArgs& a = args.rule;
+  const ChunkSpace& space = a.space;
+  if (item >= static_cast<uint64_t>(a.requests) * space.value_heads) return false;
+  w.head = static_cast<uint32_t>(item % space.value_heads);
+  w.request = static_cast<uint32_t>(a.order[item / space.value_heads]);
+  if (w.request >= a.requests) return false;
+  const uint32_t slot =
+      args.slot_ids ? static_cast<uint32_t>(args.slot_ids[w.request]) : w.request;
+  if (slot >= args.slots) return false;
+  w.tile = (static_cast<uint64_t>(slot) * space.value_heads + w.head) * kTile;
+  w.resumed = args.initial && (!args.resume || args.resume[w.request] != 0);
+  w.first_row = min(static_cast<uint32_t>(a.chunk_offsets[w.request]), space.rows);
+  const uint32_t rows =
+      min(static_cast<uint32_t>(a.chunk_offsets[w.request + 1]), space.rows) - w.first_row;
+  w.begin = min(static_cast<uint32_t>(a.offsets[w.request]), a.tokens);
+  w.length = min(static_cast<uint32_t>(a.offsets[w.request + 1]), a.tokens) - w.begin;
+  w.chunks = min(rows, (w.length + kChunk - 1) / kChunk);
+  return true;
+}
+
+// A head's state in a wavefront's accumulators: tiles `first`.. of column `value`
+// (row 4 g + i of a tile is key state_key).
+template <int kTiles, typename Pool>
+__device__ __forceinline__ void load_state(const Pool* state, int first, int value, int g,
+                                           bool resumed, f32x4 (&x)[kTiles]) {
 #pragma unroll
-  for (int i = 0; i < 80 / kWaves; ++i) {
-    const int tile = i * kWaves + wave;
-    const char* from = tile < 48 ? keys + tile * kTileBytes : block + (tile - 48) * kTileBytes;
-    stage_tile(from, lane, to + tile * kTileBytes);
+  for (int t = 0; t < kTiles; ++t) {
+    x[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (resumed) x[t] = load_cells(state + value * kDim + state_key(first + t, 4 * g));
+  }
+}
+template <int kTiles, typename Pool>
+__device__ __forceinline__ void store_state(Pool* state, int first, int value, int g,
+                                            const f32x4 (&x)[kTiles]) {
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) {
+    store_cells(state + value * kDim + state_key(first + t, 4 * g), x[t]);
   }
 }
 
-template <typename Pool, int kWaves, bool kTrain>
-__global__ __launch_bounds__(64 * kWaves, 1) void delta_scan_kernel(ScanArgs args) {
-  constexpr int kSlices = kDim / (16 * kWaves);
-  __shared__ __align__(16) char stages[2][kStage];
+// bf16 rows of a tile's four accumulator rows, as a quad of lanes stores them.
+__device__ __forceinline__ uint2 output_run(const f32x4& x, int lane) {
+  return transpose_quad(make_uint2(bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3])), lane);
+}
+__device__ __forceinline__ f32x4 value_rows(const uint2& run, int lane) {
+  const uint2 x = transpose_quad(run, lane);
+  return f32x4{widen_low(x.x), widen_high(x.x), widen_low(x.y), widen_high(x.y)};
+}
+
+// ------------------------------------------------------------- whole heads
+
+// A chunk's operands in LDS, in two halves, each fetched while the other is at work:
+// the factors, N (20 KiB of the value head's block) and K rows (16 tiles), then P b,
+// Q rows and K^T.  80 KiB, so that two workgroups share a compute unit.
+constexpr int kBlockTiles = 20;
+constexpr int kStageKeys = kBlockTiles * kTileBytes;
+constexpr int kStageRead = kStageKeys + kKeyTiles * kTileBytes;
+constexpr int kStageQueries = kStageRead + kReadOutBytes;
+constexpr int kStageColumns = kStageQueries + kKeyTiles * kTileBytes;
+constexpr int kStage = kStageColumns + kKeyTiles * kTileBytes;
+static_assert(kReadOut <= kBlockTiles * kTileBytes, "factors and N");
+static_assert(workgroups_by_lds(kStage) == 2, "two workgroups share a compute unit");
+
+constexpr int kWideWaves = 4;
+constexpr int kWideSlices = kDim / (16 * kWideWaves);
+
+template <typename Pool, bool kTrain>
+__global__ __launch_bounds__(64 * kWideWaves, 2) void delta_scan_wide_kernel(ScanArgs args) {
+  __shared__ __align__(16) char stage[kStage];
   const RuleArgs& a = args.rule;
   const ChunkSpace& space = a.space;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   // A head's slices share their operands: they get consecutive places of one XCD
   // (the dispatcher deals workgroups out to the 8 XCDs in turn).
   const uint32_t turn = blockIdx.x >> 3;
-  const uint64_t item = static_cast<uint64_t>(turn / kSlices) * 8 + (blockIdx.x & 7);
-  if (item >= static_cast<uint64_t>(a.requests) * space.value_heads) return;
-  const uint32_t head = static_cast<uint32_t>(item % space.value_heads);
-  const int32_t request = a.order[item / space.value_heads];
-  if (request < 0 || static_cast<uint32_t>(request) >= a.requests) return;
-  const int value = (turn % kSlices) * 16 * kWaves + 16 * wave + r;  // this lane's column
-  const int32_t slot = args.slot_ids ? args.slot_ids[request] : request;
-  if (slot < 0 || static_cast<uint32_t>(slot) >= args.slots) return;  // padding
-  const uint64_t tile = (static_cast<uint64_t>(slot) * space.value_heads + head) * kTile +
-                        value * kDim + 4 * g;
-
-  f32x4 state[8];  // keys 16 t + 4 g + i
-  const bool resumed = args.initial && (!args.resume || args.resume[request] != 0);
-#pragma unroll
-  for (int t = 0; t < 8; ++t) state[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  if (resumed) {
-    const Pool* p = static_cast<const Pool*>(args.initial) + tile;
-#pragma unroll
-    for (int t = 0; t < 8; ++t) state[t] = load_cells(p + 16 * t);
+  Work w;
+  if (!find_work(args, static_cast<uint64_t>(turn / kWideSlices) * 8 + (blockIdx.x & 7), w)) {
+    return;
   }
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int first_value = 16 * (kWideWaves * (turn % kWideSlices) + wave);
+  const int value = first_value + r;
+  const uint32_t key_head = w.head / a.group;
+  const uint32_t length = w.length, chunks = w.chunks;
 
-  // The request's tokens and chunk rows, as far as the tables stay inside the batch.
-  const uint32_t first_row = min(static_cast<uint32_t>(a.chunk_offsets[request]), space.rows);
-  const uint32_t rows = min(static_cast<uint32_t>(a.chunk_offsets[request + 1]), space.rows) -
-                        first_row;
-  const uint32_t begin = min(static_cast<uint32_t>(a.offsets[request]), a.tokens);
-  const uint32_t length = min(static_cast<uint32_t>(a.offsets[request + 1]), a.tokens) - begin;
-  const uint32_t chunks = min(rows, (length + kChunk - 1) / kChunk);
+  f32x4 state[8];
+  load_state(static_cast<const Pool*>(args.initial) + w.tile, 0, value, g, w.resumed, state);
+
   const uint32_t stage_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
-      (__attribute__((address_space(3))) char*)&stages[0][0]));
-  const uint64_t token_step = static_cast<uint64_t>(space.value_heads) * kDim;
-
-  bf16_bits values[4][4];  // of the tokens 16 t + 4 g + i
-  const auto fetch = [&](uint32_t c) {
-    const int last = min(static_cast<int>(length - c * kChunk), kChunk) - 1;
-    stage_chunk<kWaves>(space.key_block(first_row + c, head / a.group),
-                        space.value_block(first_row + c, head), wave, lane,
-                        stage_at + (c & 1) * kStage);
-    const bf16_bits* v = a.values + static_cast<uint64_t>(begin + c * kChunk) * a.value_stride +
-                         head * kDim + value;
+      (__attribute__((address_space(3))) char*)&stage[0]));
+  // Addresses are a chunk's (scalar) and a lane's own 32-bit byte offset from it,
+  // which the last chunk's row clamps: rows past the end repeat it.  What becomes of
+  // them meets a strength of zero before it meets anything else, and is not stored.
+  const uint32_t key_step = static_cast<uint32_t>(a.key_stride) * 2;
+  const uint32_t query_step = static_cast<uint32_t>(a.query_stride) * 2;
+  const uint32_t value_step = static_cast<uint32_t>(a.value_stride) * 2;
+  const uint32_t out_step = space.value_heads * kDim * 2;
+  uint2 values[4];  // columns 4 (r / 4).. of tokens 16 t + 4 g + (r & 3)
+  const uint32_t linear = 16 * lane;
+  const auto fetch_first = [&](uint32_t c) {
+    const uint64_t token = w.begin + c * kChunk;
+    const uint32_t last = min(length - c * kChunk, static_cast<uint32_t>(kChunk)) - 1;
+    const char* k = reinterpret_cast<const char*>(a.keys + token * a.key_stride +
+                                                  key_head * kDim);
+    const char* block = space.value_block(w.first_row + c, w.head);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {  // rows 16 t.., keys 32 wave..
+      const uint32_t row = min(static_cast<uint32_t>(16 * t + r), last);
+      stage_tile(k + 64 * wave, row * key_step + 16 * g,
+                 stage_at + kStageKeys + (4 * t + wave) * kTileBytes);
+    }
+#pragma unroll
+    for (int i = 0; i < kBlockTiles / kWideWaves; ++i) {
+      const int tile = kWideWaves * i + wave;
+      stage_tile(block + tile * kTileBytes, linear, stage_at + tile * kTileBytes);
+    }
+    const char* v = reinterpret_cast<const char*>(a.values + token * a.value_stride +
+                                                  w.head * kDim + first_value);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        values[t][i] = v[min(16 * t + 4 * g + i, last) * a.value_stride];
-      }
+      const uint32_t row = min(static_cast<uint32_t>(16 * t + 4 * g + (r & 3)), last);
+      values[t] = *reinterpret_cast<const uint2*>(v + (row * value_step + 2 * (r & 12)));
     }
   };
-  if (chunks != 0) fetch(0);
+  const auto fetch_second = [&](uint32_t c) {
+    const uint64_t token = w.begin + c * kChunk;
+    const uint32_t last = min(length - c * kChunk, static_cast<uint32_t>(kChunk)) - 1;
+    const char* q = reinterpret_cast<const char*>(a.queries + token * a.query_stride +
+                                                  key_head * kDim);
+    const char* columns = space.key_block(w.first_row + c, key_head) + kKeyColumns;
+    const char* read = space.value_block(w.first_row + c, w.head) + kReadOut;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const uint32_t row = min(static_cast<uint32_t>(16 * t + r), last);
+      const int tile = 4 * t + wave;
+      stage_tile(q + 64 * wave, row * query_step + 16 * g,
+                 stage_at + kStageQueries + tile * kTileBytes);
+      stage_tile(columns + tile * kTileBytes, linear,
+                 stage_at + kStageColumns + tile * kTileBytes);
+    }
+#pragma unroll
+    for (int i = 0; i < 2 * kTriangle / kWideWaves; ++i) {
+      const int tile = kWideWaves * i + wave;
+      stage_tile(read + tile * kTileBytes, linear, stage_at + kStageRead + tile * kTileBytes);
+    }
+  };
+  if (chunks != 0) fetch_first(0);
 
   f32x4 error[4], out[4];
-  const auto store_outputs = [&](uint32_t c, int tokens) {
-    if constexpr (kTrain) {
-      float* e = space.errors(first_row + c, head) + value;
+  const auto store_rows = [&](uint32_t c, int tokens) {
+    char* o = reinterpret_cast<char*>(args.outputs) +
+              (w.begin + static_cast<uint64_t>(c) * kChunk) * out_step +
+              2 * (w.head * kDim + first_value);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < 4; ++t) {
+      const int token = 16 * t + 4 * g + (r & 3);
+      const uint2 x = output_run(out[t], lane);
+      if (token < tokens) *reinterpret_cast<uint2*>(o + (token * out_step + 2 * (r & 12))) = x;
+      if constexpr (kTrain) {
+        float* e = space.errors(w.first_row + c, w.head) + value;
 #pragma unroll
         for (int i = 0; i < 4; ++i) e[(16 * t + 4 * g + i) * kDim] = error[t][i];
       }
     }
-    bf16_bits* o = args.outputs + (begin + c * kChunk) * token_step + head * kDim + value;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int token = 16 * t + 4 * g + i;
-        if (token < tokens) {
-          o[token * token_step] = static_cast<bf16_bits>(bf16_pair(out[t][i], 0.0f));
-        }
-      }
-    }
   };
 
+  const uint4* const k_rows = reinterpret_cast<const uint4*>(stage + kStageKeys) + lane;
+  const uint4* const q_rows = reinterpret_cast<const uint4*>(stage + kStageQueries) + lane;
+  const uint4* const k_columns = reinterpret_cast<const uint4*>(stage + kStageColumns) + lane;
+  const uint4* const solve = reinterpret_cast<const uint4*>(stage + kSolve) + lane;
+  const uint4* const read_out = reinterpret_cast<const uint4*>(stage + kStageRead) + lane;
   for (uint32_t c = 0; c < chunks; ++c) {
-    stage_ready();
-    const uint32_t row = first_row + c;
-    const char* const keys = stages[c & 1];
-    const char* const block = keys + kKeyStage;
-    const uint4* const k_rows = reinterpret_cast<const uint4*>(keys + kKeyRows) + lane;
-    const uint4* const q_rows = reinterpret_cast<const uint4*>(keys + kQueryRows) + lane;
-    const uint4* const k_columns = reinterpret_cast<const uint4*>(keys + kKeyColumns) + lane;
-    const uint4* const solve = reinterpret_cast<const uint4*>(block + kSolve) + lane;
-    const uint4* const read_out = reinterpret_cast<const uint4*>(block + kReadOut) + lane;
-    const float* const factors = reinterpret_cast<const float*>(block) + 4 * g;
-    const int tokens = min(static_cast<int>(length - c * kChunk), kChunk);
-    f32x4 value_rows[4];
+    stage_ready();  // the first half is there, the second has been read
+    f32x4 factors[4];  // of tokens 16 t + 4 g + (r & 3)
+    float queries[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        value_rows[t][i] = 16 * t + 4 * g + i < tokens ? widen(values[t][i]) : 0.0f;
-        // Used before the next loads are issued, so that no wait for it covers them.
-        asm volatile("" : "+v"(value_rows[t][i]));
-      }
+      const int token = 16 * t + 4 * g + (r & 3);
+      factors[t] = reinterpret_cast<const f32x4*>(stage)[token];
+      queries[t] = reinterpret_cast<const float*>(stage)[kReadQuery + token];
+      // Used before the next loads are issued, so that no wait for it covers them.
+      asm volatile("" : "+v"(values[t].x), "+v"(values[t].y));
     }
-    // The next chunk's loads and the last one's stores have this chunk's products
-    // to finish in.
-    if (c + 1 < chunks) fetch(c + 1);
-    if (c != 0) store_outputs(c - 1, kChunk);  // only the last chunk can be short
+    fetch_second(c);
+    if (c != 0) store_rows(c - 1, kChunk);  // only the last chunk can be short
     if constexpr (kTrain) {
-      float* p = space.state(row, head) + value;
+      float* p = space.state(w.first_row + c, w.head) + value;
 #pragma unroll
       for (int t = 0; t < 8; ++t) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[(16 * t + 4 * g + i) * kDim] = state[t][i];
+        for (int i = 0; i < 4; ++i) p[state_key(t, 4 * g + i) * kDim] = state[t][i];
       }
     }
-
-    {
-      uint4 part[4][3];  // of the state, over the keys
+    uint4 part[4][3];  // of the state, over the keys
+#pragma unroll
+    for (int step = 0; step < 4; ++step) {
+      split3(state[2 * step], state[2 * step + 1], part[step]);
+    }
+    // R = V - exp(G) K S0
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      f32x4 seen[2] = {};  // two sums, so that each product waits for the last but one
 #pragma unroll
       for (int step = 0; step < 4; ++step) {
-        split3(state[2 * step], state[2 * step + 1], part[step]);
+        const uint4 k = k_rows[(4 * t + step) * 64];
+#pragma unroll
+        for (int p = 2; p >= 0; --p) seen[p & 1] = mfma(k, part[step][p], seen[p & 1]);
       }
-      // R = V - exp(G) K S0
+      const f32x4 read_key = of_rows(factors[t][kReadKey]);
+      const f32x4 x = value_rows(values[t], lane);
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        f32x4 seen = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int step = 0; step < 4; ++step) {
-          seen = mfma3(k_rows[(4 * t + step) * 64], part[step], seen);
-        }
-        const f32x4 factor = load4(factors + kReadKey * kChunk + 16 * t);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) error[t][i] = fmaf(-factor[i], seen[i], value_rows[t][i]);
-      }
-      // exp(G) Q S0, from two of the state's parts: 2^-15 of terms whose sums
-      // become bf16 outputs.
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        f32x4 read = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int step = 0; step < 4; ++step) {
-          const uint4 q = q_rows[(4 * t + step) * 64];
-          read = mfma(q, part[step][1], read);
-          read = mfma(q, part[step][0], read);
-        }
-        const f32x4 factor = load4(factors + kReadQuery * kChunk + 16 * t);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) out[t][i] = factor[i] * read[i];
-      }
+      for (int i = 0; i < 4; ++i) error[t][i] = fmaf(-read_key[i], seen[0][i] + seen[1][i], x[i]);
     }
     // E = R + N (b R)
     {
@@ -210,7 +272,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void delta_scan_kernel(ScanArgs arg
         f32x4 x[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const f32x4 b = load4(factors + kStrength * kChunk + 32 * step + 16 * u);
+          const f32x4 b = of_rows(factors[2 * step + u][kStrength]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[u][i] = b[i] * error[2 * step + u][i];
         }
@@ -227,12 +289,28 @@ __global__ __launch_bounds__(64 * kWaves, 1) void delta_scan_kernel(ScanArgs arg
         }
       }
     }
+    stage_ready();  // the second half is there, the first has been read
+    if (c + 1 < chunks) fetch_first(c + 1);
+    // exp(G) Q S0 from two of the state's parts: 2^-15 of terms whose sums become
+    // bf16 outputs.
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      f32x4 read[2] = {};
+#pragma unroll
+      for (int step = 0; step < 4; ++step) {
+        const uint4 q = q_rows[(4 * t + step) * 64];
+        read[0] = mfma(q, part[step][1], read[0]);
+        read[1] = mfma(q, part[step][0], read[1]);
+      }
+      const f32x4 read_query = of_rows(queries[t]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out[t][i] = read_query[i] * (read[0][i] + read[1][i]);
+    }
     // S1 = exp(G_63) S0 + K^T (write b E), and O += (P b) E
-    const float whole = factors[kWhole * kChunk];
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) state[t][i] *= whole;
+      for (int i = 0; i < 4; ++i) state[t][i] *= factors[0][kWhole];
     }
 #pragma unroll
     for (int step = 0; step < 2; ++step) {
@@ -240,10 +318,9 @@ __global__ __launch_bounds__(64 * kWaves, 1) void delta_scan_kernel(ScanArgs arg
       f32x4 x[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const f32x4 b = load4(factors + kStrength * kChunk + 32 * step + 16 * u);
-        const f32x4 w = load4(factors + kWrite * kChunk + 32 * step + 16 * u);
+        const f32x4 write = of_rows(factors[2 * step + u][kWrite]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[u][i] = w[i] * (b[i] * error[2 * step + u][i]);
+        for (int i = 0; i < 4; ++i) x[u][i] = write[i] * error[2 * step + u][i];
       }
       split3(x[0], x[1], written);
       split3(error[2 * step], error[2 * step + 1], plain);
@@ -253,38 +330,331 @@ __global__ __launch_bounds__(64 * kWaves, 1) void delta_scan_kernel(ScanArgs arg
       }
 #pragma unroll
       for (int t = 2 * step; t < 4; ++t) {  // rows 0..31 end in step 0
-        const int place = lower_tile(t, step);
-        const uint4 high = read_out[place * 64], low = read_out[(kTriangle + place) * 64];
+        const int tile = lower_tile(t, step);
+        const uint4 high = read_out[tile * 64], low = read_out[(kTriangle + tile) * 64];
         out[t] = mfma(low, plain[0], out[t]);
         out[t] = mfma(high, plain[1], out[t]);
         out[t] = mfma(high, plain[0], out[t]);
       }
     }
   }
-  if (chunks != 0) store_outputs(chunks - 1, length - (chunks - 1) * kChunk);
-
-  Pool* p = static_cast<Pool*>(args.final_states) + tile;
-#pragma unroll
-  for (int t = 0; t < 8; ++t) store_cells(p + 16 * t, state[t]);
+  if (chunks != 0) store_rows(chunks - 1, length - (chunks - 1) * kChunk);
+  store_state(static_cast<Pool*>(args.final_states) + w.tile, 0, value, g, state);
 }
 
-template <typename Pool, int kWaves, bool kTrain>
-int32_t launch_scan(void* stream, const ScanArgs& args) {
-  constexpr uint64_t kSlices = kDim / (16 * kWaves);
+// ------------------------------------------------------------ 16 columns
+
+template <typename Pool, bool kTrain>
+__global__ __launch_bounds__(512) void delta_scan_narrow_kernel(ScanArgs args) {
+  constexpr int kSlices = kDim / 16;
+  // Parts of S0 (4 steps over the keys), b R, write b E and E (2 steps over the
+  // tokens).
+  __shared__ uint4 state_parts[4][3][64];
+  __shared__ uint4 row_parts[2][3][64];
+  __shared__ uint4 written_parts[2][3][64];
+  __shared__ uint4 error_parts[2][2][64];
+  const RuleArgs& a = args.rule;
+  const ChunkSpace& space = a.space;
+  // A head's slices share their operands: they get consecutive places of one XCD
+  // (the dispatcher deals workgroups out to the 8 XCDs in turn).
+  const uint32_t turn = blockIdx.x >> 3;
+  Work w;
+  if (!find_work(args, static_cast<uint64_t>(turn / kSlices) * 8 + (blockIdx.x & 7), w)) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int rows = wave & 3;           // this wavefront's token rows, 16 rows..
+  const int steps = lower_steps(rows);
+  const int first_value = (turn % kSlices) * 16, value = first_value + r;
+  const uint32_t key_head = w.head / a.group;
+  const uint32_t length = w.length, chunks = w.chunks;
+  const uint32_t mine = 16 * rows + 4 * g + (r & 3);  // the token whose factors it loads
+
+  // Addresses as in the wide form; past the last chunk, the same again.
+  uint64_t token = w.begin;
+  uint32_t row = w.first_row;
+  uint32_t last = min(length, static_cast<uint32_t>(kChunk)) - 1;
+  const auto advance = [&](uint32_t c) {  // to chunk c + 1, if there is one
+    const uint32_t on = c + 1 < chunks ? 1 : 0;
+    token += on * kChunk;
+    row += on;
+    last = min(length - (c + on) * kChunk, static_cast<uint32_t>(kChunk)) - 1;
+  };
+
+  if (wave >= 4) {  // the outputs: O = exp(G) Q S0 + (P b) E
+    const uint32_t query_step = static_cast<uint32_t>(a.query_stride) * 2;
+    const uint32_t out_step = space.value_heads * kDim * 2;
+    uint4 q_rows[4], read_out[2][2];
+    float query;
+    const auto fetch_queries = [&]() {
+      const char* q = reinterpret_cast<const char*>(a.queries + token * a.query_stride +
+                                                    key_head * kDim);
+      const uint32_t at = min(static_cast<uint32_t>(16 * rows + r), last) * query_step + 16 * g;
+#pragma unroll
+      for (int step = 0; step < 4; ++step) {
+        q_rows[step] = *reinterpret_cast<const uint4*>(q + 64 * step + at);
+      }
+      query = reinterpret_cast<const float*>(space.value_block(row, w.head))[kReadQuery + mine];
+    };
+    const auto fetch_read_out = [&]() {
+      const uint4* p =
+          reinterpret_cast<const uint4*>(space.value_block(row, w.head) + kReadOut);
+#pragma unroll
+      for (int step = 0; step < 2; ++step) {  // rows 0..31 have no second step
+        const int tile = lower_tile(rows, step < steps ? step : 0);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) read_out[u][step] = p[(u * kTriangle + tile) * 64 + lane];
+      }
+    };
+    if (chunks != 0) fetch_queries();
+    for (uint32_t c = 0; c < chunks; ++c) {
+      char* const o = reinterpret_cast<char*>(args.outputs) + token * out_step +
+                      2 * (w.head * kDim + first_value);
+      const uint32_t live = last;
+      exchange();
+      fetch_read_out();
+      advance(c);
+      exchange();  // S0's parts stay until the third
+      uint4 part[4][2];
+#pragma unroll
+      for (int step = 0; step < 4; ++step) {
+        part[step][0] = state_parts[step][0][lane];
+        part[step][1] = state_parts[step][1][lane];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      // From two of the state's parts: 2^-15 of terms whose sums become bf16 outputs.
+      f32x4 read[2] = {};
+#pragma unroll
+      for (int p = 1; p >= 0; --p) {
+#pragma unroll
+        for (int step = 0; step < 4; ++step) {
+          read[step & 1] = mfma(q_rows[step], part[step][p], read[step & 1]);
+        }
+      }
+      const f32x4 read_query = of_rows(query);
+      f32x4 out;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) out[i] = read_query[i] * (read[0][i] + read[1][i]);
+      exchange();
+      uint4 part_e[2][2];
+#pragma unroll
+      for (int step = 0; step < 2; ++step) {
+        part_e[step][0] = error_parts[step][0][lane];
+        part_e[step][1] = error_parts[step][1][lane];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      fetch_queries();
+#pragma unroll
+      for (int step = 0; step < 2; ++step) {
+        if (step < steps) {
+          out = mfma(read_out[1][step], part_e[step][0], out);
+          out = mfma(read_out[0][step], part_e[step][1], out);
+          out = mfma(read_out[0][step], part_e[step][0], out);
+        }
+      }
+      const uint2 x = output_run(out, lane);
+      if (mine <= live) *reinterpret_cast<uint2*>(o + (mine * out_step + 2 * (r & 12))) = x;
+    }
+    return;
+  }
+
+  // The chain: token rows 16 wave.., state tiles 2 wave and 2 wave + 1.
+  f32x4 state[2];
+  load_state(static_cast<const Pool*>(args.initial) + w.tile, 2 * wave, value, g, w.resumed,
+             state);
+  const uint32_t key_step = static_cast<uint32_t>(a.key_stride) * 2;
+  const uint32_t value_step = static_cast<uint32_t>(a.value_stride) * 2;
+  uint4 k_rows[4], k_columns[2][2], solve[2][3];
+  f32x4 factors;
+  uint2 values;
+  const auto fetch_keys = [&]() {
+    const char* k = reinterpret_cast<const char*>(a.keys + token * a.key_stride +
+                                                  key_head * kDim);
+    const uint32_t at = min(static_cast<uint32_t>(16 * wave + r), last) * key_step + 16 * g;
+#pragma unroll
+    for (int step = 0; step < 4; ++step) {
+      k_rows[step] = *reinterpret_cast<const uint4*>(k + 64 * step + at);
+    }
+    const char* v = reinterpret_cast<const char*>(a.values + token * a.value_stride +
+                                                  w.head * kDim + first_value);
+    values = *reinterpret_cast<const uint2*>(v + (min(mine, last) * value_step + 2 * (r & 12)));
+  };
+  const auto fetch_solve = [&]() {
+    const char* const block = space.value_block(row, w.head);
+    const uint4* p = reinterpret_cast<const uint4*>(block + kSolve);
+    factors = reinterpret_cast<const f32x4*>(block)[mine];
+#pragma unroll
+    for (int step = 0; step < 2; ++step) {  // rows 0..31 have no second step
+      const int tile = lower_tile(wave, step < steps ? step : 0);
+#pragma unroll
+      for (int u = 0; u < 3; ++u) solve[step][u] = p[(u * kTriangle + tile) * 64 + lane];
+    }
+  };
+  const auto fetch_columns = [&]() {
+    const uint4* k =
+        reinterpret_cast<const uint4*>(space.key_block(row, key_head) + kKeyColumns);
+#pragma unroll
+    for (int step = 0; step < 2; ++step) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        k_columns[u][step] = k[(2 * (2 * wave + u) + step) * 64 + lane];
+      }
+    }
+  };
+  if (chunks != 0) {
+    fetch_keys();
+    fetch_solve();
+  }
+
+  for (uint32_t c = 0; c < chunks; ++c) {
+    {  // S0, cut into parts
+      uint4 part[3];
+      split3(state[0], state[1], part);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) state_parts[wave][p][lane] = part[p];
+      if constexpr (kTrain) {
+        float* p = space.state(row, w.head) + (32 * wave + 8 * g) * kDim + value;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[i * kDim] = state[0][i];
+          p[(4 + i) * kDim] = state[1][i];
+        }
+      }
+    }
+    float* const e = kTrain ? space.errors(row, w.head) : nullptr;
+    exchange();
+    // R = V - exp(G) K S0.  An exchange's values are all asked for before the first
+    // is used, and the operands two products ahead (of the next chunk, where this one
+    // has no more) are asked for while those are on their way: a wavefront's loads
+    // go out one every 16 cycles of the compute unit, and nothing behind them moves.
+    uint4 part_s[4][3];
+#pragma unroll
+    for (int p = 2; p >= 0; --p) {
+#pragma unroll
+      for (int step = 0; step < 4; ++step) part_s[step][p] = state_parts[step][p][lane];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_columns();
+    advance(c);
+    __builtin_amdgcn_sched_barrier(0);
+    const f32x4 read_key = of_rows(factors[kReadKey]), strength = of_rows(factors[kStrength]);
+    const f32x4 write = of_rows(factors[kWrite]), v = value_rows(values, lane);
+    f32x4 seen[2] = {};  // two sums, so that each product waits for the last but one
+#pragma unroll
+    for (int p = 2; p >= 0; --p) {
+#pragma unroll
+      for (int step = 0; step < 4; ++step) {
+        seen[step & 1] = mfma(k_rows[step], part_s[step][p], seen[step & 1]);
+      }
+    }
+    f32x4 error, scaled;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      error[i] = fmaf(-read_key[i], seen[0][i] + seen[1][i], v[i]);
+      scaled[i] = strength[i] * error[i];
+    }
+    uint2 half[3];
+    split3_half(scaled, half);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      reinterpret_cast<uint2*>(&row_parts[wave >> 1][p][lane])[wave & 1] = half[p];
+    }
+    exchange();
+    // E = R + N (b R)
+    uint4 part_r[2][3];
+#pragma unroll
+    for (int p = 2; p >= 0; --p) {
+#pragma unroll
+      for (int step = 0; step < 2; ++step) part_r[step][p] = row_parts[step][p][lane];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_keys();
+    __builtin_amdgcn_sched_barrier(0);
+    if (steps == 2) {
+      f32x4 more = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int v = 2; v >= 0; --v) {  // parts u and v with u + v <= 2
+#pragma unroll
+        for (int u = 2 - v; u >= 0; --u) {
+          error = mfma(solve[0][u], part_r[0][v], error);
+          more = mfma(solve[1][u], part_r[1][v], more);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) error[i] += more[i];
+    } else {
+      error = mfma6(solve[0], part_r[0], error);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) scaled[i] = write[i] * error[i];
+    split3_half(scaled, half);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) {
+      reinterpret_cast<uint2*>(&written_parts[wave >> 1][p][lane])[wave & 1] = half[p];
+    }
+    split3_half(error, half);
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      reinterpret_cast<uint2*>(&error_parts[wave >> 1][p][lane])[wave & 1] = half[p];
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) state[t][i] *= factors[kWhole];
+    }
+    exchange();
+    // S1 = exp(G_63) S0 + K^T (write b E)
+    uint4 part_w[2][3];
+#pragma unroll
+    for (int p = 2; p >= 0; --p) {
+#pragma unroll
+      for (int step = 0; step < 2; ++step) part_w[step][p] = written_parts[step][p][lane];
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_solve();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int p = 2; p >= 0; --p) {
+#pragma unroll
+      for (int step = 0; step < 2; ++step) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          state[u] = mfma(k_columns[u][step], part_w[step][p], state[u]);
+        }
+      }
+    }
+    if constexpr (kTrain) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[(16 * wave + 4 * g + i) * kDim + value] = error[i];
+    }
+  }
+  store_state(static_cast<Pool*>(args.final_states) + w.tile, 2 * wave, value, g, state);
+}
+
+template <typename Pool, bool kTrain>
+int32_t scan_by_size(void* stream, const ScanArgs& args) {
   const uint64_t items = static_cast<uint64_t>(args.rule.requests) * args.rule.space.value_heads;
-  const uint64_t blocks = (items + 7) / 8 * 8 * kSlices;
+  // A compute unit runs one narrow workgroup at a time; where they all run at once, a
+  // chunk takes 2.0 us (32 heads of one request), in the wide form 4.1 us.  From twice
+  // as many on, two rounds of the one are no faster than one of the other, which
+  // issues an eighth of the loads.
+  const bool narrow = items * (kDim / 16) <= 256;
+  const uint64_t blocks = (items + 7) / 8 * 8 * (narrow ? kDim / 16 : kWideSlices);
   if (blocks > kMaxGrid) return kStatusInvalidArgument;
-  return launch(delta_scan_kernel<Pool, kWaves, kTrain>, dim3(static_cast<uint32_t>(blocks)),
-                dim3(64 * kWaves), stream, args);
+  const dim3 grid(static_cast<uint32_t>(blocks));
+  return narrow ? launch(delta_scan_narrow_kernel<Pool, kTrain>, grid, dim3(512), stream, args)
+                : launch(delta_scan_wide_kernel<Pool, kTrain>, grid, dim3(64 * kWideWaves), stream,
+                         args);
 }
 
 }  // namespace
 
 int32_t launch_delta_scan(void* stream, const ScanArgs& args, uint32_t dtype) {
-  if (args.rule.space.train) return launch_scan<float, 4, true>(stream, args);
-  return dtype == kDtypeF32 ? launch_scan<float, 4, false>(stream, args)
-                            : launch_scan<bf16_bits, 4, false>(stream, args);
+  if (args.rule.space.train) return scan_by_size<float, true>(stream, args);
+  return dtype == kDtypeF32 ? scan_by_size<float, false>(stream, args)
+                            : scan_by_size<bf16_bits, false>(stream, args);
 }
+
+constexpr uint64_t kMaxStride = 1u << 24;  // elements between tokens
 
 // Checks the caller's arguments and fills the kernels'; false: a bad argument.
 bool rule_args(const gdn_state_codec_rule* rule, bool train, RuleArgs& a) {
@@ -294,6 +664,9 @@ bool rule_args(const gdn_state_codec_rule* rule, bool train, RuleArgs& a) {
       rule->tokens > 0x7FFFFFFFu || rule->rows != rule->tokens / kChunk + rule->requests ||
       rule->key_heads == 0 || rule->value_heads == 0 ||
       rule->value_heads % rule->key_heads != 0 || rule->normalize > 1 ||
+      // a chunk's rows are addressed with 32-bit byte offsets
+      rule->query_stride > kMaxStride || rule->key_stride > kMaxStride ||
+      rule->value_stride > kMaxStride || rule->value_heads > kMaxStride / kDim ||
       rule->query_stride % 8 != 0 || rule->key_stride % 8 != 0 || rule->value_stride % 8 != 0 ||
       static_cast<uint64_t>(rule->rows) * rule->value_heads > kMaxGrid ||
       !aligned16(rule->queries, rule->keys, rule->values, rule->log_decay, rule->beta,

@@ -24,13 +24,18 @@ QUERY_SCALE = DIM ** -0.5
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 
 
+# The current stream's handle, without the Stream object around it: a decode step
+# is a few microseconds of host work, and this is asked for on every call.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+
+
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    return _raw_stream(_current_device())
 
 
-def _require(condition: bool, message: str) -> None:
-    if not condition:
-        raise RuntimeError(f"GDN State Codec {message}")
+def _fail(message: str) -> None:
+    raise RuntimeError(f"GDN State Codec {message}")
 
 
 def _launched(status: int, what: str) -> None:
@@ -38,17 +43,21 @@ def _launched(status: int, what: str) -> None:
         raise RuntimeError(f"GDN State Codec {what} launch failed: {status}")
 
 
+# Messages are put together only when a check fails: formatting a tensor's shape
+# and strides costs more than the whole call.
+
 def _on_device(t: torch.Tensor, name: str) -> None:
-    _require(t.is_cuda and t.get_device() == torch.cuda.current_device(),
-             f"{name} must be on the current GPU")
+    if t.get_device() != _current_device():
+        _fail(f"{name} must be on the current GPU")
 
 
 def _dense(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype) -> None:
     """A contiguous tensor of exactly this shape and type, on the current GPU."""
-    _require(t.dtype == dtype and t.shape == shape and t.is_contiguous(),
-             f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}, got "
-             f"{t.dtype} {tuple(t.shape)} with strides {tuple(t.stride())}")
-    _on_device(t, name)
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
+        _fail(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)}, got "
+              f"{t.dtype} {tuple(t.shape)} with strides {tuple(t.stride())}")
+    if t.get_device() != _current_device():
+        _fail(f"{name} must be on the current GPU")
 
 
 class RequestTables(NamedTuple):
@@ -71,19 +80,20 @@ def request_tables(lengths: torch.Tensor, slot_ids: torch.Tensor,
     ``max_tokens``-row buffer, from device int32 ``lengths`` and ``slot_ids`` [N]
     (N in 1..4096; slot -1: padding).  A negative length counts as 0, and tokens
     past ``max_tokens`` are cut off."""
-    _require(lengths.dim() == 1 and 1 <= lengths.numel() <= MAX_REQUESTS,
-             f"request lengths must be [1..{MAX_REQUESTS}]")
     n = lengths.numel()
+    if lengths.dim() != 1 or not 1 <= n <= MAX_REQUESTS:
+        _fail(f"request lengths must be [1..{MAX_REQUESTS}]")
     _dense(lengths, "request lengths", (n,), torch.int32)
     _dense(slot_ids, "request slot ids", (n,), torch.int32)
-    _require(0 <= max_tokens < 2 ** 31, "request tables' max_tokens must be in 0..2^31-1")
+    if not 0 <= max_tokens < 2 ** 31:
+        _fail("request tables' max_tokens must be in 0..2^31-1")
     rows = table_rows(max_tokens, n)
     # One allocation; each table starts on a 16-byte boundary.
-    step = (n + 4) // 4 * 4
-    buffer = torch.empty(4 * rows + 3 * step, dtype=torch.int32, device=lengths.device)
-    chunks, offsets, chunk_offsets, order = buffer.split((4 * rows, step, step, step))
-    tables = RequestTables(offsets[:n + 1], chunk_offsets[:n + 1], chunks.view(rows, 4),
-                           order[:n])
+    buffer = torch.empty(4 * rows + 2 * (n // 4 * 4 + 4) + n, dtype=torch.int32,
+                         device=lengths.device)
+    chunks, offsets, _, chunk_offsets, _, order = buffer.split_with_sizes(
+        (4 * rows, n + 1, 3 - n % 4, n + 1, 3 - n % 4, n))
+    tables = RequestTables(offsets, chunk_offsets, chunks.view(rows, 4), order)
     _launched(native().request_tables_launch_v1(
         _stream(), lengths.data_ptr(), slot_ids.data_ptr(), n, max_tokens, rows,
         tables.offsets.data_ptr(), tables.chunk_offsets.data_ptr(), tables.chunks.data_ptr(),
@@ -97,15 +107,16 @@ def _token_rows(t: torch.Tensor, name: str, tokens: int) -> int:
     """Checks bf16 [tokens,heads,128] whose heads are packed; the distance between
     tokens may be any multiple of 8 elements (a slice of a fused projection).
     Returns that distance."""
-    _require(t.dtype == torch.bfloat16 and t.dim() == 3 and t.shape[0] == tokens
-             and t.shape[1] > 0 and t.shape[2] == DIM,
-             f"{name} must be bf16 [{tokens},heads,128], got {t.dtype} {tuple(t.shape)}")
+    shape, (step, head_step, one) = t.shape, t.stride() if t.dim() == 3 else (0, 0, 0)
+    if t.dtype is not torch.bfloat16 or len(shape) != 3 or shape[0] != tokens or \
+            shape[1] < 1 or shape[2] != DIM:
+        _fail(f"{name} must be bf16 [{tokens},heads,128], got {t.dtype} {tuple(shape)}")
     _on_device(t, name)
-    stride = t.stride(0) if tokens > 1 else t.shape[1] * DIM
-    _require(t.stride(2) == 1 and (t.shape[1] == 1 or t.stride(1) == DIM) and stride % 8 == 0
-             and stride >= t.shape[1] * DIM,
-             f"{name} must hold whole [heads,128] rows a multiple of 8 elements apart, got "
-             f"strides {tuple(t.stride())}")
+    width = shape[1] * DIM
+    stride = step if tokens > 1 else width
+    if one != 1 or (head_step != DIM and shape[1] != 1) or stride % 8 or stride < width:
+        _fail(f"{name} must hold whole [heads,128] rows a multiple of 8 elements apart, got "
+              f"strides {tuple(t.stride())}")
     return stride
 
 
@@ -115,17 +126,18 @@ def _rule_inputs(queries, keys, values, log_decay, beta):
     strides = (_token_rows(queries, "queries", tokens), _token_rows(keys, "keys", tokens),
                _token_rows(values, "values", tokens))
     heads, key_heads = values.shape[1], keys.shape[1]
-    _require(queries.shape[1] == key_heads and heads % key_heads == 0,
-             "queries and keys must have as many heads, and values a multiple of them")
+    if queries.shape[1] != key_heads or heads % key_heads:
+        _fail("queries and keys must have as many heads, and values a multiple of them")
     _dense(log_decay, "log decay", (tokens, heads), torch.float32)
     _dense(beta, "beta", (tokens, heads), torch.bfloat16)
     return tokens, heads, key_heads, strides
 
 
 def _pool(pool: torch.Tensor, heads: int) -> int:
-    _require(pool.dtype in _TYPES and pool.dim() == 4 and pool.shape[0] > 0
-             and tuple(pool.shape[1:]) == (heads, DIM, DIM) and pool.is_contiguous(),
-             f"state pool must be contiguous fp32 or bf16 [slots,{heads},128 value,128 key]")
+    if pool.dtype not in _TYPES or pool.dim() != 4 or pool.shape[0] < 1 or \
+            pool.shape[1:] != (heads, DIM, DIM) or not pool.is_contiguous():
+        _fail(f"state pool must be contiguous fp32 or bf16 [slots,{heads},128 value,128 key], "
+              f"got {pool.dtype} {tuple(pool.shape)}")
     _on_device(pool, "state pool")
     return _TYPES[pool.dtype]
 
@@ -161,7 +173,8 @@ def gated_delta_step(queries: torch.Tensor, keys: torch.Tensor, values: torch.Te
 def _check_tables(tables: RequestTables, tokens: int) -> int:
     """Checks that the tables are a batch's of `tokens` token rows; returns N."""
     requests = tables.order.numel()
-    _require(1 <= requests <= MAX_REQUESTS, f"tables must hold 1..{MAX_REQUESTS} requests")
+    if not 1 <= requests <= MAX_REQUESTS:
+        _fail(f"tables must hold 1..{MAX_REQUESTS} requests")
     for t, name, shape in ((tables.offsets, "offsets", (requests + 1,)),
                            (tables.chunk_offsets, "chunk_offsets", (requests + 1,)),
                            (tables.chunks, "chunks", (table_rows(tokens, requests), 4)),
@@ -185,9 +198,9 @@ def _rule(queries, keys, values, log_decay, beta, tables, scale, normalize, work
     if workspace is None:
         workspace = torch.empty(needed, dtype=torch.uint8, device=values.device)
     else:
-        _require(workspace.dtype == torch.uint8 and workspace.is_contiguous()
-                 and workspace.numel() >= needed,
-                 f"workspace must be contiguous uint8 of at least {needed} bytes")
+        if workspace.dtype is not torch.uint8 or not workspace.is_contiguous() or \
+                workspace.numel() < needed:
+            _fail(f"workspace must be contiguous uint8 of at least {needed} bytes")
         _on_device(workspace, "workspace")
     rule = RuleStruct(queries.data_ptr(), keys.data_ptr(), values.data_ptr(),
                       log_decay.data_ptr(), beta.data_ptr(), *strides,
@@ -293,9 +306,9 @@ def gated_delta_rule(queries: torch.Tensor, keys: torch.Tensor, values: torch.Te
 # ------------------------------------------------------------------ the norms
 
 def _rows_of(t: torch.Tensor, name: str, width: int) -> int:
-    _require(t.dtype in _TYPES and t.dim() >= 1 and t.shape[-1] == width and t.is_contiguous(),
-             f"{name} must be contiguous fp32 or bf16 [...,{width}], got {t.dtype} "
-             f"{tuple(t.shape)}")
+    if t.dtype not in _TYPES or t.shape[-1] != width or not t.is_contiguous():
+        _fail(f"{name} must be contiguous fp32 or bf16 [...,{width}], got {t.dtype} "
+              f"{tuple(t.shape)}")
     _on_device(t, name)
     return t.numel() // width
 
@@ -344,10 +357,12 @@ def gated_norm(x: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor,
 
     x and gate [...,128] of one type (bf16 or fp32), weight fp32 [128]; the result
     has x's type.  Differentiable in all three."""
+    if x.dim() < 1:
+        _fail("gated norm input must have a last dimension of 128")
     _rows_of(x, "gated norm input", DIM)
+    if gate.shape != x.shape or gate.dtype is not x.dtype:
+        _fail("gate must have the input's shape and type")
     _rows_of(gate, "gate", DIM)
-    _require(gate.shape == x.shape and gate.dtype == x.dtype,
-             "gate must have the input's shape and type")
     _dense(weight, "gated norm weight", (DIM,), torch.float32)
     if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad
                                     or weight.requires_grad):
@@ -407,13 +422,15 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
     x [...,D] and residual [...,D] bf16 or fp32 (each its own), weight fp32 [D], D
     a multiple of 8 up to 16384.  The norm is of the stored (rounded) sum.
     Differentiable in x, residual and weight."""
-    _require(x.dim() >= 1, "residual norm input must have a last dimension")
+    if x.dim() < 1:
+        _fail("residual norm input must have a last dimension")
     width = x.shape[-1]
-    _require(width % 8 == 0 and 0 < width <= 16384,
-             "residual norm width must be a multiple of 8 up to 16384")
+    if width % 8 or not 0 < width <= 16384:
+        _fail("residual norm width must be a multiple of 8 up to 16384")
     _rows_of(x, "residual norm input", width)
+    if residual.shape != x.shape:
+        _fail("the residual stream must have the input's shape")
     _rows_of(residual, "residual stream", width)
-    _require(residual.shape == x.shape, "the residual stream must have the input's shape")
     _dense(weight, "residual norm weight", (width,), torch.float32)
     if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad
                                     or weight.requires_grad):
