@@ -346,6 +346,11 @@ __device__ __forceinline__ float sum16(float x) {  // over the 16 lanes of a DPP
   return add_partner<8>(x);
 }
 
+// By value: a choice between elements of an array would put it into memory.
+__device__ __forceinline__ uint4 pick(bool first, uint4 x, uint4 y) {
+  return make_uint4(first ? x.x : y.x, first ? x.y : y.y, first ? x.z : y.z, first ? x.w : y.w);
+}
+
 struct Gradient {
   // X and E cut into parts, 16 tiles a part; then the four kinds of F and H, 6 tiles
   // a part.
@@ -408,6 +413,11 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
   f32x4 d_q[2][2] = {}, d_k[2][2] = {};  // [state tile 2 pair + c][token tile 2 half + i]
   for (uint32_t member = 0; member < a.group; ++member) {
     const uint32_t value_head = head * a.group + member;
+    // Taken afresh for each head: the addresses that follow from it would otherwise
+    // be kept over the loop, in more registers than there are.
+    int lane = t & 63;
+    asm volatile("" : "+v"(lane));
+    const int r = lane & 15, g = lane >> 4;
     const float* const s0 = space.state(row, value_head);
     const float* const s1 = space.state_gradient(row, value_head);
     const float* const errors = space.errors(row, value_head);
@@ -421,17 +431,15 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
       x[u][0] = load4(xs + at), x[u][1] = load4(xs + at + 4);
       e[u][0] = load4(errors + at), e[u][1] = load4(errors + at + 4);
     }
-    f32x4 start[4][2], grad[4][2];  // S0's and dS1's rows of a tile of keys
-    const auto load_rows = [&](const float* state, int c, f32x4 (&rows)[4][2]) {
+    f32x4 cells[4][2];  // S0's or dS1's rows of a tile of keys
+    const auto load_rows = [&](const float* state, int c) {
       const float* p = state + state_key(2 * pair + c, r) * kDim + 8 * g;
 #pragma unroll
       for (int step = 0; step < 4; ++step) {
-        rows[step][0] = load4(p + 32 * step);
-        rows[step][1] = load4(p + 32 * step + 4);
+        cells[step][0] = load4(p + 32 * step);
+        cells[step][1] = load4(p + 32 * step + 4);
       }
     };
-    load_rows(s0, 0, start);
-    load_rows(s1, 0, grad);
     if (member != 0) __syncthreads();  // the last head's values have been read
     {  // dO as an operand over the values: rows past the end repeat the last, and
        // meet rows of K and Q that are zeros
@@ -503,22 +511,17 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
       }
     }
 
-    // S0 dO, S0 X and dS1 E of this wavefront's keys and tokens.
+    // S0 dO and S0 X, then dS1 E, of this wavefront's keys and tokens; the rows of the
+    // next tile of keys come while this one's products are formed.
     f32x4 read_q[2][2] = {}, read_k[2][2] = {}, written[2][2] = {};
-    float end = 0.0f;
+    load_rows(s0, 0);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       uint4 part[4][3];
 #pragma unroll
-      for (int step = 0; step < 4; ++step) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          end = fmaf(start[step][0][j], grad[step][0][j],
-                     fmaf(start[step][1][j], grad[step][1][j], end));
-        }
-        split_row(start[step], part[step]);
-      }
-      if (c == 0) load_rows(s0, 1, start);
+      for (int step = 0; step < 4; ++step) split_row(cells[step], part[step]);
+      load_rows(c == 0 ? s0 : s1, c == 0 ? 1 : 0);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -531,9 +534,15 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
           read_k[c][i] = mfma6(x_part, part[step], read_k[c][i]);
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
+    }
 #pragma unroll
-      for (int step = 0; step < 4; ++step) split_row(grad[step], part[step]);
-      if (c == 0) load_rows(s1, 1, grad);
+    for (int c = 0; c < 2; ++c) {
+      uint4 part[4][3];
+#pragma unroll
+      for (int step = 0; step < 4; ++step) split_row(cells[step], part[step]);
+      if (c == 0) load_rows(s1, 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -545,9 +554,20 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
           written[c][i] = mfma6(e_part, part[step], written[c][i]);
         }
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
-    // Both halves of the tokens hold these keys; one of them counts.
-    end = half == 0 ? end * s.factors[kWhole] : 0.0f;
+    // <dS1, S0>, an eighth of the cells a wavefront
+    float end = 0.0f;
+    {
+      const uint32_t from = wave * (kTile / 8) + 4 * lane;
+#pragma unroll
+      for (int i = 0; i < kTile / 8; i += 256) {
+        const f32x4 x = load4(s0 + from + i), y = load4(s1 + from + i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) end = fmaf(x[j], y[j], end);
+      }
+      end *= s.factors[kWhole];
+    }
     __syncthreads();  // f and h are whole, X's and E's parts have been read
 
     // The four kinds, six units each: F and H by rows (over the tokens before), their
@@ -597,8 +617,8 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
     float cells_k[2][8], cells_q[2][8];  // of the token tiles: 4 i + j
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      widen8(half == 0 ? k_columns[c][0] : k_columns[c][1], cells_k[c]);
-      widen8(half == 0 ? q_columns[c][0] : q_columns[c][1], cells_q[c]);
+      widen8(pick(half == 0, k_columns[c][0], k_columns[c][1]), cells_k[c]);
+      widen8(pick(half == 0, q_columns[c][0], q_columns[c][1]), cells_q[c]);
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
