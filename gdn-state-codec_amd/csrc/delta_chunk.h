@@ -149,6 +149,13 @@ struct ChunkSpace {
     return state(row, head) + 2 * kTile + kChunk * kDim;
   }
 };
+// The two inputs that are read element by element, which a slice of a batch may
+// start anywhere.
+inline bool element_aligned(const float* log_decay, const bf16_bits* beta) {
+  return reinterpret_cast<uintptr_t>(log_decay) % sizeof(float) == 0 &&
+         reinterpret_cast<uintptr_t>(beta) % sizeof(bf16_bits) == 0;
+}
+
 struct RuleArgs {
   const bf16_bits* queries;
   const bf16_bits* keys;

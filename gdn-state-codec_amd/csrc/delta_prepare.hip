@@ -374,7 +374,9 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(RuleArgs a,
     const uint32_t value_head = head * a.group + member;
     char* const block = a.space.value_block(row, value_head);
     const uint64_t at = (first + lane) * a.space.value_heads + value_head;
-    double total = lane < count ? static_cast<double>(a.log_decay[at]) * kInverseLn2 : 0.0;
+    // exp of anything below -10000 is 0; a sum of -inf would leave no differences.
+    const float g = lane < count ? a.log_decay[at] : 0.0f;
+    double total = static_cast<double>(g < -1.0e4f ? -1.0e4f : g) * kInverseLn2;
     const float strength = lane < count ? widen(a.beta[at]) : 0.0f;
 #pragma unroll
     for (int step = 1; step < 64; step <<= 1) {

@@ -669,8 +669,8 @@ bool rule_args(const gdn_state_codec_rule* rule, bool train, RuleArgs& a) {
       rule->value_stride > kMaxStride || rule->value_heads > kMaxStride / kDim ||
       rule->query_stride % 8 != 0 || rule->key_stride % 8 != 0 || rule->value_stride % 8 != 0 ||
       static_cast<uint64_t>(rule->rows) * rule->value_heads > kMaxGrid ||
-      !aligned16(rule->queries, rule->keys, rule->values, rule->log_decay, rule->beta,
-                 rule->offsets, rule->chunk_offsets, rule->chunks, rule->order,
+      !element_aligned(rule->log_decay, rule->beta) ||
+      !aligned16(rule->queries, rule->keys, rule->values, rule->offsets, rule->chunk_offsets, rule->chunks, rule->order,
                  rule->workspace)) {
     return false;
   }

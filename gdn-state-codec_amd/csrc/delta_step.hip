@@ -186,7 +186,8 @@ extern "C" int32_t statecentric_gdn_state_codec_gated_delta_step_launch_v1(
       batch == 0 || slots == 0 || key_heads == 0 || value_heads == 0 ||
       value_heads % key_heads != 0 || slots > 0x7FFFFFFFu || pool_dtype > gdn::kDtypeBF16 ||
       normalize > 1 || query_stride % 8 != 0 || key_stride % 8 != 0 || value_stride % 8 != 0 ||
-      !gdn::aligned16(queries, keys, values, log_decay, beta, pool, slot_ids, outputs)) {
+      !gdn::element_aligned(log_decay, beta) ||
+      !gdn::aligned16(queries, keys, values, pool, slot_ids, outputs)) {
     return gdn::kStatusInvalidArgument;
   }
   const gdn::StepArgs args{queries, keys, values, log_decay, beta, pool, slot_ids, outputs,

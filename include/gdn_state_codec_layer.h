@@ -21,7 +21,8 @@
  *
  * Same conventions as gdn_state_codec_kernel.h: asynchronous on `stream` (NULL
  * = HIP's null stream), no allocation, status 0 / 1 (bad argument) / 5 (launch
- * failed), and every device pointer 16-byte aligned.
+ * failed), and every device pointer 16-byte aligned but log_decay and beta, which
+ * need their element's alignment only (a slice of a batch may start anywhere).
  */
 #ifndef GDN_STATE_CODEC_LAYER_H
 #define GDN_STATE_CODEC_LAYER_H
