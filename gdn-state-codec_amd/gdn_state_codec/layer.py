@@ -60,6 +60,12 @@ def _dense(t: torch.Tensor, name: str, shape: tuple, dtype: torch.dtype) -> None
         _fail(f"{name} must be on the current GPU")
 
 
+def _once() -> None:
+    """In a backward pass: there is no gradient of the gradients."""
+    if torch.is_grad_enabled():
+        _fail("layer operators cannot be differentiated twice")
+
+
 class RequestTables(NamedTuple):
     """The device tables of a ragged batch of N requests (all int32)."""
 
@@ -265,18 +271,17 @@ class _GatedDeltaRule(torch.autograd.Function):
         return out, final
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_out, d_final):
+        _once()
         queries, keys, values, log_decay, beta = ctx.saved_tensors[:5]
         rule = ctx.rule
         shape = (rule.requests, rule.value_heads, DIM, DIM)
         if d_out is None:
             d_out = torch.zeros(values.shape, dtype=torch.bfloat16, device=values.device)
-        d_out = d_out.to(torch.bfloat16).contiguous()
+        d_out = _given(d_out, torch.bfloat16)
         if d_final is not None:
-            d_final = d_final.to(torch.float32).contiguous()
-        new = lambda t: torch.empty(t.shape, dtype=t.dtype, device=t.device)  # noqa: E731
-        grads = [new(t) for t in (queries, keys, values, log_decay, beta)]
+            d_final = _given(d_final, torch.float32)
+        grads = [t.new_empty(t.shape) for t in (queries, keys, values, log_decay, beta)]
         d_initial = (torch.empty(shape, dtype=torch.float32, device=values.device)
                      if ctx.resumed else None)
         _launched(native().gated_delta_backward_launch_v1(
@@ -313,9 +318,15 @@ def _rows_of(t: torch.Tensor, name: str, width: int) -> int:
     return t.numel() // width
 
 
-def _partials(rows: int, width: int, device) -> torch.Tensor:
-    return torch.empty((native().norm_partials_v1(rows, width), width), dtype=torch.float32,
-                       device=device)
+def _given(d: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """An output's gradient as the kernels read it."""
+    return d if d.dtype is dtype and d.is_contiguous() else d.to(dtype).contiguous()
+
+
+def _weight_sums(weight: torch.Tensor, rows: int):
+    """The weight's gradient and the scratch its sum goes through."""
+    parts = native().norm_partials_v1(rows, weight.numel())
+    return torch.empty_like(weight), weight.new_empty(parts * weight.numel())
 
 
 def _gated_norm(x, gate, weight, eps: float) -> torch.Tensor:
@@ -335,18 +346,19 @@ class _GatedNorm(torch.autograd.Function):
         return _gated_norm(x, gate, weight, eps)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
+        _once()
         x, gate, weight = ctx.saved_tensors
         rows = x.numel() // DIM
-        d_out = d_out.to(x.dtype).contiguous()
-        d_x, d_gate, d_weight = torch.empty_like(x), torch.empty_like(x), torch.zeros_like(weight)
-        if rows:
-            _launched(native().gated_norm_backward_launch_v1(
-                _stream(), x.data_ptr(), gate.data_ptr(), weight.data_ptr(), d_out.data_ptr(),
-                d_x.data_ptr(), d_gate.data_ptr(), d_weight.data_ptr(),
-                _partials(rows, DIM, x.device).data_ptr(), rows, _TYPES[x.dtype], ctx.eps),
-                "gated norm backward")
+        d_x, d_gate = torch.empty_like(x), torch.empty_like(x)
+        if not rows:
+            return d_x, d_gate, torch.zeros_like(weight), None
+        d_out = _given(d_out, x.dtype)
+        d_weight, partials = _weight_sums(weight, rows)
+        _launched(native().gated_norm_backward_launch_v1(
+            _stream(), x.data_ptr(), gate.data_ptr(), weight.data_ptr(), d_out.data_ptr(),
+            d_x.data_ptr(), d_gate.data_ptr(), d_weight.data_ptr(), partials.data_ptr(), rows,
+            _TYPES[x.dtype], ctx.eps), "gated norm backward")
         return d_x, d_gate, d_weight, None
 
 
@@ -391,25 +403,23 @@ class _ResidualNorm(torch.autograd.Function):
         return out, total
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_out, d_total):
+        _once()
         total, weight = ctx.saved_tensors
-        width = total.shape[-1]
+        width = weight.numel()
         rows = total.numel() // width
-        d_out = (torch.zeros_like(total, dtype=ctx.dtype) if d_out is None
-                 else d_out.to(ctx.dtype).contiguous())
+        d_x, d_residual = torch.empty_like(total, dtype=ctx.dtype), torch.empty_like(total)
+        if not rows:
+            return d_x, d_residual, torch.zeros_like(weight), None, None
+        d_out = torch.zeros_like(d_x) if d_out is None else _given(d_out, ctx.dtype)
         if d_total is not None:
-            d_total = d_total.to(total.dtype).contiguous()
-        d_x, d_residual = torch.empty_like(d_out), torch.empty_like(total)
-        d_weight = torch.zeros_like(weight)
-        if rows:
-            _launched(native().residual_norm_backward_launch_v1(
-                _stream(), total.data_ptr(), weight.data_ptr(), d_out.data_ptr(),
-                0 if d_total is None else d_total.data_ptr(), d_x.data_ptr(),
-                d_residual.data_ptr(), d_weight.data_ptr(),
-                _partials(rows, width, total.device).data_ptr(), rows, width,
-                _TYPES[ctx.dtype], _TYPES[total.dtype], ctx.scale, ctx.eps),
-                "residual norm backward")
+            d_total = _given(d_total, total.dtype)
+        d_weight, partials = _weight_sums(weight, rows)
+        _launched(native().residual_norm_backward_launch_v1(
+            _stream(), total.data_ptr(), weight.data_ptr(), d_out.data_ptr(),
+            0 if d_total is None else d_total.data_ptr(), d_x.data_ptr(), d_residual.data_ptr(),
+            d_weight.data_ptr(), partials.data_ptr(), rows, width, _TYPES[ctx.dtype],
+            _TYPES[total.dtype], ctx.scale, ctx.eps), "residual norm backward")
         return d_x, d_residual, d_weight, None, None
 
 
