@@ -15,7 +15,7 @@
 //
 // Precision.  q, k, v and the outputs' gradients are bf16, exact as they are.
 // fp32 values enter v_mfma_f32_16x16x32_bf16 as three bf16 parts that sum to
-// them exactly (truncation: 8 significant bits each), so a product with a bf16
+// them exactly (8 significant bits each), so a product with a bf16
 // operand takes 3 instructions and loses nothing, and a product of two fp32
 // operands takes 6 (the parts left out are below 2^-24 of the product).
 // Accumulators, states, sums and factors are fp32; the decays' running sums are
@@ -184,19 +184,30 @@ __device__ __forceinline__ f32x4 mfma(const uint4& a, const uint4& b, const f32x
                                                  __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-__device__ __forceinline__ float upper(float x) {
-  return __uint_as_float(__float_as_uint(x) & 0xFFFF0000u);
-}
-
-// Three parts of a pair: each the upper half of what the ones before left over
-// (8 significant bits at a time, so the third is exact and their sum is x).
+// Three parts of a pair, each what the ones before left over, rounded to bf16.  The
+// rest x - part is v_dot2_f32_bf16 of the pair of parts with (-1, 0) or (0, -1), exact
+// like the subtraction (the rest of a rounding fits fp32), so that a pair takes 7
+// instructions; 8 significant bits a part leave nothing of fp32's 24 (checked over
+// 2^22 values of every size: what three parts miss is where the third would be a
+// denormal).  The two constants are kept in registers: as inline constants the
+// instruction reads them as fp32.  A value above the largest bf16 (0x1.fep127), an
+// infinity and a NaN make their pair's other value a NaN too, which the products they
+// enter would do anyway.
 __device__ __forceinline__ void split3_pair(float x, float y, uint32_t& a, uint32_t& b,
                                             uint32_t& c) {
-  a = upper_halves(__float_as_uint(x), __float_as_uint(y));
-  x -= upper(x), y -= upper(y);
-  b = upper_halves(__float_as_uint(x), __float_as_uint(y));
-  x -= upper(x), y -= upper(y);
-  c = upper_halves(__float_as_uint(x), __float_as_uint(y));
+  uint32_t first = 0x0000BF80u, second = 0xBF800000u;
+  asm("" : "+s"(first), "+s"(second));
+  const bf16x2_t minus_first = __builtin_bit_cast(bf16x2_t, first);
+  const bf16x2_t minus_second = __builtin_bit_cast(bf16x2_t, second);
+  bf16x2_t part = __builtin_convertvector((f32x2_t){x, y}, bf16x2_t);
+  a = __builtin_bit_cast(uint32_t, part);
+  x = __builtin_amdgcn_fdot2_f32_bf16(part, minus_first, x, false);
+  y = __builtin_amdgcn_fdot2_f32_bf16(part, minus_second, y, false);
+  part = __builtin_convertvector((f32x2_t){x, y}, bf16x2_t);
+  b = __builtin_bit_cast(uint32_t, part);
+  x = __builtin_amdgcn_fdot2_f32_bf16(part, minus_first, x, false);
+  y = __builtin_amdgcn_fdot2_f32_bf16(part, minus_second, y, false);
+  c = bf16_pair(x, y);
 }
 
 // The parts of 8 places of a contraction: two accumulator tiles, or 8 values.
@@ -280,6 +291,19 @@ __device__ __forceinline__ uint2 transpose_quad(const uint2& x, int lane) {
 __device__ __forceinline__ float decay_between(float sum_i, float rest_i, float sum_j,
                                                float rest_j) {
   return __builtin_amdgcn_exp2f((sum_i - sum_j) + (rest_i - rest_j));
+}
+
+// The same of fp32: from lane j's column j (rows 0..3) to its row j (columns 0..3).
+__device__ __forceinline__ f32x4 transpose_quad(const f32x4& x, int lane) {
+  const bool odd = (lane & 1) != 0, up = (lane & 2) != 0;
+  const float a = quad<kDppQuadSwap1>(odd ? x[0] : x[1]);
+  const float b = quad<kDppQuadSwap1>(odd ? x[2] : x[3]);
+  // rows (0 or 1) and (2 or 3), two columns each
+  const float u0 = odd ? a : x[0], u1 = odd ? x[1] : a;
+  const float v0 = odd ? b : x[2], v1 = odd ? x[3] : b;
+  const float c = quad<kDppQuadSwap2>(up ? u0 : v0);
+  const float d = quad<kDppQuadSwap2>(up ? u1 : v1);
+  return f32x4{up ? c : u0, up ? d : u1, up ? v0 : c, up ? v1 : d};
 }
 
 // One tile into LDS at `to` (bytes, the same for the wavefront), 16 bytes a lane at

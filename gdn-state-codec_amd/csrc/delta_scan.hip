@@ -150,54 +150,52 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void delta_scan_wide_kernel(Sca
   const uint32_t out_step = space.value_heads * kDim * 2;
   uint2 values[4];  // columns 4 (r / 4).. of tokens 16 t + 4 g + (r & 3)
   const uint32_t linear = 16 * lane;
-  const auto fetch_first = [&](uint32_t c) {
+  // Piece i of a chunk's first half (0..8; and 9..12, its rows of V) and of its second
+  // (0..10).  They are issued one by one between other work: the compute unit takes a
+  // tile about every 20 cycles, and a wavefront that issues several waits for them.
+  const auto fetch_first = [&](uint32_t c, int i) {
     const uint64_t token = w.begin + c * kChunk;
     const uint32_t last = min(length - c * kChunk, static_cast<uint32_t>(kChunk)) - 1;
-    const char* k = reinterpret_cast<const char*>(a.keys + token * a.key_stride +
-                                                  key_head * kDim);
-    const char* block = space.value_block(w.first_row + c, w.head);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {  // rows 16 t.., keys 32 wave..
-      const uint32_t row = min(static_cast<uint32_t>(16 * t + r), last);
+    if (i < 4) {  // K rows 16 i.., keys 32 wave..
+      const char* k = reinterpret_cast<const char*>(a.keys + token * a.key_stride +
+                                                    key_head * kDim);
+      const uint32_t row = min(static_cast<uint32_t>(16 * i + r), last);
       stage_tile(k + 64 * wave, row * key_step + 16 * g,
-                 stage_at + kStageKeys + (4 * t + wave) * kTileBytes);
-    }
-#pragma unroll
-    for (int i = 0; i < kBlockTiles / kWideWaves; ++i) {
-      const int tile = kWideWaves * i + wave;
-      stage_tile(block + tile * kTileBytes, linear, stage_at + tile * kTileBytes);
-    }
-    const char* v = reinterpret_cast<const char*>(a.values + token * a.value_stride +
-                                                  w.head * kDim + first_value);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const uint32_t row = min(static_cast<uint32_t>(16 * t + 4 * g + (r & 3)), last);
-      values[t] = *reinterpret_cast<const uint2*>(v + (row * value_step + 2 * (r & 12)));
+                 stage_at + kStageKeys + (4 * i + wave) * kTileBytes);
+    } else if (i < 9) {
+      const int tile = kWideWaves * (i - 4) + wave;
+      stage_tile(space.value_block(w.first_row + c, w.head) + tile * kTileBytes, linear,
+                 stage_at + tile * kTileBytes);
+    } else {
+      const char* v = reinterpret_cast<const char*>(a.values + token * a.value_stride +
+                                                    w.head * kDim + first_value);
+      const uint32_t row = min(static_cast<uint32_t>(16 * (i - 9) + 4 * g + (r & 3)), last);
+      values[i - 9] = *reinterpret_cast<const uint2*>(v + (row * value_step + 2 * (r & 12)));
     }
   };
-  const auto fetch_second = [&](uint32_t c) {
-    const uint64_t token = w.begin + c * kChunk;
-    const uint32_t last = min(length - c * kChunk, static_cast<uint32_t>(kChunk)) - 1;
-    const char* q = reinterpret_cast<const char*>(a.queries + token * a.query_stride +
-                                                  key_head * kDim);
-    const char* columns = space.key_block(w.first_row + c, key_head) + kKeyColumns;
-    const char* read = space.value_block(w.first_row + c, w.head) + kReadOut;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const uint32_t row = min(static_cast<uint32_t>(16 * t + r), last);
-      const int tile = 4 * t + wave;
+  const auto fetch_second = [&](uint32_t c, int i) {
+    if (i < 4) {  // Q rows 16 i.., keys 32 wave..
+      const uint64_t token = w.begin + c * kChunk;
+      const uint32_t last = min(length - c * kChunk, static_cast<uint32_t>(kChunk)) - 1;
+      const char* q = reinterpret_cast<const char*>(a.queries + token * a.query_stride +
+                                                    key_head * kDim);
+      const uint32_t row = min(static_cast<uint32_t>(16 * i + r), last);
       stage_tile(q + 64 * wave, row * query_step + 16 * g,
-                 stage_at + kStageQueries + tile * kTileBytes);
-      stage_tile(columns + tile * kTileBytes, linear,
-                 stage_at + kStageColumns + tile * kTileBytes);
-    }
-#pragma unroll
-    for (int i = 0; i < 2 * kTriangle / kWideWaves; ++i) {
-      const int tile = kWideWaves * i + wave;
-      stage_tile(read + tile * kTileBytes, linear, stage_at + kStageRead + tile * kTileBytes);
+                 stage_at + kStageQueries + (4 * i + wave) * kTileBytes);
+    } else if (i < 8) {
+      const int tile = kWideWaves * (i - 4) + wave;
+      stage_tile(space.key_block(w.first_row + c, key_head) + kKeyColumns + tile * kTileBytes,
+                 linear, stage_at + kStageColumns + tile * kTileBytes);
+    } else {
+      const int tile = kWideWaves * (i - 8) + wave;
+      stage_tile(space.value_block(w.first_row + c, w.head) + kReadOut + tile * kTileBytes,
+                 linear, stage_at + kStageRead + tile * kTileBytes);
     }
   };
-  if (chunks != 0) fetch_first(0);
+  if (chunks != 0) {
+#pragma unroll
+    for (int i = 0; i < 13; ++i) fetch_first(0, i);
+  }
 
   f32x4 error[4], out[4];
   const auto store_rows = [&](uint32_t c, int tokens) {
@@ -210,9 +208,8 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void delta_scan_wide_kernel(Sca
       const uint2 x = output_run(out[t], lane);
       if (token < tokens) *reinterpret_cast<uint2*>(o + (token * out_step + 2 * (r & 12))) = x;
       if constexpr (kTrain) {
-        float* e = space.errors(w.first_row + c, w.head) + value;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) e[(16 * t + 4 * g + i) * kDim] = error[t][i];
+        float* e = space.errors(w.first_row + c, w.head) + first_value + (r & 12);
+        *reinterpret_cast<f32x4*>(e + token * kDim) = transpose_quad(error[t], lane);
       }
     }
   };
@@ -234,20 +231,23 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void delta_scan_wide_kernel(Sca
       // Used before the next loads are issued, so that no wait for it covers them.
       asm volatile("" : "+v"(values[t].x), "+v"(values[t].y));
     }
-    fetch_second(c);
-    if (c != 0) store_rows(c - 1, kChunk);  // only the last chunk can be short
-    if constexpr (kTrain) {
-      float* p = space.state(w.first_row + c, w.head) + value;
-#pragma unroll
-      for (int t = 0; t < 8; ++t) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[state_key(t, 4 * g + i) * kDim] = state[t][i];
-      }
-    }
     uint4 part[4][3];  // of the state, over the keys
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
       split3(state[2 * step], state[2 * step + 1], part[step]);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 3 * step; i < min(3 * step + 3, 11); ++i) fetch_second(c, i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (c != 0) store_rows(c - 1, kChunk);  // only the last chunk can be short
+    if constexpr (kTrain) {
+      float* p = space.state(w.first_row + c, w.head) + first_value + (r & 12);
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        *reinterpret_cast<f32x4*>(p + state_key(t, 4 * g + (r & 3)) * kDim) =
+            transpose_quad(state[t], lane);
+      }
     }
     // R = V - exp(G) K S0
 #pragma unroll
@@ -290,7 +290,6 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void delta_scan_wide_kernel(Sca
       }
     }
     stage_ready();  // the second half is there, the first has been read
-    if (c + 1 < chunks) fetch_first(c + 1);
     // exp(G) Q S0 from two of the state's parts: 2^-15 of terms whose sums become
     // bf16 outputs.
 #pragma unroll
@@ -305,6 +304,12 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void delta_scan_wide_kernel(Sca
       const f32x4 read_query = of_rows(queries[t]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) out[t][i] = read_query[i] * (read[0][i] + read[1][i]);
+      if (c + 1 < chunks) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = t; i < 13; i += 4) fetch_first(c + 1, i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
     // S1 = exp(G_63) S0 + K^T (write b E), and O += (P b) E
 #pragma unroll
