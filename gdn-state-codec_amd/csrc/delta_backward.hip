@@ -42,24 +42,33 @@ struct BackArgs {
 };
 
 // A chunk's operands in LDS, in two halves, each fetched while the other is at work:
-// the factors (2 KiB), N^T and K rows; then K^T, Q^T and the first two parts of the
-// next chunk's P^T.  80 KiB, so that two workgroups share a compute unit; P^T's third
-// part goes to registers instead.
+// the factors (2 KiB), N^T, K rows and Q^T; then K^T and the next chunk's P^T and dO.
+// Beside them 48 KiB through which the chain and the wavefronts beside it hand each
+// other accumulators, each lane to the same lane: dS1 and, once that has been taken,
+// (exp(G) Q)^T dO; P^T dO and, once that has been taken, X.
 constexpr int kStageSolve = 2 * kTileBytes;
 constexpr int kStageKeys = kStageSolve + kTriangleBytes;
-constexpr int kStageColumns = kStageKeys + kKeyTiles * kTileBytes;
-constexpr int kStageRead = kStageColumns + 2 * kKeyTiles * kTileBytes;
-constexpr int kStage = kStageRead + 2 * kTriangle * kTileBytes;
-static_assert(kHeadFactors <= 2 * kTileBytes, "the factors' tiles");
-static_assert(workgroups_by_lds(kStage) == 2, "two workgroups share a compute unit");
+constexpr int kStageQueryColumns = kStageKeys + kKeyTiles * kTileBytes;
+constexpr int kStageColumns = kStageQueryColumns + kKeyTiles * kTileBytes;
+constexpr int kStageRead = kStageColumns + kKeyTiles * kTileBytes;
+constexpr int kStageOuts = kStageRead + kTriangleBytes;
 constexpr int kWaves = 4;
 constexpr int kSlices = kDim / (16 * kWaves);
+constexpr int kOutBytes = 32 * kWaves;  // of a token's dO
+constexpr int kStageState = kStageOuts + kChunk * kOutBytes;
+constexpr int kStageRows = kStageState + kWaves * 8 * kTileBytes;
+constexpr int kStage = kStageRows + kWaves * 4 * kTileBytes;
+static_assert(kHeadFactors <= 2 * kTileBytes, "the factors' tiles");
+static_assert(kStage <= kLdsPerCu, "a compute unit's LDS");
 
-__global__ __launch_bounds__(64 * kWaves, 2) void delta_back_scan_kernel(BackArgs args) {
+// A workgroup takes 64 columns, two wavefronts for each 16: one the chain, the other
+// the operands' loads, the two products that need no state, and the stores.
+__global__ __launch_bounds__(128 * kWaves) void delta_back_scan_kernel(BackArgs args) {
   __shared__ __align__(16) char stage[kStage];
   const RuleArgs& a = args.rule;
   const ChunkSpace& space = a.space;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int place = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = place % kWaves;
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const uint32_t turn = blockIdx.x >> 3;  // slices of a head on one XCD, as forward
   const uint64_t item = static_cast<uint64_t>(turn / kSlices) * 8 + (blockIdx.x & 7);
@@ -68,183 +77,231 @@ __global__ __launch_bounds__(64 * kWaves, 2) void delta_back_scan_kernel(BackArg
   const uint32_t key_head = head / a.group;
   const uint32_t request = static_cast<uint32_t>(a.order[item / space.value_heads]);
   if (request >= a.requests) return;
-  const int first_value = 16 * (kWaves * (turn % kSlices) + wave), value = first_value + r;
-  const uint64_t tile = (static_cast<uint64_t>(request) * space.value_heads + head) * kTile +
-                        value * kDim;
-
-  f32x4 state[8];  // the state's gradient, rows as in the forward scan
-#pragma unroll
-  for (int t = 0; t < 8; ++t) {
-    state[t] = args.d_final ? load4(args.d_final + tile + state_key(t, 4 * g))
-                            : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  }
-
+  const int slice = kWaves * (turn % kSlices) + wave;
   const uint32_t first_row = min(static_cast<uint32_t>(a.chunk_offsets[request]), space.rows);
   const uint32_t rows = min(static_cast<uint32_t>(a.chunk_offsets[request + 1]), space.rows) -
                         first_row;
   const uint32_t begin = min(static_cast<uint32_t>(a.offsets[request]), a.tokens);
   const uint32_t length = min(static_cast<uint32_t>(a.offsets[request + 1]), a.tokens) - begin;
   const uint32_t chunks = min(rows, (length + kChunk - 1) / kChunk);
-  const uint32_t stage_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
-      (__attribute__((address_space(3))) char*)&stage[0]));
-  const uint32_t key_step = static_cast<uint32_t>(a.key_stride) * 2;
-  const uint32_t out_step = space.value_heads * kDim * 2;
-  const uint32_t linear = 16 * lane;
+  f32x4* const state_cells =
+      reinterpret_cast<f32x4*>(stage + kStageState) + wave * 8 * 64 + lane;
+  f32x4* const row_cells = reinterpret_cast<f32x4*>(stage + kStageRows) + wave * 4 * 64 + lane;
+  const int own = 4 * g + (r & 3);  // a lane's token of each tile, where it has one
 
-  const auto fetch_first = [&](uint32_t c) {
-    const uint64_t token = begin + c * kChunk;
-    const uint32_t last = min(length - c * kChunk, static_cast<uint32_t>(kChunk)) - 1;
-    const char* k = reinterpret_cast<const char*>(a.keys + token * a.key_stride +
-                                                  key_head * kDim);
-    const char* block = space.value_block(first_row + c, head);
+  if (place >= kWaves) {
+    const uint32_t stage_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+        (__attribute__((address_space(3))) char*)&stage[0]));
+    const uint32_t key_step = static_cast<uint32_t>(a.key_stride) * 2;
+    const uint32_t out_step = space.value_heads * kDim * 2;
+    const uint32_t linear = 16 * lane;
+    const auto fetch_first = [&](uint32_t c) {
+      const uint64_t token = begin + c * kChunk;
+      const uint32_t last = min(length - c * kChunk, static_cast<uint32_t>(kChunk)) - 1;
+      const char* k = reinterpret_cast<const char*>(a.keys + token * a.key_stride +
+                                                    key_head * kDim);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {  // rows 16 t.., keys 32 wave..
-      const uint32_t row = min(static_cast<uint32_t>(16 * t + r), last);
-      stage_tile(k + 64 * wave, row * key_step + 16 * g,
-                 stage_at + kStageKeys + (4 * t + wave) * kTileBytes);
-    }
-#pragma unroll
-    for (int i = 0; i < 5; ++i) {
-      const int at = kWaves * i + wave;
-      const char* from = at < 2 ? block + at * kTileBytes
-                                : block + kSolveBack + (at - 2) * kTileBytes;
-      stage_tile(from, linear, stage_at + at * kTileBytes);
-    }
-  };
-  // The gradient of the outputs: columns 4 (r / 4).. of tokens 16 t + 4 g + (r & 3).
-  uint2 next_out[4];
-  uint4 read_low[kTriangle];  // P^T's third part
-  const auto fetch_read = [&](uint32_t c) {
-    const char* block = space.value_block(first_row + c, head) + kReadBack;
-#pragma unroll
-    for (int i = 0; i < 2 * kTriangle / kWaves; ++i) {
-      const int at = kWaves * i + wave;
-      stage_tile(block + at * kTileBytes, linear, stage_at + kStageRead + at * kTileBytes);
-    }
-#pragma unroll
-    for (int i = 0; i < kTriangle; ++i) {
-      read_low[i] = reinterpret_cast<const uint4*>(block + (2 * kTriangle + i) * kTileBytes)[lane];
-    }
-    const uint32_t last = min(length - c * kChunk, static_cast<uint32_t>(kChunk)) - 1;
-    const char* d = reinterpret_cast<const char*>(args.d_outputs) +
-                    (begin + static_cast<uint64_t>(c) * kChunk) * out_step +
-                    2 * (head * kDim + first_value);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const uint32_t row = min(static_cast<uint32_t>(16 * t + 4 * g + (r & 3)), last);
-      next_out[t] = *reinterpret_cast<const uint2*>(d + (row * out_step + 2 * (r & 12)));
-    }
-  };
-  const auto fetch_columns = [&](uint32_t c) {
-    const char* columns = space.key_block(first_row + c, key_head);
-#pragma unroll
-    for (int i = 0; i < 2 * kKeyTiles / kWaves; ++i) {
-      const int at = kWaves * i + wave;
-      stage_tile(columns + at * kTileBytes, linear, stage_at + kStageColumns + at * kTileBytes);
-    }
-  };
-  const uint4* const k_rows = reinterpret_cast<const uint4*>(stage + kStageKeys) + lane;
-  const uint4* const k_columns = reinterpret_cast<const uint4*>(stage + kStageColumns) + lane;
-  const uint4* const q_columns = k_columns + kKeyTiles * 64;
-  const uint4* const solve = reinterpret_cast<const uint4*>(stage + kStageSolve) + lane;
-  const uint4* const read_back = reinterpret_cast<const uint4*>(stage + kStageRead) + lane;
-
-  // dO of a chunk as an operand over its tokens (rows past its end are zeros), and
-  // P^T dO, which needs no state: both a chunk ahead of the state.
-  uint4 d_part[2];
-  f32x4 v[4];
-  const auto take_outputs = [&](uint32_t c) {
-    const int tokens = min(static_cast<int>(length - c * kChunk), kChunk);
-    uint2 x[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const bool live = 16 * t + 4 * g + (r & 3) < tokens;
-      x[t] = transpose_quad(make_uint2(live ? next_out[t].x : 0, live ? next_out[t].y : 0), lane);
-    }
-    d_part[0] = make_uint4(x[0].x, x[0].y, x[1].x, x[1].y);
-    d_part[1] = make_uint4(x[2].x, x[2].y, x[3].x, x[3].y);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      v[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int step = upper_first(t); step < 2; ++step) {
-        const int at = upper_tile(t, step);
-        v[t] = mfma(read_low[at], d_part[step], v[t]);
-        v[t] = mfma(read_back[(kTriangle + at) * 64], d_part[step], v[t]);
-        v[t] = mfma(read_back[at * 64], d_part[step], v[t]);
+      for (int i = 0; i < 4; ++i) {  // rows 16 i.., keys 32 wave..
+        const uint32_t row = min(static_cast<uint32_t>(16 * i + r), last);
+        stage_tile(k + 64 * wave, row * key_step + 16 * g,
+                   stage_at + kStageKeys + (4 * i + wave) * kTileBytes);
       }
-    }
-  };
-
-  if (chunks != 0) {
-    fetch_read(chunks - 1);
-    fetch_first(chunks - 1);
-    stage_ready();
-    take_outputs(chunks - 1);
-  }
-
-  f32x4 x[4];
-  uint2 y[4];
-  const auto store_rows = [&](uint32_t c, int tokens) {
-    float* e = space.error_gradient(first_row + c, head) + value;
-    char* d = reinterpret_cast<char*>(args.d_values) +
-              (begin + static_cast<uint64_t>(c) * kChunk) * out_step +
-              2 * (head * kDim + first_value);
+      const char* block = space.value_block(first_row + c, head);
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) e[(16 * t + 4 * g + i) * kDim] = x[t][i];
-      const int token = 16 * t + 4 * g + (r & 3);
-      const uint2 run = transpose_quad(y[t], lane);
-      if (token < tokens) *reinterpret_cast<uint2*>(d + (token * out_step + 2 * (r & 12))) = run;
-    }
-  };
-
-  for (uint32_t c = chunks; c-- > 0;) {
-    stage_ready();  // the first half is there, the second has been read
-    f32x4 factors[4];  // of tokens 16 t + 4 g + (r & 3)
-    float queries[4], carries[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int token = 16 * t + 4 * g + (r & 3);
-      factors[t] = reinterpret_cast<const f32x4*>(stage)[token];
-      queries[t] = reinterpret_cast<const float*>(stage)[kReadQuery + token];
-      carries[t] = reinterpret_cast<const float*>(stage)[kCarry + token];
-    }
-    fetch_columns(c);
-    if (c != 0) fetch_read(c - 1);
-    if (c + 1 != chunks) {
-      store_rows(c + 1, min(static_cast<int>(length - (c + 1) * kChunk), kChunk));
-    }
-    {
-      float* p = space.state_gradient(first_row + c, head) + value;
-#pragma unroll
-      for (int t = 0; t < 8; ++t) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[state_key(t, 4 * g + i) * kDim] = state[t][i];
+      for (int i = 0; i < 5; ++i) {
+        const int at = kWaves * i + wave;
+        const char* from = at < 2 ? block + at * kTileBytes
+                                  : block + kSolveBack + (at - 2) * kTileBytes;
+        stage_tile(from, linear, stage_at + at * kTileBytes);
       }
-    }
-    {
-      uint4 part[4][3];
+      const char* columns = space.key_block(first_row + c, key_head) + kQueryColumns;
 #pragma unroll
-      for (int step = 0; step < 4; ++step) {
-        split3(state[2 * step], state[2 * step + 1], part[step]);
+      for (int i = 0; i < kKeyTiles / kWaves; ++i) {
+        const int at = kWaves * i + wave;
+        stage_tile(columns + at * kTileBytes, linear,
+                   stage_at + kStageQueryColumns + at * kTileBytes);
       }
+    };
+    const auto fetch_columns = [&](uint32_t c) {
+      const char* columns = space.key_block(first_row + c, key_head) + kKeyColumns;
+#pragma unroll
+      for (int i = 0; i < kKeyTiles / kWaves; ++i) {
+        const int at = kWaves * i + wave;
+        stage_tile(columns + at * kTileBytes, linear, stage_at + kStageColumns + at * kTileBytes);
+      }
+    };
+    const auto fetch_read = [&](uint32_t c) {
+      const char* block = space.value_block(first_row + c, head) + kReadBack;
+#pragma unroll
+      for (int i = 0; i < (3 * kTriangle + kWaves - 1) / kWaves; ++i) {  // the last one twice
+        const int at = min(kWaves * i + wave, 3 * kTriangle - 1);
+        stage_tile(block + at * kTileBytes, linear, stage_at + kStageRead + at * kTileBytes);
+      }
+      const uint32_t last = min(length - c * kChunk, static_cast<uint32_t>(kChunk)) - 1;
+      const char* d = reinterpret_cast<const char*>(args.d_outputs) +
+                      (begin + static_cast<uint64_t>(c) * kChunk) * out_step +
+                      2 * (head * kDim) + kOutBytes * (turn % kSlices);
+      constexpr int kLanes = kOutBytes / 16, kRows = 64 / kLanes;  // of one tile
+#pragma unroll
+      for (int i = 0; i < kChunk / kRows / kWaves; ++i) {
+        const int at = kWaves * i + wave;
+        const uint32_t row = min(static_cast<uint32_t>(kRows * at + lane / kLanes), last);
+        stage_tile(d, row * out_step + 16 * (lane % kLanes),
+                   stage_at + kStageOuts + at * kTileBytes);
+      }
+    };
+    const uint4* const q_columns =
+        reinterpret_cast<const uint4*>(stage + kStageQueryColumns) + lane;
+    const uint4* const read_back = reinterpret_cast<const uint4*>(stage + kStageRead) + lane;
+    const char* const outs = stage + kStageOuts + own * kOutBytes + 32 * wave + 2 * (r & 12);
+
+    // dO of a chunk as an operand over its tokens (rows past its end are zeros), and
+    // P^T dO, which the chain takes.
+    uint4 d_part[2];
+    const auto take_outputs = [&](uint32_t c) {
+      const int tokens = min(static_cast<int>(length - c * kChunk), kChunk);
+      uint2 x[4];
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        f32x4 seen[2] = {};
-#pragma unroll
-        for (int step = 0; step < 4; ++step) {
-          const uint4 k = k_rows[(4 * t + step) * 64];
-#pragma unroll
-          for (int p = 2; p >= 0; --p) seen[p & 1] = mfma(k, part[step][p], seen[p & 1]);
-        }
-        const f32x4 carry = of_rows(carries[t]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[t][i] = fmaf(carry[i], seen[0][i] + seen[1][i], v[t][i]);
+        const uint2 run = *reinterpret_cast<const uint2*>(outs + 16 * t * kOutBytes);
+        const bool live = 16 * t + own < tokens;
+        x[t] = transpose_quad(make_uint2(live ? run.x : 0, live ? run.y : 0), lane);
       }
+      d_part[0] = make_uint4(x[0].x, x[0].y, x[1].x, x[1].y);
+      d_part[1] = make_uint4(x[2].x, x[2].y, x[3].x, x[3].y);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int step = upper_first(t); step < 2; ++step) {
+          const int at = upper_tile(t, step);
+          const uint4 parts[3] = {read_back[at * 64], read_back[(kTriangle + at) * 64],
+                                  read_back[(2 * kTriangle + at) * 64]};
+          v = mfma3(parts, d_part[step], v);
+        }
+        row_cells[64 * t] = v;
+      }
+    };
+    if (chunks != 0) {
+      fetch_read(chunks - 1);
+      fetch_first(chunks - 1);
+      stage_ready();
+      take_outputs(chunks - 1);
     }
-    // X = V' + N^T (b V'), Y = b X
+    for (uint32_t c = chunks; c-- > 0;) {
+      // The first half is there, the second has been read.  Stores issued after the
+      // tiles stay in flight (the last chunk's rows may be fewer).
+      if (c + 2 < chunks) {
+        stage_ready<8>();
+      } else {
+        stage_ready();
+      }
+      fetch_columns(c);
+      if (c != 0) fetch_read(c - 1);
+      float queries[4], strengths[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const float* const factors = reinterpret_cast<const float*>(stage);
+        queries[t] = factors[kReadQuery + 16 * t + own];
+        strengths[t] = factors[4 * (16 * t + own) + kStrength];
+      }
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {  // dS1
+        store_run(space.state_gradient(first_row + c, head) + slice * slice_cells(8),
+                  t * kTileBytes + linear, transpose_quad(state_cells[64 * t], lane));
+      }
+      {  // (exp(G) Q)^T dO
+        f32x4 sum[8] = {};
+#pragma unroll
+        for (int step = 0; step < 2; ++step) {
+          uint4 part[3];
+          f32x4 p[2];
+          float d[8];
+          widen8(d_part[step], d);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const f32x4 q = of_rows(queries[2 * step + u]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[u][i] = q[i] * d[4 * u + i];
+          }
+          split3(p[0], p[1], part);
+#pragma unroll
+          for (int t = 0; t < 8; ++t) {
+            sum[t] = mfma3(q_columns[(2 * t + step) * 64], part, sum[t]);
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < 8; ++t) state_cells[64 * t] = sum[t];
+      }
+      // The second half, X and the sum are there, the first half has been read.
+      stage_ready<8>();
+      if (c != 0) fetch_first(c - 1);
+      const int tokens = min(static_cast<int>(length - c * kChunk), kChunk);
+      char* const d = reinterpret_cast<char*>(args.d_values) +
+                      (begin + static_cast<uint64_t>(c) * kChunk) * out_step +
+                      2 * (head * kDim + 16 * slice);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {  // X, and Y = b X
+        const f32x4 x = row_cells[64 * t], b = of_rows(strengths[t]);
+        store_run(space.error_gradient(first_row + c, head) + slice * slice_cells(4),
+                  t * kTileBytes + linear, transpose_quad(x, lane));
+        const uint2 run = transpose_quad(
+            make_uint2(bf16_pair(b[0] * x[0], b[1] * x[1]), bf16_pair(b[2] * x[2], b[3] * x[3])),
+            lane);
+        if (16 * t + own < tokens) store_run(d, (16 * t + own) * out_step + 2 * (r & 12), run);
+      }
+      if (c != 0) take_outputs(c - 1);
+    }
+    return;
+  }
+
+  // The chain.
+  const uint64_t tile = (static_cast<uint64_t>(request) * space.value_heads + head) * kTile +
+                        (16 * slice + r) * kDim;
+  f32x4 state[8];  // the state's gradient, rows as in the forward scan
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    state[t] = args.d_final ? load4(args.d_final + tile + state_key(t, 4 * g))
+                            : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  const uint4* const k_rows = reinterpret_cast<const uint4*>(stage + kStageKeys) + lane;
+  const uint4* const k_columns = reinterpret_cast<const uint4*>(stage + kStageColumns) + lane;
+  const uint4* const solve = reinterpret_cast<const uint4*>(stage + kStageSolve) + lane;
+  if (chunks != 0) exchange();  // the first chunk's operands
+  __builtin_amdgcn_s_setprio(1);
+  for (uint32_t c = chunks; c-- > 0;) {
+    uint4 part[4][3];
+#pragma unroll
+    for (int t = 0; t < 8; ++t) state_cells[64 * t] = state[t];
+#pragma unroll
+    for (int step = 0; step < 4; ++step) {
+      split3(state[2 * step], state[2 * step + 1], part[step]);
+    }
+    exchange();
+    f32x4 factors[4];
+    float carries[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      factors[t] = reinterpret_cast<const f32x4*>(stage)[16 * t + own];
+      carries[t] = reinterpret_cast<const float*>(stage)[kCarry + 16 * t + own];
+    }
+    // V' = P^T dO + exp(G_63 - G) K dS1
+    f32x4 v[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const f32x4 read = row_cells[64 * t];
+      f32x4 seen[2] = {};
+#pragma unroll
+      for (int step = 0; step < 4; ++step) {
+        const uint4 k = k_rows[(4 * t + step) * 64];
+#pragma unroll
+        for (int p = 2; p >= 0; --p) seen[p & 1] = mfma(k, part[step][p], seen[p & 1]);
+      }
+      const f32x4 carry = of_rows(carries[t]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[t][i] = fmaf(carry[i], seen[0][i] + seen[1][i], read[i]);
+    }
+    // X = V' + N^T (b V')
     {
       uint4 part[2][3];
 #pragma unroll
@@ -260,65 +317,42 @@ __global__ __launch_bounds__(64 * kWaves, 2) void delta_back_scan_kernel(BackArg
       }
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        x[t] = v[t];
 #pragma unroll
         for (int step = upper_first(t); step < 2; ++step) {
           uint4 n[3];
 #pragma unroll
           for (int p = 0; p < 3; ++p) n[p] = solve[(p * kTriangle + upper_tile(t, step)) * 64];
-          x[t] = mfma6(n, part[step], x[t]);
+          v[t] = mfma6(n, part[step], v[t]);
         }
+        row_cells[64 * t] = v[t];
       }
     }
-    stage_ready();  // the second half is there, the first has been read
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      // Used before the next loads are issued, so that no wait for it covers them.
-      asm volatile("" : "+v"(next_out[t].x), "+v"(next_out[t].y));
-    }
-#pragma unroll
-    for (int i = 0; i < kTriangle; ++i) {
-      asm volatile("" : "+v"(read_low[i].x), "+v"(read_low[i].y), "+v"(read_low[i].z),
-                   "+v"(read_low[i].w));
-    }
-    if (c != 0) fetch_first(c - 1);
+    exchange();
     // dS0
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
+      const f32x4 sum = state_cells[64 * t];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) state[t][i] *= factors[0][kWhole];
+      for (int i = 0; i < 4; ++i) state[t][i] = fmaf(factors[0][kWhole], state[t][i], sum[i]);
     }
 #pragma unroll
     for (int step = 0; step < 2; ++step) {
-      uint4 by_query[3], by_key[3];
-      f32x4 p[2], m[2];
-      float d[8];
-      widen8(d_part[step], d);
+      uint4 by_key[3];
+      f32x4 m[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int t = 2 * step + u;
-        const f32x4 b = of_rows(factors[t][kStrength]);
-        const f32x4 k = of_rows(factors[t][kReadKey]), q = of_rows(queries[t]);
-        f32x4 row;
+        const f32x4 b = of_rows(factors[t][kStrength]), k = of_rows(factors[t][kReadKey]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          row[i] = b[i] * x[t][i];
-          p[u][i] = q[i] * d[4 * u + i];
-          m[u][i] = -k[i] * row[i];
-        }
-        y[t] = make_uint2(bf16_pair(row[0], row[1]), bf16_pair(row[2], row[3]));
+        for (int i = 0; i < 4; ++i) m[u][i] = -k[i] * (b[i] * v[t][i]);
       }
-      split3(p[0], p[1], by_query);
       split3(m[0], m[1], by_key);
 #pragma unroll
       for (int t = 0; t < 8; ++t) {
-        state[t] = mfma3(q_columns[(2 * t + step) * 64], by_query, state[t]);
         state[t] = mfma3(k_columns[(2 * t + step) * 64], by_key, state[t]);
       }
     }
-    if (c != 0) take_outputs(c - 1);
   }
-  if (chunks != 0) store_rows(0, min(static_cast<int>(length), kChunk));
 
   if (args.d_initial) {
 #pragma unroll
@@ -427,17 +461,17 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int unit = wave + 8 * u;
-      const int at = (16 * (unit >> 2) + r) * kDim + 32 * (unit & 3) + 8 * g;
-      x[u][0] = load4(xs + at), x[u][1] = load4(xs + at + 4);
-      e[u][0] = load4(errors + at), e[u][1] = load4(errors + at + 4);
+      const int at = cells_at(4, unit >> 2, r, g) + 2 * (unit & 3) * slice_cells(4);
+      x[u][0] = load4(xs + at), x[u][1] = load4(xs + at + 16);
+      e[u][0] = load4(errors + at), e[u][1] = load4(errors + at + 16);
     }
     f32x4 cells[4][2];  // S0's or dS1's rows of a tile of keys
     const auto load_rows = [&](const float* state, int c) {
-      const float* p = state + state_key(2 * pair + c, r) * kDim + 8 * g;
+      const float* p = state + cells_at(8, 2 * pair + c, r, g);
 #pragma unroll
       for (int step = 0; step < 4; ++step) {
-        cells[step][0] = load4(p + 32 * step);
-        cells[step][1] = load4(p + 32 * step + 4);
+        cells[step][0] = load4(p + 2 * step * slice_cells(8));
+        cells[step][1] = load4(p + 2 * step * slice_cells(8) + 16);
       }
     };
     if (member != 0) __syncthreads();  // the last head's values have been read
@@ -800,7 +834,7 @@ extern "C" int32_t statecentric_gdn_state_codec_gated_delta_backward_launch_v1(
   if (scans > gdn::kMaxGrid) return gdn::kStatusInvalidArgument;
   const int32_t status = gdn::launch(gdn::delta_back_scan_kernel,
                                      dim3(static_cast<uint32_t>(scans)),
-                                     dim3(64 * gdn::kWaves), stream, args);
+                                     dim3(128 * gdn::kWaves), stream, args);
   return status != gdn::kStatusOk
              ? status
              : gdn::launch(gdn::delta_gradient_kernel, dim3(space.rows * space.key_heads),

@@ -120,8 +120,9 @@ struct ChunkSpace {
   __host__ __device__ uint64_t states_at() const {
     return values_at() + static_cast<uint64_t>(rows) * value_heads * value_block_bytes(train);
   }
-  // Training: the start state and the end state's gradient of each chunk and
-  // value head (fp32 [key][value]), then E and X (fp32 [64][128] each).
+  // Training: the start state and the end state's gradient of each chunk and value
+  // head (fp32, 8 tiles of keys), then E and X (4 tiles of tokens each), in cells_at's
+  // order.
   __host__ __device__ uint64_t total() const {
     return states_at() + (train ? static_cast<uint64_t>(rows) * value_heads *
                                       (2 * kTile + 2 * kChunk * kDim) * 4
@@ -149,6 +150,18 @@ struct ChunkSpace {
     return state(row, head) + 2 * kTile + kChunk * kDim;
   }
 };
+
+// fp32 matrices that the scans leave to the gradients: 16 columns by 16 rows at a time,
+// as a wavefront's accumulator tile gives them after transpose_quad, 16 bytes a lane:
+// 1 KiB a store (rows of the whole matrix, 64 bytes of each a store, took 1.3 times as
+// long).  The floats from one slice of 16 columns to the next, of `tiles` row tiles:
+__host__ __device__ constexpr int slice_cells(int tiles) { return tiles * 256; }
+// Columns 8 g .. 8 g + 3 of the first two slices in row r of a tile; columns 4 on are
+// 16 floats on, columns 32 on two slices.
+__device__ __forceinline__ int cells_at(int tiles, int tile, int r, int g) {
+  return (g >> 1) * slice_cells(tiles) + tile * 256 + 64 * (r >> 2) + 32 * (g & 1) + 4 * (r & 3);
+}
+
 // The two inputs that are read element by element, which a slice of a batch may
 // start anywhere.
 inline bool element_aligned(const float* log_decay, const bf16_bits* beta) {
@@ -318,9 +331,26 @@ __device__ __forceinline__ void stage_tile(const char* from, uint32_t offset, ui
 }
 
 // Every staged tile of the workgroup is in LDS, and the stage read before may be
-// overwritten, after this.
+// overwritten, after this.  `kAfter` memory operations that each wavefront has issued
+// after its last tile (store_run's, so that their number is known) stay in flight.
+template <int kAfter = 0>
 __device__ __forceinline__ void stage_ready() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(kAfter) : "memory");
+}
+
+// One store of 16 or 8 bytes a lane, `offset` bytes from `to` (the same for the
+// wavefront).  The s_nop keeps the next instruction off the registers it reads.
+__device__ __forceinline__ void store_run(void* to, uint32_t offset, const f32x4& x) {
+  asm volatile("global_store_dwordx4 %0, %1, %2\n\ts_nop 1"
+               :
+               : "v"(offset), "v"(x), "s"(to)
+               : "memory");
+}
+__device__ __forceinline__ void store_run(void* to, uint32_t offset, const uint2& x) {
+  asm volatile("global_store_dwordx2 %0, %1, %2\n\ts_nop 1"
+               :
+               : "v"(offset), "v"(__builtin_bit_cast(uint64_t, x)), "s"(to)
+               : "memory");
 }
 
 // LDS written before it may be read by the workgroup's other wavefronts after it.

@@ -8,16 +8,22 @@
 //   K S0: 48, N (b R): 36, K^T U: 48, and beside the chain Q S0: 32, (P b) E: 18
 // matrix instructions.  Two forms:
 //
-// delta_scan_wide_kernel, for throughput: a workgroup takes a whole head, each of its
-// eight wavefronts 16 columns with all 64 tokens, the state in its accumulators.
-// What one product hands to the next are accumulators cut into parts, in registers:
-// no exchange.  The operands, the same for all eight, come through LDS a chunk ahead.
+// delta_scan_wide_kernel, for throughput: a workgroup takes 64 columns, with two
+// wavefronts for each 16.  One runs the chain with all 64 tokens, the state in its
+// accumulators: what one product hands to the next are accumulators cut into parts, in
+// registers, with no exchange.  The other loads the operands, which all share, into LDS
+// half a chunk ahead, forms the outputs half a chunk behind and stores what training
+// keeps; it takes S0 and E from LDS.  Bound by the chain's 132 matrix instructions and
+// the vector instructions between them: 3.1 us a chunk (32 heads of one request), where
+// the products alone would take 0.9; in training by the 96 KiB a chunk and head that it
+// stores as well, 5.6 us (128 heads at once, 3 TB/s).  With one wavefront for both the
+// chain and the rest these were 4.1 and 6.8.
 //
 // delta_scan_narrow_kernel, for few heads, where a long request's chain is all there
 // is: a workgroup takes 16 columns, and its wavefronts share each product by token
 // rows (or state rows), four on the chain and four on the outputs.  What a product
 // hands to the next goes through LDS, three exchanges a chunk; a wavefront's own
-// operands go from global memory to its registers a chunk ahead.
+// operands go from global memory to its registers a chunk ahead.  2.1 us a chunk.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -100,25 +106,36 @@ __device__ __forceinline__ f32x4 value_rows(const uint2& run, int lane) {
   return f32x4{widen_low(x.x), widen_high(x.x), widen_low(x.y), widen_high(x.y)};
 }
 
-// ------------------------------------------------------------- whole heads
-
-// A chunk's operands in LDS, in two halves, each fetched while the other is at work:
-// the factors, N (20 KiB of the value head's block) and K rows (16 tiles), then P b,
-// Q rows and K^T.  80 KiB, so that two workgroups share a compute unit.
-constexpr int kBlockTiles = 20;
-constexpr int kStageKeys = kBlockTiles * kTileBytes;
-constexpr int kStageRead = kStageKeys + kKeyTiles * kTileBytes;
-constexpr int kStageQueries = kStageRead + kReadOutBytes;
-constexpr int kStageColumns = kStageQueries + kKeyTiles * kTileBytes;
-constexpr int kStage = kStageColumns + kKeyTiles * kTileBytes;
-static_assert(kReadOut <= kBlockTiles * kTileBytes, "factors and N");
-static_assert(workgroups_by_lds(kStage) == 2, "two workgroups share a compute unit");
+// ------------------------------------------------------------ 64 columns
 
 constexpr int kWideWaves = 4;
 constexpr int kWideSlices = kDim / (16 * kWideWaves);
 
+// A chunk's operands in LDS, in two halves, each fetched while the other is at work:
+// the factors, N (20 KiB of the value head's block) and K rows (16 tiles), then Q rows,
+// K^T and P b (two stages: it is read a phase later).  Beside them S0 and E (two stages)
+// as the chain's accumulators hold them.  156 KiB: a workgroup has the compute unit to
+// itself.
+constexpr int kBlockTiles = 20;
+constexpr int kStageKeys = kBlockTiles * kTileBytes;
+constexpr int kStageQueries = kStageKeys + kKeyTiles * kTileBytes;
+constexpr int kStageColumns = kStageQueries + kKeyTiles * kTileBytes;
+constexpr int kStageRead = kStageColumns + kKeyTiles * kTileBytes;
+constexpr int kStageState = kStageRead + 2 * kReadOutBytes;
+constexpr int kStageErrors = kStageState + kWideWaves * 8 * kTileBytes;
+constexpr int kStage = kStageErrors + 2 * kWideWaves * 4 * kTileBytes;
+static_assert(kReadOut <= kBlockTiles * kTileBytes, "factors and N");
+static_assert(kStage <= 160 * 1024, "a compute unit's LDS");
+
+// Two bf16 parts of 8 places: 2^-15 of terms whose sums become bf16 outputs.
+__device__ __forceinline__ void split2(const f32x4& x, const f32x4& y, uint4 (&part)[2]) {
+  uint4 all[3];
+  split3(x, y, all);
+  part[0] = all[0], part[1] = all[1];
+}
+
 template <typename Pool, bool kTrain>
-__global__ __launch_bounds__(64 * kWideWaves, 2) void delta_scan_wide_kernel(ScanArgs args) {
+__global__ __launch_bounds__(128 * kWideWaves) void delta_scan_wide_kernel(ScanArgs args) {
   __shared__ __align__(16) char stage[kStage];
   const RuleArgs& a = args.rule;
   const ChunkSpace& space = a.space;
@@ -129,127 +146,203 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void delta_scan_wide_kernel(Sca
   if (!find_work(args, static_cast<uint64_t>(turn / kWideSlices) * 8 + (blockIdx.x & 7), w)) {
     return;
   }
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int place = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = place % kWideWaves;
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int first_value = 16 * (kWideWaves * (turn % kWideSlices) + wave);
-  const int value = first_value + r;
+  const int slice = kWideWaves * (turn % kWideSlices) + wave;
+  const int first_value = 16 * slice, value = first_value + r;
   const uint32_t key_head = w.head / a.group;
   const uint32_t length = w.length, chunks = w.chunks;
-
-  f32x4 state[8];
-  load_state(static_cast<const Pool*>(args.initial) + w.tile, 0, value, g, w.resumed, state);
-
-  const uint32_t stage_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
-      (__attribute__((address_space(3))) char*)&stage[0]));
-  // Addresses are a chunk's (scalar) and a lane's own 32-bit byte offset from it,
-  // which the last chunk's row clamps: rows past the end repeat it.  What becomes of
-  // them meets a strength of zero before it meets anything else, and is not stored.
-  const uint32_t key_step = static_cast<uint32_t>(a.key_stride) * 2;
-  const uint32_t query_step = static_cast<uint32_t>(a.query_stride) * 2;
-  const uint32_t value_step = static_cast<uint32_t>(a.value_stride) * 2;
-  const uint32_t out_step = space.value_heads * kDim * 2;
-  uint2 values[4];  // columns 4 (r / 4).. of tokens 16 t + 4 g + (r & 3)
-  const uint32_t linear = 16 * lane;
-  // Piece i of a chunk's first half (0..8; and 9..12, its rows of V) and of its second
-  // (0..10).  They are issued one by one between other work: the compute unit takes a
-  // tile about every 20 cycles, and a wavefront that issues several waits for them.
-  const auto fetch_first = [&](uint32_t c, int i) {
-    const uint64_t token = w.begin + c * kChunk;
-    const uint32_t last = min(length - c * kChunk, static_cast<uint32_t>(kChunk)) - 1;
-    if (i < 4) {  // K rows 16 i.., keys 32 wave..
-      const char* k = reinterpret_cast<const char*>(a.keys + token * a.key_stride +
-                                                    key_head * kDim);
-      const uint32_t row = min(static_cast<uint32_t>(16 * i + r), last);
-      stage_tile(k + 64 * wave, row * key_step + 16 * g,
-                 stage_at + kStageKeys + (4 * i + wave) * kTileBytes);
-    } else if (i < 9) {
-      const int tile = kWideWaves * (i - 4) + wave;
-      stage_tile(space.value_block(w.first_row + c, w.head) + tile * kTileBytes, linear,
-                 stage_at + tile * kTileBytes);
-    } else {
-      const char* v = reinterpret_cast<const char*>(a.values + token * a.value_stride +
-                                                    w.head * kDim + first_value);
-      const uint32_t row = min(static_cast<uint32_t>(16 * (i - 9) + 4 * g + (r & 3)), last);
-      values[i - 9] = *reinterpret_cast<const uint2*>(v + (row * value_step + 2 * (r & 12)));
-    }
+  f32x4* const state_cells =
+      reinterpret_cast<f32x4*>(stage + kStageState) + wave * 8 * 64 + lane;
+  const auto error_cells = [&](uint32_t c) {
+    return reinterpret_cast<f32x4*>(stage + kStageErrors) +
+           ((c & 1) * kWideWaves + wave) * 4 * 64 + lane;
   };
-  const auto fetch_second = [&](uint32_t c, int i) {
-    if (i < 4) {  // Q rows 16 i.., keys 32 wave..
+
+  if (place >= kWideWaves) {  // the operands' loads, the outputs, training's stores
+    const uint32_t stage_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+        (__attribute__((address_space(3))) char*)&stage[0]));
+    const uint32_t key_step = static_cast<uint32_t>(a.key_stride) * 2;
+    const uint32_t query_step = static_cast<uint32_t>(a.query_stride) * 2;
+    const uint32_t out_step = space.value_heads * kDim * 2;
+    const uint32_t linear = 16 * lane;
+    const auto fetch_first = [&](uint32_t c) {
       const uint64_t token = w.begin + c * kChunk;
       const uint32_t last = min(length - c * kChunk, static_cast<uint32_t>(kChunk)) - 1;
+      const char* k = reinterpret_cast<const char*>(a.keys + token * a.key_stride +
+                                                    key_head * kDim);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {  // K rows 16 i.., keys 32 wave..
+        const uint32_t row = min(static_cast<uint32_t>(16 * i + r), last);
+        stage_tile(k + 64 * wave, row * key_step + 16 * g,
+                   stage_at + kStageKeys + (4 * i + wave) * kTileBytes);
+      }
+      const char* block = space.value_block(w.first_row + c, w.head);
+#pragma unroll
+      for (int i = 0; i < kBlockTiles / kWideWaves; ++i) {
+        const int tile = kWideWaves * i + wave;
+        stage_tile(block + tile * kTileBytes, linear, stage_at + tile * kTileBytes);
+      }
+    };
+    const auto fetch_second = [&](uint32_t c) {
+      const uint64_t token = w.begin + c * kChunk;
+      const uint32_t last = min(length - c * kChunk, static_cast<uint32_t>(kChunk)) - 1;
+      const char* columns = space.key_block(w.first_row + c, key_head) + kKeyColumns;
       const char* q = reinterpret_cast<const char*>(a.queries + token * a.query_stride +
                                                     key_head * kDim);
-      const uint32_t row = min(static_cast<uint32_t>(16 * i + r), last);
-      stage_tile(q + 64 * wave, row * query_step + 16 * g,
-                 stage_at + kStageQueries + (4 * i + wave) * kTileBytes);
-    } else if (i < 8) {
-      const int tile = kWideWaves * (i - 4) + wave;
-      stage_tile(space.key_block(w.first_row + c, key_head) + kKeyColumns + tile * kTileBytes,
-                 linear, stage_at + kStageColumns + tile * kTileBytes);
-    } else {
-      const int tile = kWideWaves * (i - 8) + wave;
-      stage_tile(space.value_block(w.first_row + c, w.head) + kReadOut + tile * kTileBytes,
-                 linear, stage_at + kStageRead + tile * kTileBytes);
-    }
-  };
-  if (chunks != 0) {
+      const char* read = space.value_block(w.first_row + c, w.head) + kReadOut;
 #pragma unroll
-    for (int i = 0; i < 13; ++i) fetch_first(0, i);
-  }
-
-  f32x4 error[4], out[4];
-  const auto store_rows = [&](uint32_t c, int tokens) {
-    char* o = reinterpret_cast<char*>(args.outputs) +
-              (w.begin + static_cast<uint64_t>(c) * kChunk) * out_step +
-              2 * (w.head * kDim + first_value);
+      for (int i = 0; i < 4; ++i) {
+        const int tile = kWideWaves * i + wave;
+        stage_tile(columns + tile * kTileBytes, linear,
+                   stage_at + kStageColumns + tile * kTileBytes);
+      }
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int token = 16 * t + 4 * g + (r & 3);
-      const uint2 x = output_run(out[t], lane);
-      if (token < tokens) *reinterpret_cast<uint2*>(o + (token * out_step + 2 * (r & 12))) = x;
+      for (int i = 0; i < 4; ++i) {  // Q rows 16 i.., keys 32 wave..
+        const uint32_t row = min(static_cast<uint32_t>(16 * i + r), last);
+        stage_tile(q + 64 * wave, row * query_step + 16 * g,
+                   stage_at + kStageQueries + (4 * i + wave) * kTileBytes);
+      }
+#pragma unroll
+      for (int i = 0; i < 2 * kTriangle / kWideWaves; ++i) {
+        const int tile = kWideWaves * i + wave;
+        stage_tile(read + tile * kTileBytes, linear,
+                   stage_at + kStageRead + (c & 1) * kReadOutBytes + tile * kTileBytes);
+      }
+    };
+    f32x4 out[4], error[4];
+    const auto read_errors = [&](uint32_t c) {  // O += (P b) E
+      const f32x4* const cells = error_cells(c);
+      const uint4* const read_out =
+          reinterpret_cast<const uint4*>(stage + kStageRead + (c & 1) * kReadOutBytes) + lane;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) error[t] = cells[64 * t];
+#pragma unroll
+      for (int step = 0; step < 2; ++step) {
+        uint4 part[2];
+        split2(error[2 * step], error[2 * step + 1], part);
+#pragma unroll
+        for (int t = 2 * step; t < 4; ++t) {  // rows 0..31 end in step 0
+          const int tile = lower_tile(t, step);
+          const uint4 high = read_out[tile * 64], low = read_out[(kTriangle + tile) * 64];
+          out[t] = mfma(low, part[0], out[t]);
+          out[t] = mfma(high, part[1], out[t]);
+          out[t] = mfma(high, part[0], out[t]);
+        }
+      }
+    };
+    // kTrain ? 8 : 4 stores, of which the tokens past `tokens` have none.
+    const auto store_rows = [&](uint32_t c, int tokens) {
+      char* o = reinterpret_cast<char*>(args.outputs) +
+                (w.begin + static_cast<uint64_t>(c) * kChunk) * out_step +
+                2 * (w.head * kDim + first_value);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int token = 16 * t + 4 * g + (r & 3);
+        const uint2 x = output_run(out[t], lane);
+        if (token < tokens) store_run(o, token * out_step + 2 * (r & 12), x);
+        if constexpr (kTrain) {
+          store_run(space.errors(w.first_row + c, w.head) + slice * slice_cells(4),
+                    t * kTileBytes + linear, transpose_quad(error[t], lane));
+        }
+      }
+    };
+    const uint4* const q_rows = reinterpret_cast<const uint4*>(stage + kStageQueries) + lane;
+    if (chunks != 0) fetch_first(0);
+    for (uint32_t c = 0; c < chunks; ++c) {
+      // The first half is there, the second has been read.  Only the stores issued after
+      // the tiles stay in flight: a store's way to memory is as long as a chunk's work.
+      if (c < 2) {
+        stage_ready();
+      } else {
+        stage_ready<kTrain ? 8 : 4>();
+      }
+      fetch_second(c);
+      f32x4 state[8];
+      float queries[4];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) state[t] = state_cells[64 * t];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        queries[t] =
+            reinterpret_cast<const float*>(stage)[kReadQuery + 16 * t + 4 * g + (r & 3)];
+      }
+      uint4 part[4][2];
+#pragma unroll
+      for (int step = 0; step < 4; ++step) {
+        split2(state[2 * step], state[2 * step + 1], part[step]);
+      }
       if constexpr (kTrain) {
-        float* e = space.errors(w.first_row + c, w.head) + first_value + (r & 12);
-        *reinterpret_cast<f32x4*>(e + token * kDim) = transpose_quad(error[t], lane);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+          store_run(space.state(w.first_row + c, w.head) + slice * slice_cells(8),
+                    t * kTileBytes + linear, transpose_quad(state[t], lane));
+        }
+      }
+      if (c != 0) read_errors(c - 1);
+      // The second half and E are there, the first half and S0 have been read.
+      stage_ready<kTrain ? 8 : 0>();
+      if (c + 1 < chunks) fetch_first(c + 1);
+      if (c != 0) store_rows(c - 1, kChunk);  // only the last chunk can be short
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        f32x4 read[2] = {};
+#pragma unroll
+        for (int step = 0; step < 4; ++step) {
+          const uint4 q = q_rows[(4 * t + step) * 64];
+          read[0] = mfma(q, part[step][1], read[0]);
+          read[1] = mfma(q, part[step][0], read[1]);
+        }
+        const f32x4 read_query = of_rows(queries[t]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[t][i] = read_query[i] * (read[0][i] + read[1][i]);
       }
     }
-  };
+    if (chunks != 0) {
+      read_errors(chunks - 1);
+      store_rows(chunks - 1, length - (chunks - 1) * kChunk);
+    }
+    return;
+  }
 
-  const uint4* const k_rows = reinterpret_cast<const uint4*>(stage + kStageKeys) + lane;
-  const uint4* const q_rows = reinterpret_cast<const uint4*>(stage + kStageQueries) + lane;
-  const uint4* const k_columns = reinterpret_cast<const uint4*>(stage + kStageColumns) + lane;
-  const uint4* const solve = reinterpret_cast<const uint4*>(stage + kSolve) + lane;
-  const uint4* const read_out = reinterpret_cast<const uint4*>(stage + kStageRead) + lane;
-  for (uint32_t c = 0; c < chunks; ++c) {
-    stage_ready();  // the first half is there, the second has been read
-    f32x4 factors[4];  // of tokens 16 t + 4 g + (r & 3)
-    float queries[4];
+  // The chain.
+  f32x4 state[8];
+  load_state(static_cast<const Pool*>(args.initial) + w.tile, 0, value, g, w.resumed, state);
+  const uint32_t value_step = static_cast<uint32_t>(a.value_stride) * 2;
+  uint2 values[4];  // columns 4 (r / 4).. of tokens 16 t + 4 g + (r & 3)
+  const auto fetch_values = [&](uint32_t c) {
+    const uint64_t token = w.begin + c * kChunk;
+    const uint32_t last = min(length - c * kChunk, static_cast<uint32_t>(kChunk)) - 1;
+    const char* v = reinterpret_cast<const char*>(a.values + token * a.value_stride +
+                                                  w.head * kDim + first_value);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      const int token = 16 * t + 4 * g + (r & 3);
-      factors[t] = reinterpret_cast<const f32x4*>(stage)[token];
-      queries[t] = reinterpret_cast<const float*>(stage)[kReadQuery + token];
-      // Used before the next loads are issued, so that no wait for it covers them.
-      asm volatile("" : "+v"(values[t].x), "+v"(values[t].y));
+      const uint32_t row = min(static_cast<uint32_t>(16 * t + 4 * g + (r & 3)), last);
+      values[t] = *reinterpret_cast<const uint2*>(v + (row * value_step + 2 * (r & 12)));
     }
+  };
+  const uint4* const k_rows = reinterpret_cast<const uint4*>(stage + kStageKeys) + lane;
+  const uint4* const k_columns = reinterpret_cast<const uint4*>(stage + kStageColumns) + lane;
+  const uint4* const solve = reinterpret_cast<const uint4*>(stage + kSolve) + lane;
+  if (chunks != 0) fetch_values(0);
+  __builtin_amdgcn_s_setprio(1);
+  for (uint32_t c = 0; c < chunks; ++c) {
     uint4 part[4][3];  // of the state, over the keys
+#pragma unroll
+    for (int t = 0; t < 8; ++t) state_cells[64 * t] = state[t];
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
       split3(state[2 * step], state[2 * step + 1], part[step]);
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = 3 * step; i < min(3 * step + 3, 11); ++i) fetch_second(c, i);
-      __builtin_amdgcn_sched_barrier(0);
     }
-    if (c != 0) store_rows(c - 1, kChunk);  // only the last chunk can be short
-    if constexpr (kTrain) {
-      float* p = space.state(w.first_row + c, w.head) + first_value + (r & 12);
+    exchange();
+    f32x4 factors[4];  // of tokens 16 t + 4 g + (r & 3)
 #pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        *reinterpret_cast<f32x4*>(p + state_key(t, 4 * g + (r & 3)) * kDim) =
-            transpose_quad(state[t], lane);
-      }
+    for (int t = 0; t < 4; ++t) {
+      factors[t] = reinterpret_cast<const f32x4*>(stage)[16 * t + 4 * g + (r & 3)];
     }
     // R = V - exp(G) K S0
+    f32x4 error[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       f32x4 seen[2] = {};  // two sums, so that each product waits for the last but one
@@ -264,6 +357,7 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void delta_scan_wide_kernel(Sca
 #pragma unroll
       for (int i = 0; i < 4; ++i) error[t][i] = fmaf(-read_key[i], seen[0][i] + seen[1][i], x[i]);
     }
+    if (c + 1 < chunks) fetch_values(c + 1);
     // E = R + N (b R)
     {
       uint4 part[2][3];
@@ -278,6 +372,7 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void delta_scan_wide_kernel(Sca
         }
         split3(x[0], x[1], part[step]);
       }
+      f32x4* const cells = error_cells(c);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
 #pragma unroll
@@ -287,31 +382,11 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void delta_scan_wide_kernel(Sca
           for (int p = 0; p < 3; ++p) n[p] = solve[(p * kTriangle + lower_tile(t, step)) * 64];
           error[t] = mfma6(n, part[step], error[t]);
         }
+        cells[64 * t] = error[t];
       }
     }
-    stage_ready();  // the second half is there, the first has been read
-    // exp(G) Q S0 from two of the state's parts: 2^-15 of terms whose sums become
-    // bf16 outputs.
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      f32x4 read[2] = {};
-#pragma unroll
-      for (int step = 0; step < 4; ++step) {
-        const uint4 q = q_rows[(4 * t + step) * 64];
-        read[0] = mfma(q, part[step][1], read[0]);
-        read[1] = mfma(q, part[step][0], read[1]);
-      }
-      const f32x4 read_query = of_rows(queries[t]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) out[t][i] = read_query[i] * (read[0][i] + read[1][i]);
-      if (c + 1 < chunks) {
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = t; i < 13; i += 4) fetch_first(c + 1, i);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-    // S1 = exp(G_63) S0 + K^T (write b E), and O += (P b) E
+    exchange();
+    // S1 = exp(G_63) S0 + K^T (write b E)
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
 #pragma unroll
@@ -319,7 +394,7 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void delta_scan_wide_kernel(Sca
     }
 #pragma unroll
     for (int step = 0; step < 2; ++step) {
-      uint4 written[3], plain[3];
+      uint4 written[3];
       f32x4 x[2];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
@@ -328,22 +403,12 @@ __global__ __launch_bounds__(64 * kWideWaves, 2) void delta_scan_wide_kernel(Sca
         for (int i = 0; i < 4; ++i) x[u][i] = write[i] * error[2 * step + u][i];
       }
       split3(x[0], x[1], written);
-      split3(error[2 * step], error[2 * step + 1], plain);
 #pragma unroll
       for (int t = 0; t < 8; ++t) {
         state[t] = mfma3(k_columns[(2 * t + step) * 64], written, state[t]);
       }
-#pragma unroll
-      for (int t = 2 * step; t < 4; ++t) {  // rows 0..31 end in step 0
-        const int tile = lower_tile(t, step);
-        const uint4 high = read_out[tile * 64], low = read_out[(kTriangle + tile) * 64];
-        out[t] = mfma(low, plain[0], out[t]);
-        out[t] = mfma(high, plain[1], out[t]);
-        out[t] = mfma(high, plain[0], out[t]);
-      }
     }
   }
-  if (chunks != 0) store_rows(chunks - 1, length - (chunks - 1) * kChunk);
   store_state(static_cast<Pool*>(args.final_states) + w.tile, 0, value, g, state);
 }
 
@@ -369,7 +434,7 @@ __global__ __launch_bounds__(512) void delta_scan_narrow_kernel(ScanArgs args) {
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int rows = wave & 3;           // this wavefront's token rows, 16 rows..
   const int steps = lower_steps(rows);
-  const int first_value = (turn % kSlices) * 16, value = first_value + r;
+  const int slice = turn % kSlices, first_value = 16 * slice, value = first_value + r;
   const uint32_t key_head = w.head / a.group;
   const uint32_t length = w.length, chunks = w.chunks;
   const uint32_t mine = 16 * rows + 4 * g + (r & 3);  // the token whose factors it loads
@@ -517,15 +582,14 @@ __global__ __launch_bounds__(512) void delta_scan_narrow_kernel(ScanArgs args) {
 #pragma unroll
       for (int p = 0; p < 3; ++p) state_parts[wave][p][lane] = part[p];
       if constexpr (kTrain) {
-        float* p = space.state(row, w.head) + (32 * wave + 8 * g) * kDim + value;
+        float* p = space.state(row, w.head) + slice * slice_cells(8) + 2 * wave * 256 + 4 * lane;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[i * kDim] = state[0][i];
-          p[(4 + i) * kDim] = state[1][i];
-        }
+        for (int u = 0; u < 2; ++u) store_cells(p + 256 * u, transpose_quad(state[u], lane));
       }
     }
-    float* const e = kTrain ? space.errors(row, w.head) : nullptr;
+    float* const e =
+        kTrain ? space.errors(row, w.head) + slice * slice_cells(4) + wave * 256 + 4 * lane
+               : nullptr;
     exchange();
     // R = V - exp(G) K S0.  An exchange's values are all asked for before the first
     // is used, and the operands two products ahead (of the next chunk, where this one
@@ -627,10 +691,7 @@ __global__ __launch_bounds__(512) void delta_scan_narrow_kernel(ScanArgs args) {
         }
       }
     }
-    if constexpr (kTrain) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) e[(16 * wave + 4 * g + i) * kDim + value] = error[i];
-    }
+    if constexpr (kTrain) store_cells(e, transpose_quad(error, lane));
   }
   store_state(static_cast<Pool*>(args.final_states) + w.tile, 2 * wave, value, g, state);
 }
@@ -638,16 +699,16 @@ __global__ __launch_bounds__(512) void delta_scan_narrow_kernel(ScanArgs args) {
 template <typename Pool, bool kTrain>
 int32_t scan_by_size(void* stream, const ScanArgs& args) {
   const uint64_t items = static_cast<uint64_t>(args.rule.requests) * args.rule.space.value_heads;
-  // A compute unit runs one narrow workgroup at a time; where they all run at once, a
-  // chunk takes 2.0 us (32 heads of one request), in the wide form 4.1 us.  From twice
-  // as many on, two rounds of the one are no faster than one of the other, which
-  // issues an eighth of the loads.
+  // Where all narrow workgroups run at once, one on each of the 256 compute units, a
+  // chunk takes 2.1 us (32 heads of one request), in the wide form 3.1 us.  Twice as many
+  // would take two rounds of the one, and one of the other, which issues a quarter of
+  // the loads (128 heads, 4 requests in training: 250 us and 180 us).
   const bool narrow = items * (kDim / 16) <= 256;
   const uint64_t blocks = (items + 7) / 8 * 8 * (narrow ? kDim / 16 : kWideSlices);
   if (blocks > kMaxGrid) return kStatusInvalidArgument;
   const dim3 grid(static_cast<uint32_t>(blocks));
   return narrow ? launch(delta_scan_narrow_kernel<Pool, kTrain>, grid, dim3(512), stream, args)
-                : launch(delta_scan_wide_kernel<Pool, kTrain>, grid, dim3(64 * kWideWaves), stream,
+                : launch(delta_scan_wide_kernel<Pool, kTrain>, grid, dim3(128 * kWideWaves), stream,
                          args);
 }
 
