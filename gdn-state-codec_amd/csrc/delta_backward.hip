@@ -380,11 +380,6 @@ __device__ __forceinline__ float sum16(float x) {  // over the 16 lanes of a DPP
   return add_partner<8>(x);
 }
 
-// By value: a choice between elements of an array would put it into memory.
-__device__ __forceinline__ uint4 pick(bool first, uint4 x, uint4 y) {
-  return make_uint4(first ? x.x : y.x, first ? x.y : y.y, first ? x.z : y.z, first ? x.w : y.w);
-}
-
 struct Gradient {
   // X and E cut into parts, 16 tiles a part; then the four kinds of F and H, 6 tiles
   // a part.
@@ -397,16 +392,17 @@ struct Gradient {
   float h[kChunk][kWide];
   float factors[kFactors];
   float norms[3][kChunk];  // 1/|k|, scale/|q|, 1/|q|
+  // Of the value head at work: exp(G), exp(G) b, exp(G_63 - G) b.
+  float decays[3][kChunk];
   float along[4][kChunk];  // X.E by step
-  float sums[2][4][kChunk];
+  float sums[2][8][kChunk];
   float ends[8];
 };
 static_assert(sizeof(Gradient) <= kLdsPerCu, "one workgroup a compute unit");
 
-// One workgroup per chunk row and key head.  Wavefront w takes keys of state tiles
-// 2 (w / 2) and the next and token tiles 2 (w & 1) and the next, so that an operand
-// read from LDS meets two others.  X and E are cut into parts once, by the wavefront
-// that loads them, and so are F and H.
+// One workgroup per chunk row and key head.  Wavefront w takes the keys of state tile w
+// and all tokens, so that a state is loaded and cut into parts once.  X and E are cut
+// once, by the wavefront that loads them, and so are F and H.
 __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args) {
   __shared__ __align__(16) Gradient s;
   const RuleArgs& a = args.rule;
@@ -437,14 +433,19 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
   if (count == 0) return;
   const uint64_t first = chunk.y;
   const char* const keys = space.key_block(row, head);
-  const int pair = wave >> 1, half = wave & 1;
   const uint32_t outs_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
       (__attribute__((address_space(3))) char*)&s.outs[0][0]));
   if (t < 3 * kChunk) {
     s.norms[t / kChunk][t % kChunk] = reinterpret_cast<const float*>(keys + kNorms)[t];
   }
 
-  f32x4 d_q[2][2] = {}, d_k[2][2] = {};  // [state tile 2 pair + c][token tile 2 half + i]
+  const auto eight = [&](int which, int token) {  // a sum over the wavefronts
+    return ((s.sums[which][0][token] + s.sums[which][1][token]) +
+            (s.sums[which][2][token] + s.sums[which][3][token])) +
+           ((s.sums[which][4][token] + s.sums[which][5][token]) +
+            (s.sums[which][6][token] + s.sums[which][7][token]));
+  };
+  f32x4 d_q[4] = {}, d_k[4] = {};  // of the token tiles
   for (uint32_t member = 0; member < a.group; ++member) {
     const uint32_t value_head = head * a.group + member;
     // Taken afresh for each head: the addresses that follow from it would otherwise
@@ -465,9 +466,9 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
       x[u][0] = load4(xs + at), x[u][1] = load4(xs + at + 16);
       e[u][0] = load4(errors + at), e[u][1] = load4(errors + at + 16);
     }
-    f32x4 cells[4][2];  // S0's or dS1's rows of a tile of keys
-    const auto load_rows = [&](const float* state, int c) {
-      const float* p = state + cells_at(8, 2 * pair + c, r, g);
+    f32x4 start[4][2], end_gradient[4][2];  // S0's and dS1's rows of the keys
+    const auto load_rows = [&](const float* state, f32x4 (&cells)[4][2]) {
+      const float* p = state + cells_at(8, wave, r, g);
 #pragma unroll
       for (int step = 0; step < 4; ++step) {
         cells[step][0] = load4(p + 2 * step * slice_cells(8));
@@ -509,6 +510,16 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
       for (int p = 0; p < 3; ++p) s.rows[1][p][unit][lane] = part[p];
     }
     stage_ready();
+    load_rows(s0, start);
+    if (t < kChunk) {
+      const float b = s.factors[4 * t + kStrength];
+      const float decay = __builtin_amdgcn_exp2f(s.factors[kSum + t]);
+      s.decays[0][t] = decay;
+      s.decays[1][t] = decay * b;
+      s.decays[2][t] = b * decay_between(s.factors[kSum + kChunk - 1],
+                                         s.factors[kSumRest + kChunk - 1], s.factors[kSum + t],
+                                         s.factors[kSumRest + t]);
+    }
 
     // F and H, ten blocks (i, j), j <= i, of 16 x 16; the two beside them that an
     // operand tile holds are zeros.
@@ -545,62 +556,53 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
       }
     }
 
-    // S0 dO and S0 X, then dS1 E, of this wavefront's keys and tokens; the rows of the
-    // next tile of keys come while this one's products are formed.
-    f32x4 read_q[2][2] = {}, read_k[2][2] = {}, written[2][2] = {};
-    load_rows(s0, 0);
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    // S0 dO and S0 X, then <dS1, S0> and dS1 E, of this wavefront's keys.
+    load_rows(s1, end_gradient);
+    __builtin_amdgcn_sched_barrier(0);
+    f32x4 read_q[4] = {}, read_k[4] = {}, written[4] = {};
+    {
       uint4 part[4][3];
 #pragma unroll
-      for (int step = 0; step < 4; ++step) split_row(cells[step], part[step]);
-      load_rows(c == 0 ? s0 : s1, c == 0 ? 1 : 0);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int step = 0; step < 4; ++step) split_row(start[step], part[step]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 4; ++i) {
 #pragma unroll
         for (int step = 0; step < 4; ++step) {
-          const int at = 4 * (2 * half + i) + step;
+          const int at = 4 * i + step;
           uint4 x_part[3];
 #pragma unroll
           for (int p = 0; p < 3; ++p) x_part[p] = s.rows[0][p][at][lane];
-          read_q[c][i] = mfma3(s.outs[at][lane], part[step], read_q[c][i]);
-          read_k[c][i] = mfma6(x_part, part[step], read_k[c][i]);
+          read_q[i] = mfma3(s.outs[at][lane], part[step], read_q[i]);
+          read_k[i] = mfma6(x_part, part[step], read_k[i]);
         }
       }
-      __builtin_amdgcn_sched_barrier(0);
     }
+    __builtin_amdgcn_sched_barrier(0);
+    float end = 0.0f;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int step = 0; step < 4; ++step) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        end = fmaf(start[step][0][i], end_gradient[step][0][i], end);
+        end = fmaf(start[step][1][i], end_gradient[step][1][i], end);
+      }
+    }
+    end *= s.factors[kWhole];
+    {
       uint4 part[4][3];
 #pragma unroll
-      for (int step = 0; step < 4; ++step) split_row(cells[step], part[step]);
-      if (c == 0) load_rows(s1, 1);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int step = 0; step < 4; ++step) split_row(end_gradient[step], part[step]);
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 4; ++i) {
 #pragma unroll
         for (int step = 0; step < 4; ++step) {
-          const int at = 4 * (2 * half + i) + step;
+          const int at = 4 * i + step;
           uint4 e_part[3];
 #pragma unroll
           for (int p = 0; p < 3; ++p) e_part[p] = s.rows[1][p][at][lane];
-          written[c][i] = mfma6(e_part, part[step], written[c][i]);
+          written[i] = mfma6(e_part, part[step], written[i]);
         }
       }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-    // <dS1, S0>, an eighth of the cells a wavefront
-    float end = 0.0f;
-    {
-      const uint32_t from = wave * (kTile / 8) + 4 * lane;
-#pragma unroll
-      for (int i = 0; i < kTile / 8; i += 256) {
-        const f32x4 x = load4(s0 + from + i), y = load4(s1 + from + i);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) end = fmaf(x[j], y[j], end);
-      }
-      end *= s.factors[kWhole];
     }
     __syncthreads();  // f and h are whole, X's and E's parts have been read
 
@@ -636,90 +638,60 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
 #pragma unroll
       for (int p = 0; p < 3; ++p) s.kinds[kind][p][at][lane] = part[p];
     }
-    uint4 k_columns[2][2], q_columns[2][2];
+    uint4 k_columns[2], q_columns[2];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-#pragma unroll
-      for (int step = 0; step < 2; ++step) {
-        const int at = (2 * (2 * pair + c) + step) * kTileBytes + 16 * lane;
-        k_columns[c][step] = *reinterpret_cast<const uint4*>(keys + kKeyColumns + at);
-        q_columns[c][step] = *reinterpret_cast<const uint4*>(keys + kQueryColumns + at);
-      }
+    for (int step = 0; step < 2; ++step) {
+      const int at = (2 * wave + step) * kTileBytes + 16 * lane;
+      k_columns[step] = *reinterpret_cast<const uint4*>(keys + kKeyColumns + at);
+      q_columns[step] = *reinterpret_cast<const uint4*>(keys + kQueryColumns + at);
     }
     __syncthreads();
 
-    float cells_k[2][8], cells_q[2][8];  // of the token tiles: 4 i + j
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      widen8(pick(half == 0, k_columns[c][0], k_columns[c][1]), cells_k[c]);
-      widen8(pick(half == 0, q_columns[c][0], q_columns[c][1]), cells_q[c]);
-    }
+    for (int i = 0; i < 4; ++i) {
+      f32x4 by_query = {0.0f, 0.0f, 0.0f, 0.0f}, by_read = by_query, by_write = by_query;
+      const auto add = [&](int kind, int at, const uint4& columns, f32x4& to) {
+        const uint4 part[3] = {s.kinds[kind][0][at][lane], s.kinds[kind][1][at][lane],
+                               s.kinds[kind][2][at][lane]};
+        to = mfma3(part, columns, to);
+      };
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int tile = 2 * half + i;
-      f32x4 by_query[2], by_read[2], by_write[2];
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        by_query[c] = by_read[c] = by_write[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int step = 0; step < lower_steps(i); ++step) {  // the tokens before
+        add(0, lower_tile(i, step), k_columns[step], by_query);
+        add(1, lower_tile(i, step), k_columns[step], by_read);
       }
 #pragma unroll
-      for (int step = 0; step < 2; ++step) {
-        uint4 part[3];
-        if (step <= half) {  // the tokens before
-          const int at = half == 0 ? i : 2 * tile - 2 + step;
-#pragma unroll
-          for (int p = 0; p < 3; ++p) part[p] = s.kinds[0][p][at][lane];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) by_query[c] = mfma3(part, k_columns[c][step], by_query[c]);
-#pragma unroll
-          for (int p = 0; p < 3; ++p) part[p] = s.kinds[1][p][at][lane];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) by_read[c] = mfma3(part, k_columns[c][step], by_read[c]);
-        }
-        if (step >= half) {  // the tokens after
-          const int at = half == 0 ? 2 * i + step : tile + 2;
-#pragma unroll
-          for (int p = 0; p < 3; ++p) part[p] = s.kinds[2][p][at][lane];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) by_write[c] = mfma3(part, q_columns[c][step], by_write[c]);
-#pragma unroll
-          for (int p = 0; p < 3; ++p) part[p] = s.kinds[3][p][at][lane];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) by_write[c] = mfma3(part, k_columns[c][step], by_write[c]);
-        }
+      for (int step = upper_first(i); step < 2; ++step) {  // the tokens after
+        add(2, upper_tile(i, step), q_columns[step], by_write);
+        add(3, upper_tile(i, step), k_columns[step], by_write);
       }
+      float cells_k[8], cells_q[8];
+      widen8(k_columns[i >> 1], cells_k);
+      widen8(q_columns[i >> 1], cells_q);
+      const int from = 16 * i + 4 * g;
+      const f32x4 k_unit = load4(&s.norms[0][from]), q_unit = load4(&s.norms[1][from]);
+      const f32x4 decay = load4(&s.decays[0][from]), read_by = load4(&s.decays[1][from]);
+      const f32x4 kept = load4(&s.decays[2][from]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int token = 16 * tile + 4 * g + j;
-        const float k_unit = s.norms[0][token], q_unit = s.norms[1][token];
-        const float b = s.factors[4 * token + kStrength];
-        const float decay = __builtin_amdgcn_exp2f(s.factors[kSum + token]);
-        const float kept = decay_between(s.factors[kSum + kChunk - 1],
-                                         s.factors[kSumRest + kChunk - 1],
-                                         s.factors[kSum + token], s.factors[kSumRest + token]);
-        float total = 0.0f;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const float dq = fmaf(decay, read_q[c][i][j], by_query[c][j]);
-          const float read = -fmaf(decay * b, read_k[c][i][j], by_read[c][j]);
-          const float carried = kept * b * written[c][i][j];
-          const float write = carried + by_write[c][j];
-          const float k = k_unit * cells_k[c][4 * i + j], q = q_unit * cells_q[c][4 * i + j];
-          total = fmaf(q, dq, fmaf(k, read - write, total));
-          end = fmaf(k, carried, end);
-          d_q[c][i][j] += dq;
-          d_k[c][i][j] += read + write;
-        }
-        total = sum16(total);
-        if (r == 0) s.sums[0][pair][token] = total;
+        const float dq = fmaf(decay[j], read_q[i][j], by_query[j]);
+        const float read = -fmaf(read_by[j], read_k[i][j], by_read[j]);
+        const float carried = kept[j] * written[i][j];
+        const float write = carried + by_write[j];
+        const float k = k_unit[j] * cells_k[4 * (i & 1) + j];
+        const float q = q_unit[j] * cells_q[4 * (i & 1) + j];
+        end = fmaf(k, carried, end);
+        d_q[i][j] += dq;
+        d_k[i][j] += read + write;
+        const float total = sum16(fmaf(q, dq, k * (read - write)));
+        if (r == 0) s.sums[0][wave][from + j] = total;
       }
     }
     end = wave_sum_valu(end);
     if (lane == 0) s.ends[wave] = end;
     __syncthreads();
     if (wave == 0) {
-      float total = (s.sums[0][0][lane] + s.sums[0][1][lane]) +
-                    (s.sums[0][2][lane] + s.sums[0][3][lane]);
+      float total = eight(0, lane);
       if (lane == 63) {
         total += ((s.ends[0] + s.ends[1]) + (s.ends[2] + s.ends[3])) +
                  ((s.ends[4] + s.ends[5]) + (s.ends[6] + s.ends[7]));
@@ -742,71 +714,55 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
   // for keys the same with scale 1.
   float cells_k[2][8], cells_q[2][8];
 #pragma unroll
-  for (int c = 0; c < 2; ++c) {
-    const int at = (2 * (2 * pair + c) + half) * kTileBytes + 16 * lane;
-    widen8(*reinterpret_cast<const uint4*>(keys + kKeyColumns + at), cells_k[c]);
-    widen8(*reinterpret_cast<const uint4*>(keys + kQueryColumns + at), cells_q[c]);
+  for (int step = 0; step < 2; ++step) {
+    const int at = (2 * wave + step) * kTileBytes + 16 * lane;
+    widen8(*reinterpret_cast<const uint4*>(keys + kKeyColumns + at), cells_k[step]);
+    widen8(*reinterpret_cast<const uint4*>(keys + kQueryColumns + at), cells_q[step]);
   }
   __syncthreads();  // the last head's sums have been read
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < 4; ++i) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      float q = 0.0f, k = 0.0f;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        q = fmaf(cells_q[c][4 * i + j], d_q[c][i][j], q);
-        k = fmaf(cells_k[c][4 * i + j], d_k[c][i][j], k);
-      }
-      q = sum16(q), k = sum16(k);
+      const float q = sum16(cells_q[i >> 1][4 * (i & 1) + j] * d_q[i][j]);
+      const float k = sum16(cells_k[i >> 1][4 * (i & 1) + j] * d_k[i][j]);
       if (r == 0) {
-        s.sums[0][pair][16 * (2 * half + i) + 4 * g + j] = q;
-        s.sums[1][pair][16 * (2 * half + i) + 4 * g + j] = k;
+        s.sums[0][wave][16 * i + 4 * g + j] = q;
+        s.sums[1][wave][16 * i + 4 * g + j] = k;
       }
     }
   }
   __syncthreads();
+  // What of a token's gradients lies along its q and k, once for all wavefronts.
+  if (t < kChunk) {
+    const float k_unit = s.norms[0][t], q_unit = s.norms[1][t];
+    s.along[0][t] = a.normalize ? eight(0, t) * q_unit * s.norms[2][t] * s.norms[2][t] : 0.0f;
+    s.along[1][t] = a.normalize ? eight(1, t) * k_unit * k_unit * k_unit : 0.0f;
+  }
+  __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int tile = 2 * half + i;
-    f32x4 dq[2], dk[2];
+  for (int i = 0; i < 4; ++i) {
+    const int from = 16 * i + 4 * g;
+    const f32x4 k_unit = load4(&s.norms[0][from]), q_unit = load4(&s.norms[1][from]);
+    const f32x4 q_along = load4(&s.along[0][from]), k_along = load4(&s.along[1][from]);
+    f32x4 dq, dk;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int token = 16 * tile + 4 * g + j;
-      const float k_unit = s.norms[0][token], q_unit = s.norms[1][token];
-      float q_along = 0.0f, k_along = 0.0f;
-      if (a.normalize) {
-        q_along = ((s.sums[0][0][token] + s.sums[0][1][token]) +
-                   (s.sums[0][2][token] + s.sums[0][3][token])) *
-                  q_unit * s.norms[2][token] * s.norms[2][token];
-        k_along = ((s.sums[1][0][token] + s.sums[1][1][token]) +
-                   (s.sums[1][2][token] + s.sums[1][3][token])) *
-                  k_unit * k_unit * k_unit;
-      }
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        dq[c][j] = fmaf(-cells_q[c][4 * i + j], q_along, q_unit * d_q[c][i][j]);
-        dk[c][j] = fmaf(-cells_k[c][4 * i + j], k_along, k_unit * d_k[c][i][j]);
-      }
+      dq[j] = fmaf(-cells_q[i >> 1][4 * (i & 1) + j], q_along[j], q_unit[j] * d_q[i][j]);
+      dk[j] = fmaf(-cells_k[i >> 1][4 * (i & 1) + j], k_along[j], k_unit[j] * d_k[i][j]);
     }
     // Four tokens by four keys of a quad, transposed: lane 4 m + j gets token j's keys
-    // 8 m.. of the pair's 32, four of each tile.
-    uint2 q_run[2], k_run[2];
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      q_run[c] = transpose_quad(make_uint2(bf16_pair(dq[c][0], dq[c][1]),
-                                           bf16_pair(dq[c][2], dq[c][3])), lane);
-      k_run[c] = transpose_quad(make_uint2(bf16_pair(dk[c][0], dk[c][1]),
-                                           bf16_pair(dk[c][2], dk[c][3])), lane);
-    }
-    const int token = 16 * tile + 4 * g + (r & 3);
+    // state_key(wave, 4 m)..
+    const uint2 q_run =
+        transpose_quad(make_uint2(bf16_pair(dq[0], dq[1]), bf16_pair(dq[2], dq[3])), lane);
+    const uint2 k_run =
+        transpose_quad(make_uint2(bf16_pair(dk[0], dk[1]), bf16_pair(dk[2], dk[3])), lane);
+    const int token = from + (r & 3);
     if (token < count) {
-      const uint64_t at = ((first + token) * space.key_heads + head) * kDim + 32 * pair +
-                          8 * (r >> 2);
-      *reinterpret_cast<uint4*>(args.d_queries + at) =
-          make_uint4(q_run[0].x, q_run[0].y, q_run[1].x, q_run[1].y);
-      *reinterpret_cast<uint4*>(args.d_keys + at) =
-          make_uint4(k_run[0].x, k_run[0].y, k_run[1].x, k_run[1].y);
+      const uint64_t at = ((first + token) * space.key_heads + head) * kDim +
+                          state_key(wave, r & 12);
+      *reinterpret_cast<uint2*>(args.d_queries + at) = q_run;
+      *reinterpret_cast<uint2*>(args.d_keys + at) = k_run;
     }
   }
 }
