@@ -61,24 +61,37 @@ __global__ __launch_bounds__(kThreads) void request_tables_kernel(
   const uint32_t first = min(t * each, requests);
   const uint32_t last = min(first + each, requests);
 
-  // Token sums, cut off at max_tokens (64-bit: 4096 lengths of up to 2^31 - 1).
+  // Token sums, cut off at max_tokens (64-bit: 4096 lengths of up to 2^31 - 1).  The
+  // lengths are all asked for before the first is used.
+  int32_t own[kMaxRequests / kThreads];
+#pragma unroll
+  for (int i = 0; i < kMaxRequests / kThreads; ++i) {
+    own[i] = lengths[min(first + i, requests - 1)];
+  }
   int64_t sum = 0;
-  for (uint32_t r = first; r < last; ++r) sum += max(lengths[r], 0);
+#pragma unroll
+  for (int i = 0; i < kMaxRequests / kThreads; ++i) {
+    own[i] = first + i < last ? max(own[i], 0) : 0;
+    sum += own[i];
+  }
   int64_t total;
   int64_t at = prefix(sum, waves, total);
   const int64_t most = max_tokens;
   int64_t count = 0;
-  for (uint32_t r = first; r < last; ++r) {
+#pragma unroll
+  for (int i = 0; i < kMaxRequests / kThreads; ++i) {
     const int64_t begin = min(at, most);
-    at += max(lengths[r], 0);
-    token_sum[r] = static_cast<int32_t>(begin);
-    count += (min(at, most) - begin + kChunk - 1) / kChunk;
+    at += own[i];
+    own[i] = static_cast<int32_t>((min(at, most) - begin + kChunk - 1) / kChunk);
+    count += own[i];
+    if (first + i < last) token_sum[first + i] = static_cast<int32_t>(begin);
   }
   if (t == 0) token_sum[requests] = static_cast<int32_t>(min(total, most));
   int64_t chunk = prefix(count, waves, total);  // its barriers publish token_sum
-  for (uint32_t r = first; r < last; ++r) {
-    chunk_sum[r] = static_cast<int32_t>(chunk);
-    chunk += (token_sum[r + 1] - token_sum[r] + kChunk - 1) / kChunk;
+#pragma unroll
+  for (int i = 0; i < kMaxRequests / kThreads; ++i) {
+    if (first + i < last) chunk_sum[first + i] = static_cast<int32_t>(chunk);
+    chunk += own[i];
   }
   if (t == 0) chunk_sum[requests] = static_cast<int32_t>(total);
   __syncthreads();
@@ -113,6 +126,7 @@ __global__ __launch_bounds__(kThreads) void request_tables_kernel(
   if (r < requests) {  // the same for the 16 lanes of a request
     const int mine = chunk_sum[r + 1] - chunk_sum[r];
     int before = 0;
+#pragma unroll 8
     for (uint32_t s = t & 15; s < requests; s += 16) {
       const int other = chunk_sum[s + 1] - chunk_sum[s];
       before += other > mine || (other == mine && s < r) ? 1 : 0;
