@@ -119,22 +119,39 @@ __global__ __launch_bounds__(kThreads) void gated_norm_backward_kernel(
   }
 }
 
-// d_w[column] = sum over `count` partials, 8 columns a workgroup: 32 threads a
-// column add every 32nd row, then one wavefront adds their sums in order.
-__global__ __launch_bounds__(kThreads) void weight_sum_kernel(
+// d_w[column] = sum over `count` partials, 8 columns a workgroup: 128 threads a column
+// add every 128th row, four of them asked for at a time, and one wavefront adds their
+// sums in a fixed order.
+constexpr int kSumThreads = 1024;
+constexpr int kSumGroups = kSumThreads / 8;
+
+__global__ __launch_bounds__(kSumThreads) void weight_sum_kernel(
     const float* __restrict__ partials, float* __restrict__ d_weight, uint32_t count,
     uint32_t width) {
-  __shared__ float parts[32][9];
-  const int column = threadIdx.x & 7, group = threadIdx.x >> 3;
+  __shared__ float parts[kSumGroups][9];
+  const int column = threadIdx.x & 7;
+  const uint32_t group = threadIdx.x >> 3;
   const float* p = partials + 8 * static_cast<uint64_t>(blockIdx.x) + column;
   float sum = 0.0f;
-  for (uint32_t i = group; i < count; i += 32) sum += p[static_cast<uint64_t>(i) * width];
+  for (uint32_t i = group; i < count; i += 4 * kSumGroups) {
+    float x[4];
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u) {
+      x[u] = p[static_cast<uint64_t>(min(i + u * kSumGroups, count - 1)) * width];
+    }
+#pragma unroll
+    for (uint32_t u = 0; u < 4; ++u) sum += i + u * kSumGroups < count ? x[u] : 0.0f;
+  }
   parts[group][column] = sum;
   __syncthreads();
-  if (threadIdx.x < 8) {
-    float total = parts[0][threadIdx.x];
-    for (int i = 1; i < 32; ++i) total += parts[i][threadIdx.x];
-    d_weight[8 * blockIdx.x + threadIdx.x] = total;
+  if (threadIdx.x < 64) {
+    float total = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSumGroups / 8; ++i) total += parts[kSumGroups / 8 * group + i][column];
+    total += __shfl_xor(total, 8);
+    total += __shfl_xor(total, 16);
+    total += __shfl_xor(total, 32);
+    if (group == 0) d_weight[8 * blockIdx.x + column] = total;
   }
 }
 
@@ -294,7 +311,7 @@ uint32_t most_partials(uint64_t rows, uint32_t width) {
 
 int32_t add_partials(void* stream, const float* partials, float* d_weight, uint32_t count,
                      uint32_t width) {
-  return launch(weight_sum_kernel, dim3(width / 8), dim3(kThreads), stream, partials, d_weight,
+  return launch(weight_sum_kernel, dim3(width / 8), dim3(kSumThreads), stream, partials, d_weight,
                 count, width);
 }
 
