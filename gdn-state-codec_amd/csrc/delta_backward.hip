@@ -412,9 +412,10 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
   const uint32_t row = blockIdx.x / space.key_heads;
   const uint32_t head = blockIdx.x % space.key_heads;
   const uint64_t token_step = static_cast<uint64_t>(space.value_heads) * kDim;
-  if (row == 0) {  // tokens of no request: zeros
+  {  // tokens of no request: zeros, a share of them for each chunk row
     const uint32_t from = min(static_cast<uint32_t>(a.offsets[a.requests]), a.tokens);
-    for (uint64_t token = from; token < a.tokens; ++token) {
+    for (uint64_t token = from + static_cast<uint64_t>(row); token < a.tokens;
+         token += space.rows) {
       for (uint32_t i = t; i < a.group * kDim; i += kThreads) {
         args.d_values[token * token_step + head * a.group * kDim + i] = 0;
       }

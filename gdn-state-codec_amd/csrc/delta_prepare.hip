@@ -252,14 +252,17 @@ __device__ __forceinline__ void read_out_head(const Staged& s, const Head& head,
   }
 }
 
-// The outputs of tokens of no request: zeros, for one key head's value heads.
-__device__ __forceinline__ void clear_rest(const RuleArgs& a, uint32_t head,
+// The outputs of tokens of no request: zeros, for one key head's value heads, a share of
+// the tokens for each chunk row.
+__device__ __forceinline__ void clear_rest(const RuleArgs& a, uint32_t row, uint32_t head,
                                            bf16_bits* outputs) {
   const uint32_t from = min(static_cast<uint32_t>(a.offsets[a.requests]), a.tokens);
   const uint32_t width = a.group * kDim;
-  for (uint64_t i = threadIdx.x; i < static_cast<uint64_t>(a.tokens - from) * width;
-       i += kThreads) {
-    outputs[(from + i / width) * a.space.value_heads * kDim + head * width + i % width] = 0;
+  for (uint64_t token = from + static_cast<uint64_t>(row); token < a.tokens;
+       token += a.space.rows) {
+    for (uint32_t i = threadIdx.x; i < width; i += kThreads) {
+      outputs[token * a.space.value_heads * kDim + head * width + i] = 0;
+    }
   }
 }
 
@@ -272,7 +275,7 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(RuleArgs a,
   const uint32_t head = blockIdx.x % a.space.key_heads;
   const int4 chunk = a.chunks[row];
   const int count = chunk_tokens(a, chunk);
-  if (kTrain && row == 0) clear_rest(a, head, outputs);
+  if (kTrain) clear_rest(a, row, head, outputs);
   if (count == 0 || (!kTrain && chunk.w < 0)) return;  // past the last chunk, or padding
   const uint64_t first = chunk.y;
 
