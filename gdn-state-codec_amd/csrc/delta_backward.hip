@@ -108,7 +108,9 @@ static_assert(kHeadFactors <= 2 * kTileBytes, "the factors' tiles");
 static_assert(kStage <= kLdsPerCu, "a compute unit's LDS");
 
 // A workgroup takes 64 columns, two wavefronts for each 16: one the chain, the other
-// the operands' loads, the two products that need no state, and the stores.
+// the operands' loads, the two products that need no state, and the stores.  5.9 us a
+// chunk of 128 heads at once, bound by the 112 KiB a chunk and head that it stores (6.9
+// with one wavefront for all of it), 4.7 of 32 heads.
 __global__ __launch_bounds__(128 * kWaves) void delta_back_wide_kernel(BackArgs args) {
   __shared__ __align__(16) char stage[kStage];
   const RuleArgs& a = args.rule;
@@ -394,7 +396,7 @@ __global__ __launch_bounds__(128 * kWaves) void delta_back_wide_kernel(BackArgs 
 
 // A workgroup takes 16 columns.  Four wavefronts share the chain's products by token
 // rows (or state rows), four the two products beside it in the same way and the stores,
-// with three exchanges a chunk, as the forward scan's narrow form.
+// with three exchanges a chunk, as the forward scan's narrow form.  3.4 us a chunk.
 __global__ __launch_bounds__(512) void delta_back_narrow_kernel(BackArgs args) {
   constexpr int kNarrow = kDim / 16;
   // Parts of dS1 (4 steps over the keys), of b V' and of -exp(G) Y / |k| (2 steps over
@@ -735,6 +737,15 @@ static_assert(sizeof(Gradient) <= kLdsPerCu, "one workgroup a compute unit");
 // One workgroup per chunk row and key head.  Wavefront w takes the keys of state tile w
 // and all tokens, so that a state is loaded and cut into parts once.  X and E are cut
 // once, by the wavefront that loads them, and so are F and H.
+//
+// 32 heads of 85 chunks take 264 us: 650 MB of states, E and X (2.5 TB/s), 2,850 matrix
+// instructions a chunk and head (18% of their rate).  The parts of X and E leave room
+// for one workgroup a compute unit, whose phases (loads, F and H, the states' products,
+// the kinds) wait for each other: of some 35,000 cycles a head, loads take a third and
+// LDS reads as much.  Measured and left out: the next head's X and E asked for a phase
+// ahead in a loop over chunks (286 us, with the registers it takes), F and H dealt out
+// evenly (274), two tiles of keys by two of tokens a wavefront (262, every state loaded
+// and cut twice).
 __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args) {
   __shared__ __align__(16) Gradient s;
   const RuleArgs& a = args.rule;

@@ -15,9 +15,9 @@
 // half a chunk ahead, forms the outputs half a chunk behind and stores what training
 // keeps; it takes S0 and E from LDS.  Bound by the chain's 132 matrix instructions and
 // the vector instructions between them: 3.1 us a chunk (32 heads of one request), where
-// the products alone would take 0.9; in training by the 96 KiB a chunk and head that it
-// stores as well, 5.6 us (128 heads at once, 3 TB/s).  With one wavefront for both the
-// chain and the rest these were 4.1 and 6.8.
+// the products alone would take 0.9; in training by the 112 KiB a chunk and head that it
+// stores, 5.8 us (128 heads at once, 2.5 TB/s; without the stores 3.8).  With one
+// wavefront for both the chain and the rest these were 4.1 and 6.8.
 //
 // delta_scan_narrow_kernel, for few heads, where a long request's chain is all there
 // is: a workgroup takes 16 columns, and its wavefronts share each product by token

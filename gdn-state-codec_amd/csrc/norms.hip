@@ -11,6 +11,10 @@
 //
 // Every kernel reads each input and writes each output once, which is what
 // bounds it (HBM); a row stays in registers between its sum and its outputs.
+// 8192 x 32 rows of 128 (bf16): forward 31 us (201 MB), backward 58 (335 MB, 5.8 TB/s)
+// and 4 for the sum of its partials.  8192 rows of 4096 (bf16, fp32 stream): forward 72
+// us (403 MB, 5.6 TB/s), backward 109 (537 MB, 4.9 TB/s) and 7.  256 rows of either:
+// 3.2 us, a launch.
 // Sums are fp32; each output is rounded once, to its own type.  The new residual
 // stream is rounded before the norm is taken, so that y is the norm of what the
 // next layer reads and the backward pass needs only the stored stream.
