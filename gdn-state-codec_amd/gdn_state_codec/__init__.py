@@ -1,7 +1,8 @@
 """MI355X (gfx950) GDN state codec: int8 codec of Qwen3.5 gated-delta-net
 recurrent-state head tiles, the encoded projection, the windowed decode step,
 its window-boundary refit and the LQCAPS01 capsule wire format, behind the
-reference's ``statecentric_gdn_state_codec_*`` C-ABI."""
+reference's ``statecentric_gdn_state_codec_*`` C-ABI; and the dense operators of a
+gated-delta-net layer around that state (``layer``)."""
 
 from ._native import NativeLibrary, library_dir, library_path, native
 from .codec import (

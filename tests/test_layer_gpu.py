@@ -161,6 +161,13 @@ def test_prefill_of_many_heads_takes_the_wide_form(device):
     _prefill(device, [100, 30, 0, 64, 129, 1, 70, 3, 65], 6, 3, torch.float32, True, seed=24)
 
 
+@pytest.mark.parametrize("pool_dtype,normalize", [
+    (torch.bfloat16, True), (torch.float32, False)])
+@pytest.mark.parametrize("lengths", [[1] * 9, [64] * 9, [0, 330, 2, 63, 65, 0, 128, 127, 5]])
+def test_prefill_variants_of_the_wide_form(device, lengths, pool_dtype, normalize):
+    _prefill(device, lengths, 4, 2, pool_dtype, normalize, seed=27)
+
+
 def _prefill(device, lengths, heads, key_heads, pool_dtype, normalize, seed, decay="mixed",
              alike=False, state_bound=FP32):
     n, total = len(lengths), sum(lengths)
@@ -371,6 +378,18 @@ def test_train_variants(device, options):
 
 def test_train_of_many_heads_takes_the_wide_form(device):
     _train(device, [65, 20, 0, 70, 1], 8, 4, 45)
+
+
+@pytest.mark.parametrize("options", [
+    dict(), dict(normalize=False, scale=0.5), dict(decay="none"), dict(decay="strong"),
+    dict(resumed=False), dict(final_used=False), dict(rest=700)])
+def test_train_variants_of_the_wide_form(device, options):
+    _train(device, [200, 1, 64, 0, 130, 63], 6, 3, 47, **options)
+
+
+def test_train_of_one_chunk_and_of_many_in_both_forms(device):
+    _train(device, [330], 2, 1, 49)
+    _train(device, [330] + [2] * 16, 2, 1, 51)
 
 
 def test_forward_differences_of_the_kernels_themselves(device):
