@@ -108,6 +108,13 @@ constexpr int kReadOut = kSolve + kTriangleBytes;
 constexpr int kSolveBack = kReadOut + kReadOutBytes;
 constexpr int kReadBack = kSolveBack + kTriangleBytes;
 
+// A long sequence of few heads is served in segments (delta_scan.hip): states between
+// them and their maps, at most as many as half the compute units of each.
+constexpr uint32_t kSplitItems = 32;    // requests x heads at most
+constexpr uint32_t kSplitChunks = 64;   // chunks of a request at least, on the average
+constexpr uint32_t kMostSegments = 16;  // after the first
+constexpr uint32_t kSegmentStates = kComputeUnits;
+
 // One chunk's key block, value block and, for training, states and rows.
 struct ChunkSpace {
   char* base;
@@ -123,12 +130,18 @@ struct ChunkSpace {
   // Training: the start state and the end state's gradient of each chunk and value
   // head (fp32, 8 tiles of keys), then E and X (4 tiles of tokens each), in cells_at's
   // order.
+  // For serving, the states between segments, where there may be any.
+  __host__ __device__ bool may_split() const {
+    return !train && value_heads <= kSplitItems && rows >= kSplitChunks;
+  }
   __host__ __device__ uint64_t total() const {
     return states_at() + (train ? static_cast<uint64_t>(rows) * value_heads *
                                       (2 * kTile + 2 * kChunk * kDim) * 4
-                                : 0) +
+                          : may_split() ? static_cast<uint64_t>(kSegmentStates) * kTile * 4
+                                        : 0) +
            kTileBytes;  // blocks are read in whole tiles
   }
+  __device__ float* segments() const { return reinterpret_cast<float*>(base + states_at()); }
   __device__ char* key_block(uint32_t row, uint32_t head) const {
     return base + (static_cast<uint64_t>(row) * key_heads + head) * key_block_bytes(train);
   }

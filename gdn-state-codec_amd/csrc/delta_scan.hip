@@ -6,7 +6,7 @@
 //   S0 -> K S0 -> R -> N (b R) -> E -> K^T U -> S1,
 // chunk after chunk.  Per chunk and 16 columns it issues
 //   K S0: 48, N (b R): 36, K^T U: 48, and beside the chain Q S0: 32, (P b) E: 18
-// matrix instructions.  Two forms:
+// matrix instructions.  Two forms, and a third made of the first:
 //
 // delta_scan_wide_kernel, for throughput: a workgroup takes 64 columns, with two
 // wavefronts for each 16.  One runs the chain with all 64 tokens, the state in its
@@ -24,8 +24,18 @@
 // rows (or state rows), four on the chain and four on the outputs.  What a product
 // hands to the next goes through LDS, three exchanges a chunk; a wavefront's own
 // operands go from global memory to its registers a chunk ahead.  2.1 us a chunk.
+//
+// delta_segment_kernel, for long requests of few heads: the chain is linear in the state,
+// S1 = M S0 + B, so a request's chunks are cut into segments whose B and M (the same
+// chain from zeros, and from the identity without values) are found at once; joined in
+// order (delta_join_kernel) they give each segment's start, from which a second pass
+// runs all segments at once.  About three times the work, on all compute units instead
+// of a few.  With unit keys and strengths of 0 to 1 every M is a contraction; with others
+// it grows as the states themselves would.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+
+#include <algorithm>
 
 #include "delta_chunk.h"
 
@@ -41,6 +51,8 @@ struct ScanArgs {
   const int32_t* resume;     // 0: start from zeros, or null: all resume
   uint32_t slots;
   bf16_bits* outputs;        // [tokens][value head][128]
+  uint32_t segments;         // after a request's first, and which of the two passes
+  uint32_t pass;
 };
 
 namespace {
@@ -74,6 +86,50 @@ __device__ __forceinline__ bool find_work(const ScanArgs& args, uint64_t item, W
   w.begin = min(static_cast<uint32_t>(a.offsets[w.request]), a.tokens);
   w.length = min(static_cast<uint32_t>(a.offsets[w.request + 1]), a.tokens) - w.begin;
   w.chunks = min(rows, (w.length + kChunk - 1) / kChunk);
+  return true;
+}
+
+// One segment of a request's chunks, and what becomes of its state.
+struct Segment {
+  const float* start;  // the state before it, as accumulators; or null: the pool's, or zeros
+  float* end;          // the state after it; or null: the pool's
+  bool map;            // from the identity, without values: end = map x start + the rest
+  bool outputs, keep;  // whether it forms outputs, and leaves its state
+};
+
+// The segments' states of an item: before segments 1.., then the maps of 1.. .
+__device__ __forceinline__ float* segment_state(const ScanArgs& args, uint64_t item,
+                                                uint32_t at) {
+  return args.rule.space.segments() + (item * (2 * args.segments - 1) + at) * kTile;
+}
+
+// Task `task` of a pass: `segments` + 1 parts of each item's chunks.  The first pass runs
+// the first part whole, and of all others but the last finds what they add (from zeros)
+// and, `second`, their maps; the second pass runs all others whole.  The first part is as
+// much longer as a chunk of both takes longer than a chunk whole.
+__device__ __forceinline__ bool find_segment(const ScanArgs& args, uint64_t task, bool second,
+                                             Work& w, Segment& s) {
+  const uint64_t items = static_cast<uint64_t>(args.rule.requests) * args.rule.space.value_heads;
+  const uint64_t item = task % items;
+  const uint32_t n = args.segments;
+  const uint32_t part = static_cast<uint32_t>(task / items) + args.pass;
+  if (part >= n + args.pass || !find_work(args, item, w)) return false;
+  const uint32_t whole = w.chunks;
+  const uint32_t first = whole < 4 * n ? whole : (3 * whole + 2 * n + 2) / (2 * n + 3);
+  const uint32_t each = (whole - first + n - 1) / n;
+  const uint32_t from = part == 0 ? 0 : min(first + (part - 1) * each, whole);
+  const uint32_t to = part == 0 ? first : min(from + each, whole);
+  s.outputs = part == 0 || args.pass != 0;
+  s.map = !s.outputs && second;
+  s.start = part == 0 || args.pass == 0 ? nullptr : segment_state(args, item, part - 1);
+  s.end = s.map ? segment_state(args, item, n + part - 1)
+          : part == n ? nullptr : segment_state(args, item, part);
+  s.keep = args.pass == 0 || part == n;
+  if (part != 0) w.resumed = false;
+  w.first_row += from;
+  w.begin += from * kChunk;
+  w.length = to == whole ? w.length - from * kChunk : (to - from) * kChunk;
+  w.chunks = to - from;
   return true;
 }
 
@@ -134,22 +190,92 @@ __device__ __forceinline__ void split2(const f32x4& x, const f32x4& y, uint4 (&p
   part[0] = all[0], part[1] = all[1];
 }
 
-template <typename Pool, bool kTrain>
-__global__ __launch_bounds__(128 * kWideWaves) void delta_scan_wide_kernel(ScanArgs args) {
-  __shared__ __align__(16) char stage[kStage];
+// The chain's three products, of one wavefront's 16 columns.  R = V - exp(G) K S0, from
+// the state's parts, and from rows of V as fetched (columns 4 (r / 4).. of tokens 16 t +
+// 4 g + (r & 3)) or none.
+__device__ __forceinline__ void chain_rest(const uint4* k_rows, const uint4 (&parts)[4][3],
+                                           const f32x4 (&factors)[4], const uint2 (&values)[4],
+                                           bool none, int lane, f32x4 (&error)[4]) {
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    f32x4 seen[2] = {};  // two sums, so that each product waits for the last but one
+#pragma unroll
+    for (int step = 0; step < 4; ++step) {
+      const uint4 k = k_rows[(4 * t + step) * 64];
+#pragma unroll
+      for (int p = 2; p >= 0; --p) seen[p & 1] = mfma(k, parts[step][p], seen[p & 1]);
+    }
+    const f32x4 read_key = of_rows(factors[t][kReadKey]);
+    f32x4 x = value_rows(values[t], lane);
+    if (none) x = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) error[t][i] = fmaf(-read_key[i], seen[0][i] + seen[1][i], x[i]);
+  }
+}
+
+// E = R + N (b R)
+__device__ __forceinline__ void chain_solve(const uint4* solve, const f32x4 (&factors)[4],
+                                            f32x4 (&error)[4]) {
+  uint4 part[2][3];
+#pragma unroll
+  for (int step = 0; step < 2; ++step) {
+    f32x4 x[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const f32x4 b = of_rows(factors[2 * step + u][kStrength]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[u][i] = b[i] * error[2 * step + u][i];
+    }
+    split3(x[0], x[1], part[step]);
+  }
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+#pragma unroll
+    for (int step = 0; step < lower_steps(t); ++step) {
+      uint4 n[3];
+#pragma unroll
+      for (int p = 0; p < 3; ++p) n[p] = solve[(p * kTriangle + lower_tile(t, step)) * 64];
+      error[t] = mfma6(n, part[step], error[t]);
+    }
+  }
+}
+
+// S1 = exp(G_63) S0 + K^T (write b E)
+__device__ __forceinline__ void chain_state(const uint4* k_columns, const f32x4 (&factors)[4],
+                                            const f32x4 (&error)[4], f32x4 (&state)[8]) {
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) state[t][i] *= factors[0][kWhole];
+  }
+#pragma unroll
+  for (int step = 0; step < 2; ++step) {
+    uint4 written[3];
+    f32x4 x[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const f32x4 write = of_rows(factors[2 * step + u][kWrite]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[u][i] = write[i] * error[2 * step + u][i];
+    }
+    split3(x[0], x[1], written);
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      state[t] = mfma3(k_columns[(2 * t + step) * 64], written, state[t]);
+    }
+  }
+}
+
+// A request's chunks, or one segment's, of the value head and columns `block` of `w`.
+template <typename Pool, bool kTrain, bool kSplit>
+__device__ __forceinline__ void scan_columns(const ScanArgs& args, const Work& w,
+                                             const Segment& part, int block, char* stage) {
   const RuleArgs& a = args.rule;
   const ChunkSpace& space = a.space;
-  // A head's slices share their operands: they get consecutive places of one XCD
-  // (the dispatcher deals workgroups out to the 8 XCDs in turn).
-  const uint32_t turn = blockIdx.x >> 3;
-  Work w;
-  if (!find_work(args, static_cast<uint64_t>(turn / kWideSlices) * 8 + (blockIdx.x & 7), w)) {
-    return;
-  }
   const int place = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wave = place % kWideWaves;
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int slice = kWideWaves * (turn % kWideSlices) + wave;
+  const int slice = kWideWaves * block + wave;
   const int first_value = 16 * slice, value = first_value + r;
   const uint32_t key_head = w.head / a.group;
   const uint32_t length = w.length, chunks = w.chunks;
@@ -162,7 +288,7 @@ __global__ __launch_bounds__(128 * kWideWaves) void delta_scan_wide_kernel(ScanA
 
   if (place >= kWideWaves) {  // the operands' loads, the outputs, training's stores
     const uint32_t stage_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
-        (__attribute__((address_space(3))) char*)&stage[0]));
+        (__attribute__((address_space(3))) char*)stage));
     const uint32_t key_step = static_cast<uint32_t>(a.key_stride) * 2;
     const uint32_t query_step = static_cast<uint32_t>(a.query_stride) * 2;
     const uint32_t out_step = space.value_heads * kDim * 2;
@@ -268,10 +394,10 @@ __global__ __launch_bounds__(128 * kWideWaves) void delta_scan_wide_kernel(ScanA
         queries[t] =
             reinterpret_cast<const float*>(stage)[kReadQuery + 16 * t + 4 * g + (r & 3)];
       }
-      uint4 part[4][2];
+      uint4 parts[4][2];
 #pragma unroll
       for (int step = 0; step < 4; ++step) {
-        split2(state[2 * step], state[2 * step + 1], part[step]);
+        split2(state[2 * step], state[2 * step + 1], parts[step]);
       }
       if constexpr (kTrain) {
 #pragma unroll
@@ -291,8 +417,8 @@ __global__ __launch_bounds__(128 * kWideWaves) void delta_scan_wide_kernel(ScanA
 #pragma unroll
         for (int step = 0; step < 4; ++step) {
           const uint4 q = q_rows[(4 * t + step) * 64];
-          read[0] = mfma(q, part[step][1], read[0]);
-          read[1] = mfma(q, part[step][0], read[1]);
+          read[0] = mfma(q, parts[step][1], read[0]);
+          read[1] = mfma(q, parts[step][0], read[1]);
         }
         const f32x4 read_query = of_rows(queries[t]);
 #pragma unroll
@@ -308,7 +434,14 @@ __global__ __launch_bounds__(128 * kWideWaves) void delta_scan_wide_kernel(ScanA
 
   // The chain.
   f32x4 state[8];
-  load_state(static_cast<const Pool*>(args.initial) + w.tile, 0, value, g, w.resumed, state);
+  if (kSplit && part.start) {
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      state[t] = load4(part.start + slice * slice_cells(8) + 256 * t + 4 * lane);
+    }
+  } else {
+    load_state(static_cast<const Pool*>(args.initial) + w.tile, 0, value, g, w.resumed, state);
+  }
   const uint32_t value_step = static_cast<uint32_t>(a.value_stride) * 2;
   uint2 values[4];  // columns 4 (r / 4).. of tokens 16 t + 4 g + (r & 3)
   const auto fetch_values = [&](uint32_t c) {
@@ -328,12 +461,12 @@ __global__ __launch_bounds__(128 * kWideWaves) void delta_scan_wide_kernel(ScanA
   if (chunks != 0) fetch_values(0);
   __builtin_amdgcn_s_setprio(1);
   for (uint32_t c = 0; c < chunks; ++c) {
-    uint4 part[4][3];  // of the state, over the keys
+    uint4 parts[4][3];  // of the state, over the keys
 #pragma unroll
     for (int t = 0; t < 8; ++t) state_cells[64 * t] = state[t];
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
-      split3(state[2 * step], state[2 * step + 1], part[step]);
+      split3(state[2 * step], state[2 * step + 1], parts[step]);
     }
     exchange();
     f32x4 factors[4];  // of tokens 16 t + 4 g + (r & 3)
@@ -341,75 +474,222 @@ __global__ __launch_bounds__(128 * kWideWaves) void delta_scan_wide_kernel(ScanA
     for (int t = 0; t < 4; ++t) {
       factors[t] = reinterpret_cast<const f32x4*>(stage)[16 * t + 4 * g + (r & 3)];
     }
-    // R = V - exp(G) K S0
     f32x4 error[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      f32x4 seen[2] = {};  // two sums, so that each product waits for the last but one
-#pragma unroll
-      for (int step = 0; step < 4; ++step) {
-        const uint4 k = k_rows[(4 * t + step) * 64];
-#pragma unroll
-        for (int p = 2; p >= 0; --p) seen[p & 1] = mfma(k, part[step][p], seen[p & 1]);
-      }
-      const f32x4 read_key = of_rows(factors[t][kReadKey]);
-      const f32x4 x = value_rows(values[t], lane);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) error[t][i] = fmaf(-read_key[i], seen[0][i] + seen[1][i], x[i]);
-    }
+    chain_rest(k_rows, parts, factors, values, false, lane, error);
     if (c + 1 < chunks) fetch_values(c + 1);
-    // E = R + N (b R)
-    {
-      uint4 part[2][3];
+    chain_solve(solve, factors, error);
+    f32x4* const cells = error_cells(c);
 #pragma unroll
-      for (int step = 0; step < 2; ++step) {
-        f32x4 x[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const f32x4 b = of_rows(factors[2 * step + u][kStrength]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[u][i] = b[i] * error[2 * step + u][i];
-        }
-        split3(x[0], x[1], part[step]);
-      }
-      f32x4* const cells = error_cells(c);
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-#pragma unroll
-        for (int step = 0; step < lower_steps(t); ++step) {
-          uint4 n[3];
-#pragma unroll
-          for (int p = 0; p < 3; ++p) n[p] = solve[(p * kTriangle + lower_tile(t, step)) * 64];
-          error[t] = mfma6(n, part[step], error[t]);
-        }
-        cells[64 * t] = error[t];
-      }
-    }
+    for (int t = 0; t < 4; ++t) cells[64 * t] = error[t];
     exchange();
-    // S1 = exp(G_63) S0 + K^T (write b E)
+    chain_state(k_columns, factors, error, state);
+  }
+  if (kSplit && !part.keep) return;
+  if (kSplit && part.end) {
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) state[t][i] *= factors[0][kWhole];
+      store_cells(part.end + slice * slice_cells(8) + 256 * t + 4 * lane, state[t]);
     }
+  } else {
+    store_state(static_cast<Pool*>(args.final_states) + w.tile, 0, value, g, state);
+  }
+}
+
+template <typename Pool, bool kTrain>
+__global__ __launch_bounds__(128 * kWideWaves) void delta_scan_wide_kernel(ScanArgs args) {
+  __shared__ __align__(16) char stage[kStage];
+  // A head's slices share their operands: they get consecutive places of one XCD
+  // (the dispatcher deals workgroups out to the 8 XCDs in turn).
+  const uint32_t turn = blockIdx.x >> 3;
+  Work w;
+  if (!find_work(args, static_cast<uint64_t>(turn / kWideSlices) * 8 + (blockIdx.x & 7), w)) {
+    return;
+  }
+  scan_columns<Pool, kTrain, false>(args, w, Segment{}, turn % kWideSlices, stage);
+}
+
+// ------------------------------------------------------------ segments
+
+// What a segment makes of its state and no more: eight wavefronts, all columns, each the
+// chain of 16.  The factors, N, K rows and K^T of a chunk come into LDS while the last
+// chunk is at work.
+constexpr int kChainKeys = kBlockTiles * kTileBytes;
+constexpr int kChainColumns = kChainKeys + kKeyTiles * kTileBytes;
+constexpr int kChainStage = kChainColumns + kKeyTiles * kTileBytes;
+static_assert(2 * kChainStage <= kStage, "two stages in the other form's LDS");
+
+__device__ __forceinline__ void scan_state(const ScanArgs& args, const Work& w,
+                                           const Segment& part, char* stage) {
+  constexpr int kWaves = 8;
+  const RuleArgs& a = args.rule;
+  const ChunkSpace& space = a.space;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int value = 16 * wave + r;
+  const uint32_t key_head = w.head / a.group;
+  const uint32_t length = w.length, chunks = w.chunks;
+  const uint32_t stage_at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+      (__attribute__((address_space(3))) char*)stage));
+  const uint32_t key_step = static_cast<uint32_t>(a.key_stride) * 2;
+  const uint32_t value_step = static_cast<uint32_t>(a.value_stride) * 2;
+  const uint32_t linear = 16 * lane;
+  uint2 values[4];
+  // Piece i of 0..6; and the values.
+  const auto fetch = [&](uint32_t c, int i) {
+    const uint32_t to = stage_at + (c & 1) * kChainStage;
+    if (i < 2) {  // K rows 16 (tile / 4).., keys 32 (tile % 4)..
+      const uint64_t token = w.begin + c * kChunk;
+      const uint32_t last = min(length - c * kChunk, static_cast<uint32_t>(kChunk)) - 1;
+      const char* k = reinterpret_cast<const char*>(a.keys + token * a.key_stride +
+                                                    key_head * kDim);
+      const int tile = kWaves * i + wave;
+      const uint32_t row = min(static_cast<uint32_t>(16 * (tile >> 2) + r), last);
+      stage_tile(k + 64 * (tile & 3), row * key_step + 16 * g,
+                 to + kChainKeys + tile * kTileBytes);
+    } else if (i < 4) {
+      const int tile = kWaves * (i - 2) + wave;
+      stage_tile(space.key_block(w.first_row + c, key_head) + kKeyColumns + tile * kTileBytes,
+                 linear, to + kChainColumns + tile * kTileBytes);
+    } else {
+      const int tile = min(kWaves * (i - 4) + wave, kBlockTiles - 1);  // the last one again
+      stage_tile(space.value_block(w.first_row + c, w.head) + tile * kTileBytes, linear,
+                 to + tile * kTileBytes);
+    }
+  };
+  const auto fetch_values = [&](uint32_t c) {
+    const uint64_t token = w.begin + c * kChunk;
+    const uint32_t last = min(length - c * kChunk, static_cast<uint32_t>(kChunk)) - 1;
+    const char* v = reinterpret_cast<const char*>(a.values + token * a.value_stride +
+                                                  w.head * kDim + 16 * wave);
 #pragma unroll
-    for (int step = 0; step < 2; ++step) {
-      uint4 written[3];
-      f32x4 x[2];
+    for (int t = 0; t < 4; ++t) {
+      const uint32_t row = min(static_cast<uint32_t>(16 * t + 4 * g + (r & 3)), last);
+      values[t] = *reinterpret_cast<const uint2*>(v + (row * value_step + 2 * (r & 12)));
+    }
+  };
+
+  f32x4 state[8];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const f32x4 write = of_rows(factors[2 * step + u][kWrite]);
+  for (int t = 0; t < 8; ++t) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x[u][i] = write[i] * error[2 * step + u][i];
-      }
-      split3(x[0], x[1], written);
-#pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        state[t] = mfma3(k_columns[(2 * t + step) * 64], written, state[t]);
-      }
+    for (int i = 0; i < 4; ++i) {
+      state[t][i] = part.map && state_key(t, 4 * g + i) == value ? 1.0f : 0.0f;
     }
   }
-  store_state(static_cast<Pool*>(args.final_states) + w.tile, 0, value, g, state);
+  if (chunks != 0) {
+#pragma unroll
+    for (int i = 0; i < 7; ++i) fetch(0, i);
+    fetch_values(0);
+  }
+  for (uint32_t c = 0; c < chunks; ++c) {
+    stage_ready();  // this chunk's operands are there, the last one's have been read
+    const char* const at = stage + (c & 1) * kChainStage;
+    const uint32_t next = min(c + 1, chunks - 1);
+    f32x4 factors[4];  // of tokens 16 t + 4 g + (r & 3)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      factors[t] = reinterpret_cast<const f32x4*>(at)[16 * t + 4 * g + (r & 3)];
+      // Used before the next loads are issued, so that no wait for it covers them.
+      asm volatile("" : "+v"(values[t].x), "+v"(values[t].y));
+    }
+    uint4 parts[4][3];  // of the state, over the keys
+#pragma unroll
+    for (int step = 0; step < 4; ++step) {
+      split3(state[2 * step], state[2 * step + 1], parts[step]);
+      __builtin_amdgcn_sched_barrier(0);
+      if (c + 1 < chunks) {
+        fetch(c + 1, 2 * step);
+        if (step < 3) fetch(c + 1, 2 * step + 1);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    f32x4 error[4];
+    chain_rest(reinterpret_cast<const uint4*>(at + kChainKeys) + lane, parts, factors, values,
+               part.map, lane, error);
+    fetch_values(next);
+    chain_solve(reinterpret_cast<const uint4*>(at + kSolve) + lane, factors, error);
+    chain_state(reinterpret_cast<const uint4*>(at + kChainColumns) + lane, factors, error,
+                state);
+  }
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    store_cells(part.end + wave * slice_cells(8) + 256 * t + 4 * lane,
+                part.map ? transpose_quad(state[t], lane) : state[t]);
+  }
+}
+
+template <typename Pool>
+__global__ __launch_bounds__(128 * kWideWaves) void delta_segment_kernel(ScanArgs args) {
+  __shared__ __align__(16) char stage[kStage];
+  const uint32_t turn = blockIdx.x >> 3;  // the two workgroups of a segment on one XCD
+  const uint64_t task = static_cast<uint64_t>(turn / 2) * 8 + (blockIdx.x & 7);
+  Work w;
+  Segment part;
+  if (!find_segment(args, task, turn % 2 != 0, w, part)) return;
+  if (part.outputs) {
+    scan_columns<Pool, false, true>(args, w, part, turn % 2, stage);
+  } else {
+    scan_state(args, w, part, stage);
+  }
+}
+
+// The states before segments 2..: a segment's map times the state before it, and what it
+// adds (which its place holds).  One workgroup per item and 16 columns, wavefront w the
+// state's tiles 2 w and 2 w + 1.
+__global__ __launch_bounds__(256) void delta_join_kernel(ScanArgs args) {
+  __shared__ uint4 parts[4][3][64];
+  const uint64_t item = blockIdx.x / 8;
+  Work w;
+  if (!find_work(args, item, w)) return;
+  const int slice = blockIdx.x % 8;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const uint32_t n = args.segments;
+  const int at = slice * slice_cells(8) + 2 * wave * 256 + 4 * lane;
+  f32x4 state[2], map[2][4][2], more[2];
+  const auto fetch = [&](uint32_t part) {  // for the state after segment `part`
+    const float* m = segment_state(args, item, n + part - 1);
+    const float* rest = segment_state(args, item, part) + at;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      more[u] = load4(rest + 256 * u);
+      const float* p = m + cells_at(8, 2 * wave + u, r, g);
+#pragma unroll
+      for (int step = 0; step < 4; ++step) {
+        map[u][step][0] = load4(p + 2 * step * slice_cells(8));
+        map[u][step][1] = load4(p + 2 * step * slice_cells(8) + 16);
+      }
+    }
+  };
+#pragma unroll
+  for (int u = 0; u < 2; ++u) state[u] = load4(segment_state(args, item, 0) + at + 256 * u);
+  fetch(1);
+  for (uint32_t part = 1; part < n; ++part) {
+    uint4 own[3], factor[2][4][3];
+    split3(state[0], state[1], own);
+#pragma unroll
+    for (int p = 0; p < 3; ++p) parts[wave][p][lane] = own[p];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      state[u] = more[u];
+#pragma unroll
+      for (int step = 0; step < 4; ++step) {
+        split3(map[u][step][0], map[u][step][1], factor[u][step]);
+      }
+    }
+    fetch(min(part + 1, n - 1));
+    exchange();
+#pragma unroll
+    for (int step = 0; step < 4; ++step) {
+      const uint4 x[3] = {parts[step][0][lane], parts[step][1][lane], parts[step][2][lane]};
+#pragma unroll
+      for (int u = 0; u < 2; ++u) state[u] = mfma6(factor[u][step], x, state[u]);
+    }
+    float* const to = segment_state(args, item, part) + at;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) store_cells(to + 256 * u, state[u]);
+    exchange();  // the parts have been read
+  }
 }
 
 // ------------------------------------------------------------ 16 columns
@@ -708,14 +988,43 @@ int32_t scan_by_size(void* stream, const ScanArgs& args) {
   if (blocks > kMaxGrid) return kStatusInvalidArgument;
   const dim3 grid(static_cast<uint32_t>(blocks));
   return narrow ? launch(delta_scan_narrow_kernel<Pool, kTrain>, grid, dim3(512), stream, args)
-                : launch(delta_scan_wide_kernel<Pool, kTrain>, grid, dim3(128 * kWideWaves), stream,
-                         args);
+                : launch(delta_scan_wide_kernel<Pool, kTrain>, grid, dim3(128 * kWideWaves),
+                         stream, args);
+}
+
+// One long request, or a few, of few heads: its chunks in segments, the states between
+// them from their maps.
+template <typename Pool>
+int32_t scan_in_segments(void* stream, ScanArgs args) {
+  const uint32_t items = args.rule.requests * args.rule.space.value_heads;
+  args.segments = std::min(kComputeUnits / kWideSlices / items, kMostSegments);
+  const auto run = [&](uint32_t pass) {
+    args.pass = pass;
+    return launch(delta_segment_kernel<Pool>, dim3((args.segments * items + 7) / 8 * 8 * 2),
+                  dim3(128 * kWideWaves), stream, args);
+  };
+  int32_t status = run(0);
+  if (status == kStatusOk) {
+    status = launch(delta_join_kernel, dim3(items * 8), dim3(256), stream, args);
+  }
+  return status == kStatusOk ? run(1) : status;
 }
 
 }  // namespace
 
 int32_t launch_delta_scan(void* stream, const ScanArgs& args, uint32_t dtype) {
   if (args.rule.space.train) return scan_by_size<float, true>(stream, args);
+  const uint64_t items = static_cast<uint64_t>(args.rule.requests) * args.rule.space.value_heads;
+  // In segments, where a request has so many chunks that the two passes, over all compute
+  // units, beat the narrow form's one chain: 64 on the average and 4 for each request x
+  // head.  32 heads of one request (narrow form in brackets, whole calls): 32,768 tokens
+  // 1,050 us (1,240), 8,192 280 (313), 4,096 158 (147).  8 heads: 32,768 tokens 362 (958),
+  // 4,096 90 (118).  One head: 4,096 tokens 78 (113).
+  const uint64_t chunks = args.rule.space.rows / args.rule.requests;
+  if (items <= kSplitItems && chunks >= std::max<uint64_t>(kSplitChunks, 4 * items)) {
+    return dtype == kDtypeF32 ? scan_in_segments<float>(stream, args)
+                              : scan_in_segments<bf16_bits>(stream, args);
+  }
   return dtype == kDtypeF32 ? scan_by_size<float, false>(stream, args)
                             : scan_by_size<bf16_bits, false>(stream, args);
 }

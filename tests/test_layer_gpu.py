@@ -168,6 +168,37 @@ def test_prefill_variants_of_the_wide_form(device, lengths, pool_dtype, normaliz
     _prefill(device, lengths, 4, 2, pool_dtype, normalize, seed=27)
 
 
+@pytest.mark.parametrize("lengths,heads,key_heads,pool_dtype,normalize,decay", [
+    ([4160], 2, 1, torch.float32, True, "mixed"),
+    ([4100], 1, 1, torch.bfloat16, True, "none"),
+    ([5003], 3, 3, torch.float32, False, "mixed"),
+    ([9000, 3, 0, 7500], 2, 2, torch.float32, True, "mixed"),
+    ([4096, 4300], 8, 4, torch.bfloat16, True, "strong"),
+    ([8300], 32, 16, torch.float32, True, "mixed"),
+    ([70, 8200], 1, 1, torch.float32, True, "none")])
+def test_prefill_of_long_sequences_in_segments(device, lengths, heads, key_heads, pool_dtype,
+                                               normalize, decay):
+    """64 chunks a request and more, and 4 for each of at most 32 requests x heads.  Many
+    times the chunks of the other tests, but a state forgets (through its decays or its
+    writes) what the first of them rounded."""
+    _prefill(device, lengths, heads, key_heads, pool_dtype, normalize, seed=29, decay=decay)
+
+
+def test_prefill_of_a_short_batch_in_a_long_buffer(device):
+    """Segments by the buffer's length; the requests fill a few chunks of it."""
+    lengths, slots = [130, 0, 64], ints([2, 1, 0], device)
+    total, room = sum(lengths), 64 * 200
+    mixed, q, k, v, g, b = tokens_of(room, 2, 1, 33)
+    inputs = on(device, mixed, q, k, v, g, b)
+    pool = torch.zeros((3, 2, 128, 128), device=device)
+    tables = gdn.request_tables(ints(lengths, device), slots, room)
+    out = gdn.gated_delta_prefill(*inputs, tables, slots, pool)
+    want, final = ref.rule(*(t[:total] for t in (q, k, v, g, b)), lengths,
+                           torch.zeros((3, 2, 128, 128), dtype=torch.float64))
+    close(out[:total], want, BF16, "out")
+    close(pool[slots.long()], final, FP32, "states")
+
+
 def _prefill(device, lengths, heads, key_heads, pool_dtype, normalize, seed, decay="mixed",
              alike=False, state_bound=FP32):
     n, total = len(lengths), sum(lengths)
