@@ -739,7 +739,7 @@ static_assert(sizeof(Gradient) <= kLdsPerCu, "one workgroup a compute unit");
 // once, by the wavefront that loads them, and so are F and H.
 //
 // 32 heads of 85 chunks take 264 us: 650 MB of states, E and X (2.5 TB/s), 2,850 matrix
-// instructions a chunk and head (18% of their rate).  The parts of X and E leave room
+// instructions a chunk and head (a fifth of their rate).  The parts of X and E leave room
 // for one workgroup a compute unit, whose phases (loads, F and H, the states' products,
 // the kinds) wait for each other: of some 35,000 cycles a head, loads take a third and
 // LDS reads as much.  Measured and left out: the next head's X and E asked for a phase
