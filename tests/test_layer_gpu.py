@@ -199,6 +199,46 @@ def test_prefill_of_a_short_batch_in_a_long_buffer(device):
     close(pool[slots.long()], final, FP32, "states")
 
 
+def test_segments_skip_padding_and_forget_and_replay(device):
+    """A padding request among long ones, log decays of -inf at the segments' borders and
+    inside, NaN in the padding's tokens, and a captured call's replays."""
+    lengths, slots = [4200, 4300, 4160], ints([2, -1, 0], device)
+    total, keep = sum(lengths), torch.cat([torch.arange(4200), torch.arange(8500, 12660)])
+    mixed, q, k, v, g, b = tokens_of(total, 2, 1, 35, decay="none")
+    for at in (0, 63, 64, 700, 8500, 12659):
+        g[at] = float("-inf")
+    g[1000:1100, 1] = -3.0e38
+    mixed[4200:8500] = float("nan")
+    start = 0.1 * torch.randn((3, 2, 128, 128), generator=torch.Generator().manual_seed(36))
+    x = on(device, mixed, q, k, v, g, b)
+    pool = start.to(device)
+    out = torch.full((total, 2, 128), 7.0, dtype=torch.bfloat16, device=device)
+    space = torch.empty(layer.workspace_bytes(total, 3, 2, 1), dtype=torch.uint8, device=device)
+    tables = gdn.request_tables(ints(lengths, device), slots, total)
+
+    def work():
+        gdn.gated_delta_prefill(*x, tables, slots, pool, workspace=space, out=out)
+
+    work()
+    want, final = ref.rule(q[keep], k[keep], v[keep], g[keep], b[keep], [4200, 4160],
+                           start[torch.tensor([2, 0])])
+    close(out.cpu()[keep], want, BF16, "out")
+    close(pool[[2, 0]], final, FP32, "states")
+    assert (out[4200:8500].cpu() == 7.0).all() and torch.equal(pool[1].cpu(), start[1])
+    eager = [out.clone(), pool.clone()]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        work()
+    for _ in range(3):
+        pool.copy_(start)
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager[0]) and torch.equal(pool, eager[1])
+
+
 def _prefill(device, lengths, heads, key_heads, pool_dtype, normalize, seed, decay="mixed",
              alike=False, state_bound=FP32):
     n, total = len(lengths), sum(lengths)
