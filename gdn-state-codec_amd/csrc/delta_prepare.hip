@@ -15,8 +15,9 @@
 // are stable for any keys, which powers of A are not.
 //
 // Bound by what it writes: of 32,768 tokens, 16 key heads and 32 value heads it reads
-// 268 MB and writes 671 in 218 us, 4.3 TB/s (a copy: 5.2); a training pass of 5,298
-// tokens, with the transposes, takes 60 us.
+// 268 MB and writes 671 in 200 us, 4.7 TB/s (a copy: 5.2; 220 us with the matrices whole
+// and two workgroups a compute unit); a training pass of 5,298 tokens, with the
+// transposes, takes 60 us.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -28,12 +29,35 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kPitch = 136;  // bf16 a staged row: 128 and 16 bytes against bank conflicts
-constexpr int kWide = 68;    // fp32 a row of a 64 x 64 matrix
 constexpr double kInverseLn2 = 1.4426950408889634074;
 
 struct Head {  // one wavefront's value head
   float sum[kChunk], rest[kChunk];  // G / ln 2
   float strength[kChunk];
+};
+
+// A lower triangular 64 x 64 matrix: ten blocks of 16 x 16, and the two above the
+// diagonal that an operand tile holds beside them.  A row's four runs of four columns
+// are rotated by its place, so that 16 rows' runs fall on different banks.
+struct Triangle {
+  float cells[12][256];
+
+  static __device__ __forceinline__ int block(int i, int j) {
+    return j <= i ? i * (i + 1) / 2 + j : i == 0 ? 10 : 11;
+  }
+  // Four columns from `column` on (a multiple of 4), of row `row` of a block.
+  __device__ __forceinline__ float* run(int at, int row, int column) {
+    return &cells[at][16 * row + (column ^ (row & 12))];
+  }
+  __device__ __forceinline__ const float* run(int at, int row, int column) const {
+    return &cells[at][16 * row + (column ^ (row & 12))];
+  }
+  __device__ __forceinline__ float& cell(int at, int row, int column) {
+    return cells[at][16 * row + (column ^ (row & 12))];
+  }
+  __device__ __forceinline__ float cell(int at, int row, int column) const {
+    return cells[at][16 * row + (column ^ (row & 12))];
+  }
 };
 
 struct Staged {
@@ -42,15 +66,17 @@ struct Staged {
       uint16_t k[kChunk][kPitch];
       uint16_t q[kChunk][kPitch];
     };
-    float solve[2][kChunk][kWide];  // A, then N, of two wavefronts
+    struct {
+      Triangle kk, qk;
+      Triangle solve[2];  // A, then N, of two wavefronts
+    };
   };
-  float kk[kChunk][kWide];
-  float qk[kChunk][kWide];
   Head heads[4];
   float k_unit[kChunk];  // 1 / |k|
   float q_unit[kChunk];  // scale / |q|
   float q_norm[kChunk];  // 1 / |q|
 };
+static_assert(workgroups_by_lds(sizeof(Staged)) == 3, "three workgroups share a compute unit");
 
 // LDS written by other lanes of the same wavefront is read after this.
 __device__ __forceinline__ void wave_sync() {
@@ -82,8 +108,8 @@ __device__ __forceinline__ void store_tile(char* operand, int tile, int lane, co
 }
 
 template <bool kTrain>
-__device__ __forceinline__ void solve_head(Staged& s, const Head& head, float (&m)[kChunk][kWide],
-                                           int lane, char* block) {
+__device__ __forceinline__ void solve_head(Staged& s, const Head& head, Triangle& m, int lane,
+                                           char* block) {
   const int r = lane & 15, g = lane >> 4;
   // A, block by block as accumulators (row 4 g + i, column r), and in LDS.
   f32x4 a[4][4];
@@ -100,9 +126,9 @@ __device__ __forceinline__ void solve_head(Staged& s, const Head& head, float (&
       for (int c = 0; c < 4; ++c) {
         const int row = 16 * i + 4 * g + c;
         const float x = decay_between(sum[c], rest[c], sum_c, rest_c) *
-                        (unit[c] * unit_c * s.kk[row][column]);
+                        (unit[c] * unit_c * s.kk.cell(Triangle::block(i, j), 4 * g + c, r));
         a[i][j][c] = column < row ? x : 0.0f;
-        m[row][column] = a[i][j][c];
+        m.cell(Triangle::block(i, j), 4 * g + c, r) = a[i][j][c];
       }
     }
   }
@@ -110,13 +136,13 @@ __device__ __forceinline__ void solve_head(Staged& s, const Head& head, float (&
   {  // the diagonal blocks: lane group g solves block g, column r
     float n[16], scaled[16];
     const float* const strength = &head.strength[16 * g];
+    const int diagonal = g * (g + 3) / 2;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      const float* const row = &m[16 * g + i][16 * g];
-      float x = -row[r], y = 0.0f;
+      float x = -m.cell(diagonal, i, r), y = 0.0f;
 #pragma unroll
       for (int c = 0; c < i; c += 4) {
-        const f32x4 l = load4(row + c);
+        const f32x4 l = load4(m.run(diagonal, i, c));
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
           if (c + u < i) {
@@ -130,19 +156,19 @@ __device__ __forceinline__ void solve_head(Staged& s, const Head& head, float (&
     }
     wave_sync();  // A's diagonal blocks have been read
 #pragma unroll
-    for (int i = 0; i < 16; ++i) m[16 * g + i][16 * g + r] = n[i];
+    for (int i = 0; i < 16; ++i) m.cell(diagonal, i, r) = n[i];
   }
   wave_sync();
   f32x4 inverse[4];  // I + N_ii b_i, row r
   f32x4 n[4][4], scaled[4][4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const f32x4 row = load4(&m[16 * i + r][16 * i + 4 * g]);
+    const f32x4 row = load4(m.run(Triangle::block(i, i), r, 4 * g));
     const f32x4 b = load4(&head.strength[16 * i + 4 * g]);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       inverse[i][c] = fmaf(row[c], b[c], 4 * g + c == r ? 1.0f : 0.0f);
-      n[i][i][c] = m[16 * i + 4 * g + c][16 * i + r];
+      n[i][i][c] = m.cell(Triangle::block(i, i), 4 * g + c, r);
     }
     scaled[i][i] = times(b, n[i][i]);
   }
@@ -154,7 +180,7 @@ __device__ __forceinline__ void solve_head(Staged& s, const Head& head, float (&
       f32x4 x = a[i][j];
 #pragma unroll
       for (int c = j; c < i; ++c) {
-        x = block_product(load4(&m[16 * i + r][16 * c + 4 * g]), scaled[c][j], x);
+        x = block_product(load4(m.run(Triangle::block(i, c), r, 4 * g)), scaled[c][j], x);
       }
       const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
       x = block_product(inverse[i], x, zero);
@@ -171,7 +197,7 @@ __device__ __forceinline__ void solve_head(Staged& s, const Head& head, float (&
       if (j < i || empty) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          m[16 * i + 4 * g + c][16 * j + r] = empty ? 0.0f : n[i][j][c];
+          m.cell(Triangle::block(i, j), 4 * g + c, r) = empty ? 0.0f : n[i][j][c];
         }
       }
     }
@@ -182,15 +208,16 @@ __device__ __forceinline__ void solve_head(Staged& s, const Head& head, float (&
 #pragma unroll
     for (int step = 0; step < 2; ++step) {
       if (step < lower_steps(t)) {
-        const float* p = &m[16 * t + r][32 * step + 4 * g];
-        store_tile(block + kSolve, lower_tile(t, step), lane, load4(p), load4(p + 16));
+        store_tile(block + kSolve, lower_tile(t, step), lane,
+                   load4(m.run(Triangle::block(t, 2 * step), r, 4 * g)),
+                   load4(m.run(Triangle::block(t, 2 * step + 1), r, 4 * g)));
       }
       if (kTrain && step >= upper_first(t)) {
         f32x4 x, y;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          x[i] = m[token_place(step, g, i)][16 * t + r];
-          y[i] = m[token_place(step, g, i + 4)][16 * t + r];
+          x[i] = m.cell(Triangle::block(2 * step, t), 4 * g + i, r);
+          y[i] = m.cell(Triangle::block(2 * step + 1, t), 4 * g + i, r);
         }
         store_tile(block + kSolveBack, upper_tile(t, step), lane, x, y);
       }
@@ -217,7 +244,7 @@ __device__ __forceinline__ void read_out_head(const Staged& s, const Head& head,
           const int from = 32 * step + 16 * u + 4 * g;
           const f32x4 sums = load4(&head.sum[from]), rests = load4(&head.rest[from]);
           const f32x4 units = load4(&s.k_unit[from]), b = load4(&head.strength[from]);
-          const f32x4 product = load4(&s.qk[at][from]);
+          const f32x4 product = load4(s.qk.run(Triangle::block(t, 2 * step + u), r, 4 * g));
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float y = decay_between(sum, rest, sums[i], rests[i]) *
@@ -246,7 +273,8 @@ __device__ __forceinline__ void read_out_head(const Staged& s, const Head& head,
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float y = decay_between(sums[i], rests[i], sum, rest) *
-                            (units[i] * k_unit * s.qk[from + i][at]);
+                            (units[i] * k_unit *
+                             s.qk.cell(Triangle::block(2 * step + u, t), 4 * g + i, r));
             x[u][i] = at <= from + i ? y : 0.0f;
           }
         }
@@ -270,11 +298,13 @@ __device__ __forceinline__ void clear_rest(const RuleArgs& a, uint32_t row, uint
   }
 }
 
+// Three workgroups share a compute unit (training's registers allow two).
 template <bool kTrain>
-__global__ __launch_bounds__(kThreads) void delta_prepare_kernel(RuleArgs a,
+__global__ __launch_bounds__(kThreads, kTrain ? 2 : 3) void delta_prepare_kernel(RuleArgs a,
                                                                 bf16_bits* outputs) {
   __shared__ __align__(16) Staged s;
-  const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const uint32_t row = blockIdx.x / a.space.key_heads;
   const uint32_t head = blockIdx.x % a.space.key_heads;
   const int4 chunk = a.chunks[row];
@@ -323,25 +353,24 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(RuleArgs a,
 
   char* const key_block = a.space.key_block(row, head);
   const int r = lane & 15, g = lane >> 4;
-  {  // row tile `wave` of K K^T and Q K^T, up to the diagonal
+  f32x4 kk[4], qk[4];  // row tile `wave` of K K^T and Q K^T, up to the diagonal
+  {
     uint4 k[4], q[4];
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
       k[step] = *reinterpret_cast<const uint4*>(&s.k[16 * wave + r][32 * step + 8 * g]);
       q[step] = *reinterpret_cast<const uint4*>(&s.q[16 * wave + r][32 * step + 8 * g]);
     }
-    for (int c = 0; c <= wave; ++c) {
-      f32x4 kk = {0.0f, 0.0f, 0.0f, 0.0f}, qk = kk;
 #pragma unroll
-      for (int step = 0; step < 4; ++step) {
-        const uint4 b = *reinterpret_cast<const uint4*>(&s.k[16 * c + r][32 * step + 8 * g]);
-        kk = mfma(k[step], b, kk);
-        qk = mfma(q[step], b, qk);
-      }
+    for (int c = 0; c < 4; ++c) {
+      kk[c] = qk[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (c <= wave) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s.kk[16 * wave + 4 * g + i][16 * c + r] = kk[i];
-        s.qk[16 * wave + 4 * g + i][16 * c + r] = qk[i];
+        for (int step = 0; step < 4; ++step) {
+          const uint4 b = *reinterpret_cast<const uint4*>(&s.k[16 * c + r][32 * step + 8 * g]);
+          kk[c] = mfma(k[step], b, kk[c]);
+          qk[c] = mfma(q[step], b, qk[c]);
+        }
       }
     }
     // Two row tiles of the transposes: rows = keys in state order, over the tokens.
@@ -373,7 +402,19 @@ __global__ __launch_bounds__(kThreads) void delta_prepare_kernel(RuleArgs a,
       norms[2 * kChunk + t] = s.q_norm[t];
     }
   }
-  __syncthreads();  // K and Q have been read; K K^T and Q K^T are whole
+  __syncthreads();  // K and Q have been read
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    if (c <= wave) {
+      const int at = wave * (wave + 1) / 2 + c;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s.kk.cell(at, 4 * g + i, r) = kk[c][i];
+        s.qk.cell(at, 4 * g + i, r) = qk[c][i];
+      }
+    }
+  }
+  __syncthreads();
 
   // Wavefronts 0 and 2 solve, 1 and 3 form P b, each for every second value head.
   Head& mine = s.heads[wave];
