@@ -108,7 +108,7 @@ static_assert(kHeadFactors <= 2 * kTileBytes, "the factors' tiles");
 static_assert(kStage <= kLdsPerCu, "a compute unit's LDS");
 
 // A workgroup takes 64 columns, two wavefronts for each 16: one the chain, the other
-// the operands' loads, the two products that need no state, and the stores.  5.9 us a
+// the operands' loads, the two products that need no state, and the stores.  5.7 us a
 // chunk of 128 heads at once, bound by the 112 KiB a chunk and head that it stores (6.9
 // with one wavefront for all of it), 4.7 of 32 heads.
 __global__ __launch_bounds__(128 * kWaves) void delta_back_wide_kernel(BackArgs args) {
@@ -738,7 +738,7 @@ static_assert(sizeof(Gradient) <= kLdsPerCu, "one workgroup a compute unit");
 // and all tokens, so that a state is loaded and cut into parts once.  X and E are cut
 // once, by the wavefront that loads them, and so are F and H.
 //
-// 32 heads of 85 chunks take 264 us: 650 MB of states, E and X (2.5 TB/s), 2,850 matrix
+// 32 heads of 85 chunks take 255 us: 650 MB of states, E and X (2.5 TB/s), 2,850 matrix
 // instructions a chunk and head (a fifth of their rate).  The parts of X and E leave room
 // for one workgroup a compute unit, whose phases (loads, F and H, the states' products,
 // the kinds) wait for each other: of some 35,000 cycles a head, loads take a third and

@@ -16,7 +16,7 @@
 // keeps; it takes S0 and E from LDS.  Bound by the chain's 132 matrix instructions and
 // the vector instructions between them: 3.1 us a chunk (32 heads of one request), where
 // the products alone would take 0.9; in training by the 112 KiB a chunk and head that it
-// stores, 5.8 us (128 heads at once, 2.5 TB/s; without the stores 3.8).  With one
+// stores, 5.7 us (128 heads at once, 2.6 TB/s; without the stores 3.8).  With one
 // wavefront for both the chain and the rest these were 4.1 and 6.8.
 //
 // delta_scan_narrow_kernel, for few heads, where a long request's chain is all there
