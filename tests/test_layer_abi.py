@@ -144,3 +144,15 @@ def test_sizes(lib):
     assert 0 < one < two < 2 * one
     # Training keeps each chunk's start state and its gradient (64 KiB a head) too.
     assert lib.gated_delta_workspace_v1(1, 4, 2, 1) - one > 4 * 2 * 65536
+
+
+def test_workspace_holds_the_states_between_segments(lib):
+    """256 states of 64 KiB from 64 chunk rows on, for up to 32 heads, serving only."""
+    def step(rows, heads, train):
+        size = lib.gated_delta_workspace_v1
+        return size(rows, heads, 1, train) - size(rows - 1, heads, 1, train)
+
+    states = 256 * 65536
+    assert step(64, 32, 0) == step(63, 32, 0) + states
+    assert step(64, 33, 0) == step(63, 33, 0)
+    assert step(64, 32, 1) == step(63, 32, 1)
