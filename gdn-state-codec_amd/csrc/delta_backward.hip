@@ -88,7 +88,7 @@ __device__ __forceinline__ void store_initial(float* d_initial, uint64_t tile, i
 // ------------------------------------------------------------ 64 columns
 
 // A chunk's operands in LDS, in two halves, each fetched while the other is at work:
-// the factors (2 KiB), N^T, K rows and Q^T; then K^T and the next chunk's P^T and dO.
+// the factors (2 KiB), N^T b, K rows and Q^T; then K^T and the next chunk's P^T and dO.
 // Beside them 48 KiB through which the chain and the wavefronts beside it hand each
 // other accumulators, each lane to the same lane: dS1 and, once that has been taken,
 // (exp(G) Q)^T dO; P^T dO and, once that has been taken, X.
@@ -336,20 +336,11 @@ __global__ __launch_bounds__(128 * kWaves) void delta_back_wide_kernel(BackArgs 
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[t][i] = fmaf(carry[i], seen[0][i] + seen[1][i], read[i]);
     }
-    // X = V' + N^T (b V')
+    // X = V' + (N^T b) V'
     {
       uint4 part[2][3];
 #pragma unroll
-      for (int step = 0; step < 2; ++step) {
-        f32x4 w[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const f32x4 b = of_rows(factors[2 * step + u][kStrength]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[u][i] = b[i] * v[2 * step + u][i];
-        }
-        split3(w[0], w[1], part[step]);
-      }
+      for (int step = 0; step < 2; ++step) split3(v[2 * step], v[2 * step + 1], part[step]);
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
 #pragma unroll
@@ -377,9 +368,9 @@ __global__ __launch_bounds__(128 * kWaves) void delta_back_wide_kernel(BackArgs 
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int t = 2 * step + u;
-        const f32x4 b = of_rows(factors[t][kStrength]), k = of_rows(factors[t][kReadKey]);
+        const f32x4 k = of_rows(factors[t][kStrength] * -factors[t][kReadKey]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) m[u][i] = -k[i] * (b[i] * v[t][i]);
+        for (int i = 0; i < 4; ++i) m[u][i] = k[i] * v[t][i];
       }
       split3(m[0], m[1], by_key);
 #pragma unroll
@@ -399,7 +390,7 @@ __global__ __launch_bounds__(128 * kWaves) void delta_back_wide_kernel(BackArgs 
 // with three exchanges a chunk, as the forward scan's narrow form.  3.4 us a chunk.
 __global__ __launch_bounds__(512) void delta_back_narrow_kernel(BackArgs args) {
   constexpr int kNarrow = kDim / 16;
-  // Parts of dS1 (4 steps over the keys), of b V' and of -exp(G) Y / |k| (2 steps over
+  // Parts of dS1 (4 steps over the keys), of V' and of -exp(G) Y / |k| (2 steps over
   // the tokens), and the fp32 accumulators that pass between the two kinds of wavefront.
   __shared__ uint4 state_parts[4][3][64];
   __shared__ uint4 row_parts[2][3][64];
@@ -608,8 +599,8 @@ __global__ __launch_bounds__(512) void delta_back_narrow_kernel(BackArgs args) {
     fetch_columns();
     if (c != 0) go_to(c - 1);
     __builtin_amdgcn_sched_barrier(0);
-    const f32x4 carried = of_rows(carry), strength = of_rows(factors[kStrength]);
-    const f32x4 read_key = of_rows(factors[kReadKey]);
+    const f32x4 carried = of_rows(carry);
+    const f32x4 written = of_rows(factors[kStrength] * -factors[kReadKey]);
     f32x4 seen[2] = {};
 #pragma unroll
     for (int p = 2; p >= 0; --p) {
@@ -618,20 +609,16 @@ __global__ __launch_bounds__(512) void delta_back_narrow_kernel(BackArgs args) {
         seen[step & 1] = mfma(k_rows[step], part_s[step][p], seen[step & 1]);
       }
     }
-    f32x4 scaled;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = fmaf(carried[i], seen[0][i] + seen[1][i], v[i]);
-      scaled[i] = strength[i] * v[i];
-    }
+    for (int i = 0; i < 4; ++i) v[i] = fmaf(carried[i], seen[0][i] + seen[1][i], v[i]);
     uint2 half[3];
-    split3_half(scaled, half);
+    split3_half(v, half);
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
       reinterpret_cast<uint2*>(&row_parts[wave >> 1][p][lane])[wave & 1] = half[p];
     }
     exchange();
-    // X = V' + N^T (b V')
+    // X = V' + (N^T b) V'
     uint4 part_r[2][3];
 #pragma unroll
     for (int p = 2; p >= 0; --p) {
@@ -657,8 +644,9 @@ __global__ __launch_bounds__(512) void delta_back_narrow_kernel(BackArgs args) {
       v = mfma6(solve[1], part_r[1], v);
     }
     error_cells[wave][lane] = v;
+    f32x4 scaled;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) scaled[i] = -read_key[i] * (strength[i] * v[i]);
+    for (int i = 0; i < 4; ++i) scaled[i] = written[i] * v[i];
     split3_half(scaled, half);
 #pragma unroll
     for (int p = 0; p < 3; ++p) {

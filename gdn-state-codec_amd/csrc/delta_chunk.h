@@ -51,7 +51,7 @@ constexpr float kUnitEps = 1e-6f;  // inside the square root of q's and k's norm
 constexpr int kTileBytes = 1024;
 constexpr int kKeyTiles = 16;
 // Triangular operands (rows and contraction = tokens): 6 of the 8 tiles hold
-// anything.  N, P and their transposes are three bf16 parts, 18 KiB (cut once
+// anything.  N b, N^T b and P^T are three bf16 parts, 18 KiB (cut once
 // here instead of by every slice that reads them); P b is two, since the outputs it
 // makes are bf16.
 constexpr int kTriangle = 6;
@@ -102,7 +102,7 @@ __host__ __device__ constexpr uint64_t value_block_bytes(bool train) {
 constexpr int kKeyColumns = 0;
 constexpr int kQueryColumns = kKeyTiles * kTileBytes;
 constexpr int kNorms = 2 * kKeyTiles * kTileBytes;
-// Places inside a value block: factors, N, P b, then for training N^T and P^T.
+// Places inside a value block: factors, N b, P b, then for training N^T b and P^T.
 constexpr int kSolve = kHeadFactors;
 constexpr int kReadOut = kSolve + kTriangleBytes;
 constexpr int kSolveBack = kReadOut + kReadOutBytes;

@@ -1,11 +1,11 @@
 // The state-independent half of the gated delta rule's chunked form, for every
 // chunk and key head at once: the transposed operands, the norms, and for each
-// value head of the group the factors, N and P b (and for training N^T and P^T);
+// value head of the group the factors, N b and P b (and for training N^T b and P^T);
 // formulas and layouts in delta_chunk.h.
 //
 // One workgroup per chunk row and key head.  K K^T and Q K^T are formed once per
 // key head on the matrix cores (exact bf16 products), then each wavefront takes a
-// value head's N or its P b, with no barrier between them.
+// value head's N b or its P b, with no barrier between them.
 //
 // N by blocks of 16 tokens.  The four diagonal blocks are solved at once by forward
 // substitution, one column a lane (120 fmas).  Below them
@@ -208,9 +208,10 @@ __device__ __forceinline__ void solve_head(Staged& s, const Head& head, Triangle
 #pragma unroll
     for (int step = 0; step < 2; ++step) {
       if (step < lower_steps(t)) {
+        const float* const b = &head.strength[32 * step + 4 * g];
         store_tile(block + kSolve, lower_tile(t, step), lane,
-                   load4(m.run(Triangle::block(t, 2 * step), r, 4 * g)),
-                   load4(m.run(Triangle::block(t, 2 * step + 1), r, 4 * g)));
+                   times(load4(m.run(Triangle::block(t, 2 * step), r, 4 * g)), load4(b)),
+                   times(load4(m.run(Triangle::block(t, 2 * step + 1), r, 4 * g)), load4(b + 16)));
       }
       if (kTrain && step >= upper_first(t)) {
         f32x4 x, y;
@@ -219,7 +220,9 @@ __device__ __forceinline__ void solve_head(Staged& s, const Head& head, Triangle
           x[i] = m.cell(Triangle::block(2 * step, t), 4 * g + i, r);
           y[i] = m.cell(Triangle::block(2 * step + 1, t), 4 * g + i, r);
         }
-        store_tile(block + kSolveBack, upper_tile(t, step), lane, x, y);
+        const float* const b = &head.strength[32 * step + 4 * g];
+        store_tile(block + kSolveBack, upper_tile(t, step), lane, times(x, load4(b)),
+                   times(y, load4(b + 16)));
       }
     }
   }

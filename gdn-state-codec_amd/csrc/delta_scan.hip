@@ -3,9 +3,9 @@
 //
 // Column v of a state [key][value] meets only column v of V, E and O, so columns
 // go to wavefronts and workgroups as they like, but from S0 to S1 is one chain,
-//   S0 -> K S0 -> R -> N (b R) -> E -> K^T U -> S1,
+//   S0 -> K S0 -> R -> (N b) R -> E -> K^T U -> S1,
 // chunk after chunk.  Per chunk and 16 columns it issues
-//   K S0: 48, N (b R): 36, K^T U: 48, and beside the chain Q S0: 32, (P b) E: 18
+//   K S0: 48, (N b) R: 36, K^T U: 48, and beside the chain Q S0: 32, (P b) E: 18
 // matrix instructions.  Two forms, and a third made of the first:
 //
 // delta_scan_wide_kernel, for throughput: a workgroup takes 64 columns, with two
@@ -168,7 +168,7 @@ constexpr int kWideWaves = 4;
 constexpr int kWideSlices = kDim / (16 * kWideWaves);
 
 // A chunk's operands in LDS, in two halves, each fetched while the other is at work:
-// the factors, N (20 KiB of the value head's block) and K rows (16 tiles), then Q rows,
+// the factors, N b (20 KiB of the value head's block) and K rows (16 tiles), then Q rows,
 // K^T and P b (two stages: it is read a phase later).  Beside them S0 and E (two stages)
 // as the chain's accumulators hold them.  156 KiB: a workgroup has the compute unit to
 // itself.
@@ -213,20 +213,12 @@ __device__ __forceinline__ void chain_rest(const uint4* k_rows, const uint4 (&pa
   }
 }
 
-// E = R + N (b R)
-__device__ __forceinline__ void chain_solve(const uint4* solve, const f32x4 (&factors)[4],
-                                            f32x4 (&error)[4]) {
+// E = R + (N b) R
+__device__ __forceinline__ void chain_solve(const uint4* solve, f32x4 (&error)[4]) {
   uint4 part[2][3];
 #pragma unroll
   for (int step = 0; step < 2; ++step) {
-    f32x4 x[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const f32x4 b = of_rows(factors[2 * step + u][kStrength]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[u][i] = b[i] * error[2 * step + u][i];
-    }
-    split3(x[0], x[1], part[step]);
+    split3(error[2 * step], error[2 * step + 1], part[step]);
   }
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
@@ -477,7 +469,7 @@ __device__ __forceinline__ void scan_columns(const ScanArgs& args, const Work& w
     f32x4 error[4];
     chain_rest(k_rows, parts, factors, values, false, lane, error);
     if (c + 1 < chunks) fetch_values(c + 1);
-    chain_solve(solve, factors, error);
+    chain_solve(solve, error);
     f32x4* const cells = error_cells(c);
 #pragma unroll
     for (int t = 0; t < 4; ++t) cells[64 * t] = error[t];
@@ -511,7 +503,7 @@ __global__ __launch_bounds__(128 * kWideWaves) void delta_scan_wide_kernel(ScanA
 // ------------------------------------------------------------ segments
 
 // What a segment makes of its state and no more: eight wavefronts, all columns, each the
-// chain of 16.  The factors, N, K rows and K^T of a chunk come into LDS while the last
+// chain of 16.  The factors, N b, K rows and K^T of a chunk come into LDS while the last
 // chunk is at work.
 constexpr int kChainKeys = kBlockTiles * kTileBytes;
 constexpr int kChainColumns = kChainKeys + kKeyTiles * kTileBytes;
@@ -607,7 +599,7 @@ __device__ __forceinline__ void scan_state(const ScanArgs& args, const Work& w,
     chain_rest(reinterpret_cast<const uint4*>(at + kChainKeys) + lane, parts, factors, values,
                part.map, lane, error);
     fetch_values(next);
-    chain_solve(reinterpret_cast<const uint4*>(at + kSolve) + lane, factors, error);
+    chain_solve(reinterpret_cast<const uint4*>(at + kSolve) + lane, error);
     chain_state(reinterpret_cast<const uint4*>(at + kChainColumns) + lane, factors, error,
                 state);
   }
@@ -697,7 +689,7 @@ __global__ __launch_bounds__(256) void delta_join_kernel(ScanArgs args) {
 template <typename Pool, bool kTrain>
 __global__ __launch_bounds__(512) void delta_scan_narrow_kernel(ScanArgs args) {
   constexpr int kSlices = kDim / 16;
-  // Parts of S0 (4 steps over the keys), b R, write b E and E (2 steps over the
+  // Parts of S0 (4 steps over the keys), R, write b E and E (2 steps over the
   // tokens).
   __shared__ uint4 state_parts[4][3][64];
   __shared__ uint4 row_parts[2][3][64];
@@ -885,8 +877,8 @@ __global__ __launch_bounds__(512) void delta_scan_narrow_kernel(ScanArgs args) {
     fetch_columns();
     advance(c);
     __builtin_amdgcn_sched_barrier(0);
-    const f32x4 read_key = of_rows(factors[kReadKey]), strength = of_rows(factors[kStrength]);
-    const f32x4 write = of_rows(factors[kWrite]), v = value_rows(values, lane);
+    const f32x4 read_key = of_rows(factors[kReadKey]), write = of_rows(factors[kWrite]);
+    const f32x4 v = value_rows(values, lane);
     f32x4 seen[2] = {};  // two sums, so that each product waits for the last but one
 #pragma unroll
     for (int p = 2; p >= 0; --p) {
@@ -899,16 +891,15 @@ __global__ __launch_bounds__(512) void delta_scan_narrow_kernel(ScanArgs args) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       error[i] = fmaf(-read_key[i], seen[0][i] + seen[1][i], v[i]);
-      scaled[i] = strength[i] * error[i];
     }
     uint2 half[3];
-    split3_half(scaled, half);
+    split3_half(error, half);
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
       reinterpret_cast<uint2*>(&row_parts[wave >> 1][p][lane])[wave & 1] = half[p];
     }
     exchange();
-    // E = R + N (b R)
+    // E = R + (N b) R
     uint4 part_r[2][3];
 #pragma unroll
     for (int p = 2; p >= 0; --p) {
