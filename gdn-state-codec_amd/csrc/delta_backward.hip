@@ -142,10 +142,8 @@ __global__ __launch_bounds__(128 * kWaves) void delta_back_wide_kernel(BackArgs 
       const char* k = reinterpret_cast<const char*>(a.keys + token * a.key_stride +
                                                     key_head * kDim);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {  // rows 16 i.., keys 32 wave..
-        const uint32_t row = min(static_cast<uint32_t>(16 * i + r), last);
-        stage_tile(k + 64 * wave, row * key_step + 16 * g,
-                   stage_at + kStageKeys + (4 * i + wave) * kTileBytes);
+      for (int i = 0; i < 4; ++i) {
+        stage_rows(k, key_step, last, kWaves * i + wave, lane, stage_at + kStageKeys);
       }
       const char* block = space.value_block(first_row + c, head);
 #pragma unroll
@@ -299,11 +297,11 @@ __global__ __launch_bounds__(128 * kWaves) void delta_back_wide_kernel(BackArgs 
   // The chain.
   f32x4 state[8];  // the state's gradient, rows as in the forward scan
   load_final(args.d_final, w.tile, 0, 16 * slice + r, g, state);
-  const uint4* const k_rows = reinterpret_cast<const uint4*>(stage + kStageKeys) + lane;
+  const uint4* k_rows[4];
+  row_operands(stage + kStageKeys, lane, k_rows);
   const uint4* const k_columns = reinterpret_cast<const uint4*>(stage + kStageColumns) + lane;
   const uint4* const solve = reinterpret_cast<const uint4*>(stage + kStageSolve) + lane;
   if (chunks != 0) exchange();  // the first chunk's operands
-  __builtin_amdgcn_s_setprio(1);
   for (uint32_t c = chunks; c-- > 0;) {
     uint4 part[4][3];
 #pragma unroll
@@ -328,7 +326,7 @@ __global__ __launch_bounds__(128 * kWaves) void delta_back_wide_kernel(BackArgs 
       f32x4 seen[2] = {};
 #pragma unroll
       for (int step = 0; step < 4; ++step) {
-        const uint4 k = k_rows[(4 * t + step) * 64];
+        const uint4 k = k_rows[step][256 * t];
 #pragma unroll
         for (int p = 2; p >= 0; --p) seen[p & 1] = mfma(k, part[step][p], seen[p & 1]);
       }

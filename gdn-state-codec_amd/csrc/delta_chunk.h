@@ -343,6 +343,28 @@ __device__ __forceinline__ void stage_tile(const char* from, uint32_t offset, ui
                : "memory");
 }
 
+// 64 rows of q or k (one head's 256 bytes each) in LDS: four whole rows a tile, `step`
+// bytes apart at `from`, rows past `last` the last again.  A row's 16-byte pieces are
+// exchanged by its place, p to p ^ (row & 15), so that 16 rows' pieces of one operand fall
+// on different banks.  (A tile of 16 rows by 64 bytes takes the address unit twice as
+// long.)
+__device__ __forceinline__ void stage_rows(const char* from, uint32_t step, uint32_t last,
+                                           int tile, int lane, uint32_t to) {
+  const uint32_t row = 4 * tile + (lane >> 4);
+  stage_tile(from, min(row, last) * step + 16 * ((lane & 15) ^ (row & 15)),
+             to + tile * kTileBytes);
+}
+// A lane's places of row tile 0, step by step, of rows staged so; the next row tile is 256
+// on.
+__device__ __forceinline__ void row_operands(const char* rows, int lane,
+                                             const uint4* (&operand)[4]) {
+  const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int step = 0; step < 4; ++step) {
+    operand[step] = reinterpret_cast<const uint4*>(rows) + 16 * r + ((4 * step + g) ^ r);
+  }
+}
+
 // Every staged tile of the workgroup is in LDS, and the stage read before may be
 // overwritten, after this.  `kAfter` memory operations that each wavefront has issued
 // after its last tile (store_run's, so that their number is known) stay in flight.

@@ -193,7 +193,8 @@ __device__ __forceinline__ void split2(const f32x4& x, const f32x4& y, uint4 (&p
 // The chain's three products, of one wavefront's 16 columns.  R = V - exp(G) K S0, from
 // the state's parts, and from rows of V as fetched (columns 4 (r / 4).. of tokens 16 t +
 // 4 g + (r & 3)) or none.
-__device__ __forceinline__ void chain_rest(const uint4* k_rows, const uint4 (&parts)[4][3],
+__device__ __forceinline__ void chain_rest(const uint4* const (&k_rows)[4],
+                                           const uint4 (&parts)[4][3],
                                            const f32x4 (&factors)[4], const uint2 (&values)[4],
                                            bool none, int lane, f32x4 (&error)[4]) {
 #pragma unroll
@@ -201,7 +202,7 @@ __device__ __forceinline__ void chain_rest(const uint4* k_rows, const uint4 (&pa
     f32x4 seen[2] = {};  // two sums, so that each product waits for the last but one
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
-      const uint4 k = k_rows[(4 * t + step) * 64];
+      const uint4 k = k_rows[step][256 * t];
 #pragma unroll
       for (int p = 2; p >= 0; --p) seen[p & 1] = mfma(k, parts[step][p], seen[p & 1]);
     }
@@ -291,10 +292,8 @@ __device__ __forceinline__ void scan_columns(const ScanArgs& args, const Work& w
       const char* k = reinterpret_cast<const char*>(a.keys + token * a.key_stride +
                                                     key_head * kDim);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {  // K rows 16 i.., keys 32 wave..
-        const uint32_t row = min(static_cast<uint32_t>(16 * i + r), last);
-        stage_tile(k + 64 * wave, row * key_step + 16 * g,
-                   stage_at + kStageKeys + (4 * i + wave) * kTileBytes);
+      for (int i = 0; i < 4; ++i) {
+        stage_rows(k, key_step, last, kWideWaves * i + wave, lane, stage_at + kStageKeys);
       }
       const char* block = space.value_block(w.first_row + c, w.head);
 #pragma unroll
@@ -317,10 +316,8 @@ __device__ __forceinline__ void scan_columns(const ScanArgs& args, const Work& w
                    stage_at + kStageColumns + tile * kTileBytes);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {  // Q rows 16 i.., keys 32 wave..
-        const uint32_t row = min(static_cast<uint32_t>(16 * i + r), last);
-        stage_tile(q + 64 * wave, row * query_step + 16 * g,
-                   stage_at + kStageQueries + (4 * i + wave) * kTileBytes);
+      for (int i = 0; i < 4; ++i) {
+        stage_rows(q, query_step, last, kWideWaves * i + wave, lane, stage_at + kStageQueries);
       }
 #pragma unroll
       for (int i = 0; i < 2 * kTriangle / kWideWaves; ++i) {
@@ -330,7 +327,8 @@ __device__ __forceinline__ void scan_columns(const ScanArgs& args, const Work& w
       }
     };
     f32x4 out[4], error[4];
-    const auto read_errors = [&](uint32_t c) {  // O += (P b) E
+    uint2 runs[4];
+    const auto read_errors = [&](uint32_t c) {  // O += (P b) E, and both as they are stored
       const f32x4* const cells = error_cells(c);
       const uint4* const read_out =
           reinterpret_cast<const uint4*>(stage + kStageRead + (c & 1) * kReadOutBytes) + lane;
@@ -349,6 +347,11 @@ __device__ __forceinline__ void scan_columns(const ScanArgs& args, const Work& w
           out[t] = mfma(high, part[0], out[t]);
         }
       }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        runs[t] = output_run(out[t], lane);
+        if constexpr (kTrain) error[t] = transpose_quad(error[t], lane);
+      }
     };
     // kTrain ? 8 : 4 stores, of which the tokens past `tokens` have none.
     const auto store_rows = [&](uint32_t c, int tokens) {
@@ -358,15 +361,15 @@ __device__ __forceinline__ void scan_columns(const ScanArgs& args, const Work& w
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const int token = 16 * t + 4 * g + (r & 3);
-        const uint2 x = output_run(out[t], lane);
-        if (token < tokens) store_run(o, token * out_step + 2 * (r & 12), x);
+        if (token < tokens) store_run(o, token * out_step + 2 * (r & 12), runs[t]);
         if constexpr (kTrain) {
           store_run(space.errors(w.first_row + c, w.head) + slice * slice_cells(4),
-                    t * kTileBytes + linear, transpose_quad(error[t], lane));
+                    t * kTileBytes + linear, error[t]);
         }
       }
     };
-    const uint4* const q_rows = reinterpret_cast<const uint4*>(stage + kStageQueries) + lane;
+    const uint4* q_rows[4];
+    row_operands(stage + kStageQueries, lane, q_rows);
     if (chunks != 0) fetch_first(0);
     for (uint32_t c = 0; c < chunks; ++c) {
       // The first half is there, the second has been read.  Only the stores issued after
@@ -408,7 +411,7 @@ __device__ __forceinline__ void scan_columns(const ScanArgs& args, const Work& w
         f32x4 read[2] = {};
 #pragma unroll
         for (int step = 0; step < 4; ++step) {
-          const uint4 q = q_rows[(4 * t + step) * 64];
+          const uint4 q = q_rows[step][256 * t];
           read[0] = mfma(q, parts[step][1], read[0]);
           read[1] = mfma(q, parts[step][0], read[1]);
         }
@@ -447,11 +450,11 @@ __device__ __forceinline__ void scan_columns(const ScanArgs& args, const Work& w
       values[t] = *reinterpret_cast<const uint2*>(v + (row * value_step + 2 * (r & 12)));
     }
   };
-  const uint4* const k_rows = reinterpret_cast<const uint4*>(stage + kStageKeys) + lane;
+  const uint4* k_rows[4];
+  row_operands(stage + kStageKeys, lane, k_rows);
   const uint4* const k_columns = reinterpret_cast<const uint4*>(stage + kStageColumns) + lane;
   const uint4* const solve = reinterpret_cast<const uint4*>(stage + kSolve) + lane;
   if (chunks != 0) fetch_values(0);
-  __builtin_amdgcn_s_setprio(1);
   for (uint32_t c = 0; c < chunks; ++c) {
     uint4 parts[4][3];  // of the state, over the keys
 #pragma unroll
@@ -529,15 +532,12 @@ __device__ __forceinline__ void scan_state(const ScanArgs& args, const Work& w,
   // Piece i of 0..6; and the values.
   const auto fetch = [&](uint32_t c, int i) {
     const uint32_t to = stage_at + (c & 1) * kChainStage;
-    if (i < 2) {  // K rows 16 (tile / 4).., keys 32 (tile % 4)..
+    if (i < 2) {
       const uint64_t token = w.begin + c * kChunk;
       const uint32_t last = min(length - c * kChunk, static_cast<uint32_t>(kChunk)) - 1;
       const char* k = reinterpret_cast<const char*>(a.keys + token * a.key_stride +
                                                     key_head * kDim);
-      const int tile = kWaves * i + wave;
-      const uint32_t row = min(static_cast<uint32_t>(16 * (tile >> 2) + r), last);
-      stage_tile(k + 64 * (tile & 3), row * key_step + 16 * g,
-                 to + kChainKeys + tile * kTileBytes);
+      stage_rows(k, key_step, last, kWaves * i + wave, lane, to + kChainKeys);
     } else if (i < 4) {
       const int tile = kWaves * (i - 2) + wave;
       stage_tile(space.key_block(w.first_row + c, key_head) + kKeyColumns + tile * kTileBytes,
@@ -596,8 +596,9 @@ __device__ __forceinline__ void scan_state(const ScanArgs& args, const Work& w,
       __builtin_amdgcn_sched_barrier(0);
     }
     f32x4 error[4];
-    chain_rest(reinterpret_cast<const uint4*>(at + kChainKeys) + lane, parts, factors, values,
-               part.map, lane, error);
+    const uint4* k_rows[4];
+    row_operands(at + kChainKeys, lane, k_rows);
+    chain_rest(k_rows, parts, factors, values, part.map, lane, error);
     fetch_values(next);
     chain_solve(reinterpret_cast<const uint4*>(at + kSolve) + lane, error);
     chain_state(reinterpret_cast<const uint4*>(at + kChainColumns) + lane, factors, error,
