@@ -108,7 +108,7 @@ static_assert(kHeadFactors <= 2 * kTileBytes, "the factors' tiles");
 static_assert(kStage <= kLdsPerCu, "a compute unit's LDS");
 
 // A workgroup takes 64 columns, two wavefronts for each 16: one the chain, the other
-// the operands' loads, the two products that need no state, and the stores.  5.7 us a
+// the operands' loads, the two products that need no state, and the stores.  5.5 us a
 // chunk of 128 heads at once, bound by the 112 KiB a chunk and head that it stores (6.9
 // with one wavefront for all of it), 4.7 of 32 heads.
 __global__ __launch_bounds__(128 * kWaves) void delta_back_wide_kernel(BackArgs args) {

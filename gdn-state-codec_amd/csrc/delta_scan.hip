@@ -16,7 +16,7 @@
 // keeps; it takes S0 and E from LDS.  Bound by the chain's 132 matrix instructions and
 // the vector instructions between them: 3.1 us a chunk (32 heads of one request), where
 // the products alone would take 0.9; in training by the 112 KiB a chunk and head that it
-// stores, 5.7 us (128 heads at once, 2.6 TB/s; without the stores 3.8).  With one
+// stores, 5.4 us (128 heads at once, 2.7 TB/s; without the stores 3.8).  With one
 // wavefront for both the chain and the rest these were 4.1 and 6.8.
 //
 // delta_scan_narrow_kernel, for few heads, where a long request's chain is all there
@@ -1010,7 +1010,7 @@ int32_t launch_delta_scan(void* stream, const ScanArgs& args, uint32_t dtype) {
   // In segments, where a request has so many chunks that the two passes, over all compute
   // units, beat the narrow form's one chain: 64 on the average and 4 for each request x
   // head.  32 heads of one request (narrow form in brackets, whole calls): 32,768 tokens
-  // 1,050 us (1,240), 8,192 280 (313), 4,096 158 (147).  8 heads: 32,768 tokens 362 (958),
+  // 1,000 us (1,240), 8,192 280 (313), 4,096 158 (147).  8 heads: 32,768 tokens 362 (958),
   // 4,096 90 (118).  One head: 4,096 tokens 78 (113).
   const uint64_t chunks = args.rule.space.rows / args.rule.requests;
   if (items <= kSplitItems && chunks >= std::max<uint64_t>(kSplitChunks, 4 * items)) {
