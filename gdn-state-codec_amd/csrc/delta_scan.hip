@@ -974,7 +974,7 @@ int32_t scan_by_size(void* stream, const ScanArgs& args) {
   // Where all narrow workgroups run at once, one on each of the 256 compute units, a
   // chunk takes 2.1 us (32 heads of one request), in the wide form 3.1 us.  Twice as many
   // would take two rounds of the one, and one of the other, which issues a quarter of
-  // the loads (128 heads, 4 requests in training: 250 us and 180 us).
+  // the loads (128 heads, 4 requests in training: 250 us and 172 us).
   const bool narrow = items * (kDim / 16) <= kComputeUnits;
   const uint64_t blocks = (items + 7) / 8 * 8 * (narrow ? kDim / 16 : kWideSlices);
   if (blocks > kMaxGrid) return kStatusInvalidArgument;
