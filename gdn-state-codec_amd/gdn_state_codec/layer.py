@@ -252,6 +252,10 @@ def gated_delta_prefill(queries: torch.Tensor, keys: torch.Tensor, values: torch
     return out
 
 
+def _sizes(rule: RuleStruct) -> tuple:
+    return rule.tokens, rule.requests, rule.value_heads, rule.key_heads
+
+
 class _GatedDeltaRule(torch.autograd.Function):
     @staticmethod
     def forward(ctx, queries, keys, values, log_decay, beta, initial, tables, scale, normalize):
@@ -264,17 +268,22 @@ class _GatedDeltaRule(torch.autograd.Function):
         _launched(native().gated_delta_forward_launch_v1(
             _stream(), ctypes.byref(rule), 0 if initial is None else initial.data_ptr(),
             final.data_ptr(), out.data_ptr()), "gated delta forward")
-        # The struct's pointers stay good as long as these tensors are kept.
         ctx.save_for_backward(queries, keys, values, log_decay, beta, *tables, workspace)
-        ctx.rule, ctx.resumed = rule, initial is not None
+        ctx.sizes, ctx.scale, ctx.normalize = _sizes(rule), scale, normalize
+        ctx.resumed = initial is not None
         ctx.set_materialize_grads(False)
         return out, final
 
     @staticmethod
     def backward(ctx, d_out, d_final):
         _once()
-        queries, keys, values, log_decay, beta = ctx.saved_tensors[:5]
-        rule = ctx.rule
+        # Under hooks on saved tensors (checkpointing, offloading) these are others than the
+        # forward pass's, which may be gone: their addresses, strides and checks are taken anew.
+        queries, keys, values, log_decay, beta, *tables, workspace = ctx.saved_tensors
+        rule, _ = _rule(queries, keys, values, log_decay, beta, RequestTables(*tables), ctx.scale,
+                        ctx.normalize, workspace, True)
+        if _sizes(rule) != ctx.sizes:
+            _fail("gated delta rule's saved tensors changed their shapes")
         shape = (rule.requests, rule.value_heads, DIM, DIM)
         if d_out is None:
             d_out = torch.zeros(values.shape, dtype=torch.bfloat16, device=values.device)

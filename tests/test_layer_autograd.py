@@ -1,0 +1,126 @@
+"""The layer operators' autograd functions on a machine without a GPU: the native
+library is replaced by a recorder that launches nothing, and what it is called with is
+held to the tensors that are alive at that call."""
+
+from __future__ import annotations
+
+import types
+
+import pytest
+import torch
+from torch.utils.checkpoint import checkpoint
+
+import gdn_state_codec as gdn
+from gdn_state_codec import _native, layer
+from gdn_state_codec._native import RuleStruct
+
+HEADS, KEY_HEADS, TOKENS = 4, 2, 70
+POINTERS = ("queries", "keys", "values", "log_decay", "beta", "offsets", "chunk_offsets",
+            "chunks", "order", "workspace")
+
+
+@pytest.fixture
+def calls(monkeypatch):
+    """(name, arguments) of every launch; a rule's struct as a dict of its fields."""
+    seen = []
+    real = _native.NativeLibrary()
+
+    def recorder(name):
+        def launch(*args):
+            args = [{field: getattr(a._obj, field) for field, _ in RuleStruct._fields_}
+                    if hasattr(a, "_obj") else a for a in args]
+            seen.append((name, args))
+            return 0
+        return launch
+
+    library = types.SimpleNamespace(
+        gated_delta_workspace_v1=real.gated_delta_workspace_v1,
+        norm_partials_v1=real.norm_partials_v1,
+        **{name: recorder(name) for name in (
+            "gated_delta_forward_launch_v1", "gated_delta_backward_launch_v1",
+            "gated_delta_prefill_launch_v1", "gated_delta_step_launch_v1",
+            "gated_norm_launch_v1", "gated_norm_backward_launch_v1",
+            "residual_norm_launch_v1", "residual_norm_backward_launch_v1")})
+    monkeypatch.setattr(layer, "native", lambda: library)
+    monkeypatch.setattr(layer, "_stream", lambda: 0)
+    monkeypatch.setattr(layer, "_current_device", lambda: torch.empty(0).get_device())
+    return seen
+
+
+def batch(tokens=TOKENS, requests=2):
+    """Leaves (queries, keys and values slices of one projection) and tables."""
+    mixed = torch.randn(tokens, (2 * KEY_HEADS + HEADS) * 128).bfloat16()
+    q, k, v = (x.unflatten(1, (-1, 128)) for x in
+               mixed.split((KEY_HEADS * 128, KEY_HEADS * 128, HEADS * 128), 1))
+    rest = [torch.zeros(tokens, HEADS), torch.zeros(tokens, HEADS).bfloat16()]
+    rows = layer.table_rows(tokens, requests)
+    tables = gdn.RequestTables(*(torch.zeros(shape, dtype=torch.int32) for shape in (
+        requests + 1, requests + 1, (rows, 4), requests)))
+    return [x.detach().requires_grad_() for x in (q, k, v, *rest)], tables
+
+
+def struct_of(tensors):
+    """The pointers and strides that a rule's saved tensors ask for."""
+    want = dict(zip(POINTERS, (t.data_ptr() for t in tensors)))
+    want.update(zip(("query_stride", "key_stride", "value_stride"),
+                    (t.stride(0) for t in tensors)))
+    want["workspace_bytes"] = tensors[9].numel()
+    return want
+
+
+def check(rule, tensors):
+    want = struct_of(tensors)
+    assert {name: rule[name] for name in want} == want
+
+
+def test_backward_reads_what_the_saved_tensors_were_unpacked_to(calls):
+    leaves, tables = batch()
+    unpacked = []
+
+    def unpack(t):
+        unpacked.append(t)
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.clone(), unpack):
+        out, final = gdn.gated_delta_rule(*leaves, tables)
+    torch.autograd.grad([out], leaves, [torch.ones_like(out)])
+    (_, forward), (name, backward) = calls
+    assert name == "gated_delta_backward_launch_v1" and len(unpacked) == 10
+    check(backward[1], unpacked)
+    assert unpacked[0].stride(0) == KEY_HEADS * 128  # a copy of the slice is dense
+    for field in ("requests", "rows", "tokens", "value_heads", "key_heads", "scale", "normalize"):
+        assert backward[1][field] == forward[1][field]
+
+
+def test_backward_reads_what_a_checkpoint_recomputed(calls):
+    leaves, tables = batch()
+    kept = []  # of every forward call, so that no address is used twice
+
+    def block(*inputs):
+        inputs = [x * 1.0 for x in inputs]
+        out, final = gdn.gated_delta_rule(*inputs, tables)
+        kept.append(inputs + [out, final])
+        return out, final
+
+    out, final = checkpoint(block, *leaves, use_reentrant=False)
+    torch.autograd.grad([out, final], leaves, [torch.ones_like(out), torch.ones_like(final)])
+    names = [name.split("_")[2] for name, _ in calls]
+    assert names == ["forward", "forward", "backward"]
+    for field in POINTERS:
+        assert calls[2][1][1][field] == calls[1][1][1][field], field
+
+
+def test_backward_without_hooks_reads_the_forward_call_s_tensors(calls):
+    leaves, tables = batch()
+    out, final = gdn.gated_delta_rule(*leaves, tables)
+    torch.autograd.grad([out], leaves, [torch.ones_like(out)])
+    assert calls[0][1][1] == calls[1][1][1]
+
+
+def test_backward_refuses_what_a_hook_changed(calls):
+    leaves, tables = batch()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: t[:-1]):
+        out, _ = gdn.gated_delta_rule(*leaves, tables)
+    with pytest.raises(RuntimeError, match="GDN State Codec"):
+        torch.autograd.grad([out], leaves, [torch.ones_like(out)])
+    assert len(calls) == 1
