@@ -1105,8 +1105,9 @@ extern "C" int32_t statecentric_gdn_state_codec_gated_delta_backward_launch_v1(
     const float* d_final, uint16_t* d_queries, uint16_t* d_keys, uint16_t* d_values,
     float* d_log_decay, uint16_t* d_beta, float* d_initial) {
   gdn::BackArgs args{};
-  if (!gdn::rule_args(rule, true, args.rule) || !d_outputs || !d_queries || !d_keys ||
-      !d_values || !d_log_decay || !d_beta ||
+  if (!gdn::rule_args(rule, true, args.rule) ||
+      !gdn::token_rows(rule->tokens, d_outputs, d_queries, d_keys, d_values, d_log_decay,
+                       d_beta) ||
       !gdn::aligned16(d_outputs, d_final, d_queries, d_keys, d_values, d_log_decay, d_beta,
                       d_initial)) {
     return gdn::kStatusInvalidArgument;

@@ -182,6 +182,13 @@ inline bool element_aligned(const float* log_decay, const bf16_bits* beta) {
          reinterpret_cast<uintptr_t>(beta) % sizeof(bf16_bits) == 0;
 }
 
+// Tensors of one row a token: all there, unless there are no tokens (an empty tensor has
+// no address, and no kernel reads a row of it).
+template <typename... Pointers>
+inline bool token_rows(uint32_t tokens, const Pointers*... pointers) {
+  return tokens == 0 || ((pointers != nullptr) && ...);
+}
+
 struct RuleArgs {
   const bf16_bits* queries;
   const bf16_bits* keys;

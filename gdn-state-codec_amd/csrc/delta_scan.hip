@@ -1025,8 +1025,9 @@ constexpr uint64_t kMaxStride = 1u << 24;  // elements between tokens
 
 // Checks the caller's arguments and fills the kernels'; false: a bad argument.
 bool rule_args(const gdn_state_codec_rule* rule, bool train, RuleArgs& a) {
-  if (!rule || !rule->queries || !rule->keys || !rule->values || !rule->log_decay ||
-      !rule->beta || !rule->offsets || !rule->chunk_offsets || !rule->chunks || !rule->order ||
+  if (!rule || !rule->offsets || !rule->chunk_offsets || !rule->chunks || !rule->order ||
+      !token_rows(rule->tokens, rule->queries, rule->keys, rule->values, rule->log_decay,
+                  rule->beta) ||
       !rule->workspace || rule->requests == 0 || rule->requests > GDN_STATE_CODEC_MAX_REQUESTS ||
       rule->tokens > 0x7FFFFFFFu || rule->rows != rule->tokens / kChunk + rule->requests ||
       rule->key_heads == 0 || rule->value_heads == 0 ||
@@ -1037,8 +1038,8 @@ bool rule_args(const gdn_state_codec_rule* rule, bool train, RuleArgs& a) {
       rule->query_stride % 8 != 0 || rule->key_stride % 8 != 0 || rule->value_stride % 8 != 0 ||
       static_cast<uint64_t>(rule->rows) * rule->value_heads > kMaxGrid ||
       !element_aligned(rule->log_decay, rule->beta) ||
-      !aligned16(rule->queries, rule->keys, rule->values, rule->offsets, rule->chunk_offsets, rule->chunks, rule->order,
-                 rule->workspace)) {
+      !aligned16(rule->queries, rule->keys, rule->values, rule->offsets, rule->chunk_offsets,
+                 rule->chunks, rule->order, rule->workspace)) {
     return false;
   }
   a = RuleArgs{rule->queries, rule->keys, rule->values, rule->log_decay, rule->beta,
@@ -1062,7 +1063,8 @@ extern "C" int32_t statecentric_gdn_state_codec_gated_delta_prefill_launch_v1(
     void* stream, const gdn_state_codec_rule* rule, const int32_t* slot_ids,
     const int32_t* resume, void* pool, uint32_t slots, uint32_t pool_dtype, uint16_t* outputs) {
   gdn::ScanArgs args{};
-  if (!gdn::rule_args(rule, false, args.rule) || !slot_ids || !pool || !outputs || slots == 0 ||
+  if (!gdn::rule_args(rule, false, args.rule) || !slot_ids || !pool ||
+      !gdn::token_rows(rule->tokens, outputs) || slots == 0 ||
       slots > 0x7FFFFFFFu || pool_dtype > gdn::kDtypeBF16 ||
       !gdn::aligned16(slot_ids, resume, pool, outputs)) {
     return gdn::kStatusInvalidArgument;
@@ -1077,7 +1079,8 @@ extern "C" int32_t statecentric_gdn_state_codec_gated_delta_forward_launch_v1(
     void* stream, const gdn_state_codec_rule* rule, const float* initial, float* final_states,
     uint16_t* outputs) {
   gdn::ScanArgs args{};
-  if (!gdn::rule_args(rule, true, args.rule) || !final_states || !outputs ||
+  if (!gdn::rule_args(rule, true, args.rule) || !final_states ||
+      !gdn::token_rows(rule->tokens, outputs) ||
       !gdn::aligned16(initial, final_states, outputs)) {
     return gdn::kStatusInvalidArgument;
   }

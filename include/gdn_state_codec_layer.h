@@ -72,7 +72,9 @@ int32_t statecentric_gdn_state_codec_gated_delta_step_launch_v1(
     uint64_t query_stride, uint64_t key_stride, uint64_t value_stride,
     uint32_t pool_dtype, float scale, uint32_t normalize);
 
-/* A packed ragged batch and the scratch its whole-sequence form works in. */
+/* A packed ragged batch and the scratch its whole-sequence form works in.  Where
+ * tokens is 0, every pointer to rows of tokens, here and in the calls, may be NULL:
+ * each request is then empty. */
 typedef struct gdn_state_codec_rule {
   const uint16_t* queries;      /* bf16 [tokens][key_heads][128] */
   const uint16_t* keys;         /* bf16 [tokens][key_heads][128] */
