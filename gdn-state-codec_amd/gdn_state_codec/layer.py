@@ -328,8 +328,11 @@ def _rows_of(t: torch.Tensor, name: str, width: int) -> int:
 
 
 def _given(d: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
-    """An output's gradient as the kernels read it."""
-    return d if d.dtype is dtype and d.is_contiguous() else d.to(dtype).contiguous()
+    """An output's gradient as the kernels read it: dense, of its type, and on a 16-byte
+    boundary (autograd hands over slices of larger gradients as they lie)."""
+    if d.dtype is not dtype or not d.is_contiguous():
+        d = d.to(dtype).contiguous()
+    return d if d.data_ptr() % 16 == 0 else d.clone()
 
 
 def _weight_sums(weight: torch.Tensor, rows: int):

@@ -124,3 +124,28 @@ def test_backward_refuses_what_a_hook_changed(calls):
     with pytest.raises(RuntimeError, match="GDN State Codec"):
         torch.autograd.grad([out], leaves, [torch.ones_like(out)])
     assert len(calls) == 1
+
+
+@pytest.mark.parametrize("operator", ["rule", "gated norm", "residual norm"])
+def test_gradients_that_start_anywhere(calls, operator):
+    """The gradient of a torch.cat's operand is a slice of the whole one, and starts where
+    the operand did: no 16-byte boundary."""
+    if operator == "rule":
+        leaves, tables = batch()
+        outs = gdn.gated_delta_rule(*leaves, tables)
+    elif operator == "gated norm":
+        leaves = [torch.randn(3, 128).requires_grad_() for _ in range(2)]
+        leaves.append(torch.ones(128).requires_grad_())
+        outs = (gdn.gated_norm(*leaves),)
+    else:
+        leaves = [torch.randn(3, 64).requires_grad_() for _ in range(2)]
+        leaves.append(torch.ones(64).requires_grad_())
+        outs = gdn.residual_norm(*leaves)
+    joined = torch.cat([torch.zeros(3)] + [x.float().flatten() for x in outs])
+    torch.autograd.grad([joined], leaves, [torch.randn_like(joined)])
+    name, args = calls[-1]
+    assert "backward" in name
+    pointers = args[2:] if operator == "rule" else args[1:9]
+    assert len(pointers) == 8
+    for pointer in pointers:
+        assert pointer % 16 == 0
