@@ -14,6 +14,7 @@ import ctypes
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from ._native import RuleStruct, native
 
@@ -64,6 +65,13 @@ def _once() -> None:
     """In a backward pass: there is no gradient of the gradients."""
     if torch.is_grad_enabled():
         _fail("layer operators cannot be differentiated twice")
+
+
+def _no_tangents(*tensors: torch.Tensor) -> None:
+    """Refuses dual tensors, whose tangents a launch would drop."""
+    if forward_ad._current_level >= 0 and any(
+            forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        _fail("layer operators have no forward-mode derivative")
 
 
 class RequestTables(NamedTuple):
@@ -388,6 +396,7 @@ def gated_norm(x: torch.Tensor, gate: torch.Tensor, weight: torch.Tensor,
         _fail("gate must have the input's shape and type")
     _rows_of(gate, "gate", DIM)
     _dense(weight, "gated norm weight", (DIM,), torch.float32)
+    _no_tangents(x, gate, weight)
     if torch.is_grad_enabled() and (x.requires_grad or gate.requires_grad
                                     or weight.requires_grad):
         return _GatedNorm.apply(x, gate, weight, eps)
@@ -454,6 +463,7 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
         _fail("the residual stream must have the input's shape")
     _rows_of(residual, "residual stream", width)
     _dense(weight, "residual norm weight", (width,), torch.float32)
+    _no_tangents(x, residual, weight)
     if torch.is_grad_enabled() and (x.requires_grad or residual.requires_grad
                                     or weight.requires_grad):
         return _ResidualNorm.apply(x, residual, weight, scale, eps)

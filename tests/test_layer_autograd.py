@@ -149,3 +149,23 @@ def test_gradients_that_start_anywhere(calls, operator):
     assert len(pointers) == 8
     for pointer in pointers:
         assert pointer % 16 == 0
+
+
+def norm_inputs():
+    return {gdn.gated_norm: [torch.randn(3, 128), torch.randn(3, 128), torch.ones(128)],
+            gdn.residual_norm: [torch.randn(3, 64), torch.randn(3, 64), torch.ones(64)]}
+
+
+@pytest.mark.parametrize("norm", [gdn.gated_norm, gdn.residual_norm])
+@pytest.mark.parametrize("place", range(3))
+def test_norms_refuse_tangents(calls, norm, place):
+    """There is no forward-mode derivative: a dual tensor is refused, not cut off."""
+    inputs = norm_inputs()[norm]
+    with torch.autograd.forward_ad.dual_level():
+        norm(*inputs)  # no dual among them
+        inputs[place] = torch.autograd.forward_ad.make_dual(inputs[place],
+                                                            torch.ones_like(inputs[place]))
+        launched = len(calls)
+        with pytest.raises(RuntimeError, match="GDN State Codec"):
+            norm(*inputs)
+    assert len(calls) == launched == 1
