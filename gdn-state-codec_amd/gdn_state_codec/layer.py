@@ -74,6 +74,14 @@ def _no_tangents(*tensors: torch.Tensor) -> None:
         _fail("layer operators have no forward-mode derivative")
 
 
+def _not_differentiated(what: str, *tensors: torch.Tensor) -> None:
+    """Refuses tensors that ask for a gradient, which a call in place cannot give."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        _fail(f"{what} has no gradient: call it under torch.no_grad(), or "
+              "gated_delta_rule to train")
+    _no_tangents(*tensors)
+
+
 class RequestTables(NamedTuple):
     """The device tables of a ragged batch of N requests (all int32)."""
 
@@ -167,9 +175,12 @@ def gated_delta_step(queries: torch.Tensor, keys: torch.Tensor, values: torch.Te
 
     queries, keys bf16 [B,Hk,128], values bf16 [B,H,128] (rows of a fused
     projection are fine), log_decay fp32 and beta bf16 [B,H]; returns bf16
-    [B,H,128].  ``normalize`` divides queries and keys by their 2-norm."""
+    [B,H,128].  ``normalize`` divides queries and keys by their 2-norm.  Not
+    differentiable: inputs that require gradients are refused outside
+    ``torch.no_grad()``."""
     batch, heads, key_heads, strides = _rule_inputs(queries, keys, values, log_decay, beta)
     pool_dtype = _pool(pool, heads)
+    _not_differentiated("gated delta step", queries, keys, values, log_decay, beta, pool)
     _dense(slot_ids, "slot ids", (batch,), torch.int32)
     if out is None:
         out = torch.zeros((batch, heads, DIM), dtype=torch.bfloat16, device=values.device)
@@ -241,11 +252,13 @@ def gated_delta_prefill(queries: torch.Tensor, keys: torch.Tensor, values: torch
     projection are fine), log_decay fp32 and beta bf16 [T,H]; ``tables`` are
     :func:`request_tables`' for ``max_tokens`` T and the same slot ids.  Returns
     bf16 [T,H,128]; rows of no request, and padding's, stay as they were.
-    ``workspace`` (uint8, :func:`workspace_bytes`) may be kept between calls."""
+    ``workspace`` (uint8, :func:`workspace_bytes`) may be kept between calls.  Not
+    differentiable, as :func:`gated_delta_step`; :func:`gated_delta_rule` is."""
     rule, workspace = _rule(queries, keys, values, log_decay, beta, tables, scale, normalize,
                             workspace, False)
     heads = values.shape[1]
     pool_dtype = _pool(pool, heads)
+    _not_differentiated("gated delta prefill", queries, keys, values, log_decay, beta, pool)
     _dense(slot_ids, "slot ids", (rule.requests,), torch.int32)
     if resume is not None:
         _dense(resume, "resume", (rule.requests,), torch.int32)

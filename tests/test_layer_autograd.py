@@ -169,3 +169,36 @@ def test_norms_refuse_tangents(calls, norm, place):
         with pytest.raises(RuntimeError, match="GDN State Codec"):
             norm(*inputs)
     assert len(calls) == launched == 1
+
+def serving_calls():
+    """The two calls that update a pool in place, as functions of their float inputs."""
+    leaves, tables = batch()
+    inputs = [x.detach() for x in leaves]
+    slots = torch.zeros(TOKENS, dtype=torch.int32)
+    inputs.append(torch.zeros(3, HEADS, 128, 128))
+    return inputs, {
+        "step": lambda *x: gdn.gated_delta_step(*x, slots),
+        "prefill": lambda *x: gdn.gated_delta_prefill(*x[:5], tables, slots[:2], x[5])}
+
+
+@pytest.mark.parametrize("call", ["step", "prefill"])
+@pytest.mark.parametrize("place", range(6))
+def test_serving_calls_refuse_what_they_cannot_differentiate(calls, call, place):
+    """Inputs and states of a serving call that require gradients, or hold tangents."""
+    inputs, functions = serving_calls()
+    functions[call](*inputs)
+    wanted = list(inputs)
+    wanted[place] = inputs[place].clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="GDN State Codec"):
+        functions[call](*wanted)
+    with torch.autograd.forward_ad.dual_level():
+        functions[call](*inputs)
+        dual = list(inputs)
+        dual[place] = torch.autograd.forward_ad.make_dual(
+            inputs[place].clone(), torch.ones_like(inputs[place]))
+        with pytest.raises(RuntimeError, match="GDN State Codec"):
+            functions[call](*dual)
+    assert len(calls) == 2
+    with torch.no_grad():
+        functions[call](*wanted)
+    assert len(calls) == 3
