@@ -12,11 +12,16 @@
 //   dk_i = - exp(G_i) S0 Y_i - sum_j H_ij k_j                     (as it is read)
 //          + exp(G_63 - G_i) dS1 U_i + sum_j F_ji q_j - sum_j H_ji k_j  (as it is written)
 //   db_i = X_i.E_i
-//   dG_i = q_i.dq_i + k_i.(dk_i as read) - k_i.(dk_i as written),
-//   dG_63 += exp(G_63) <dS1, S0> + sum_j k_j.(exp(G_63 - G_j) dS1 U_j)
-// for unit k and scaled unit q; dg is the sum of dG from a token to the chunk's
-// end, and the raw gradients follow through the norms.  A key head's gradients are
-// summed over its value heads in registers, in order.
+//   dg_t = exp(G_63) <dS1, S0> + sum_(i>=t) exp(G_i) (q_i.S0 dO_i - k_i.S0 Y_i)
+//          + sum_(j<t) exp(G_63 - G_j) k_j.dS1 U_j
+//          + sum_(j<t<=i) (F_ij q_i.k_j - H_ij k_i.k_j)
+// for unit k and scaled unit q; the raw gradients follow through the norms.  A key
+// head's gradients are summed over its value heads in registers, in order.
+//
+// dg_t takes exactly what crosses token t, every term with its exp(g_t).  (q_i.dq_i +
+// k_i.dk_i as read - k_i.dk_i as written, summed from t to the chunk's end, is the same,
+// but there the pairs on one side of t, and each token's own, cancel: with log decays of
+// -12 their rounding was 5% of the gradients.)
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -700,6 +705,26 @@ __device__ __forceinline__ float sum16(float x) {  // over the 16 lanes of a DPP
   return add_partner<8>(x);
 }
 
+// x of the lane `kCtrl`'s row shift names, 0 where that lies outside the 16 lanes.
+template <int kCtrl>
+__device__ __forceinline__ float shifted(float x) {
+  return __int_as_float(
+      __builtin_amdgcn_update_dpp(0, __float_as_int(x), kCtrl, 0xF, 0xF, true));
+}
+constexpr int kDppUp = 0x110, kDppDown = 0x100;  // row_shr, row_shl: from lane - n, lane + n
+__device__ __forceinline__ float sum_to_here(float x) {  // of lanes 0.. to this one
+  x += shifted<kDppUp + 1>(x);
+  x += shifted<kDppUp + 2>(x);
+  x += shifted<kDppUp + 4>(x);
+  return x + shifted<kDppUp + 8>(x);
+}
+__device__ __forceinline__ float sum_from_here(float x) {  // of this one to lane 15
+  x += shifted<kDppDown + 1>(x);
+  x += shifted<kDppDown + 2>(x);
+  x += shifted<kDppDown + 4>(x);
+  return x + shifted<kDppDown + 8>(x);
+}
+
 struct Gradient {
   // X and E cut into parts, 16 tiles a part; then the four kinds of F and H, 6 tiles
   // a part.
@@ -717,6 +742,9 @@ struct Gradient {
   float along[4][kChunk];  // X.E by step
   float sums[2][8][kChunk];
   float ends[8];
+  // What pairs of tokens add to dg, block by block: by column (its tokens after the pair's
+  // first), by row, and the whole block's.
+  float pairs_to[kBlocks][16], pairs_from[kBlocks][16], pairs[kBlocks];
 };
 static_assert(sizeof(Gradient) <= kLdsPerCu, "one workgroup a compute unit");
 
@@ -737,7 +765,7 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
   const RuleArgs& a = args.rule;
   const ChunkSpace& space = a.space;
   const int t = threadIdx.x, lane = t & 63, r = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int first_wave = __builtin_amdgcn_readfirstlane(t >> 6);
   const uint32_t row = blockIdx.x / space.key_heads;
   const uint32_t head = blockIdx.x % space.key_heads;
   const uint64_t token_step = static_cast<uint64_t>(space.value_heads) * kDim;
@@ -778,10 +806,10 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
   f32x4 d_q[4] = {}, d_k[4] = {};  // of the token tiles
   for (uint32_t member = 0; member < a.group; ++member) {
     const uint32_t value_head = head * a.group + member;
-    // Taken afresh for each head: the addresses that follow from it would otherwise
+    // Taken afresh for each head: the addresses that follow from them would otherwise
     // be kept over the loop, in more registers than there are.
-    int lane = t & 63;
-    asm volatile("" : "+v"(lane));
+    int lane = t & 63, wave = first_wave;
+    asm volatile("" : "+v"(lane), "+s"(wave));
     const int r = lane & 15, g = lane >> 4;
     const float* const s0 = space.state(row, value_head);
     const float* const s1 = space.state_gradient(row, value_head);
@@ -818,9 +846,9 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
                    outs_at + unit * kTileBytes);
       }
     }
-    for (int i = t; i < kFactors; i += kThreads) {
-      s.factors[i] = reinterpret_cast<const float*>(space.value_block(row, value_head))[i];
-    }
+    static_assert(kFactors == kThreads, "one a thread");
+    s.factors[64 * wave + lane] = reinterpret_cast<const float*>(
+        space.value_block(row, value_head))[64 * wave + lane];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const int unit = wave + 8 * u;
@@ -841,14 +869,14 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
     }
     stage_ready();
     load_rows(s0, start);
-    if (t < kChunk) {
-      const float b = s.factors[4 * t + kStrength];
-      const float decay = __builtin_amdgcn_exp2f(s.factors[kSum + t]);
-      s.decays[0][t] = decay;
-      s.decays[1][t] = decay * b;
-      s.decays[2][t] = b * decay_between(s.factors[kSum + kChunk - 1],
-                                         s.factors[kSumRest + kChunk - 1], s.factors[kSum + t],
-                                         s.factors[kSumRest + t]);
+    if (wave == 0) {
+      const float b = s.factors[4 * lane + kStrength];
+      const float decay = __builtin_amdgcn_exp2f(s.factors[kSum + lane]);
+      s.decays[0][lane] = decay;
+      s.decays[1][lane] = decay * b;
+      s.decays[2][lane] = b * decay_between(s.factors[kSum + kChunk - 1],
+                                         s.factors[kSumRest + kChunk - 1], s.factors[kSum + lane],
+                                         s.factors[kSumRest + lane]);
     }
 
     // F and H, ten blocks (i, j), j <= i, of 16 x 16; the two beside them that an
@@ -875,14 +903,38 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
       const int column = 16 * j + r;
       const float b_column = s.factors[4 * column + kStrength];
       const float sum = s.factors[kSum + column], rest = s.factors[kSumRest + column];
+      const f32x4* const dots = reinterpret_cast<const f32x4*>(
+          keys + kDots + 2 * min(block, kBlocks - 1) * kTileBytes);
+      const f32x4 qk = dots[lane], kk = dots[64 + lane];
+      float to = 0.0f, whole = 0.0f;
+      f32x4 from;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const int line = 16 * i + 4 * g + c;
         const float decay =
             decay_between(s.factors[kSum + line], s.factors[kSumRest + line], sum, rest);
-        s.f[line][column] = column <= line ? decay * (fx[c] * b_column) : 0.0f;
-        s.h[line][column] =
+        const float f = column <= line ? decay * (fx[c] * b_column) : 0.0f;
+        const float h =
             column < line ? decay * (s.factors[4 * line + kStrength] * hx[c] * b_column) : 0.0f;
+        s.f[line][column] = f;
+        s.h[line][column] = h;
+        // The pairs of this row up to this column: they cross the tokens after it and,
+        // within the row's block, up to the row.
+        const float pair = column < line ? fmaf(f, qk[c], -(h * kk[c])) : 0.0f;
+        const float upto = sum_to_here(pair);
+        const float before = shifted<kDppUp + 1>(upto);
+        to += column <= line ? before : 0.0f;
+        from[c] = upto;  // in lane 15, the row's
+        whole += upto;
+      }
+      to = add_partner<32>(add_partner<16>(to));
+      whole = add_partner<32>(add_partner<16>(whole));
+      if (block < kBlocks) {
+        if (g == 0) s.pairs_to[block][r] = to;
+        if (r == 15) {
+          *reinterpret_cast<f32x4*>(&s.pairs_from[block][4 * g]) = from;
+          if (g == 0) s.pairs[block] = whole;
+        }
       }
     }
 
@@ -1005,32 +1057,60 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float dq = fmaf(decay[j], read_q[i][j], by_query[j]);
-        const float read = -fmaf(read_by[j], read_k[i][j], by_read[j]);
+        const float seen = read_by[j] * read_k[i][j];
         const float carried = kept[j] * written[i][j];
-        const float write = carried + by_write[j];
         const float k = k_unit[j] * cells_k[4 * (i & 1) + j];
         const float q = q_unit[j] * cells_q[4 * (i & 1) + j];
-        end = fmaf(k, carried, end);
         d_q[i][j] += dq;
-        d_k[i][j] += read + write;
-        const float total = sum16(fmaf(q, dq, k * (read - write)));
-        if (r == 0) s.sums[0][wave][from + j] = total;
+        d_k[i][j] += (carried + by_write[j]) - (seen + by_read[j]);
+        const float first = sum16(fmaf(q, decay[j] * read_q[i][j], -(k * seen)));
+        const float last = sum16(k * carried);
+        if (r == 0) {
+          s.sums[0][wave][from + j] = first;
+          s.sums[1][wave][from + j] = last;
+        }
       }
     }
     end = wave_sum_valu(end);
     if (lane == 0) s.ends[wave] = end;
     __syncthreads();
     if (wave == 0) {
-      float total = eight(0, lane);
-      if (lane == 63) {
-        total += ((s.ends[0] + s.ends[1]) + (s.ends[2] + s.ends[3])) +
-                 ((s.ends[4] + s.ends[5]) + (s.ends[6] + s.ends[7]));
+      const int tile = lane >> 4, place = lane & 15;
+      const auto of = [](float x, int from) {
+        return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), from));
+      };
+      // What S0 gives to this token and those after it.
+      float from_start = sum_from_here(eight(0, lane));
+      {
+        const float second = of(from_start, 16), third = of(from_start, 32), fourth = of(from_start, 48);
+        from_start += tile == 0 ? (second + third) + fourth
+                : tile == 1 ? third + fourth
+                : tile == 2 ? fourth : 0.0f;
       }
+      // What the tokens before it give to dS1.
+      float to_end = sum_to_here(eight(1, lane));
+      {
+        const float first_three[3] = {of(to_end, 15), of(to_end, 31), of(to_end, 47)};
+        const float before = tile == 0 ? 0.0f
+                             : tile == 1 ? first_three[0]
+                             : tile == 2 ? first_three[0] + first_three[1]
+                             : (first_three[0] + first_three[1]) + first_three[2];
+        to_end = shifted<kDppUp + 1>(to_end) + before;
+      }
+      // Between tokens: pairs whose first is in this token's tile of 16, whose second is,
+      // and, for the two tiles in the middle, whose ends lie on either side of it.
+      float between = 0.0f, from = 0.0f;
 #pragma unroll
-      for (int step = 1; step < 64; step <<= 1) {  // from each token to the chunk's end
-        const float after = __shfl_down(total, step);
-        if (lane + step < 64) total += after;
+      for (int i = 0; i < 4; ++i) {
+        if (i >= tile) between += s.pairs_to[i * (i + 1) / 2 + tile][place];
+        if (i < tile) from += s.pairs_from[tile * (tile + 1) / 2 + i][place];
       }
+      between += sum_from_here(from);
+      if (tile == 1) between += s.pairs[3] + s.pairs[6];
+      if (tile == 2) between += s.pairs[6] + s.pairs[7];
+      const float ends = ((s.ends[0] + s.ends[1]) + (s.ends[2] + s.ends[3])) +
+                         ((s.ends[4] + s.ends[5]) + (s.ends[6] + s.ends[7]));
+      const float total = (ends + between) + (from_start + to_end);
       const float b = (s.along[0][lane] + s.along[1][lane]) + (s.along[2][lane] + s.along[3][lane]);
       if (lane < count) {
         const uint64_t at = (first + lane) * space.value_heads + value_head;
@@ -1040,6 +1120,7 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
     }
   }
 
+  const int wave = first_wave;
   // Through the norms: with u = scale / |q|, d(raw) = u dq - q (u q.dq) / |q|^2, and
   // for keys the same with scale 1.
   float cells_k[2][8], cells_q[2][8];

@@ -63,6 +63,8 @@ __device__ __forceinline__ constexpr int lower_tile(int row, int step) {
 __device__ __forceinline__ constexpr int upper_tile(int row, int step) {
   return row < 2 ? 2 * row + step : row + 2;  // (0,0) (0,1) (1,0) (1,1) (2,1) (3,1)
 }
+// Its blocks of 16 x 16 on and below the diagonal, (i, j) at i (i + 1) / 2 + j.
+constexpr int kBlocks = 10;
 __device__ __forceinline__ constexpr int lower_steps(int row) { return row < 2 ? 1 : 2; }
 __device__ __forceinline__ constexpr int upper_first(int row) { return row < 2 ? 0 : 1; }
 
@@ -92,16 +94,19 @@ enum : int {
 // Bytes of the workspace's parts.
 constexpr int kHeadFactors = kFactors * 4;
 __host__ __device__ constexpr uint64_t key_block_bytes(bool train) {
-  return train ? 2 * kKeyTiles * kTileBytes + 3 * kChunk * 4 : kKeyTiles * kTileBytes;
+  return train ? 2 * kKeyTiles * kTileBytes + 3 * kChunk * 4 + 2 * kBlocks * kTileBytes
+               : kKeyTiles * kTileBytes;
 }
 __host__ __device__ constexpr uint64_t value_block_bytes(bool train) {
   return kHeadFactors + kReadOutBytes + (train ? 3 : 1) * kTriangleBytes;
 }
-// Places inside a key block: K^T, then for training Q^T and the norms (fp32 1/|k|,
-// scale/|q|, 1/|q|).
+// Places inside a key block: K^T, then for training Q^T, the norms (fp32 1/|k|,
+// scale/|q|, 1/|q|), and q_i.k_j and k_i.k_j of scaled unit rows (fp32 accumulators, the
+// two of each block side by side).
 constexpr int kKeyColumns = 0;
 constexpr int kQueryColumns = kKeyTiles * kTileBytes;
 constexpr int kNorms = 2 * kKeyTiles * kTileBytes;
+constexpr int kDots = kNorms + 3 * kChunk * 4;
 // Places inside a value block: factors, N b, P b, then for training N^T b and P^T.
 constexpr int kSolve = kHeadFactors;
 constexpr int kReadOut = kSolve + kTriangleBytes;

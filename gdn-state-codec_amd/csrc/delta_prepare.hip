@@ -415,6 +415,20 @@ __global__ __launch_bounds__(kThreads, kTrain ? 2 : 3) void delta_prepare_kernel
         s.kk.cell(at, 4 * g + i, r) = kk[c][i];
         s.qk.cell(at, 4 * g + i, r) = qk[c][i];
       }
+      if constexpr (kTrain) {  // of unit rows, for the decays' gradients
+        const f32x4 k_unit = load4(&s.k_unit[16 * wave + 4 * g]);
+        const f32x4 q_unit = load4(&s.q_unit[16 * wave + 4 * g]);
+        const float unit = s.k_unit[16 * c + r];
+        f32x4* const dots = reinterpret_cast<f32x4*>(key_block + kDots + 2 * at * kTileBytes);
+        f32x4 x, y;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] = qk[c][i] * (q_unit[i] * unit);
+          y[i] = kk[c][i] * (k_unit[i] * unit);
+        }
+        dots[lane] = x;
+        dots[64 + lane] = y;
+      }
     }
   }
   __syncthreads();
