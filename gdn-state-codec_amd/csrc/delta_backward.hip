@@ -868,6 +868,15 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
       for (int p = 0; p < 3; ++p) s.rows[1][p][unit][lane] = part[p];
     }
     stage_ready();
+    // Products of unit rows for blocks `wave` and `wave` + 8, asked for ahead of S0: loads
+    // come back in order.
+    f32x4 qk[2], kk[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const f32x4* const dots = reinterpret_cast<const f32x4*>(
+          keys + kDots + 2 * min(wave + 8 * u, kBlocks - 1) * kTileBytes);
+      qk[u] = dots[lane], kk[u] = dots[64 + lane];
+    }
     load_rows(s0, start);
     if (wave == 0) {
       const float b = s.factors[4 * lane + kStrength];
@@ -881,7 +890,10 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
 
     // F and H, ten blocks (i, j), j <= i, of 16 x 16; the two beside them that an
     // operand tile holds are zeros.
-    for (int block = wave; block < 12; block += 8) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int block = wave + 8 * u;
+      if (block >= 12) break;
       const int i = block < 1 ? 0 : block < 3 ? 1 : block < 6 ? 2 : block < 10 ? 3
                     : block == 10 ? 0 : 2;
       const int j = block < 10 ? block - i * (i + 1) / 2 : i + 1;
@@ -903,9 +915,6 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
       const int column = 16 * j + r;
       const float b_column = s.factors[4 * column + kStrength];
       const float sum = s.factors[kSum + column], rest = s.factors[kSumRest + column];
-      const f32x4* const dots = reinterpret_cast<const f32x4*>(
-          keys + kDots + 2 * min(block, kBlocks - 1) * kTileBytes);
-      const f32x4 qk = dots[lane], kk = dots[64 + lane];
       float to = 0.0f, whole = 0.0f;
       f32x4 from;
 #pragma unroll
@@ -920,7 +929,7 @@ __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args)
         s.h[line][column] = h;
         // The pairs of this row up to this column: they cross the tokens after it and,
         // within the row's block, up to the row.
-        const float pair = column < line ? fmaf(f, qk[c], -(h * kk[c])) : 0.0f;
+        const float pair = column < line ? fmaf(f, qk[u][c], -(h * kk[u][c])) : 0.0f;
         const float upto = sum_to_here(pair);
         const float before = shifted<kDppUp + 1>(upto);
         to += column <= line ? before : 0.0f;
