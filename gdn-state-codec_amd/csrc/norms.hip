@@ -36,9 +36,22 @@ namespace {
 constexpr int kThreads = 256;
 constexpr uint32_t kMaxWidth = 16384;
 
-// sigmoid on the transcendental unit (exp2 and reciprocal, about an ulp each).
+// sigmoid of a T on the transcendental unit (exp2 and reciprocal, about an ulp each).  The
+// exponent's rounding puts up to |z| 2^-24 on the exponential: nothing beside a bf16
+// value's own, but 65 x 2^-24 of an fp32 output at z = -80.  For fp32 what the product (and
+// log2 e) left out is therefore put back as a factor: 6 x 2^-24 at any z.  The bounds, which
+// only infinities and NaN reach, leave those what the exponential makes of them.
+template <typename T>
 __device__ __forceinline__ float sigmoid(float z) {
-  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.44269504088896341f * z));
+  constexpr float kLog2E = 1.44269502162933349609375f, kLog2ERest = 1.92596303e-8f;
+  constexpr float kLn2 = 0.693147180559945309f;
+  const float t = -kLog2E * z;
+  float power = __builtin_amdgcn_exp2f(t);
+  if constexpr (sizeof(T) == sizeof(float)) {
+    const float rest = fmaf(-kLog2ERest, z, fmaf(-kLog2E, z, -t));
+    power *= fmaf(fminf(fmaxf(rest, -1.0e-4f), 1.0e-4f), kLn2, 1.0f);
+  }
+  return __builtin_amdgcn_rcpf(1.0f + power);
 }
 
 __device__ __forceinline__ float sum16(float x) {  // over the 16 lanes of a DPP row
@@ -75,7 +88,7 @@ __global__ __launch_bounds__(kThreads) void gated_norm_kernel(
   load8(weight + 8 * l, w);
   const float r = 1.0f / sqrtf(sum16(dot8(v, v)) * (1.0f / kDim) + eps);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = v[i] * r * w[i] * (z[i] * sigmoid(z[i]));
+  for (int i = 0; i < 8; ++i) v[i] = v[i] * r * w[i] * (z[i] * sigmoid<T>(z[i]));
   store8(out + row * kDim + 8 * l, v);
 }
 
@@ -99,7 +112,7 @@ __global__ __launch_bounds__(kThreads) void gated_norm_backward_kernel(
     float d_n[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float s = sigmoid(z[i]);
+      const float s = sigmoid<T>(z[i]);
       v[i] *= r;  // the normalized row
       const float through = z[i] * s;
       const float dn = d[i] * v[i];
