@@ -86,3 +86,56 @@ def test_saved_elsewhere(batch, hooks):
         outs = block(*leaves, tables)
     for a, b in zip(gradients(outs, leaves, given), want):
         assert torch.equal(a, b)
+
+
+def test_gradients_that_start_anywhere(batch):
+    """Outputs joined behind an odd number of values: their gradients are unaligned slices."""
+    leaves, tables, given = batch
+    want = gradients(block(*leaves, tables), leaves, given)
+    outs = block(*leaves, tables)
+    joined = torch.cat([given[1].new_zeros(3)] + [x.float().flatten() for x in outs])
+    d = torch.cat([given[1].new_zeros(3)] + [x.float().flatten() for x in given])
+    for a, b in zip(gradients([joined], leaves, [d]), want):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("lengths", [[130, 0, 64, 7], [130, 0, 64, 7] * 3])
+def test_a_captured_training_pass_replays(device, lengths):
+    gen = torch.Generator().manual_seed(73)
+    total = sum(lengths)
+
+    def made(*shape):
+        return torch.randn(shape, generator=gen).to(device)
+
+    leaves = [made(total, (2 * KEY_HEADS + HEADS) * 128).bfloat16(),
+              -0.2 * made(total, HEADS).abs(), torch.sigmoid(made(total, HEADS)).bfloat16(),
+              0.1 * made(len(lengths), HEADS, 128, 128), made(total, HEADS, 128).bfloat16(),
+              1.0 + 0.1 * made(128)]
+    leaves = [x.requires_grad_() for x in leaves]
+    given = [made(total, HEADS, 128).bfloat16(), made(len(lengths), HEADS, 128, 128)]
+    lens, slots = ints(lengths, device), ints(range(len(lengths)), device)
+
+    def work():
+        tables = gdn.request_tables(lens, slots, total)
+        outs = block(*leaves, tables)
+        return [*(x.detach() for x in outs), *torch.autograd.grad(outs, leaves, given)]
+
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        work()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = work()
+    for i in range(3):
+        with torch.no_grad():
+            leaves[0].mul_(0.5 + 0.25 * i)
+        eager = [x.clone() for x in work()]
+        for x in held:
+            x.fill_(3.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(held, eager):
+            assert torch.equal(a, b)
