@@ -144,7 +144,7 @@ def _token_rows(t: torch.Tensor, name: str, tokens: int) -> int:
 
 def _rule_inputs(queries, keys, values, log_decay, beta):
     """Checks one batch of tokens; returns (tokens, value heads, key heads, strides)."""
-    tokens = queries.shape[0]
+    tokens = queries.shape[0] if queries.dim() else 0
     strides = (_token_rows(queries, "queries", tokens), _token_rows(keys, "keys", tokens),
                _token_rows(values, "values", tokens))
     heads, key_heads = values.shape[1], keys.shape[1]
@@ -282,7 +282,9 @@ class _GatedDeltaRule(torch.autograd.Function):
     def forward(ctx, queries, keys, values, log_decay, beta, initial, tables, scale, normalize):
         rule, workspace = _rule(queries, keys, values, log_decay, beta, tables, scale, normalize,
                                 None, True)
-        heads = values.shape[1]
+        heads = rule.value_heads
+        if initial is not None:
+            _dense(initial, "initial states", (rule.requests, heads, DIM, DIM), torch.float32)
         out = torch.empty((rule.tokens, heads, DIM), dtype=torch.bfloat16, device=values.device)
         final = torch.empty((rule.requests, heads, DIM, DIM), dtype=torch.float32,
                             device=values.device)
@@ -331,9 +333,6 @@ def gated_delta_rule(queries: torch.Tensor, keys: torch.Tensor, values: torch.Te
     None: zeros) in the pool's place.  out is bf16 [T,H,128] (zeros in rows of no
     request), final fp32 like initial.  The graph keeps a workspace of
     ``workspace_bytes(T, N, H, Hk, train=True)`` until its backward pass."""
-    if initial is not None:
-        _dense(initial, "initial states", (tables.order.numel(), values.shape[1], DIM, DIM),
-               torch.float32)
     return _GatedDeltaRule.apply(queries, keys, values, log_decay, beta, initial, tables, scale,
                                  normalize)
 

@@ -202,3 +202,20 @@ def test_serving_calls_refuse_what_they_cannot_differentiate(calls, call, place)
     with torch.no_grad():
         functions[call](*wanted)
     assert len(calls) == 3
+
+
+@pytest.mark.parametrize("place,shape", [(0, ()), (0, (TOKENS,)), (1, ()), (1, (TOKENS,)),
+                                         (2, ()), (2, (TOKENS,)), (3, ()), (4, ())])
+def test_inputs_without_dimensions_are_refused(calls, place, shape):
+    leaves, tables = batch()
+    inputs = [x.detach() for x in leaves]
+    inputs[place] = torch.zeros(shape, dtype=inputs[place].dtype)
+    pool = torch.zeros(3, HEADS, 128, 128)
+    slots = torch.zeros(TOKENS, dtype=torch.int32)
+    for call in (lambda: gdn.gated_delta_step(*inputs, pool, slots),
+                 lambda: gdn.gated_delta_prefill(*inputs, tables, slots[:2], pool),
+                 lambda: gdn.gated_delta_rule(*inputs, tables),
+                 lambda: gdn.gated_delta_rule(*inputs, tables, pool[:2])):
+        with pytest.raises(RuntimeError, match="GDN State Codec"):
+            call()
+    assert not calls
