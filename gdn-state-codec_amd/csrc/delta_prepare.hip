@@ -15,9 +15,9 @@
 // are stable for any keys, which powers of A are not.
 //
 // Bound by what it writes: of 32,768 tokens, 16 key heads and 32 value heads it reads
-// 268 MB and writes 671 in 200 us, 4.7 TB/s (a copy: 5.2; 220 us with the matrices whole
+// 268 MB and writes 671 in 200 us, 4.7 TB/s (a copy: 6.1; 220 us with the matrices whole
 // and two workgroups a compute unit); a training pass of 5,298 tokens, with the
-// transposes, takes 60 us.
+// transposes and the products of unit rows, takes 63 us.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -426,8 +426,8 @@ __global__ __launch_bounds__(kThreads, kTrain ? 2 : 3) void delta_prepare_kernel
           x[i] = qk[c][i] * (q_unit[i] * unit);
           y[i] = kk[c][i] * (k_unit[i] * unit);
         }
-        dots[lane] = x;
-        dots[64 + lane] = y;
+        __builtin_nontemporal_store(x, dots + lane);  // read when both scans are done
+        __builtin_nontemporal_store(y, dots + 64 + lane);
       }
     }
   }
