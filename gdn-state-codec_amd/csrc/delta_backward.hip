@@ -752,14 +752,14 @@ static_assert(sizeof(Gradient) <= kLdsPerCu, "one workgroup a compute unit");
 // and all tokens, so that a state is loaded and cut into parts once.  X and E are cut
 // once, by the wavefront that loads them, and so are F and H.
 //
-// 32 heads of 85 chunks take 255 us: 650 MB of states, E and X (2.5 TB/s), 2,850 matrix
+// 32 heads of 85 chunks take 260 us: 535 MB of S0, dS1, E and X (2.1 TB/s), 2,850 matrix
 // instructions a chunk and head (a fifth of their rate).  The parts of X and E leave room
 // for one workgroup a compute unit, whose phases (loads, F and H, the states' products,
-// the kinds) wait for each other: of some 35,000 cycles a head, loads take a third and
-// LDS reads as much.  Measured and left out: the next head's X and E asked for a phase
-// ahead in a loop over chunks (286 us, with the registers it takes), F and H dealt out
-// evenly (274), two tiles of keys by two of tokens a wavefront (262, every state loaded
-// and cut twice).
+// the kinds) wait for each other: loads take a third of a head's time and LDS reads as
+// much.  The pairs' sums for dg take 18 us of it.  Measured without them (255 us then) and
+// left out: the next head's X and E asked for a phase ahead in a loop over chunks (286 us, with
+// the registers it takes), F and H dealt out evenly (274), two tiles of keys by two of
+// tokens a wavefront (262, every state loaded and cut twice).
 __global__ __launch_bounds__(kThreads) void delta_gradient_kernel(BackArgs args) {
   __shared__ __align__(16) Gradient s;
   const RuleArgs& a = args.rule;

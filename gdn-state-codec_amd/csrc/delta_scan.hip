@@ -1011,7 +1011,9 @@ int32_t launch_delta_scan(void* stream, const ScanArgs& args, uint32_t dtype) {
   // units, beat the narrow form's one chain: 64 on the average and 4 for each request x
   // head.  32 heads of one request (narrow form in brackets, whole calls): 32,768 tokens
   // 1,000 us (1,240), 8,192 280 (313), 4,096 158 (147).  8 heads: 32,768 tokens 362 (958),
-  // 4,096 90 (118).  One head: 4,096 tokens 78 (113).
+  // 4,096 90 (118).  One head: 4,096 tokens 78 (113).  The average hides one long request
+  // among short ones: 32,768 tokens and one more of another request, 32 heads, go through
+  // the wide form's one chain in 1,550 us.
   const uint64_t chunks = args.rule.space.rows / args.rule.requests;
   if (items <= kSplitItems && chunks >= std::max<uint64_t>(kSplitChunks, 4 * items)) {
     return dtype == kDtypeF32 ? scan_in_segments<float>(stream, args)

@@ -35,11 +35,12 @@ constexpr uint32_t kDtypeBF16 = 1;
 // Largest grid the launchers issue along x (hardware limit 2^31 - 1).
 constexpr uint64_t kMaxGrid = 0x7FFFFFFFull;
 
+constexpr uint32_t kComputeUnits = 256;
+
 // A CU has 163,840 bytes of LDS, and gfx950 allocates a workgroup's LDS in
 // 1,280-byte granules (measured: csrc/bench/lds_probe.hip), so k workgroups
 // share a CU only while k x ceil(bytes / 1280) x 1280 <= 163,840.  One byte
 // past a multiple of 1,280 costs a whole granule.
-constexpr uint32_t kComputeUnits = 256;
 constexpr uint32_t kLdsPerCu = 163840;
 constexpr uint32_t kLdsGranule = 1280;
 constexpr uint32_t workgroups_by_lds(uint64_t bytes) {

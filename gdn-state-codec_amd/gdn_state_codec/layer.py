@@ -252,7 +252,9 @@ def gated_delta_prefill(queries: torch.Tensor, keys: torch.Tensor, values: torch
     projection are fine), log_decay fp32 and beta bf16 [T,H]; ``tables`` are
     :func:`request_tables`' for ``max_tokens`` T and the same slot ids.  Returns
     bf16 [T,H,128]; rows of no request, and padding's, stay as they were.
-    ``workspace`` (uint8, :func:`workspace_bytes`) may be kept between calls.  Not
+    ``workspace`` (uint8, :func:`workspace_bytes`) may be kept between calls; without
+    ``out`` a call also clears a new one.  An output's terms are good to 2^-15 each (the
+    states to fp32).  Not
     differentiable, as :func:`gated_delta_step`; :func:`gated_delta_rule` is."""
     rule, workspace = _rule(queries, keys, values, log_decay, beta, tables, scale, normalize,
                             workspace, False)
@@ -332,7 +334,8 @@ def gated_delta_rule(queries: torch.Tensor, keys: torch.Tensor, values: torch.Te
     :func:`gated_delta_prefill` with ``initial`` fp32 [N,H,128 value,128 key] (or
     None: zeros) in the pool's place.  out is bf16 [T,H,128] (zeros in rows of no
     request), final fp32 like initial.  The graph keeps a workspace of
-    ``workspace_bytes(T, N, H, Hk, train=True)`` until its backward pass."""
+    ``workspace_bytes(T, N, H, Hk, train=True)`` until its backward pass; under hooks on
+    saved tensors (checkpointing, offloading) that and the inputs are the hooks'."""
     return _GatedDeltaRule.apply(queries, keys, values, log_decay, beta, initial, tables, scale,
                                  normalize)
 

@@ -19,6 +19,13 @@
  * sqrt(sum of squares + 1e-6), and q is multiplied by `scale`.  Value head h
  * reads key head h / (value_heads / key_heads).
  *
+ * States and their gradients are formed in fp32 throughout.  In the whole-sequence
+ * calls an output is a sum over its chunk's start state and the writes since, whose
+ * terms are good to 2^-15 each before the sum is rounded to bf16: an output far below
+ * its terms (under 2^-6 of them) has fewer bits than bf16 holds.  A NaN or an infinity
+ * in a token may reach its request's outputs from its 64-token chunk's start on; other
+ * requests never see it.
+ *
  * Same conventions as gdn_state_codec_kernel.h: asynchronous on `stream` (NULL
  * = HIP's null stream), no allocation, status 0 / 1 (bad argument) / 5 (launch
  * failed), and every device pointer 16-byte aligned but log_decay and beta, which
@@ -105,7 +112,7 @@ uint64_t statecentric_gdn_state_codec_gated_delta_workspace_v1(
     uint32_t rows, uint32_t value_heads, uint32_t key_heads, uint32_t train);
 
 /* Whole sequences on a slot-indexed pool [slots][value_heads][128 value]
- * [128 key] of pool_dtype: request r starts from its slot's state (resume NULL or
+ * [128 key] of pool_dtype (the tables made with the same slot ids): request r starts from its slot's state (resume NULL or
  * resume[r] != 0) or from zeros, and leaves its final state there.  slot_ids int32
  * [requests] (distinct); a request whose slot is outside 0..slots-1 (padding, -1)
  * is skipped, its outputs left as they were.  An empty request leaves its state, or
