@@ -1,0 +1,457 @@
+// Copies between the slots of a state cache: the order in which any pairs (source,
+// target) can be copied in place, the moves that pack live slots to the front, and the
+// copies.
+//
+// A pair has to be carried out before the pair that overwrites its source, if there is
+// one (its successor); every pair has at most one.  The pairs then form trees that end in
+// a pair whose source nobody overwrites, and cycles.  A cycle is cut before the pair of
+// its lowest number, which first keeps what its target held, and its last pair writes that.
+// Ordered by tree and by falling distance from the tree's end, every pair comes before
+// its successor, and pairs of different trees share no slot that is written.
+//
+// copy_slots needs no order between threads: a thread owns a run of 16 bytes of every
+// slot and carries the rows out in turn, 8 loads at a time.  A load may come before any
+// store (each reads what its slot held before the call), a store never before the loads
+// of the rows before it.  Trees are dealt over the grid's second dimension, so that many
+// small slots fill the card too.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "gdn_state_codec_slots.h"
+#include "launch.h"
+#include "stream_memory.h"
+
+namespace gdn {
+namespace {
+
+constexpr int kMaxPairs = GDN_STATE_CODEC_MAX_MOVES;
+constexpr int kMaxCompacted = GDN_STATE_CODEC_MAX_COMPACTED;
+constexpr int kSaves = GDN_STATE_CODEC_MOVE_SAVES;
+constexpr int kSaved = GDN_STATE_CODEC_MOVE_SAVED;
+
+// ---------------------------------------------------------------- the order
+
+constexpr int kPlanThreads = 1024;
+constexpr int kEach = kMaxPairs / kPlanThreads;
+constexpr int kHashed = 2 * kMaxPairs;
+
+struct Plan {
+  int32_t source[kMaxPairs];
+  int32_t target[kMaxPairs];
+  union {
+    int32_t hashed[kHashed];   // pairs by target, -1 free
+    uint64_t key[kMaxPairs];   // pairs in their order
+  };
+  int32_t next[kMaxPairs];     // a pair 2^i steps on
+  int32_t steps[kMaxPairs];    // how many of them are real
+  int32_t lowest[kMaxPairs];   // of the pairs passed
+  uint8_t flags[kMaxPairs];
+  uint8_t on_cycle[kMaxPairs];
+  int chained, cycles;
+};
+
+__device__ __forceinline__ uint32_t hash_of(int32_t target) {
+  return (static_cast<uint32_t>(target) * 2654435761u) >> (32 - 13);
+}
+static_assert(kHashed == 1 << 13, "the hash gives 13 bits");
+
+// The pair that writes `slot`, or -1.
+__device__ __forceinline__ int writer_of(const Plan& p, int32_t slot) {
+  uint32_t at = hash_of(slot);
+  for (int probe = 0; probe < kHashed; ++probe) {
+    const int pair = p.hashed[at];
+    if (pair < 0) return -1;
+    if (p.target[pair] == slot) return pair;
+    at = (at + 1) & (kHashed - 1);
+  }
+  return -1;
+}
+
+// next, steps and lowest after 2^rounds >= pairs steps, from one step.
+__device__ __forceinline__ void follow(Plan& p, int pairs) {
+  for (int reach = 1; reach < pairs; reach <<= 1) {
+    int32_t next[kEach], steps[kEach], lowest[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int i = threadIdx.x + e * kPlanThreads;
+      if (i >= pairs) break;
+      const int n = p.next[i];
+      next[e] = p.next[n];
+      steps[e] = p.steps[i] + p.steps[n];
+      lowest[e] = min(p.lowest[i], p.lowest[n]);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int i = threadIdx.x + e * kPlanThreads;
+      if (i >= pairs) break;
+      p.next[i] = next[e];
+      p.steps[i] = steps[e];
+      p.lowest[i] = lowest[e];
+    }
+    __syncthreads();
+  }
+}
+
+__global__ __launch_bounds__(kPlanThreads) void slot_moves_kernel(
+    const int32_t* __restrict__ sources, const int32_t* __restrict__ targets, int pairs,
+    uint32_t slots, int4* __restrict__ steps) {
+  __shared__ Plan p;
+  const int t = threadIdx.x;
+  for (int i = t; i < kHashed; i += kPlanThreads) p.hashed[i] = -1;
+  if (t == 0) p.chained = p.cycles = 0;
+  for (int i = t; i < pairs; i += kPlanThreads) {
+    const int32_t source = sources[i], target = targets[i];
+    const bool counts = static_cast<uint32_t>(target) < slots &&
+                        (source == -1 || static_cast<uint32_t>(source) < slots);
+    p.source[i] = source;
+    p.target[i] = counts ? target : -1;
+    p.flags[i] = p.on_cycle[i] = 0;
+  }
+  __syncthreads();
+  for (int i = t; i < pairs; i += kPlanThreads) {
+    const int32_t target = p.target[i];
+    if (target < 0) continue;
+    uint32_t at = hash_of(target);
+    while (true) {  // at most 4096 of 8192 places are ever taken
+      const int before = atomicCAS(&p.hashed[at], -1, i);
+      if (before < 0) break;
+      if (p.target[before] == target) {  // the last pair of a target counts
+        atomicMax(&p.hashed[at], i);
+        break;
+      }
+      at = (at + 1) & (kHashed - 1);
+    }
+  }
+  __syncthreads();
+  bool live[kEach];
+  int after[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = t + e * kPlanThreads;
+    live[e] = false;
+    after[e] = -1;
+    if (i >= pairs) break;
+    live[e] = p.target[i] >= 0 && writer_of(p, p.target[i]) == i;
+    if (live[e] && p.source[i] >= 0) {
+      after[e] = writer_of(p, p.source[i]);
+      if (after[e] == i) after[e] = -1;  // onto itself
+    }
+    p.next[i] = after[e] >= 0 ? after[e] : i;
+    p.steps[i] = after[e] >= 0 ? 1 : 0;
+    p.lowest[i] = i;
+    if (after[e] >= 0) p.chained = 1;
+  }
+  __syncthreads();
+  if (!p.chained) {  // no source is overwritten: any order will do
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int i = t + e * kPlanThreads;
+      if (i >= pairs) break;
+      steps[i] = live[e] ? make_int4(p.source[i], p.target[i], 0, i + 1)
+                         : make_int4(-1, -1, 0, i + 1);
+    }
+    return;
+  }
+
+  follow(p, pairs);
+  // Whoever has not come to an end is on a cycle now, and every pair of a cycle is
+  // reached by one of its own.
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = t + e * kPlanThreads;
+    if (i >= pairs) break;
+    // An end is its own successor; 2^rounds >= pairs real steps are taken only on cycles.
+    if (p.steps[i] >= pairs) {
+      p.on_cycle[p.next[i]] = 1;
+      p.cycles = 1;
+    }
+  }
+  __syncthreads();
+  if (p.cycles) {
+    int head[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int i = t + e * kPlanThreads;
+      head[e] = i < pairs && p.on_cycle[i] ? p.lowest[i] : -1;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int i = t + e * kPlanThreads;
+      if (i >= pairs) break;
+      if (head[e] == i) p.flags[i] |= kSaves;
+      if (head[e] >= 0 && after[e] == head[e]) {
+        p.flags[i] |= kSaved;
+        after[e] = -1;
+      }
+      p.next[i] = after[e] >= 0 ? after[e] : i;
+      p.steps[i] = after[e] >= 0 ? 1 : 0;
+    }
+    __syncthreads();
+    follow(p, pairs);
+  }
+
+  // Order by tree (the pair at its end; what is left out last), then by falling distance.
+  int size = 1;
+  while (size < pairs) size <<= 1;
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = t + e * kPlanThreads;
+    if (i >= size) break;
+    uint64_t key = ~0ull;
+    if (i < pairs) {
+      const uint64_t tree = live[e] ? p.next[i] : kMaxPairs;
+      const uint64_t away = live[e] ? kMaxPairs - p.steps[i] : 0;
+      key = tree << 32 | away << 16 | i;
+    }
+    p.key[i] = key;
+  }
+  __syncthreads();
+  for (int run = 2; run <= size; run <<= 1) {
+    for (int gap = run >> 1; gap > 0; gap >>= 1) {
+      for (int i = t; i < size; i += kPlanThreads) {
+        const int other = i ^ gap;
+        if (other > i) {
+          const uint64_t x = p.key[i], y = p.key[other];
+          if ((x > y) == ((i & run) == 0)) {
+            p.key[i] = y;
+            p.key[other] = x;
+          }
+        }
+      }
+      __syncthreads();
+    }
+  }
+  for (int place = t; place < pairs; place += kPlanThreads) {
+    const uint64_t key = p.key[place];
+    const int i = static_cast<int>(key & 0xFFFF);
+    const uint32_t tree = static_cast<uint32_t>(key >> 32);
+    if (tree == kMaxPairs) {
+      steps[place] = make_int4(-1, -1, 0, place + 1);
+      continue;
+    }
+    int low = place + 1, high = pairs;  // the first place of another tree
+    while (low < high) {
+      const int middle = (low + high) / 2;
+      if (static_cast<uint32_t>(p.key[middle] >> 32) == tree) low = middle + 1;
+      else high = middle;
+    }
+    steps[place] = make_int4(p.source[i], p.target[i], p.flags[i], low);
+  }
+}
+
+// --------------------------------------------------------------- compaction
+
+// Sum of the threads before this one; `total` is the workgroup's.
+__device__ __forceinline__ int sum_before(int x, int (&waves)[16], int& total) {
+  const int lane = threadIdx.x & 63;
+  int sum = x;
+#pragma unroll
+  for (int step = 1; step < 64; step <<= 1) {
+    const int other = __shfl_up(sum, step);
+    if (lane >= step) sum += other;
+  }
+  if (lane == 63) waves[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    if (w < static_cast<int>(threadIdx.x >> 6)) before += waves[w];
+    total += waves[w];
+  }
+  return before + sum - x;
+}
+
+__global__ __launch_bounds__(kPlanThreads) void compaction_kernel(
+    const int32_t* __restrict__ live, int slots, int4* __restrict__ steps,
+    int32_t* __restrict__ placed, int32_t* __restrict__ count) {
+  __shared__ uint16_t free_slot[kMaxCompacted / 2];
+  __shared__ int waves[16];
+  __shared__ int before_count;
+  const int t = threadIdx.x;
+  const int each = (slots + kPlanThreads - 1) / kPlanThreads;  // consecutive slots a thread
+  const int first = min(t * each, slots), last = min(first + each, slots);
+  int own = 0;
+  for (int i = first; i < last; ++i) own += live[i] != 0 ? 1 : 0;
+  int total;
+  const int before = sum_before(own, waves, total);
+  if (t == 0) {
+    *count = total;
+    before_count = total;  // where every place before `total` is live
+  }
+  __syncthreads();
+  // The free places before `total`, in order; how many live ones there are.
+  int seen = before;
+  for (int i = first; i < last; ++i) {
+    if (i == total) before_count = seen;
+    const bool is = live[i] != 0;
+    if (i < total && !is) free_slot[i - seen] = static_cast<uint16_t>(i);
+    seen += is ? 1 : 0;
+  }
+  __syncthreads();
+  seen = before;
+  const int moves = total - before_count;
+  for (int i = first; i < last; ++i) {
+    const bool is = live[i] != 0;
+    int to = is ? i : -1;
+    if (is && i >= total) {
+      const int place = seen - before_count;
+      to = free_slot[place];
+      steps[place] = make_int4(i, to, 0, place + 1);
+    }
+    placed[i] = to;
+    seen += is ? 1 : 0;
+  }
+  for (int i = moves + t; i < (slots + 1) / 2; i += kPlanThreads) {
+    steps[i] = make_int4(-1, -1, 0, i + 1);
+  }
+}
+
+// ------------------------------------------------------------------- copies
+
+constexpr int kCopyThreads = 256;
+constexpr int kBatch = 8;         // rows whose loads are all asked for before the first store
+constexpr int kMostBuffers = 64;  // of one launch
+constexpr uint32_t kFill = 8 * kComputeUnits;  // workgroups that fill the card
+
+struct CopyBuffer {
+  const char* from;
+  char* to;
+  uint64_t bytes;       // a slot
+  uint32_t first;       // its first workgroup
+  uint32_t unit;        // bytes a thread: 16, 4 or 1
+};
+
+struct CopyArgs {
+  CopyBuffer buffers[kMostBuffers];
+  const int4* steps;
+  uint32_t count, rows, slots;
+};
+
+// A thread's run of `sizeof(Unit)` bytes of every slot, for rows begin .. end - 1.
+template <typename Unit>
+__device__ __forceinline__ void copy_rows(const CopyBuffer& b, uint64_t at, const int4* steps,
+                                          uint32_t begin, uint32_t end, uint32_t slots) {
+  if (at >= b.bytes) return;
+  const char* const from = b.from + at;
+  char* const to = b.to + at;
+  Unit kept = {};
+  for (uint32_t first = begin; first < end; first += kBatch) {
+    int4 row[kBatch];
+    Unit x[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      row[i] = first + i < end ? steps[first + i] : make_int4(-1, -1, 0, 0);
+      if (static_cast<uint32_t>(row[i].y) >= slots) row[i].y = -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      x[i] = Unit{};
+      if (row[i].y >= 0 && static_cast<uint32_t>(row[i].x) < slots && !(row[i].z & kSaved)) {
+        x[i] = __builtin_nontemporal_load(
+            reinterpret_cast<const Unit*>(from + row[i].x * b.bytes));
+      }
+      if (row[i].y >= 0 && (row[i].z & kSaves)) {
+        kept = *reinterpret_cast<const Unit*>(from + row[i].y * b.bytes);
+      }
+      if (row[i].z & kSaved) x[i] = kept;
+    }
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (row[i].y >= 0) {
+        __builtin_nontemporal_store(x[i], reinterpret_cast<Unit*>(to + row[i].y * b.bytes));
+      }
+    }
+  }
+}
+
+// The first row of part `part` of `parts`, moved on to the end of a tree.
+__device__ __forceinline__ uint32_t part_begin(const int4* steps, uint32_t rows, uint32_t part,
+                                               uint32_t parts) {
+  const uint32_t at = static_cast<uint32_t>(static_cast<uint64_t>(rows) * part / parts);
+  if (at == 0 || at >= rows) return min(at, rows);
+  return min(max(static_cast<uint32_t>(steps[at - 1].w), at), rows);
+}
+
+__global__ __launch_bounds__(kCopyThreads) void copy_slots_kernel(CopyArgs a) {
+  uint32_t i = 0;
+  while (i + 1 < a.count && a.buffers[i + 1].first <= blockIdx.x) ++i;
+  const CopyBuffer b = a.buffers[i];
+  const uint32_t begin = part_begin(a.steps, a.rows, blockIdx.y, gridDim.y);
+  const uint32_t end = part_begin(a.steps, a.rows, blockIdx.y + 1, gridDim.y);
+  const uint64_t at =
+      (static_cast<uint64_t>(blockIdx.x - b.first) * kCopyThreads + threadIdx.x) * b.unit;
+  if (b.unit == 16) copy_rows<u32x4_t>(b, at, a.steps, begin, end, a.slots);
+  else if (b.unit == 4) copy_rows<uint32_t>(b, at, a.steps, begin, end, a.slots);
+  else copy_rows<uint8_t>(b, at, a.steps, begin, end, a.slots);
+}
+
+}  // namespace
+}  // namespace gdn
+
+extern "C" int32_t statecentric_gdn_state_codec_slot_moves_launch_v1(
+    void* stream, const int32_t* sources, const int32_t* targets, uint32_t pairs, uint32_t slots,
+    int32_t* steps) {
+  if (!sources || !targets || !steps || pairs == 0 || pairs > GDN_STATE_CODEC_MAX_MOVES ||
+      slots == 0 || slots > 0x7FFFFFFFu || !gdn::aligned16(sources, targets, steps)) {
+    return gdn::kStatusInvalidArgument;
+  }
+  return gdn::launch(gdn::slot_moves_kernel, dim3(1), dim3(gdn::kPlanThreads), stream, sources,
+                     targets, static_cast<int>(pairs), slots, reinterpret_cast<int4*>(steps));
+}
+
+extern "C" int32_t statecentric_gdn_state_codec_compaction_moves_launch_v1(
+    void* stream, const int32_t* live, uint32_t slots, int32_t* steps, int32_t* placed,
+    int32_t* count) {
+  if (!live || !steps || !placed || !count || slots == 0 ||
+      slots > GDN_STATE_CODEC_MAX_COMPACTED || !gdn::aligned16(live, steps, placed, count)) {
+    return gdn::kStatusInvalidArgument;
+  }
+  return gdn::launch(gdn::compaction_kernel, dim3(1), dim3(gdn::kPlanThreads), stream, live,
+                     static_cast<int>(slots), reinterpret_cast<int4*>(steps), placed, count);
+}
+
+extern "C" int32_t statecentric_gdn_state_codec_copy_slots_launch_v1(
+    void* stream, const gdn_state_codec_slot_buffer* buffers, uint32_t count,
+    const int32_t* steps, uint32_t rows, uint32_t slots) {
+  if (!buffers || !steps || count == 0 || rows == 0 || rows > 0x7FFFFFFFu || slots == 0 ||
+      slots > 0x7FFFFFFFu || !gdn::aligned16(steps)) {
+    return gdn::kStatusInvalidArgument;
+  }
+  for (uint32_t i = 0; i < count; ++i) {
+    const uint64_t bytes = buffers[i].bytes;
+    // A buffer's size has to fit an address.
+    if (!buffers[i].from || !buffers[i].to || bytes == 0 || bytes > (1ull << 47) / slots ||
+        (bytes + 15) / 16 / gdn::kCopyThreads + 1 > gdn::kMaxGrid / gdn::kMostBuffers / 16) {
+      return gdn::kStatusInvalidArgument;
+    }
+  }
+  for (uint32_t done = 0; done < count; done += gdn::kMostBuffers) {
+    gdn::CopyArgs args;
+    args.steps = reinterpret_cast<const int4*>(steps);
+    args.count = count - done < gdn::kMostBuffers ? count - done : gdn::kMostBuffers;
+    args.rows = rows;
+    args.slots = slots;
+    uint64_t blocks = 0;
+    for (uint32_t i = 0; i < args.count; ++i) {
+      const gdn_state_codec_slot_buffer& b = buffers[done + i];
+      const uint64_t bits = reinterpret_cast<uintptr_t>(b.from) |
+                            reinterpret_cast<uintptr_t>(b.to) | b.bytes;
+      const uint32_t unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
+      args.buffers[i] = {static_cast<const char*>(b.from), static_cast<char*>(b.to), b.bytes,
+                         static_cast<uint32_t>(blocks), unit};
+      const uint64_t run = static_cast<uint64_t>(unit) * gdn::kCopyThreads;
+      blocks += (b.bytes + run - 1) / run;
+    }
+    uint64_t parts = (gdn::kFill + blocks - 1) / blocks;
+    if (parts > rows) parts = rows;
+    const int32_t status =
+        gdn::launch(gdn::copy_slots_kernel,
+                    dim3(static_cast<uint32_t>(blocks), static_cast<uint32_t>(parts)),
+                    dim3(gdn::kCopyThreads), stream, args);
+    if (status != gdn::kStatusOk) return status;
+  }
+  return gdn::kStatusOk;
+}

@@ -35,6 +35,24 @@ class RuleStruct(ctypes.Structure):
         + [("scale", _F), ("normalize", _U32)])
 
 
+class DraftsStruct(ctypes.Structure):
+    """``gdn_state_codec_drafts`` (include/gdn_state_codec_layer.h)."""
+
+    _fields_ = (
+        [(name, _P) for name in ("queries", "keys", "values", "log_decay", "beta")]
+        + [(name, _U64) for name in ("query_stride", "key_stride", "value_stride")]
+        + [(name, _P) for name in ("parents", "offsets", "slot_ids")]
+        + [(name, _U32) for name in ("requests", "tokens", "value_heads", "key_heads",
+                                     "max_nodes")]
+        + [("scale", _F), ("normalize", _U32)])
+
+
+class SlotBufferStruct(ctypes.Structure):
+    """``gdn_state_codec_slot_buffer`` (include/gdn_state_codec_slots.h)."""
+
+    _fields_ = [("source", _P), ("to", _P), ("bytes", _U64)]
+
+
 # name -> argtypes (all return int32 status)
 SIGNATURES: dict[str, list] = {
     # codec, reference entry points
@@ -100,12 +118,18 @@ SIGNATURES: dict[str, list] = {
         [_P] * 5 + [_U32, _U32, _P],
     "statecentric_gdn_state_codec_gated_delta_forward_launch_v1": [_P] * 5,
     "statecentric_gdn_state_codec_gated_delta_backward_launch_v1": [_P] * 10,
+    "statecentric_gdn_state_codec_gated_delta_tree_launch_v1": [_P] * 3 + [_U32, _U32, _P],
+    "statecentric_gdn_state_codec_gated_delta_commit_launch_v1": [_P] * 4 + [_U32, _U32],
     "statecentric_gdn_state_codec_gated_norm_launch_v1": [_P] * 5 + [_U64, _U32, _F],
     "statecentric_gdn_state_codec_gated_norm_backward_launch_v1": [_P] * 9 + [_U64, _U32, _F],
     "statecentric_gdn_state_codec_residual_norm_launch_v1":
         [_P] * 6 + [_U64, _U32, _U32, _U32, _F, _F],
     "statecentric_gdn_state_codec_residual_norm_backward_launch_v1":
         [_P] * 9 + [_U64, _U32, _U32, _U32, _F, _F],
+    # include/gdn_state_codec_slots.h
+    "statecentric_gdn_state_codec_slot_moves_launch_v1": [_P] * 3 + [_U32, _U32, _P],
+    "statecentric_gdn_state_codec_compaction_moves_launch_v1": [_P] * 2 + [_U32] + [_P] * 3,
+    "statecentric_gdn_state_codec_copy_slots_launch_v1": [_P] * 2 + [_U32, _P, _U32, _U32],
 }
 
 # Entry points that do not return a status: name -> (argtypes, restype).

@@ -1,6 +1,7 @@
 """torch-facing dense operators of a gated-delta-net layer
 (include/gdn_state_codec_layer.h): the tables of a ragged batch, the gated delta
-rule for one token, for prefill and for training, and the norms around it.
+rule for one token, for prefill, for training and for trees of drafted tokens, and
+the norms around it.
 
 Each function checks shapes, dtypes, devices and strides on the host (raising
 ``RuntimeError``, as the codec's do), launches the gfx950 kernels on torch's
@@ -16,11 +17,12 @@ from typing import NamedTuple
 import torch
 from torch.autograd import forward_ad
 
-from ._native import RuleStruct, native
+from ._native import DraftsStruct, RuleStruct, native
 
 DIM = 128
 CHUNK = 64             # tokens of a row of RequestTables.chunks
 MAX_REQUESTS = 4096
+MAX_NODES = 64         # of a request's tree of drafted tokens
 QUERY_SCALE = DIM ** -0.5
 _TYPES = {torch.float32: 0, torch.bfloat16: 1}
 
@@ -338,6 +340,84 @@ def gated_delta_rule(queries: torch.Tensor, keys: torch.Tensor, values: torch.Te
     saved tensors (checkpointing, offloading) that and the inputs are the hooks'."""
     return _GatedDeltaRule.apply(queries, keys, values, log_decay, beta, initial, tables, scale,
                                  normalize)
+
+
+# ------------------------------------------------- trees of drafted tokens
+
+def _drafts(queries, keys, values, log_decay, beta, parents, tables, slot_ids, normalize,
+            max_nodes, scale):
+    """The checked argument struct of a batch of trees (queries None: a commit)."""
+    tokens, heads, key_heads, strides = _rule_inputs(keys if queries is None else queries, keys,
+                                                     values, log_decay, beta)
+    _dense(parents, "parents", (tokens,), torch.int32)
+    requests = slot_ids.numel()
+    if not 1 <= requests <= MAX_REQUESTS:
+        _fail(f"a batch of trees must hold 1..{MAX_REQUESTS} requests")
+    _dense(slot_ids, "slot ids", (requests,), torch.int32)
+    _dense(tables.offsets, "tables.offsets", (requests + 1,), torch.int32)
+    if not 1 <= max_nodes <= MAX_NODES:
+        _fail(f"max_nodes must be in 1..{MAX_NODES}")
+    return DraftsStruct(None if queries is None else queries.data_ptr(), keys.data_ptr(),
+                        values.data_ptr(), log_decay.data_ptr(), beta.data_ptr(), *strides,
+                        parents.data_ptr(), tables.offsets.data_ptr(), slot_ids.data_ptr(),
+                        requests, tokens, heads, key_heads, max_nodes, scale, normalize)
+
+
+def gated_delta_tree(queries: torch.Tensor, keys: torch.Tensor, values: torch.Tensor,
+                     log_decay: torch.Tensor, beta: torch.Tensor, parents: torch.Tensor,
+                     tables: RequestTables, slot_ids: torch.Tensor, pool: torch.Tensor,
+                     scale: float = QUERY_SCALE, normalize: bool = True,
+                     max_nodes: int = MAX_NODES, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The gated delta rule's output of every node of a tree of drafted tokens for each
+    of N requests, from the states ``pool`` [slots,H,128 value,128 key] (fp32 or bf16,
+    one layer) at ``slot_ids`` int32 [N], which stay as they are (so two requests may name
+    one slot; outside the pool, as -1: padding, skipped).
+
+    The nodes are token rows packed as :func:`gated_delta_prefill`'s (``tables`` are
+    :func:`request_tables`' of the trees' sizes): queries, keys bf16 [T,Hk,128], values
+    bf16 [T,H,128] (rows of a fused projection are fine), log_decay fp32 and beta bf16
+    [T,H].  ``parents`` int32 [T] gives each node's parent as a place in its own request,
+    an earlier node's; anything else, as -1, is the cached state, so that a request may
+    have several roots and a chain is -1, 0, 1, ..  A node sees the cached state, the nodes
+    above it and itself.  Only a request's first ``max_nodes`` (1..64) nodes are looked at:
+    where all trees are smaller, saying so saves time.
+
+    Returns bf16 [T,H,128]; rows of no request, of padding and of nodes past ``max_nodes``
+    stay as they were (zeros without ``out``).  A NaN or an infinity in a node's token
+    reaches outputs of that node and those below it only.  Not differentiable, as
+    :func:`gated_delta_step`."""
+    drafts = _drafts(queries, keys, values, log_decay, beta, parents, tables, slot_ids,
+                     normalize, max_nodes, scale)
+    pool_dtype = _pool(pool, drafts.value_heads)
+    _not_differentiated("gated delta tree", queries, keys, values, log_decay, beta, pool)
+    shape = (drafts.tokens, drafts.value_heads, DIM)
+    if out is None:
+        out = torch.zeros(shape, dtype=torch.bfloat16, device=values.device)
+    else:
+        _dense(out, "output", shape, torch.bfloat16)
+    _launched(native().gated_delta_tree_launch_v1(
+        _stream(), ctypes.byref(drafts), pool.data_ptr(), pool.shape[0], pool_dtype,
+        out.data_ptr()), "gated delta tree")
+    return out
+
+
+def gated_delta_commit(keys: torch.Tensor, values: torch.Tensor, log_decay: torch.Tensor,
+                       beta: torch.Tensor, parents: torch.Tensor, accepted: torch.Tensor,
+                       tables: RequestTables, slot_ids: torch.Tensor, pool: torch.Tensor,
+                       normalize: bool = True) -> None:
+    """Advances the states ``pool`` at ``slot_ids`` (distinct) in place by the accepted
+    nodes of :func:`gated_delta_tree`'s trees: those on the path from the cached state
+    down to ``accepted[r]`` (int32 [N], a node's place in its request, among its first 64).
+    A request that accepts nothing (-1, or no node's place) keeps its state.  The other
+    arguments are that call's.  A bf16 state is rounded once, however long the path."""
+    drafts = _drafts(None, keys, values, log_decay, beta, parents, tables, slot_ids, normalize,
+                     MAX_NODES, 1.0)
+    pool_dtype = _pool(pool, drafts.value_heads)
+    _not_differentiated("gated delta commit", keys, values, log_decay, beta, pool)
+    _dense(accepted, "accepted nodes", (drafts.requests,), torch.int32)
+    _launched(native().gated_delta_commit_launch_v1(
+        _stream(), ctypes.byref(drafts), accepted.data_ptr(), pool.data_ptr(), pool.shape[0],
+        pool_dtype), "gated delta commit")
 
 
 # ------------------------------------------------------------------ the norms

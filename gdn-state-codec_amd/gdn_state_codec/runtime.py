@@ -41,6 +41,7 @@ import torch
 
 from . import codec
 from ._native import OTHER_SIGNATURES, SIGNATURES, library_dir as default_library_dir
+from .slots import copy_slots, slot_moves
 from .window import POSITION_STRIDE, RANK, WINDOW, WindowSlot
 
 DIM = 128
@@ -230,6 +231,15 @@ class _Slot:
     def window_full(self) -> bool:
         return self.steps >= WINDOW
 
+    def blank(self) -> "_Slot":
+        """A slot of the same geometry and step count, its boundary and window not yet
+        written."""
+        window = self.window
+        other = _Slot(_Generation(*(torch.empty_like(getattr(window, name))
+                                    for name in _BOUNDARY_FIELDS)))
+        other.steps = self.steps
+        return other
+
     def trade_generations(self) -> None:
         """Make the freshly written spare boundary live; the old one becomes the spare."""
         for name in _BOUNDARY_FIELDS:
@@ -360,6 +370,22 @@ class GdnStateCodecRuntime:
         """Forget the slots of `cache_indices` (their dense state changed)."""
         for cache_index in cache_indices:
             self._slots.pop(cache_index, None)
+
+    def fork(self, cache_index: int, targets) -> None:
+        """Give each cache index of `targets` a slot of its own that goes on from where the
+        one of `cache_index` stands: its boundary, window and step count (a prefix's further
+        samples).  Slots they had are forgotten.  Raises where `cache_index` has no slot."""
+        slot = self._slots.get(cache_index)
+        if slot is None:
+            raise RuntimeError(f"GDN State Codec: cache index {cache_index} has no slot to fork")
+        targets = [target for target in dict.fromkeys(targets) if target != cache_index]
+        forks = [slot.blank() for _ in targets]
+        if forks:
+            live = slot.window.slot_rows(slot.heads)
+            whole = torch.zeros(1, dtype=torch.int32, device=slot.window.device)
+            copy_slots(live * len(forks), slot_moves(whole, whole, 1),
+                       into=[t for fork in forks for t in fork.window.slot_rows(slot.heads)])
+        self._slots.update(zip(targets, forks))
 
     @staticmethod
     def decode_fallback_reason(*, num_prefills: int, num_decodes: int, speculative: bool,

@@ -90,6 +90,14 @@ class WindowSlot:
         _check(self.record_corrections, "record_corrections", (s, WINDOW, DIM), _HALF, dev)
         _check(self.positions, "positions", (s, POSITION_STRIDE), _POS, dev)
 
+    def slot_rows(self, heads: int) -> list[torch.Tensor]:
+        """The nine buffers as [slots,heads,...] views, for slots of ``heads`` states each:
+        what :func:`copy_slots` takes."""
+        if heads < 1 or self.states % heads:
+            raise RuntimeError(f"slots of {heads} heads do not divide {self.states} states")
+        return [getattr(self, name).view(-1, heads, *getattr(self, name).shape[1:])
+                for name in self.__dataclass_fields__]
+
     def pointers(self) -> tuple:
         return (self.residual.data_ptr(), self.smoothing.data_ptr(), self.scales.data_ptr(),
                 self.compensator_keys.data_ptr(), self.compensator_values.data_ptr(),

@@ -9,6 +9,9 @@
  *   gated_delta_prefill     the rule over whole ragged sequences, on the pool
  *   gated_delta_forward,
  *   gated_delta_backward    the rule over packed sequences with every gradient
+ *   gated_delta_tree        the rule over a tree of drafted tokens per request,
+ *                           read from the pool and leaving it as it is
+ *   gated_delta_commit      the pool's states after an accepted path of such trees
  *   gated_norm, residual_norm (and _backward)
  *                           the norms after and before the block
  *
@@ -28,8 +31,8 @@
  *
  * Same conventions as gdn_state_codec_kernel.h: asynchronous on `stream` (NULL
  * = HIP's null stream), no allocation, status 0 / 1 (bad argument) / 5 (launch
- * failed), and every device pointer 16-byte aligned but log_decay and beta, which
- * need their element's alignment only (a slice of a batch may start anywhere).
+ * failed), and every device pointer 16-byte aligned but log_decay, beta and parents,
+ * which need their element's alignment only (a slice of a batch may start anywhere).
  */
 #ifndef GDN_STATE_CODEC_LAYER_H
 #define GDN_STATE_CODEC_LAYER_H
@@ -140,6 +143,57 @@ int32_t statecentric_gdn_state_codec_gated_delta_backward_launch_v1(
     void* stream, const gdn_state_codec_rule* rule, const uint16_t* d_outputs,
     const float* d_final, uint16_t* d_queries, uint16_t* d_keys, uint16_t* d_values,
     float* d_log_decay, uint16_t* d_beta, float* d_initial);
+
+/* Drafted tokens of each request as a tree: node i of request r is token row
+ * offsets[r] + i, and its parent is an earlier node of the request, or the cached
+ * state.  Only a request's first max_nodes nodes are looked at. */
+#define GDN_STATE_CODEC_MAX_NODES 64u
+
+typedef struct gdn_state_codec_drafts {
+  const uint16_t* queries;      /* bf16 [tokens][key_heads][128]; commit: NULL */
+  const uint16_t* keys;         /* bf16 [tokens][key_heads][128] */
+  const uint16_t* values;       /* bf16 [tokens][value_heads][128] */
+  const float* log_decay;       /* [tokens][value_heads] */
+  const uint16_t* beta;         /* bf16 [tokens][value_heads] */
+  uint64_t query_stride;        /* elements between tokens, multiples of 8 */
+  uint64_t key_stride;
+  uint64_t value_stride;
+  const int32_t* parents;       /* [tokens], 4-byte aligned: the parent's place in its
+                                   request; anything that is no earlier node, as -1:
+                                   the cached state */
+  const int32_t* offsets;       /* [requests + 1], as request_tables' */
+  const int32_t* slot_ids;      /* [requests] */
+  uint32_t requests;            /* 1..4096 */
+  uint32_t tokens;
+  uint32_t value_heads;
+  uint32_t key_heads;
+  uint32_t max_nodes;           /* 1..64 */
+  float scale;
+  uint32_t normalize;
+} gdn_state_codec_drafts;
+
+/* The rule's output of every node, from the state that its path leaves: with S the
+ * cached state, a node's own token is applied after those of the nodes above it.  pool
+ * [slots][value_heads][128 value][128 key] of pool_dtype is only read (two requests may
+ * name one slot).  A request whose slot is outside 0..slots-1 (padding, -1) is skipped.
+ * outputs bf16 [tokens][value_heads][128]: rows of skipped requests, of nodes past
+ * max_nodes and of no request stay as they were.
+ *
+ * A NaN or an infinity in a node's token leaves the outputs that it reaches in that node
+ * and in those below it without a finite value, and no other node's: of a value its own
+ * column's, of a key, a log decay or a write strength the head's, of a query the node's
+ * alone.  A log decay of -inf is no such value: it forgets. */
+int32_t statecentric_gdn_state_codec_gated_delta_tree_launch_v1(
+    void* stream, const gdn_state_codec_drafts* drafts, const void* pool, uint32_t slots,
+    uint32_t pool_dtype, uint16_t* outputs);
+
+/* The pool's states after the nodes from the cached state down to accepted[r] (int32
+ * [requests], a node's place in its request), in place, rounded to the pool's type once.
+ * A request that accepts no node (accepted[r] outside 0..min(nodes, max_nodes)-1, as -1)
+ * or whose slot is outside the pool keeps its state.  Slot ids are distinct. */
+int32_t statecentric_gdn_state_codec_gated_delta_commit_launch_v1(
+    void* stream, const gdn_state_codec_drafts* drafts, const int32_t* accepted, void* pool,
+    uint32_t slots, uint32_t pool_dtype);
 
 /* out = x / sqrt(mean(x^2) + eps) * weight * gate * sigmoid(gate) over rows of
  * 128.  x, gate, out [rows][128] of `dtype`, weight fp32 [128]. */
