@@ -287,6 +287,24 @@ __device__ __forceinline__ f32x4 load4(const float* p) {
   return *reinterpret_cast<const f32x4*>(p);
 }
 
+// A row of 128 over 16 lanes, 8 cells each: products of a lane's, and the sum over the
+// lanes, in all of them.
+__device__ __forceinline__ float dot8(const float (&a)[8], const float (&b)[8]) {
+  float x = a[0] * b[0], y = a[1] * b[1];
+#pragma unroll
+  for (int i = 2; i < 8; i += 2) {
+    x = fmaf(a[i], b[i], x);
+    y = fmaf(a[i + 1], b[i + 1], y);
+  }
+  return x + y;
+}
+__device__ __forceinline__ float row_sum(float x) {
+  x = add_partner<1>(x);
+  x = add_partner<2>(x);
+  x = add_partner<4>(x);
+  return add_partner<8>(x);
+}
+
 // Four neighbouring cells of a state.
 __device__ __forceinline__ f32x4 load_cells(const float* p) { return load4(p); }
 __device__ __forceinline__ f32x4 load_cells(const bf16_bits* p) {

@@ -47,23 +47,6 @@ struct StepArgs {
   uint32_t normalize;
 };
 
-__device__ __forceinline__ float row_sum(float x) {  // over the 16 lanes of a row
-  x = add_partner<1>(x);
-  x = add_partner<2>(x);
-  x = add_partner<4>(x);
-  return add_partner<8>(x);
-}
-
-__device__ __forceinline__ float dot8(const float (&a)[8], const float (&b)[8]) {
-  float x = a[0] * b[0], y = a[1] * b[1];
-#pragma unroll
-  for (int i = 2; i < 8; i += 2) {
-    x = fmaf(a[i], b[i], x);
-    y = fmaf(a[i + 1], b[i + 1], y);
-  }
-  return x + y;
-}
-
 template <typename Pool>
 struct RowCells;
 

@@ -3,25 +3,43 @@
 //
 // With S0 the cached state of one value head ([value][key]), G_t the sum of the log
 // decays from it down to node t, b_t the write strength, unit keys k and scaled unit
-// queries q:
-//   u_t = b_t (v_t - exp(G_t) S0 k_t - sum_(i above t) exp(G_t - G_i) (k_i . k_t) u_i)
-//   o_t = exp(G_t) S0 q_t + sum_(i above t, and t) exp(G_t - G_i) (k_i . q_t) u_i
+// queries q, and i above t where i is on t's path:
+//   r_t = b_t (v_t - exp(G_t) S0 k_t)
+//   u_t = r_t - sum_(i above t) A_ti u_i,        A_ti = b_t exp(G_t - G_i) k_t . k_i
+//   o_t = exp(G_t) S0 q_t + sum_(i above t, and t) M_ti u_i,  M_ti = exp(G_t - G_i) q_t . k_i
 // and after the path down to node c
 //   S = exp(G_c) S0 + sum_(i on the path) exp(G_c - G_i) u_i k_i^T.
+// So the state is read once for all nodes, by S0 K^T and S0 Q^T; what the tree is enters
+// by which cells of A and M are there.
 //
-// A workgroup takes one head of one request, a thread one row of its state; the products
-// of the nodes' keys and queries are formed once, in LDS.
+// Products with the state are on the bf16 matrix cores: k and q are exact as they are
+// (their norms are factors of the results), an fp32 state is three parts (delta_chunk.h),
+// a bf16 one itself.  What follows, A, M and u, is fp32 on the fp32 matrix cores, whose
+// accumulators are the next product's operand as they are.  (I + A)^-1 of 16 x 16 blocks
+// on the diagonal is formed by substitution, which is stable for any keys.
+//
+// Bad values.  A product takes every cell, also those that are zero, so a NaN or an
+// infinity in r or A would reach every node.  Those cells are set to zero, and the nodes
+// that they belong to noted, for their outputs and those below them.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "activations.h"
 #include "delta_chunk.h"
 #include "gdn_state_codec_layer.h"
+#include "lane_exchange.h"
 #include "launch.h"
+#include "stream_memory.h"
+#include "work_order.h"
 
 namespace gdn {
 namespace {
 
 constexpr int kMaxNodes = GDN_STATE_CODEC_MAX_NODES;
+constexpr double kInverseLn2 = 1.4426950408889634074;
+// exp of less is 0 in fp32; sums of it stay far from what fp64 cannot tell apart.
+constexpr double kLeastLogDecay = -200.0;
+constexpr float kLargest = 0x1.fffffep127f;
 
 struct DraftArgs {
   const bf16_bits* queries;
@@ -41,116 +59,709 @@ struct DraftArgs {
   uint32_t normalize;
 };
 
-struct Shared {
-  float k[kMaxNodes][kDim + 1], q[kMaxNodes][kDim + 1];
-  float u[kMaxNodes][kDim];
-  float kk[kMaxNodes][kMaxNodes], qk[kMaxNodes][kMaxNodes];
-  float decay[kMaxNodes], strength[kMaxNodes];
-  int parent[kMaxNodes];
+// A lane's 8 keys of a row of the state, in steps of 32: an operand's places.
+template <typename Pool>
+struct Cells;
+
+template <>
+struct Cells<float> {
+  static constexpr int kParts = 3;
+  f32x4 x, y;
+  __device__ __forceinline__ void load(const float* p) {
+    x = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p));
+    y = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p + 4));
+  }
+  __device__ __forceinline__ void parts(uint4 (&part)[3]) const { split3(x, y, part); }
 };
 
-__device__ __forceinline__ float cell(const float* p) { return *p; }
-__device__ __forceinline__ float cell(const bf16_bits* p) { return widen(*p); }
-__device__ __forceinline__ void put(float* p, float x) { *p = x; }
-__device__ __forceinline__ void put(bf16_bits* p, float x) {
-  *p = static_cast<bf16_bits>(bf16_pair(x, 0.0f));
+template <>
+struct Cells<bf16_bits> {
+  static constexpr int kParts = 1;
+  uint4 w;
+  __device__ __forceinline__ void load(const bf16_bits* p) {
+    w = stream_load(reinterpret_cast<const uint4*>(p));
+  }
+  __device__ __forceinline__ void parts(uint4 (&part)[1]) const { part[0] = w; }
+};
+
+__device__ __forceinline__ f32x4 product(const uint4& a, const uint4 (&b)[3], f32x4 c) {
+  return mfma3(a, b, c);
+}
+__device__ __forceinline__ f32x4 product(const uint4& a, const uint4 (&b)[1], f32x4 c) {
+  return mfma(a, b[0], c);
 }
 
-template <typename Pool, bool kCommit>
-__global__ __launch_bounds__(kDim) void draft_kernel(DraftArgs a) {
-  __shared__ Shared s;
-  const int t = threadIdx.x;
-  const uint32_t r = blockIdx.x / a.value_heads, h = blockIdx.x % a.value_heads;
-  const int32_t slot = a.slot_ids[r];
-  if (slot < 0 || static_cast<uint32_t>(slot) >= a.slots) return;
-  const int64_t begin = max(a.offsets[r], 0);
-  const int64_t end = min(static_cast<int64_t>(a.offsets[r + 1]), static_cast<int64_t>(a.tokens));
-  const int nodes = static_cast<int>(min(end - begin, static_cast<int64_t>(a.max_nodes)));
-  if (nodes <= 0) return;
-  int last = nodes - 1;
-  if (kCommit) {
-    last = a.accepted[r];
-    if (last < 0 || last >= nodes) return;
+// c + a b for 16 x 16 fp32 blocks: lane l has row l & 15, columns 4 g.. of a, and
+// rows 4 g.. of b's column l & 15 (an accumulator).
+__device__ __forceinline__ f32x4 block_product(const f32x4& a, const f32x4& b, f32x4 c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+  return c;
+}
+
+// A 16 x 16 block in LDS.  A row's four runs of four columns are rotated by its place, so
+// that 16 rows' runs fall on different banks.
+struct Block {
+  float cells[256];
+  __device__ __forceinline__ float& at(int row, int column) {
+    return cells[16 * row + (column ^ (row & 12))];
   }
-  for (int i = 0; i < nodes; ++i) {
-    const uint64_t row = begin + i;
-    s.k[i][t] = widen(a.keys[row * a.key_stride + h / a.group * kDim + t]);
-    if (!kCommit) s.q[i][t] = widen(a.queries[row * a.query_stride + h / a.group * kDim + t]);
+  __device__ __forceinline__ f32x4 run(int row, int column) const {
+    return load4(&cells[16 * row + (column ^ (row & 12))]);
   }
-  if (t < nodes) {
-    const uint64_t row = begin + t;
-    const int p = a.parents[row];
-    s.parent[t] = p < 0 || p >= t ? -1 : p;
-    s.decay[t] = expf(a.log_decay[row * a.value_heads + h]);
-    s.strength[t] = widen(a.beta[row * a.value_heads + h]);
-  }
-  __syncthreads();
-  if (t < nodes) {
-    float kk = kUnitEps, qq = kUnitEps;
-    for (int j = 0; j < kDim; ++j) {
-      kk = fmaf(s.k[t][j], s.k[t][j], kk);
-      if (!kCommit) qq = fmaf(s.q[t][j], s.q[t][j], qq);
-    }
-    const float k_unit = a.normalize ? 1.0f / sqrtf(kk) : 1.0f;
-    const float q_unit = a.normalize ? a.scale / sqrtf(qq) : a.scale;
-    for (int j = 0; j < kDim; ++j) {
-      s.k[t][j] *= k_unit;
-      if (!kCommit) s.q[t][j] *= q_unit;
-    }
-  }
-  __syncthreads();
-  for (int pair = t; pair < nodes * nodes; pair += kDim) {
-    const int i = pair / nodes, j = pair % nodes;
-    if (j > i) continue;
-    float kk = 0.0f, qk = 0.0f;
-    for (int d = 0; d < kDim; ++d) {
-      kk = fmaf(s.k[i][d], s.k[j][d], kk);
-      if (!kCommit) qk = fmaf(s.q[i][d], s.k[j][d], qk);
-    }
-    s.kk[i][j] = kk;
-    if (!kCommit) s.qk[i][j] = qk;
-  }
-  __syncthreads();
-  Pool* const state = static_cast<Pool*>(a.pool) +
-                      (static_cast<uint64_t>(slot) * a.value_heads + h) * kTile + t * kDim;
-  uint64_t on_path = 0;
-  if (kCommit) {
-    for (int i = last; i >= 0; i = s.parent[i]) on_path |= 1ull << i;
-  }
-  for (int i = 0; i <= last; ++i) {
-    if (kCommit && !(on_path >> i & 1)) continue;
-    const uint64_t row = begin + i;
-    float seen = 0.0f, read = 0.0f;
-    for (int j = 0; j < kDim; ++j) {
-      const float x = cell(state + j);
-      seen = fmaf(x, s.k[i][j], seen);
-      if (!kCommit) read = fmaf(x, s.q[i][j], read);
-    }
-    float decay = s.decay[i], seen_writes = 0.0f, read_writes = 0.0f;
-    for (int j = s.parent[i]; j >= 0; j = s.parent[j]) {
-      const float u = decay * s.u[j][t];
-      seen_writes = fmaf(u, s.kk[i][j], seen_writes);
-      if (!kCommit) read_writes = fmaf(u, s.qk[i][j], read_writes);
-      decay *= s.decay[j];
-    }
-    const float v = widen(a.values[row * a.value_stride + h * kDim + t]);
-    const float u = s.strength[i] * (v - fmaf(decay, seen, seen_writes));
-    s.u[i][t] = u;  // read by this thread alone
-    if (!kCommit) {
-      put(a.outputs + (row * a.value_heads + h) * kDim + t,
-          fmaf(u, s.qk[i][i], fmaf(decay, read, read_writes)));
-    }
-  }
-  if (kCommit) {
-    for (int j = 0; j < kDim; ++j) {
-      float decay = 1.0f, x = 0.0f;
-      for (int i = last; i >= 0; i = s.parent[i]) {
-        x = fmaf(decay * s.u[i][t], s.k[i][j], x);
-        decay *= s.decay[i];
+};
+
+// LDS written by other lanes of the same wavefront is read after this.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+}
+
+// -A of a diagonal block becomes N = (I + A)^-1 - I, column `column` by each lane that
+// stores it: N_i = -A_i - sum_(m<i) A_im N_m.  The others compute whatever is there.
+__device__ __forceinline__ void invert(Block& block, int column, bool stores) {
+  float n[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    float x = block.at(i, column), y = 0.0f;
+#pragma unroll
+    for (int c = 0; c < i; c += 4) {
+      const f32x4 l = block.run(i, c);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (c + u < i) {
+          if (u & 1) y = fmaf(l[u], n[c + u], y);
+          else x = fmaf(l[u], n[c + u], x);
+        }
       }
-      put(state + j, fmaf(decay, cell(state + j), x));
+    }
+    n[i] = x + y;
+    // Formed here, not where it is stored: all rows' operands would wait in registers.
+    asm volatile("" : "+v"(n[i]));
+  }
+  wave_sync();  // -A has been read
+  if (stores) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) block.at(i, column) = n[i];
+  }
+}
+
+// The request's nodes: first token row and how many, 0 where there is nothing to do.
+__device__ __forceinline__ int request_nodes(const DraftArgs& a, uint32_t r, int32_t& slot,
+                                             uint64_t& begin) {
+  slot = a.slot_ids[r];
+  const int64_t first = max(a.offsets[r], 0);
+  const int64_t last = min(static_cast<int64_t>(a.offsets[r + 1]),
+                           static_cast<int64_t>(a.tokens));
+  begin = static_cast<uint64_t>(first);
+  if (slot < 0 || static_cast<uint32_t>(slot) >= a.slots) return 0;
+  return static_cast<int>(max(min(last - first, static_cast<int64_t>(a.max_nodes)),
+                              static_cast<int64_t>(0)));
+}
+
+// 16 bytes of a row of k or q (16 lanes a row), into LDS, and its sum of squares.  A row's
+// pieces are exchanged by its place, p to p ^ (row & 15), so that 16 rows' pieces of one
+// operand fall on different banks.
+__device__ __forceinline__ float stage_piece(uint4* rows, int row, int piece, const uint4& w) {
+  rows[16 * row + (piece ^ (row & 15))] = w;
+  float x[8];
+  widen8(w, x);
+  return row_sum(dot8(x, x));
+}
+__device__ __forceinline__ const uint4& staged(const uint4* rows, int row, int piece) {
+  return rows[16 * row + (piece ^ (row & 15))];
+}
+
+// Four tokens' values of a lane's column, from the four columns of one token of each
+// lane of a quad.
+__device__ __forceinline__ f32x4 value_columns(const uint2& w, int lane) {
+  const uint2 t = transpose_quad(w, lane);
+  return f32x4{widen_low(t.x), widen_high(t.x), widen_low(t.y), widen_high(t.y)};
+}
+
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= kLargest; }
+
+// -------------------------------------------------------------------- the tree
+
+constexpr int blocks_of(int tiles) { return tiles * (tiles + 1) / 2; }
+// Block (i, j <= i) of a lower triangular matrix.
+__host__ __device__ constexpr int block_at(int i, int j) { return i * (i + 1) / 2 + j; }
+
+template <int kTiles>
+struct TreeShared {
+  static constexpr int kNodes = 16 * kTiles;
+  uint4 k[kNodes * 16], q[kNodes * 16];
+  Block step[blocks_of(kTiles)];  // -A; on the diagonal then N
+  Block read[blocks_of(kTiles)];  // M
+  float k_unit[kNodes], q_unit[kNodes];  // 1 / |k|, scale / |q|
+  float sum[kNodes], rest[kNodes];       // G / ln 2, and what fp32 left of it
+  float strength[kNodes];
+  uint64_t above[kNodes];
+  uint32_t bad_node[2], bad_output[2];   // a bit a node
+};
+
+// Sums and paths of the nodes, one a lane of one wavefront, by doubling: after round i a
+// lane's sum is of 2^i nodes up from its own.
+template <int kTiles>
+__device__ __forceinline__ void tree_tables(TreeShared<kTiles>& s, int lane, int nodes,
+                                            int parent, float log_decay, float strength) {
+  const bool real = lane < nodes;
+  int up = real && parent >= 0 && parent < lane ? parent : -1;
+  uint64_t above = up >= 0 ? 1ull << up : 0;
+  const bool bad = real && !(log_decay <= kLargest);
+  double sum = real && !bad ? fmax(static_cast<double>(log_decay), kLeastLogDecay) : 0.0;
+  for (int reach = 1; reach < nodes; reach <<= 1) {
+    const int from = up >= 0 ? up : lane;
+    const double sum_up = __shfl(sum, from);
+    const uint64_t above_up = __shfl(above, from);
+    const int next = __shfl(up, from);
+    if (up >= 0) {
+      sum += sum_up;
+      above |= above_up;
+      up = next;
     }
   }
+  sum *= kInverseLn2;
+  const uint64_t all_bad = __ballot(bad);
+  if (lane < TreeShared<kTiles>::kNodes) {
+    const float high = static_cast<float>(sum);
+    s.sum[lane] = high;
+    s.rest[lane] = static_cast<float>(sum - high);
+    s.strength[lane] = real ? strength : 0.0f;
+    s.above[lane] = above;
+  }
+  if (lane < 2) {
+    s.bad_node[lane] = static_cast<uint32_t>(all_bad >> (32 * lane));
+    s.bad_output[lane] = 0;
+  }
+}
+
+// A workgroup takes kWaves x kSlices slices of 16 rows of one head's state.  The first
+// wavefront forms the tables and inverts, the others form the nodes' products; the
+// state's are between, wherever a wavefront would wait.
+template <typename Pool, int kTiles, int kSlices, int kWaves>
+__global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
+  constexpr int kThreads = 64 * kWaves;
+  constexpr int kPerHead = 8 / (kSlices * kWaves);
+  constexpr int kNodes = 16 * kTiles;
+  constexpr int kPasses = kNodes * 16 / kThreads;
+  constexpr int kBlocks = blocks_of(kTiles);
+  constexpr int kPairs = (kBlocks + kWaves - 2) / (kWaves - 1);
+  static_assert(kWaves >= 2 && kNodes * 16 % kThreads == 0, "the roles above");
+  __shared__ TreeShared<kTiles> s;
+
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t item = static_cast<uint32_t>(xcd_contiguous_item(blockIdx.x, gridDim.x));
+  const uint32_t head = item / kPerHead;
+  const uint32_t n = head / a.value_heads, h = head % a.value_heads, hk = h / a.group;
+  int32_t slot;
+  uint64_t begin;
+  const int nodes = request_nodes(a, n, slot, begin);
+  if (nodes == 0) return;
+  const int tiles = (nodes + 15) / 16;
+
+  // Everything from memory is asked for here: the nodes first, which are waited for first.
+  int parent = -1;
+  float log_decay = 0.0f, strength = 0.0f;
+  if (wave == 0 && lane < nodes) {
+    const uint64_t row = begin + lane;
+    parent = a.parents[row];
+    log_decay = a.log_decay[row * a.value_heads + h];
+    strength = widen(a.beta[row * a.value_heads + h]);
+  }
+  const int piece = threadIdx.x & 15;
+  uint4 k_piece[kPasses], q_piece[kPasses];
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int row = p * (kThreads / 16) + (threadIdx.x >> 4);
+    if (p * (kThreads / 16) < 16 * tiles) {  // the same for the workgroup
+      const uint64_t token = begin + min(row, nodes - 1);
+      k_piece[p] = *reinterpret_cast<const uint4*>(a.keys + token * a.key_stride + hk * kDim +
+                                                   8 * piece);
+      q_piece[p] = *reinterpret_cast<const uint4*>(a.queries + token * a.query_stride +
+                                                   hk * kDim + 8 * piece);
+    }
+  }
+  const int first_row = 16 * kSlices * static_cast<int>((item % kPerHead) * kWaves + wave);
+  uint2 v[kSlices][kTiles];
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) {
+    if (i < tiles) {
+      const uint64_t token = begin + min(16 * i + 4 * g + (r & 3), nodes - 1);
+#pragma unroll
+      for (int slice = 0; slice < kSlices; ++slice) {
+        v[slice][i] = *reinterpret_cast<const uint2*>(
+            a.values + token * a.value_stride + h * kDim + first_row + 16 * slice +
+            (r & 12));
+      }
+    }
+  }
+  Cells<Pool> cells[kSlices][4];
+  {
+    const Pool* const state = static_cast<const Pool*>(a.pool) +
+                              (static_cast<uint64_t>(slot) * a.value_heads + h) * kTile +
+                              (first_row + r) * kDim + 8 * g;
+#pragma unroll
+    for (int slice = 0; slice < kSlices; ++slice) {
+#pragma unroll
+      for (int step = 0; step < 4; ++step) {
+        cells[slice][step].load(state + 16 * slice * kDim + 32 * step);
+      }
+    }
+  }
+
+#pragma unroll
+  for (int p = 0; p < kPasses; ++p) {
+    const int row = p * (kThreads / 16) + (threadIdx.x >> 4);
+    if (p * (kThreads / 16) < 16 * tiles) {
+      const float kk = stage_piece(s.k, row, piece, k_piece[p]);
+      const float qq = stage_piece(s.q, row, piece, q_piece[p]);
+      if (piece == 0) {
+        s.k_unit[row] = a.normalize ? 1.0f / sqrtf(kk + kUnitEps) : 1.0f;
+        s.q_unit[row] = a.normalize ? a.scale * (1.0f / sqrtf(qq + kUnitEps)) : a.scale;
+      }
+    }
+  }
+  exchange();
+
+  f32x4 seen[kSlices][kTiles], read[kSlices][kTiles];  // S0 K^T and S0 Q^T, a token a row
+  auto state_products = [&]() {
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int slice = 0; slice < kSlices; ++slice) {
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) seen[slice][i] = read[slice][i] = zero;
+    }
+#pragma unroll
+    for (int step = 0; step < 4; ++step) {
+      uint4 part[kSlices][Cells<Pool>::kParts];
+#pragma unroll
+      for (int slice = 0; slice < kSlices; ++slice) cells[slice][step].parts(part[slice]);
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) {
+        if (i < tiles) {
+          const uint4 k = staged(s.k, 16 * i + r, 4 * step + g);
+          const uint4 q = staged(s.q, 16 * i + r, 4 * step + g);
+#pragma unroll
+          for (int slice = 0; slice < kSlices; ++slice) {
+            seen[slice][i] = product(k, part[slice], seen[slice][i]);
+            read[slice][i] = product(q, part[slice], read[slice][i]);
+          }
+        }
+      }
+    }
+  };
+
+  if (wave == 0) {
+    tree_tables(s, lane, nodes, parent, log_decay, strength);
+    exchange();
+    state_products();
+    exchange();
+    const int diagonal = min(g, kTiles - 1);
+    invert(s.step[block_at(diagonal, diagonal)], r, g < tiles);
+    exchange();
+  } else {
+    f32x4 kk[kPairs], qk[kPairs];
+#pragma unroll
+    for (int e = 0; e < kPairs; ++e) {
+      const int block = wave - 1 + e * (kWaves - 1);
+      const int i = block < 1 ? 0 : block < 3 ? 1 : block < 6 ? 2 : 3;
+      const int j = block - block_at(i, 0);
+      if (block < kBlocks && i < tiles) {
+        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+        kk[e] = qk[e] = zero;
+#pragma unroll
+        for (int step = 0; step < 4; ++step) {
+          const uint4 column = staged(s.k, 16 * j + r, 4 * step + g);
+          kk[e] = mfma(staged(s.k, 16 * i + r, 4 * step + g), column, kk[e]);
+          qk[e] = mfma(staged(s.q, 16 * i + r, 4 * step + g), column, qk[e]);
+        }
+      }
+    }
+    exchange();
+#pragma unroll
+    for (int e = 0; e < kPairs; ++e) {
+      const int block = wave - 1 + e * (kWaves - 1);
+      const int i = block < 1 ? 0 : block < 3 ? 1 : block < 6 ? 2 : 3;
+      const int j = block - block_at(i, 0);
+      if (block < kBlocks && i < tiles) {
+        const int first = 16 * i + 4 * g, column = 16 * j + r;
+        const f32x4 sum = load4(&s.sum[first]), rest = load4(&s.rest[first]);
+        const f32x4 k_unit = load4(&s.k_unit[first]), q_unit = load4(&s.q_unit[first]);
+        const f32x4 b = load4(&s.strength[first]);
+        const float sum_c = s.sum[column], rest_c = s.rest[column], unit_c = s.k_unit[column];
+        uint32_t bad_node = 0, bad_output = 0;  // a bit a row
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const bool up = (s.above[first + c] >> column & 1) != 0;
+          const bool self = first + c == column && column < nodes;
+          const float decay = decay_between(sum[c], rest[c], sum_c, rest_c);
+          float x = up ? -b[c] * decay * (k_unit[c] * unit_c * kk[e][c]) : 0.0f;
+          float y = up || self ? decay * (q_unit[c] * unit_c * qk[e][c]) : 0.0f;
+          if (!finite(x)) bad_node |= 1u << c, x = 0.0f;
+          if (!finite(y)) bad_output |= 1u << c, y = 0.0f;
+          s.step[block].at(4 * g + c, r) = x;
+          s.read[block].at(4 * g + c, r) = y;
+        }
+        if (bad_node) atomicOr(&s.bad_node[first >> 5], bad_node << (first & 31));
+        if (bad_output) atomicOr(&s.bad_output[first >> 5], bad_output << (first & 31));
+      }
+    }
+    exchange();
+    state_products();
+    exchange();
+  }
+
+  const uint64_t bad_nodes = static_cast<uint64_t>(s.bad_node[1]) << 32 | s.bad_node[0];
+  const uint64_t bad_outputs = static_cast<uint64_t>(s.bad_output[1]) << 32 | s.bad_output[0];
+  uint64_t bad[kSlices];  // nodes whose r is bad in this column
+#pragma unroll
+  for (int slice = 0; slice < kSlices; ++slice) bad[slice] = bad_nodes;
+  f32x4 u[kSlices][kTiles];
+#pragma unroll
+  for (int i = 0; i < kTiles; ++i) {
+    if (i >= tiles) break;
+    const int first = 16 * i + 4 * g;
+    const f32x4 sum = load4(&s.sum[first]), rest = load4(&s.rest[first]);
+    const f32x4 k_unit = load4(&s.k_unit[first]), q_unit = load4(&s.q_unit[first]);
+    const f32x4 b = load4(&s.strength[first]);
+    f32x4 see, look;  // factors of S0 k and S0 q
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float decay = decay_between(sum[c], rest[c], 0.0f, 0.0f);
+      see[c] = decay * k_unit[c];
+      look[c] = decay * q_unit[c];
+    }
+    f32x4 x[kSlices], out[kSlices];
+#pragma unroll
+    for (int slice = 0; slice < kSlices; ++slice) {
+      const f32x4 values = value_columns(v[slice][i], lane);
+      uint32_t odd = 0;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        float y = b[c] * fmaf(-see[c], seen[slice][i][c], values[c]);
+        if (first + c >= nodes) y = 0.0f;
+        if (!finite(y)) odd |= 1u << c, y = 0.0f;
+        x[slice][c] = y;
+        out[slice][c] = look[c] * read[slice][i][c];
+      }
+      if (__any(odd != 0)) {
+        uint64_t column = static_cast<uint64_t>(odd) << first;
+        column |= __shfl_xor(column, 16);
+        column |= __shfl_xor(column, 32);
+        bad[slice] |= column;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < i; ++j) {
+      const f32x4 step = s.step[block_at(i, j)].run(r, 4 * g);
+      const f32x4 looked = s.read[block_at(i, j)].run(r, 4 * g);
+#pragma unroll
+      for (int slice = 0; slice < kSlices; ++slice) {
+        x[slice] = block_product(step, u[slice][j], x[slice]);
+        out[slice] = block_product(looked, u[slice][j], out[slice]);
+      }
+    }
+    const f32x4 inverse = s.step[block_at(i, i)].run(r, 4 * g);
+    const f32x4 looked = s.read[block_at(i, i)].run(r, 4 * g);
+#pragma unroll
+    for (int slice = 0; slice < kSlices; ++slice) {
+      u[slice][i] = block_product(inverse, x[slice], x[slice]);
+      f32x4 y = block_product(looked, u[slice][i], out[slice]);
+      if (__any(bad[slice] != 0) || bad_outputs != 0) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint64_t self = 1ull << (first + c);
+          if ((bad[slice] & (s.above[first + c] | self)) | (bad_outputs & self)) {
+            y[c] = __uint_as_float(0x7FC00000u);
+          }
+        }
+      }
+      const uint2 packed = transpose_quad(
+          make_uint2(bf16_pair(y[0], y[1]), bf16_pair(y[2], y[3])), lane);
+      const int node = first + (r & 3);
+      if (node < nodes) {
+        *reinterpret_cast<uint2*>(a.outputs +
+                                  ((begin + node) * a.value_heads + h) * kDim + first_row +
+                                  16 * slice + (r & 12)) = packed;
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ the commit
+
+struct CommitShared {
+  uint4 k[16 * 16];
+  Block step;              // -A, then N
+  float k_unit[16];
+  float sum[kMaxNodes], rest[kMaxNodes];  // G / ln 2 from the start of each 16
+  float strength[kMaxNodes];
+  float log_decay[kMaxNodes];
+  int path[kMaxNodes];
+};
+
+template <typename Pool>
+struct StateRow;  // the same 8 keys as accumulators
+
+template <>
+struct StateRow<float> {
+  static __device__ __forceinline__ void load(const float* p, f32x4& x, f32x4& y) {
+    x = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p));
+    y = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p + 4));
+  }
+  static __device__ __forceinline__ void store(float* p, const f32x4& x, const f32x4& y) {
+    __builtin_nontemporal_store(x, reinterpret_cast<f32x4*>(p));
+    __builtin_nontemporal_store(y, reinterpret_cast<f32x4*>(p + 4));
+  }
+};
+
+template <>
+struct StateRow<bf16_bits> {
+  static __device__ __forceinline__ void load(const bf16_bits* p, f32x4& x, f32x4& y) {
+    float w[8];
+    widen8(stream_load(reinterpret_cast<const uint4*>(p)), w);
+    x = f32x4{w[0], w[1], w[2], w[3]};
+    y = f32x4{w[4], w[5], w[6], w[7]};
+  }
+  static __device__ __forceinline__ void store(bf16_bits* p, const f32x4& x, const f32x4& y) {
+    const u32x4_t w = {bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]), bf16_pair(y[0], y[1]),
+                       bf16_pair(y[2], y[3])};
+    __builtin_nontemporal_store(w, reinterpret_cast<u32x4_t*>(p));
+  }
+};
+
+typedef __attribute__((ext_vector_type(4))) short bf16x4_bits;
+__device__ __forceinline__ f32x4 mfma_half(const uint2& a, const uint2& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(bf16x4_bits, a),
+                                                   __builtin_bit_cast(bf16x4_bits, b), c, 0, 0,
+                                                   0);
+}
+
+// A workgroup takes kWaves x kSlices slices of 16 rows of one head's state, which stay in
+// registers while the path's nodes are applied 16 at a time.  Accumulator tile m of a
+// slice is keys state_key(m, ..) by values, so that a lane's registers are 8 neighbouring
+// keys of its row, the products' operand and the update's accumulators.
+template <typename Pool, int kSlices, int kWaves>
+__global__ __launch_bounds__(64 * kWaves) void commit_kernel(DraftArgs a) {
+  constexpr int kThreads = 64 * kWaves;
+  constexpr int kPerHead = 8 / (kSlices * kWaves);
+  constexpr int kPasses = 16 * 16 / kThreads;
+  static_assert(kWaves >= 2 && 256 % kThreads == 0, "the roles below");
+  __shared__ CommitShared s;
+
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t item = static_cast<uint32_t>(xcd_contiguous_item(blockIdx.x, gridDim.x));
+  const uint32_t head = item / kPerHead;
+  const uint32_t n = head / a.value_heads, h = head % a.value_heads, hk = h / a.group;
+  int32_t slot;
+  uint64_t begin;
+  const int nodes = request_nodes(a, n, slot, begin);
+  const int last = a.accepted[n];
+  if (last < 0 || last >= nodes) return;
+
+  int parent = -1;
+  float log_decay = 0.0f, strength = 0.0f;
+  if (wave == 0 && lane < nodes) {
+    const uint64_t row = begin + lane;
+    parent = a.parents[row];
+    log_decay = a.log_decay[row * a.value_heads + h];
+    strength = widen(a.beta[row * a.value_heads + h]);
+  }
+  const int first_row = 16 * kSlices * static_cast<int>((item % kPerHead) * kWaves + wave);
+  Pool* const state = static_cast<Pool*>(a.pool) +
+                      (static_cast<uint64_t>(slot) * a.value_heads + h) * kTile +
+                      (first_row + r) * kDim + 8 * g;
+  f32x4 cells[kSlices][8];
+#pragma unroll
+  for (int slice = 0; slice < kSlices; ++slice) {
+#pragma unroll
+    for (int step = 0; step < 4; ++step) {
+      StateRow<Pool>::load(state + 16 * slice * kDim + 32 * step, cells[slice][2 * step],
+                           cells[slice][2 * step + 1]);
+    }
+  }
+
+  if (wave == 0) {
+    if (parent >= lane) parent = -1;
+    uint64_t on_path = 0;
+    for (int node = last; node >= 0; node = __builtin_amdgcn_readlane(parent, node)) {
+      on_path |= 1ull << node;
+    }
+    s.path[lane] = -1;
+    wave_sync();
+    if (on_path >> lane & 1) {
+      const int place = __popcll(on_path & ((1ull << lane) - 1));
+      s.path[place] = lane;
+      s.log_decay[place] = log_decay;
+      s.strength[place] = strength;
+    }
+    wave_sync();
+    const bool real = s.path[lane] >= 0;
+    // A NaN stays: it is on the path.
+    const float own = real ? s.log_decay[lane] : 0.0f;
+    double sum = own < static_cast<float>(kLeastLogDecay) ? kLeastLogDecay : own;
+#pragma unroll
+    for (int reach = 1; reach < 16; reach <<= 1) {
+      const double before = __shfl_up(sum, reach);
+      if (r >= reach) sum += before;
+    }
+    sum *= kInverseLn2;
+    const float high = static_cast<float>(sum);
+    s.sum[lane] = high;
+    s.rest[lane] = static_cast<float>(sum - high);
+    if (!real) s.strength[lane] = 0.0f;
+  }
+  exchange();
+
+  for (int at = 0; at < kMaxNodes && s.path[at] >= 0; at += 16) {
+    const int length = __popcll(__ballot(s.path[at + r] >= 0)) / 4;  // nodes of this 16
+    const int piece = threadIdx.x & 15;
+    uint4 k_piece[kPasses];
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int row = p * (kThreads / 16) + (threadIdx.x >> 4);
+      const uint64_t token = begin + s.path[at + min(row, length - 1)];
+      k_piece[p] = *reinterpret_cast<const uint4*>(a.keys + token * a.key_stride + hk * kDim +
+                                                   8 * piece);
+    }
+    uint2 v[kSlices];
+    {
+      const uint64_t token = begin + s.path[at + min(4 * g + (r & 3), length - 1)];
+#pragma unroll
+      for (int slice = 0; slice < kSlices; ++slice) {
+        v[slice] = *reinterpret_cast<const uint2*>(a.values + token * a.value_stride + h * kDim +
+                                                   first_row + 16 * slice + (r & 12));
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int row = p * (kThreads / 16) + (threadIdx.x >> 4);
+      const float kk = stage_piece(s.k, row, piece, k_piece[p]);
+      if (piece == 0) s.k_unit[row] = a.normalize ? 1.0f / sqrtf(kk + kUnitEps) : 1.0f;
+    }
+    exchange();
+
+    const f32x4 sum = load4(&s.sum[at + 4 * g]), rest = load4(&s.rest[at + 4 * g]);
+    const f32x4 b = load4(&s.strength[at + 4 * g]), k_unit = load4(&s.k_unit[4 * g]);
+    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (wave == 0) {
+      f32x4 kk = zero;
+#pragma unroll
+      for (int step = 0; step < 4; ++step) {
+        const uint4 k = staged(s.k, r, 4 * step + g);
+        kk = mfma(k, k, kk);
+      }
+      const float sum_c = s.sum[at + r], rest_c = s.rest[at + r], unit_c = s.k_unit[r];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float decay = decay_between(sum[c], rest[c], sum_c, rest_c);
+        const bool up = 4 * g + c > r && 4 * g + c < length;
+        s.step.at(4 * g + c, r) = up ? -b[c] * decay * (k_unit[c] * unit_c * kk[c]) : 0.0f;
+      }
+      wave_sync();
+      invert(s.step, r, g == 0);
+    }
+    f32x4 seen[kSlices];
+#pragma unroll
+    for (int slice = 0; slice < kSlices; ++slice) seen[slice] = zero;
+#pragma unroll
+    for (int step = 0; step < 4; ++step) {
+      const uint4 k = staged(s.k, r, 4 * step + g);
+#pragma unroll
+      for (int slice = 0; slice < kSlices; ++slice) {
+        uint4 part[3];
+        split3(cells[slice][2 * step], cells[slice][2 * step + 1], part);
+        seen[slice] = mfma3(k, part, seen[slice]);
+      }
+    }
+    exchange();
+
+    const f32x4 inverse = s.step.run(r, 4 * g);
+    const float end_sum = s.sum[at + length - 1], end_rest = s.rest[at + length - 1];
+    const float whole = decay_between(end_sum, end_rest, 0.0f, 0.0f);
+    uint2 part[kSlices][3];  // u, weighted
+#pragma unroll
+    for (int slice = 0; slice < kSlices; ++slice) {
+      const f32x4 values = value_columns(v[slice], lane);
+      f32x4 x;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float decay = decay_between(sum[c], rest[c], 0.0f, 0.0f);
+        x[c] = b[c] * fmaf(-decay * k_unit[c], seen[slice][c], values[c]);
+        if (4 * g + c >= length) x[c] = 0.0f;
+      }
+      f32x4 u = block_product(inverse, x, x);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        u[c] *= decay_between(end_sum, end_rest, sum[c], rest[c]) * k_unit[c];
+        if (4 * g + c >= length) u[c] = 0.0f;
+      }
+      split3_half(u, part[slice]);
+    }
+    const int token = 4 * g + (r & 3);
+#pragma unroll
+    for (int step = 0; step < 4; ++step) {
+      const uint4 keys = staged(s.k, token, 4 * step + (r >> 2));
+      const uint2 low = transpose_quad(make_uint2(keys.x, keys.y), lane);
+      const uint2 high = transpose_quad(make_uint2(keys.z, keys.w), lane);
+#pragma unroll
+      for (int slice = 0; slice < kSlices; ++slice) {
+        f32x4 x = cells[slice][2 * step] * whole, y = cells[slice][2 * step + 1] * whole;
+#pragma unroll
+        for (int p = 2; p >= 0; --p) {
+          x = mfma_half(low, part[slice][p], x);
+          y = mfma_half(high, part[slice][p], y);
+        }
+        cells[slice][2 * step] = x;
+        cells[slice][2 * step + 1] = y;
+      }
+    }
+    exchange();  // k and the inverse have been read
+    if (at + 16 >= kMaxNodes) break;
+  }
+
+#pragma unroll
+  for (int slice = 0; slice < kSlices; ++slice) {
+#pragma unroll
+    for (int step = 0; step < 4; ++step) {
+      StateRow<Pool>::store(state + 16 * slice * kDim + 32 * step, cells[slice][2 * step],
+                            cells[slice][2 * step + 1]);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------- launch
+
+constexpr uint32_t kFewHeads = kComputeUnits;
+
+template <typename Pool, int kTiles>
+int32_t launch_tree(void* stream, const DraftArgs& args, uint64_t heads) {
+  return heads <= kFewHeads
+             ? launch(tree_kernel<Pool, kTiles, 1, 2>, dim3(static_cast<uint32_t>(4 * heads)),
+                      dim3(128), stream, args)
+             : launch(tree_kernel<Pool, kTiles, 2, 4>, dim3(static_cast<uint32_t>(heads)),
+                      dim3(256), stream, args);
+}
+
+template <typename Pool>
+int32_t launch_tree(void* stream, const DraftArgs& args, uint64_t heads) {
+  const uint32_t most = args.max_nodes < args.tokens ? args.max_nodes : args.tokens;
+  return most <= 16   ? launch_tree<Pool, 1>(stream, args, heads)
+         : most <= 32 ? launch_tree<Pool, 2>(stream, args, heads)
+                      : launch_tree<Pool, 4>(stream, args, heads);
+}
+
+template <typename Pool>
+int32_t launch_commit(void* stream, const DraftArgs& args, uint64_t heads) {
+  return heads <= kFewHeads
+             ? launch(commit_kernel<Pool, 1, 2>, dim3(static_cast<uint32_t>(4 * heads)),
+                      dim3(128), stream, args)
+             : launch(commit_kernel<Pool, 2, 4>, dim3(static_cast<uint32_t>(heads)), dim3(256),
+                      stream, args);
 }
 
 template <bool kCommit>
@@ -171,16 +782,20 @@ int32_t launch_drafts(void* stream, const gdn_state_codec_drafts* d, const int32
                  outputs)) {
     return kStatusInvalidArgument;
   }
-  const uint64_t blocks = static_cast<uint64_t>(d->requests) * d->value_heads;
-  if (blocks > kMaxGrid) return kStatusInvalidArgument;
+  const uint64_t heads = static_cast<uint64_t>(d->requests) * d->value_heads;
+  if (heads > kMaxGrid / 256) return kStatusInvalidArgument;  // threads of the grid
   if (d->tokens == 0) return kStatusOk;  // every tree is empty
   const DraftArgs args{d->queries, d->keys, d->values, d->log_decay, d->beta, d->query_stride,
                        d->key_stride, d->value_stride, d->parents, d->offsets, d->slot_ids,
                        accepted, pool, outputs, d->tokens, slots, d->value_heads,
                        d->value_heads / d->key_heads, d->max_nodes, d->scale, d->normalize};
-  const auto kernel = pool_dtype == kDtypeF32 ? draft_kernel<float, kCommit>
-                                              : draft_kernel<bf16_bits, kCommit>;
-  return launch(kernel, dim3(static_cast<uint32_t>(blocks)), dim3(kDim), stream, args);
+  const bool f32 = pool_dtype == kDtypeF32;
+  if (kCommit) {
+    return f32 ? launch_commit<float>(stream, args, heads)
+               : launch_commit<bf16_bits>(stream, args, heads);
+  }
+  return f32 ? launch_tree<float>(stream, args, heads)
+             : launch_tree<bf16_bits>(stream, args, heads);
 }
 
 }  // namespace
