@@ -147,17 +147,19 @@ __device__ __forceinline__ void invert(Block& block, int column, bool stores) {
   }
 }
 
+// A value that all lanes share, known to be one.
+__device__ __forceinline__ int32_t uniform(int32_t x) { return __builtin_amdgcn_readfirstlane(x); }
+
 // The request's nodes: first token row and how many, 0 where there is nothing to do.
 __device__ __forceinline__ int request_nodes(const DraftArgs& a, uint32_t r, int32_t& slot,
                                              uint64_t& begin) {
-  slot = a.slot_ids[r];
-  const int64_t first = max(a.offsets[r], 0);
-  const int64_t last = min(static_cast<int64_t>(a.offsets[r + 1]),
-                           static_cast<int64_t>(a.tokens));
-  begin = static_cast<uint64_t>(first);
-  if (slot < 0 || static_cast<uint32_t>(slot) >= a.slots) return 0;
-  return static_cast<int>(max(min(last - first, static_cast<int64_t>(a.max_nodes)),
-                              static_cast<int64_t>(0)));
+  slot = uniform(a.slot_ids[r]);
+  const int32_t first = max(uniform(a.offsets[r]), 0);
+  const int32_t last = static_cast<int32_t>(
+      min(static_cast<int64_t>(uniform(a.offsets[r + 1])), static_cast<int64_t>(a.tokens)));
+  begin = static_cast<uint32_t>(first);
+  if (slot < 0 || static_cast<uint32_t>(slot) >= a.slots || last <= first) return 0;
+  return min(last - first, static_cast<int32_t>(a.max_nodes));
 }
 
 // 16 bytes of a row of k or q (16 lanes a row), into LDS, and its sum of squares.  A row's
@@ -191,21 +193,30 @@ __host__ __device__ constexpr int block_at(int i, int j) { return i * (i + 1) / 
 template <int kTiles>
 struct TreeShared {
   static constexpr int kNodes = 16 * kTiles;
-  uint4 k[kNodes * 16], q[kNodes * 16];
+  union {
+    struct {
+      uint4 k[kNodes * 16], q[kNodes * 16];
+    };
+    uint4 out[kNodes * 16];       // once all products of k and q are formed
+  };
   Block step[blocks_of(kTiles)];  // -A; on the diagonal then N
   Block read[blocks_of(kTiles)];  // M
-  float k_unit[kNodes], q_unit[kNodes];  // 1 / |k|, scale / |q|
+  float k_square[kNodes], q_square[kNodes];
+  // Factors of a node: of a key, -b / |k|, scale / |q|; then -b exp(G) / |k| of S0 k,
+  // exp(G) scale / |q| of S0 q, and b.
+  float k_unit[kNodes], k_step[kNodes], q_unit[kNodes];
+  float seen[kNodes], look[kNodes], strength[kNodes];
   float sum[kNodes], rest[kNodes];       // G / ln 2, and what fp32 left of it
-  float strength[kNodes];
   uint64_t above[kNodes];
   uint32_t bad_node[2], bad_output[2];   // a bit a node
 };
 
-// Sums and paths of the nodes, one a lane of one wavefront, by doubling: after round i a
-// lane's sum is of 2^i nodes up from its own.
+// The tables of the nodes, one a lane of one wavefront.  Sums and paths by doubling: after
+// round i a lane's sum is of 2^i nodes up from its own.
 template <int kTiles>
-__device__ __forceinline__ void tree_tables(TreeShared<kTiles>& s, int lane, int nodes,
-                                            int parent, float log_decay, float strength) {
+__device__ __forceinline__ void tree_tables(TreeShared<kTiles>& s, const DraftArgs& a, int lane,
+                                            int nodes, int parent, float log_decay,
+                                            float strength) {
   const bool real = lane < nodes;
   int up = real && parent >= 0 && parent < lane ? parent : -1;
   uint64_t above = up >= 0 ? 1ull << up : 0;
@@ -225,16 +236,34 @@ __device__ __forceinline__ void tree_tables(TreeShared<kTiles>& s, int lane, int
   sum *= kInverseLn2;
   const uint64_t all_bad = __ballot(bad);
   if (lane < TreeShared<kTiles>::kNodes) {
-    const float high = static_cast<float>(sum);
+    const float high = static_cast<float>(sum), low = static_cast<float>(sum - high);
+    float k_unit = 1.0f, q_unit = a.scale;
+    if (a.normalize) {
+      k_unit = 1.0f / sqrtf(s.k_square[lane] + kUnitEps);
+      q_unit *= 1.0f / sqrtf(s.q_square[lane] + kUnitEps);
+    }
+    const float decay = decay_between(high, low, 0.0f, 0.0f);
+    const float b = real ? strength : 0.0f;
+    s.k_unit[lane] = k_unit;
+    s.k_step[lane] = -b * k_unit;
+    s.q_unit[lane] = q_unit;
+    s.seen[lane] = -b * (decay * k_unit);
+    s.look[lane] = decay * q_unit;
+    s.strength[lane] = b;
     s.sum[lane] = high;
-    s.rest[lane] = static_cast<float>(sum - high);
-    s.strength[lane] = real ? strength : 0.0f;
+    s.rest[lane] = low;
     s.above[lane] = above;
   }
   if (lane < 2) {
     s.bad_node[lane] = static_cast<uint32_t>(all_bad >> (32 * lane));
     s.bad_output[lane] = 0;
   }
+}
+
+// 16 bytes of a token's row: `row` tokens after `base`, `step` elements apart.
+__device__ __forceinline__ const void* row_at(const bf16_bits* base, uint32_t row, uint32_t step,
+                                              uint32_t offset) {
+  return reinterpret_cast<const char*>(base) + (row * step + offset) * 2u;
 }
 
 // A workgroup takes kWaves x kSlices slices of 16 rows of one head's state.  The first
@@ -244,11 +273,12 @@ template <typename Pool, int kTiles, int kSlices, int kWaves>
 __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
   constexpr int kThreads = 64 * kWaves;
   constexpr int kPerHead = 8 / (kSlices * kWaves);
+  constexpr int kRows = 16 * kSlices * kWaves;  // of the state
   constexpr int kNodes = 16 * kTiles;
-  constexpr int kPasses = kNodes * 16 / kThreads;
+  constexpr int kPasses = 2 * kNodes * 16 / kThreads;
   constexpr int kBlocks = blocks_of(kTiles);
   constexpr int kPairs = (kBlocks + kWaves - 2) / (kWaves - 1);
-  static_assert(kWaves >= 2 && kNodes * 16 % kThreads == 0, "the roles above");
+  static_assert(kWaves >= 2 && 2 * kNodes * 16 % kThreads == 0, "the roles above");
   __shared__ TreeShared<kTiles> s;
 
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
@@ -266,35 +296,43 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
   int parent = -1;
   float log_decay = 0.0f, strength = 0.0f;
   if (wave == 0 && lane < nodes) {
-    const uint64_t row = begin + lane;
-    parent = a.parents[row];
-    log_decay = a.log_decay[row * a.value_heads + h];
-    strength = widen(a.beta[row * a.value_heads + h]);
+    const uint64_t first = begin * a.value_heads + h;
+    parent = (a.parents + begin)[lane];
+    log_decay = (a.log_decay + first)[lane * a.value_heads];
+    strength = widen((a.beta + first)[lane * a.value_heads]);
   }
   const int piece = threadIdx.x & 15;
-  uint4 k_piece[kPasses], q_piece[kPasses];
+  const bf16_bits* const keys = a.keys + begin * a.key_stride + hk * kDim;
+  const bf16_bits* const queries = a.queries + begin * a.query_stride + hk * kDim;
+  const uint32_t key_step = static_cast<uint32_t>(a.key_stride);
+  const uint32_t query_step = static_cast<uint32_t>(a.query_stride);
+  uint4 pieces[kPasses];  // the keys', then the queries'
 #pragma unroll
   for (int p = 0; p < kPasses; ++p) {
-    const int row = p * (kThreads / 16) + (threadIdx.x >> 4);
-    if (p * (kThreads / 16) < 16 * tiles) {  // the same for the workgroup
-      const uint64_t token = begin + min(row, nodes - 1);
-      k_piece[p] = *reinterpret_cast<const uint4*>(a.keys + token * a.key_stride + hk * kDim +
-                                                   8 * piece);
-      q_piece[p] = *reinterpret_cast<const uint4*>(a.queries + token * a.query_stride +
-                                                   hk * kDim + 8 * piece);
+    // The same for a wavefront, like the row's tile.
+    const int place = p * (kThreads / 16) + 4 * wave;
+    const bool query = place >= kNodes;
+    const int first = place % kNodes;
+    if (first < 16 * tiles) {
+      const uint32_t row = min(first + g, nodes - 1);
+      pieces[p] = *static_cast<const uint4*>(
+          row_at(query ? queries : keys, row, query ? query_step : key_step, 8 * piece));
     }
   }
   const int first_row = 16 * kSlices * static_cast<int>((item % kPerHead) * kWaves + wave);
   uint2 v[kSlices][kTiles];
+  {
+    const bf16_bits* const values = a.values + begin * a.value_stride + h * kDim + first_row;
+    const uint32_t step = static_cast<uint32_t>(a.value_stride);
 #pragma unroll
-  for (int i = 0; i < kTiles; ++i) {
-    if (i < tiles) {
-      const uint64_t token = begin + min(16 * i + 4 * g + (r & 3), nodes - 1);
+    for (int i = 0; i < kTiles; ++i) {
+      if (i < tiles) {
+        const uint32_t row = min(16 * i + 4 * g + (r & 3), nodes - 1);
 #pragma unroll
-      for (int slice = 0; slice < kSlices; ++slice) {
-        v[slice][i] = *reinterpret_cast<const uint2*>(
-            a.values + token * a.value_stride + h * kDim + first_row + 16 * slice +
-            (r & 12));
+        for (int slice = 0; slice < kSlices; ++slice) {
+          v[slice][i] = *static_cast<const uint2*>(
+              row_at(values, row, step, 16 * slice + (r & 12)));
+        }
       }
     }
   }
@@ -302,26 +340,25 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
   {
     const Pool* const state = static_cast<const Pool*>(a.pool) +
                               (static_cast<uint64_t>(slot) * a.value_heads + h) * kTile +
-                              (first_row + r) * kDim + 8 * g;
+                              first_row * kDim;
+    const uint32_t place = r * kDim + 8 * g;
 #pragma unroll
     for (int slice = 0; slice < kSlices; ++slice) {
 #pragma unroll
       for (int step = 0; step < 4; ++step) {
-        cells[slice][step].load(state + 16 * slice * kDim + 32 * step);
+        cells[slice][step].load(state + (place + 16 * slice * kDim + 32 * step));
       }
     }
   }
 
 #pragma unroll
   for (int p = 0; p < kPasses; ++p) {
-    const int row = p * (kThreads / 16) + (threadIdx.x >> 4);
-    if (p * (kThreads / 16) < 16 * tiles) {
-      const float kk = stage_piece(s.k, row, piece, k_piece[p]);
-      const float qq = stage_piece(s.q, row, piece, q_piece[p]);
-      if (piece == 0) {
-        s.k_unit[row] = a.normalize ? 1.0f / sqrtf(kk + kUnitEps) : 1.0f;
-        s.q_unit[row] = a.normalize ? a.scale * (1.0f / sqrtf(qq + kUnitEps)) : a.scale;
-      }
+    const int place = p * (kThreads / 16) + 4 * wave;
+    const bool query = place >= kNodes;
+    const int first = place % kNodes;
+    if (first < 16 * tiles) {
+      const float square = stage_piece(query ? s.q : s.k, first + g, piece, pieces[p]);
+      if (piece == 0) (query ? s.q_square : s.k_square)[first + g] = square;
     }
   }
   exchange();
@@ -339,15 +376,15 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
       uint4 part[kSlices][Cells<Pool>::kParts];
 #pragma unroll
       for (int slice = 0; slice < kSlices; ++slice) cells[slice][step].parts(part[slice]);
+      const uint4* const k = &staged(s.k, r, 4 * step + g);
+      const uint4* const q = &staged(s.q, r, 4 * step + g);
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) {
         if (i < tiles) {
-          const uint4 k = staged(s.k, 16 * i + r, 4 * step + g);
-          const uint4 q = staged(s.q, 16 * i + r, 4 * step + g);
 #pragma unroll
           for (int slice = 0; slice < kSlices; ++slice) {
-            seen[slice][i] = product(k, part[slice], seen[slice][i]);
-            read[slice][i] = product(q, part[slice], read[slice][i]);
+            seen[slice][i] = product(k[256 * i], part[slice], seen[slice][i]);
+            read[slice][i] = product(q[256 * i], part[slice], read[slice][i]);
           }
         }
       }
@@ -355,7 +392,7 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
   };
 
   if (wave == 0) {
-    tree_tables(s, lane, nodes, parent, log_decay, strength);
+    tree_tables(s, a, lane, nodes, parent, log_decay, strength);
     exchange();
     state_products();
     exchange();
@@ -369,14 +406,15 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
       const int block = wave - 1 + e * (kWaves - 1);
       const int i = block < 1 ? 0 : block < 3 ? 1 : block < 6 ? 2 : 3;
       const int j = block - block_at(i, 0);
+      kk[e] = qk[e] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       if (block < kBlocks && i < tiles) {
-        const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-        kk[e] = qk[e] = zero;
 #pragma unroll
         for (int step = 0; step < 4; ++step) {
-          const uint4 column = staged(s.k, 16 * j + r, 4 * step + g);
-          kk[e] = mfma(staged(s.k, 16 * i + r, 4 * step + g), column, kk[e]);
-          qk[e] = mfma(staged(s.q, 16 * i + r, 4 * step + g), column, qk[e]);
+          const uint4* const k = &staged(s.k, r, 4 * step + g);
+          const uint4* const q = &staged(s.q, r, 4 * step + g);
+          const uint4 column = k[256 * j];
+          kk[e] = mfma(k[256 * i], column, kk[e]);
+          qk[e] = mfma(q[256 * i], column, qk[e]);
         }
       }
     }
@@ -388,25 +426,37 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
       const int j = block - block_at(i, 0);
       if (block < kBlocks && i < tiles) {
         const int first = 16 * i + 4 * g, column = 16 * j + r;
-        const f32x4 sum = load4(&s.sum[first]), rest = load4(&s.rest[first]);
-        const f32x4 k_unit = load4(&s.k_unit[first]), q_unit = load4(&s.q_unit[first]);
-        const f32x4 b = load4(&s.strength[first]);
         const float sum_c = s.sum[column], rest_c = s.rest[column], unit_c = s.k_unit[column];
-        uint32_t bad_node = 0, bad_output = 0;  // a bit a row
+        float worst_node = 0.0f, worst_output = 0.0f;  // NaN where a cell is no number
+        f32x4 x, y;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const bool up = (s.above[first + c] >> column & 1) != 0;
-          const bool self = first + c == column && column < nodes;
-          const float decay = decay_between(sum[c], rest[c], sum_c, rest_c);
-          float x = up ? -b[c] * decay * (k_unit[c] * unit_c * kk[e][c]) : 0.0f;
-          float y = up || self ? decay * (q_unit[c] * unit_c * qk[e][c]) : 0.0f;
-          if (!finite(x)) bad_node |= 1u << c, x = 0.0f;
-          if (!finite(y)) bad_output |= 1u << c, y = 0.0f;
-          s.step[block].at(4 * g + c, r) = x;
-          s.read[block].at(4 * g + c, r) = y;
+          const int row = first + c;
+          const bool up = (s.above[row] >> column & 1) != 0;
+          const bool self = row == column && column < nodes;
+          const float decay = decay_between(s.sum[row], s.rest[row], sum_c, rest_c) * unit_c;
+          x[c] = up ? decay * s.k_step[row] * kk[e][c] : 0.0f;
+          y[c] = up || self ? decay * s.q_unit[row] * qk[e][c] : 0.0f;
+          worst_node = fmaf(x[c], 0.0f, worst_node);
+          worst_output = fmaf(y[c], 0.0f, worst_output);
+          // A row at a time: all rows' factors would take as many registers as the state.
+          __builtin_amdgcn_sched_barrier(0);
         }
-        if (bad_node) atomicOr(&s.bad_node[first >> 5], bad_node << (first & 31));
-        if (bad_output) atomicOr(&s.bad_output[first >> 5], bad_output << (first & 31));
+        if (__any(worst_node != 0.0f || worst_output != 0.0f)) {
+          uint32_t bad_node = 0, bad_output = 0;  // a bit a row
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (!finite(x[c])) bad_node |= 1u << c, x[c] = 0.0f;
+            if (!finite(y[c])) bad_output |= 1u << c, y[c] = 0.0f;
+          }
+          if (bad_node) atomicOr(&s.bad_node[first >> 5], bad_node << (first & 31));
+          if (bad_output) atomicOr(&s.bad_output[first >> 5], bad_output << (first & 31));
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          s.step[block].at(4 * g + c, r) = x[c];
+          s.read[block].at(4 * g + c, r) = y[c];
+        }
       }
     }
     exchange();
@@ -414,41 +464,36 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
     exchange();
   }
 
-  const uint64_t bad_nodes = static_cast<uint64_t>(s.bad_node[1]) << 32 | s.bad_node[0];
   const uint64_t bad_outputs = static_cast<uint64_t>(s.bad_output[1]) << 32 | s.bad_output[0];
-  uint64_t bad[kSlices];  // nodes whose r is bad in this column
+  uint64_t bad[kSlices];  // nodes that are bad, or whose r is in this column
 #pragma unroll
-  for (int slice = 0; slice < kSlices; ++slice) bad[slice] = bad_nodes;
+  for (int slice = 0; slice < kSlices; ++slice) {
+    bad[slice] = static_cast<uint64_t>(s.bad_node[1]) << 32 | s.bad_node[0];
+  }
   f32x4 u[kSlices][kTiles];
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) {
     if (i >= tiles) break;
     const int first = 16 * i + 4 * g;
-    const f32x4 sum = load4(&s.sum[first]), rest = load4(&s.rest[first]);
-    const f32x4 k_unit = load4(&s.k_unit[first]), q_unit = load4(&s.q_unit[first]);
+    const f32x4 see = load4(&s.seen[first]), look = load4(&s.look[first]);
     const f32x4 b = load4(&s.strength[first]);
-    f32x4 see, look;  // factors of S0 k and S0 q
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const float decay = decay_between(sum[c], rest[c], 0.0f, 0.0f);
-      see[c] = decay * k_unit[c];
-      look[c] = decay * q_unit[c];
-    }
     f32x4 x[kSlices], out[kSlices];
 #pragma unroll
     for (int slice = 0; slice < kSlices; ++slice) {
       const f32x4 values = value_columns(v[slice][i], lane);
-      uint32_t odd = 0;
+      float worst = 0.0f;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        float y = b[c] * fmaf(-see[c], seen[slice][i][c], values[c]);
-        if (first + c >= nodes) y = 0.0f;
-        if (!finite(y)) odd |= 1u << c, y = 0.0f;
-        x[slice][c] = y;
+        x[slice][c] = fmaf(see[c], seen[slice][i][c], b[c] * values[c]);
         out[slice][c] = look[c] * read[slice][i][c];
+        worst = fmaf(x[slice][c], 0.0f, worst);
       }
-      if (__any(odd != 0)) {
-        uint64_t column = static_cast<uint64_t>(odd) << first;
+      if (__any(worst != 0.0f)) {
+        uint64_t column = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (!finite(x[slice][c])) column |= 1ull << (first + c), x[slice][c] = 0.0f;
+        }
         column |= __shfl_xor(column, 16);
         column |= __shfl_xor(column, 32);
         bad[slice] |= column;
@@ -479,15 +524,23 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
           }
         }
       }
+      // A node's outputs side by side, in pieces of 16 bytes as the keys were.
       const uint2 packed = transpose_quad(
           make_uint2(bf16_pair(y[0], y[1]), bf16_pair(y[2], y[3])), lane);
       const int node = first + (r & 3);
-      if (node < nodes) {
-        *reinterpret_cast<uint2*>(a.outputs +
-                                  ((begin + node) * a.value_heads + h) * kDim + first_row +
-                                  16 * slice + (r & 12)) = packed;
-      }
+      const int at = 2 * (kSlices * wave + slice) + (r >> 3);  // piece
+      reinterpret_cast<uint2*>(&s.out[16 * node + (at ^ (node & 15))])[r >> 2 & 1] = packed;
     }
+  }
+  exchange();
+  constexpr int kOutPieces = kRows / 8;
+  bf16_bits* const outputs = a.outputs + (begin * a.value_heads + h) * kDim +
+                             static_cast<int>(item % kPerHead) * kRows;
+  for (int p = threadIdx.x; p < nodes * kOutPieces; p += kThreads) {
+    const int node = p / kOutPieces, at = p % kOutPieces;
+    *reinterpret_cast<uint4*>(reinterpret_cast<char*>(outputs) +
+                              (node * a.value_heads * kDim + 8 * at) * 2u) =
+        s.out[16 * node + (at ^ (node & 15))];
   }
 }
 
@@ -736,6 +789,8 @@ __global__ __launch_bounds__(64 * kWaves) void commit_kernel(DraftArgs a) {
 
 // ---------------------------------------------------------------------- launch
 
+// 64 rows of it are 2^31 bytes, which the kernels' 32-bit offsets hold.
+constexpr uint64_t kMaxStride = 1u << 24;  // elements between tokens
 constexpr uint32_t kFewHeads = kComputeUnits;
 
 template <typename Pool, int kTiles>
@@ -743,8 +798,8 @@ int32_t launch_tree(void* stream, const DraftArgs& args, uint64_t heads) {
   return heads <= kFewHeads
              ? launch(tree_kernel<Pool, kTiles, 1, 2>, dim3(static_cast<uint32_t>(4 * heads)),
                       dim3(128), stream, args)
-             : launch(tree_kernel<Pool, kTiles, 2, 4>, dim3(static_cast<uint32_t>(heads)),
-                      dim3(256), stream, args);
+             : launch(tree_kernel<Pool, kTiles, 1, 8>, dim3(static_cast<uint32_t>(heads)),
+                      dim3(512), stream, args);
 }
 
 template <typename Pool>
@@ -772,7 +827,8 @@ int32_t launch_drafts(void* stream, const gdn_state_codec_drafts* d, const int32
       d->tokens > 0x7FFFFFFFu || d->key_heads == 0 || d->value_heads == 0 ||
       d->value_heads % d->key_heads != 0 || d->max_nodes == 0 || d->max_nodes > kMaxNodes ||
       d->normalize > 1 || d->query_stride % 8 != 0 || d->key_stride % 8 != 0 ||
-      d->value_stride % 8 != 0 || !d->offsets || !d->slot_ids ||
+      d->value_stride % 8 != 0 || d->query_stride > kMaxStride || d->key_stride > kMaxStride ||
+      d->value_stride > kMaxStride || d->value_heads > kMaxStride / kDim || !d->offsets || !d->slot_ids ||
       !token_rows(d->tokens, d->keys, d->values, d->log_decay, d->beta, d->parents) ||
       (kCommit ? !accepted || d->queries != nullptr
                : !token_rows(d->tokens, d->queries, outputs)) ||
