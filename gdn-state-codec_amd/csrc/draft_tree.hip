@@ -118,32 +118,33 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
 }
 
-// -A of a diagonal block becomes N = (I + A)^-1 - I, column `column` by each lane that
-// stores it: N_i = -A_i - sum_(m<i) A_im N_m.  The others compute whatever is there.
+// N = (I + A)^-1 - I of a diagonal block that holds -A^T (row m: column m of -A), column
+// `column` by each lane that stores it:  N_i = -A_i - sum_(m<i) A_im N_m, one m after
+// another, so that each step waits for one fma alone.  The other lanes compute whatever
+// is there.
 __device__ __forceinline__ void invert(Block& block, int column, bool stores) {
-  float n[16];
+  f32x4 n[4];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    float x = block.at(i, column), y = 0.0f;
+  for (int c = 0; c < 4; ++c) n[c] = block.run(column, 4 * c);
 #pragma unroll
-    for (int c = 0; c < i; c += 4) {
-      const f32x4 l = block.run(i, c);
+  for (int m = 0; m < 15; ++m) {
+    const float done = n[m / 4][m % 4];
+#pragma unroll
+    for (int c = (m + 1) / 4; c < 4; ++c) {
+      const f32x4 l = block.run(m, 4 * c);
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
-        if (c + u < i) {
-          if (u & 1) y = fmaf(l[u], n[c + u], y);
-          else x = fmaf(l[u], n[c + u], x);
-        }
+        if (4 * c + u > m) n[c][u] = fmaf(l[u], done, n[c][u]);
       }
     }
-    n[i] = x + y;
-    // Formed here, not where it is stored: all rows' operands would wait in registers.
-    asm volatile("" : "+v"(n[i]));
   }
-  wave_sync();  // -A has been read
+  // Formed here, not where it is stored: all rows would wait in registers.
+#pragma unroll
+  for (int c = 0; c < 4; ++c) asm volatile("" : "+v"(n[c]));
+  wave_sync();  // -A^T has been read
   if (stores) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) block.at(i, column) = n[i];
+    for (int i = 0; i < 16; ++i) block.at(i, column) = n[i / 4][i % 4];
   }
 }
 
@@ -199,7 +200,7 @@ struct TreeShared {
     };
     uint4 out[kNodes * 16];       // once all products of k and q are formed
   };
-  Block step[blocks_of(kTiles)];  // -A; on the diagonal then N
+  Block step[blocks_of(kTiles)];  // -A; on the diagonal -A^T, then N
   Block read[blocks_of(kTiles)];  // M
   float k_square[kNodes], q_square[kNodes];
   // Factors of a node: of a key, -b / |k|, scale / |q|; then -b exp(G) / |k| of S0 k,
@@ -211,39 +212,49 @@ struct TreeShared {
   uint32_t bad_node[2], bad_output[2];   // a bit a node
 };
 
-// The tables of the nodes, one a lane of one wavefront.  Sums and paths by doubling: after
-// round i a lane's sum is of 2^i nodes up from its own.
-template <int kTiles>
-__device__ __forceinline__ void tree_tables(TreeShared<kTiles>& s, const DraftArgs& a, int lane,
-                                            int nodes, int parent, float log_decay,
-                                            float strength) {
+// What a node's path gives, one node a lane of one wavefront.  By doubling: after round i a
+// lane's sum is of 2^i nodes up from its own.
+struct Path {
+  double sum;      // of log decays
+  uint64_t above;  // a bit a node
+  bool bad;        // the node's own log decay
+};
+
+__device__ __forceinline__ Path tree_path(int lane, int nodes, int parent, float log_decay) {
   const bool real = lane < nodes;
   int up = real && parent >= 0 && parent < lane ? parent : -1;
-  uint64_t above = up >= 0 ? 1ull << up : 0;
-  const bool bad = real && !(log_decay <= kLargest);
-  double sum = real && !bad ? fmax(static_cast<double>(log_decay), kLeastLogDecay) : 0.0;
+  Path p;
+  p.above = up >= 0 ? 1ull << up : 0;
+  p.bad = real && !(log_decay <= kLargest);
+  p.sum = real && !p.bad ? fmax(static_cast<double>(log_decay), kLeastLogDecay) : 0.0;
   for (int reach = 1; reach < nodes; reach <<= 1) {
     const int from = up >= 0 ? up : lane;
-    const double sum_up = __shfl(sum, from);
-    const uint64_t above_up = __shfl(above, from);
+    const double sum_up = __shfl(p.sum, from);
+    const uint64_t above_up = __shfl(p.above, from);
     const int next = __shfl(up, from);
     if (up >= 0) {
-      sum += sum_up;
-      above |= above_up;
+      p.sum += sum_up;
+      p.above |= above_up;
       up = next;
     }
   }
-  sum *= kInverseLn2;
-  const uint64_t all_bad = __ballot(bad);
+  p.sum *= kInverseLn2;
+  return p;
+}
+
+template <int kTiles>
+__device__ __forceinline__ void tree_tables(TreeShared<kTiles>& s, const DraftArgs& a, int lane,
+                                            int nodes, const Path& p, float strength) {
+  const uint64_t all_bad = __ballot(p.bad);
   if (lane < TreeShared<kTiles>::kNodes) {
-    const float high = static_cast<float>(sum), low = static_cast<float>(sum - high);
+    const float high = static_cast<float>(p.sum), low = static_cast<float>(p.sum - high);
     float k_unit = 1.0f, q_unit = a.scale;
     if (a.normalize) {
       k_unit = 1.0f / sqrtf(s.k_square[lane] + kUnitEps);
       q_unit *= 1.0f / sqrtf(s.q_square[lane] + kUnitEps);
     }
     const float decay = decay_between(high, low, 0.0f, 0.0f);
-    const float b = real ? strength : 0.0f;
+    const float b = lane < nodes ? strength : 0.0f;
     s.k_unit[lane] = k_unit;
     s.k_step[lane] = -b * k_unit;
     s.q_unit[lane] = q_unit;
@@ -252,7 +263,7 @@ __device__ __forceinline__ void tree_tables(TreeShared<kTiles>& s, const DraftAr
     s.strength[lane] = b;
     s.sum[lane] = high;
     s.rest[lane] = low;
-    s.above[lane] = above;
+    s.above[lane] = p.above;
   }
   if (lane < 2) {
     s.bad_node[lane] = static_cast<uint32_t>(all_bad >> (32 * lane));
@@ -351,6 +362,8 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
     }
   }
 
+  Path path;
+  if (wave == 0) path = tree_path(lane, nodes, parent, log_decay);
 #pragma unroll
   for (int p = 0; p < kPasses; ++p) {
     const int place = p * (kThreads / 16) + 4 * wave;
@@ -392,7 +405,7 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
   };
 
   if (wave == 0) {
-    tree_tables(s, a, lane, nodes, parent, log_decay, strength);
+    tree_tables(s, a, lane, nodes, path, strength);
     exchange();
     state_products();
     exchange();
@@ -427,20 +440,19 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
       if (block < kBlocks && i < tiles) {
         const int first = 16 * i + 4 * g, column = 16 * j + r;
         const float sum_c = s.sum[column], rest_c = s.rest[column], unit_c = s.k_unit[column];
+        const f32x4 sum = load4(&s.sum[first]), rest = load4(&s.rest[first]);
+        const f32x4 k_step = load4(&s.k_step[first]), q_unit = load4(&s.q_unit[first]);
         float worst_node = 0.0f, worst_output = 0.0f;  // NaN where a cell is no number
         f32x4 x, y;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const int row = first + c;
-          const bool up = (s.above[row] >> column & 1) != 0;
-          const bool self = row == column && column < nodes;
-          const float decay = decay_between(s.sum[row], s.rest[row], sum_c, rest_c) * unit_c;
-          x[c] = up ? decay * s.k_step[row] * kk[e][c] : 0.0f;
-          y[c] = up || self ? decay * s.q_unit[row] * qk[e][c] : 0.0f;
+          const bool up = (s.above[first + c] >> column & 1) != 0;
+          const bool self = first + c == column && column < nodes;
+          const float decay = decay_between(sum[c], rest[c], sum_c, rest_c) * unit_c;
+          x[c] = up ? decay * k_step[c] * kk[e][c] : 0.0f;
+          y[c] = up || self ? decay * q_unit[c] * qk[e][c] : 0.0f;
           worst_node = fmaf(x[c], 0.0f, worst_node);
           worst_output = fmaf(y[c], 0.0f, worst_output);
-          // A row at a time: all rows' factors would take as many registers as the state.
-          __builtin_amdgcn_sched_barrier(0);
         }
         if (__any(worst_node != 0.0f || worst_output != 0.0f)) {
           uint32_t bad_node = 0, bad_output = 0;  // a bit a row
@@ -454,7 +466,7 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
         }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          s.step[block].at(4 * g + c, r) = x[c];
+          s.step[block].at(i == j ? r : 4 * g + c, i == j ? 4 * g + c : r) = x[c];
           s.read[block].at(4 * g + c, r) = y[c];
         }
       }
@@ -548,7 +560,7 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
 
 struct CommitShared {
   uint4 k[16 * 16];
-  Block step;              // -A, then N
+  Block step;              // -A^T, then N
   float k_unit[16];
   float sum[kMaxNodes], rest[kMaxNodes];  // G / ln 2 from the start of each 16
   float strength[kMaxNodes];
@@ -713,7 +725,7 @@ __global__ __launch_bounds__(64 * kWaves) void commit_kernel(DraftArgs a) {
       for (int c = 0; c < 4; ++c) {
         const float decay = decay_between(sum[c], rest[c], sum_c, rest_c);
         const bool up = 4 * g + c > r && 4 * g + c < length;
-        s.step.at(4 * g + c, r) = up ? -b[c] * decay * (k_unit[c] * unit_c * kk[c]) : 0.0f;
+        s.step.at(r, 4 * g + c) = up ? -b[c] * decay * (k_unit[c] * unit_c * kk[c]) : 0.0f;
       }
       wave_sync();
       invert(s.step, r, g == 0);
