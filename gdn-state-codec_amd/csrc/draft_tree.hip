@@ -99,6 +99,14 @@ __device__ __forceinline__ f32x4 block_product(const f32x4& a, const f32x4& b, f
   return c;
 }
 
+// c + a b of 16 places of a contraction.
+typedef __attribute__((ext_vector_type(4))) short bf16x4_bits;
+__device__ __forceinline__ f32x4 mfma_half(const uint2& a, const uint2& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(bf16x4_bits, a),
+                                                   __builtin_bit_cast(bf16x4_bits, b), c, 0, 0,
+                                                   0);
+}
+
 // A 16 x 16 block in LDS.  A row's four runs of four columns are rotated by its place, so
 // that 16 rows' runs fall on different banks.
 struct Block {
@@ -191,6 +199,61 @@ constexpr int blocks_of(int tiles) { return tiles * (tiles + 1) / 2; }
 // Block (i, j <= i) of a lower triangular matrix.
 __host__ __device__ constexpr int block_at(int i, int j) { return i * (i + 1) / 2 + j; }
 
+// -A below the diagonal and M as operands of products with u, in three parts, row tile by
+// row tile: blocks 2 s and 2 s + 1 of a row side by side (16 bytes a lane, the places of
+// delta_chunk.h), a last one without a partner by itself (8 bytes a lane).  In units of 8
+// bytes: a block takes 3 x 64, and block j of row tile i starts at
+constexpr int kBlockPlaces = 3 * 64;
+__host__ __device__ constexpr int step_at(int i, int j) {
+  return (i * (i - 1) / 2 + j / 2 * 2) * kBlockPlaces;
+}
+__host__ __device__ constexpr int read_at(int i, int j) {
+  return (i * (i + 1) / 2 + j / 2 * 2) * kBlockPlaces;
+}
+constexpr int step_places(int tiles) { return tiles > 1 ? step_at(tiles, 0) : 1; }
+constexpr int read_places(int tiles) { return read_at(tiles, 0); }
+
+// A block (an accumulator) as its part of such an operand, where it has a partner (then
+// `second` is whether it is the second of the two) or not.
+__device__ __forceinline__ void store_operand(uint2* operand, bool paired, bool second, int lane,
+                                              const f32x4& block) {
+  const f32x4 row = transpose_quad(block, lane);  // row 4 g + (r & 3), columns r & 12 ..
+  uint2 part[3];
+  split3_half(row, part);
+  const int place = 4 * (lane >> 4) + (lane & 3) + 16 * (lane >> 2 & 3);
+#pragma unroll
+  for (int p = 0; p < 3; ++p) {
+    operand[paired ? 128 * p + 2 * place + (second ? 1 : 0) : 64 * p + place] = part[p];
+  }
+}
+
+// Parts of u, tiles 2 s and 2 s + 1 side by side.
+typedef uint4 Pair[3];
+
+// c + (blocks 2 s, 2 s + 1 of a row) (u of those tiles).
+__device__ __forceinline__ f32x4 add_pair(const uint2* operand, int lane, const Pair& u, f32x4 c) {
+  uint4 a[3];
+#pragma unroll
+  for (int p = 0; p < 3; ++p) a[p] = reinterpret_cast<const uint4*>(operand)[64 * p + lane];
+  return mfma6(a, u, c);
+}
+// c + (the last block of a row, that has no partner) (u of its tile).
+__device__ __forceinline__ f32x4 add_single(const uint2* operand, int lane, const Pair& u,
+                                            f32x4 c) {
+  uint2 a[3], b[3];
+#pragma unroll
+  for (int p = 0; p < 3; ++p) {
+    a[p] = operand[64 * p + lane];
+    b[p] = make_uint2(u[p].x, u[p].y);
+  }
+  c = mfma_half(a[0], b[2], c);
+  c = mfma_half(a[1], b[1], c);
+  c = mfma_half(a[2], b[0], c);
+  c = mfma_half(a[0], b[1], c);
+  c = mfma_half(a[1], b[0], c);
+  return mfma_half(a[0], b[0], c);
+}
+
 template <int kTiles>
 struct TreeShared {
   static constexpr int kNodes = 16 * kTiles;
@@ -200,9 +263,10 @@ struct TreeShared {
     };
     uint4 out[kNodes * 16];       // once all products of k and q are formed
   };
-  Block step[blocks_of(kTiles)];  // -A; on the diagonal -A^T, then N
-  Block read[blocks_of(kTiles)];  // M
-  float k_square[kNodes], q_square[kNodes];
+  Block inverse[kTiles];          // on the diagonal: -A^T, then N
+  alignas(16) uint2 step[step_places(kTiles)];  // -A below it
+  alignas(16) uint2 read[read_places(kTiles)];  // M
+  alignas(16) float k_square[kNodes], q_square[kNodes];
   // Factors of a node: of a key, -b / |k|, scale / |q|; then -b exp(G) / |k| of S0 k,
   // exp(G) scale / |q| of S0 q, and b.
   float k_unit[kNodes], k_step[kNodes], q_unit[kNodes];
@@ -410,7 +474,7 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
     state_products();
     exchange();
     const int diagonal = min(g, kTiles - 1);
-    invert(s.step[block_at(diagonal, diagonal)], r, g < tiles);
+    invert(s.inverse[diagonal], r, g < tiles);
     exchange();
   } else {
     f32x4 kk[kPairs], qk[kPairs];
@@ -464,11 +528,13 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
           if (bad_node) atomicOr(&s.bad_node[first >> 5], bad_node << (first & 31));
           if (bad_output) atomicOr(&s.bad_output[first >> 5], bad_output << (first & 31));
         }
+        if (i == j) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          s.step[block].at(i == j ? r : 4 * g + c, i == j ? 4 * g + c : r) = x[c];
-          s.read[block].at(4 * g + c, r) = y[c];
+          for (int c = 0; c < 4; ++c) s.inverse[i].at(r, 4 * g + c) = x[c];
+        } else {
+          store_operand(s.step + step_at(i, j), (j | 1) < i, (j & 1) != 0, lane, x);
         }
+        store_operand(s.read + read_at(i, j), (j | 1) <= i, (j & 1) != 0, lane, y);
       }
     }
     exchange();
@@ -482,7 +548,7 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
   for (int slice = 0; slice < kSlices; ++slice) {
     bad[slice] = static_cast<uint64_t>(s.bad_node[1]) << 32 | s.bad_node[0];
   }
-  f32x4 u[kSlices][kTiles];
+  Pair u[kSlices][(kTiles + 1) / 2];
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) {
     if (i >= tiles) break;
@@ -511,22 +577,30 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
         bad[slice] |= column;
       }
     }
-#pragma unroll
-    for (int j = 0; j < i; ++j) {
-      const f32x4 step = s.step[block_at(i, j)].run(r, 4 * g);
-      const f32x4 looked = s.read[block_at(i, j)].run(r, 4 * g);
-#pragma unroll
-      for (int slice = 0; slice < kSlices; ++slice) {
-        x[slice] = block_product(step, u[slice][j], x[slice]);
-        out[slice] = block_product(looked, u[slice][j], out[slice]);
-      }
-    }
-    const f32x4 inverse = s.step[block_at(i, i)].run(r, 4 * g);
-    const f32x4 looked = s.read[block_at(i, i)].run(r, 4 * g);
+    const f32x4 inverse = s.inverse[i].run(r, 4 * g);
 #pragma unroll
     for (int slice = 0; slice < kSlices; ++slice) {
-      u[slice][i] = block_product(inverse, x[slice], x[slice]);
-      f32x4 y = block_product(looked, u[slice][i], out[slice]);
+#pragma unroll
+      for (int j = 0; j < i; j += 2) {
+        const uint2* const step = s.step + step_at(i, j);
+        x[slice] = j + 1 < i ? add_pair(step, lane, u[slice][j / 2], x[slice])
+                             : add_single(step, lane, u[slice][j / 2], x[slice]);
+      }
+      uint2 part[3];
+      split3_half(block_product(inverse, x[slice], x[slice]), part);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        uint4& whole = u[slice][i / 2][p];
+        if (i % 2 == 0) whole.x = part[p].x, whole.y = part[p].y;
+        else whole.z = part[p].x, whole.w = part[p].y;
+      }
+      f32x4 y = out[slice];
+#pragma unroll
+      for (int j = 0; j <= i; j += 2) {
+        const uint2* const looked = s.read + read_at(i, j);
+        y = j + 1 <= i ? add_pair(looked, lane, u[slice][j / 2], y)
+                       : add_single(looked, lane, u[slice][j / 2], y);
+      }
       if (__any(bad[slice] != 0) || bad_outputs != 0) {
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -597,13 +671,6 @@ struct StateRow<bf16_bits> {
     __builtin_nontemporal_store(w, reinterpret_cast<u32x4_t*>(p));
   }
 };
-
-typedef __attribute__((ext_vector_type(4))) short bf16x4_bits;
-__device__ __forceinline__ f32x4 mfma_half(const uint2& a, const uint2& b, const f32x4& c) {
-  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(bf16x4_bits, a),
-                                                   __builtin_bit_cast(bf16x4_bits, b), c, 0, 0,
-                                                   0);
-}
 
 // A workgroup takes kWaves x kSlices slices of 16 rows of one head's state, which stay in
 // registers while the path's nodes are applied 16 at a time.  Accumulator tile m of a
