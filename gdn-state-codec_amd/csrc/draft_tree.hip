@@ -633,58 +633,80 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
 // ------------------------------------------------------------------ the commit
 
 struct CommitShared {
-  uint4 k[16 * 16];
-  Block step;              // -A^T, then N
-  float k_unit[16];
+  uint4 k[kMaxNodes * 16];  // the path's, like all that follows
+  Block inverse[kMaxNodes / 16];  // of each 16: -A^T, then N
+  float k_square[kMaxNodes], k_unit[kMaxNodes];
   float sum[kMaxNodes], rest[kMaxNodes];  // G / ln 2 from the start of each 16
   float strength[kMaxNodes];
   float log_decay[kMaxNodes];
   int path[kMaxNodes];
 };
 
+// A lane's 8 keys of a row in step `step` (of 32), as two accumulators: which keys these are
+// keeps a wavefront's loads and stores in runs of 64 bytes of a row.  Half `half` holds four
+// keys from run `place`'s on, in runs of four (place: the lane group, or a quad's number
+// where the tile's 16 keys are an operand's rows).
 template <typename Pool>
-struct StateRow;  // the same 8 keys as accumulators
+struct StateRow;
 
 template <>
 struct StateRow<float> {
-  static __device__ __forceinline__ void load(const float* p, f32x4& x, f32x4& y) {
-    x = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p));
-    y = __builtin_nontemporal_load(reinterpret_cast<const f32x4*>(p + 4));
+  static __device__ __forceinline__ int run(int step, int half, int place) {
+    return 8 * step + 4 * half + place;
   }
-  static __device__ __forceinline__ void store(float* p, const f32x4& x, const f32x4& y) {
-    __builtin_nontemporal_store(x, reinterpret_cast<f32x4*>(p));
-    __builtin_nontemporal_store(y, reinterpret_cast<f32x4*>(p + 4));
+  static __device__ __forceinline__ void load(const float* row, int step, int g, f32x4& x,
+                                              f32x4& y) {
+    x = load4(row + 4 * run(step, 0, g));
+    y = load4(row + 4 * run(step, 1, g));
+  }
+  static __device__ __forceinline__ void store(float* row, int step, int g, const f32x4& x,
+                                               const f32x4& y) {
+    store_cells(row + 4 * run(step, 0, g), x);
+    store_cells(row + 4 * run(step, 1, g), y);
   }
 };
 
 template <>
 struct StateRow<bf16_bits> {
-  static __device__ __forceinline__ void load(const bf16_bits* p, f32x4& x, f32x4& y) {
+  static __device__ __forceinline__ int run(int step, int half, int place) {
+    return 8 * step + 2 * place + half;
+  }
+  static __device__ __forceinline__ void load(const bf16_bits* row, int step, int g, f32x4& x,
+                                              f32x4& y) {
     float w[8];
-    widen8(stream_load(reinterpret_cast<const uint4*>(p)), w);
+    load8(row + 4 * run(step, 0, g), w);
     x = f32x4{w[0], w[1], w[2], w[3]};
     y = f32x4{w[4], w[5], w[6], w[7]};
   }
-  static __device__ __forceinline__ void store(bf16_bits* p, const f32x4& x, const f32x4& y) {
-    const u32x4_t w = {bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]), bf16_pair(y[0], y[1]),
-                       bf16_pair(y[2], y[3])};
-    __builtin_nontemporal_store(w, reinterpret_cast<u32x4_t*>(p));
+  // The pool's own type: one rounding a path.
+  static __device__ __forceinline__ void store(bf16_bits* row, int step, int g, const f32x4& x,
+                                               const f32x4& y) {
+    *reinterpret_cast<uint4*>(row + 4 * run(step, 0, g)) =
+        make_uint4(bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]), bf16_pair(y[0], y[1]),
+                   bf16_pair(y[2], y[3]));
   }
 };
 
-// A workgroup takes kWaves x kSlices slices of 16 rows of one head's state, which stay in
-// registers while the path's nodes are applied 16 at a time.  Accumulator tile m of a
-// slice is keys state_key(m, ..) by values, so that a lane's registers are 8 neighbouring
-// keys of its row, the products' operand and the update's accumulators.
-template <typename Pool, int kSlices, int kWaves>
+// Run `run` of four keys of a staged row.
+__device__ __forceinline__ uint2 staged_run(const uint4* rows, int row, int run) {
+  return reinterpret_cast<const uint2*>(rows)[32 * row + ((run >> 1 ^ (row & 15)) << 1) +
+                                              (run & 1)];
+}
+
+// A workgroup takes kWaves slices of 16 rows of one head's state, which stay in registers
+// while the path's nodes are applied 16 at a time, both as the products' operand and as the
+// update's accumulators.  What depends on no state (the path, its keys in LDS, A's inverse
+// for each 16, by a wavefront each) comes first, so that nothing waits for another
+// wavefront between one 16 and the next.
+template <typename Pool, int kWaves>
 __global__ __launch_bounds__(64 * kWaves) void commit_kernel(DraftArgs a) {
+  typedef StateRow<Pool> Row;
   constexpr int kThreads = 64 * kWaves;
-  constexpr int kPerHead = 8 / (kSlices * kWaves);
-  constexpr int kPasses = 16 * 16 / kThreads;
-  static_assert(kWaves >= 2 && 256 % kThreads == 0, "the roles below");
+  constexpr int kPerHead = 8 / kWaves;
+  constexpr int kPasses = kMaxNodes * 16 / kThreads;
   __shared__ CommitShared s;
 
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t item = static_cast<uint32_t>(xcd_contiguous_item(blockIdx.x, gridDim.x));
   const uint32_t head = item / kPerHead;
@@ -692,49 +714,48 @@ __global__ __launch_bounds__(64 * kWaves) void commit_kernel(DraftArgs a) {
   int32_t slot;
   uint64_t begin;
   const int nodes = request_nodes(a, n, slot, begin);
-  const int last = a.accepted[n];
+  const int last = uniform(a.accepted[n]);
   if (last < 0 || last >= nodes) return;
 
+  // Every wavefront finds the path; the first one forms its tables.
   int parent = -1;
   float log_decay = 0.0f, strength = 0.0f;
+  if (lane < nodes) parent = (a.parents + begin)[lane];
   if (wave == 0 && lane < nodes) {
-    const uint64_t row = begin + lane;
-    parent = a.parents[row];
-    log_decay = a.log_decay[row * a.value_heads + h];
-    strength = widen(a.beta[row * a.value_heads + h]);
+    const uint64_t first = begin * a.value_heads + h;
+    log_decay = (a.log_decay + first)[lane * a.value_heads];
+    strength = widen((a.beta + first)[lane * a.value_heads]);
   }
-  const int first_row = 16 * kSlices * static_cast<int>((item % kPerHead) * kWaves + wave);
+  const int first_row = 16 * static_cast<int>((item % kPerHead) * kWaves + wave);
   Pool* const state = static_cast<Pool*>(a.pool) +
                       (static_cast<uint64_t>(slot) * a.value_heads + h) * kTile +
-                      (first_row + r) * kDim + 8 * g;
-  f32x4 cells[kSlices][8];
+                      first_row * kDim;
+  f32x4 cells[4][2];
 #pragma unroll
-  for (int slice = 0; slice < kSlices; ++slice) {
-#pragma unroll
-    for (int step = 0; step < 4; ++step) {
-      StateRow<Pool>::load(state + 16 * slice * kDim + 32 * step, cells[slice][2 * step],
-                           cells[slice][2 * step + 1]);
-    }
+  for (int step = 0; step < 4; ++step) {
+    Row::load(state + r * kDim, step, g, cells[step][0], cells[step][1]);
   }
 
+  if (parent >= lane) parent = -1;
+  uint64_t on_path = 0;
+  for (int node = last; node >= 0; node = __builtin_amdgcn_readlane(parent, node)) {
+    on_path |= 1ull << node;
+  }
+  const int length = __popcll(on_path);
   if (wave == 0) {
-    if (parent >= lane) parent = -1;
-    uint64_t on_path = 0;
-    for (int node = last; node >= 0; node = __builtin_amdgcn_readlane(parent, node)) {
-      on_path |= 1ull << node;
+    if (lane >= length) {
+      s.path[lane] = -1;
+      s.strength[lane] = 0.0f;
+      s.log_decay[lane] = 0.0f;
     }
-    s.path[lane] = -1;
-    wave_sync();
     if (on_path >> lane & 1) {
       const int place = __popcll(on_path & ((1ull << lane) - 1));
       s.path[place] = lane;
-      s.log_decay[place] = log_decay;
       s.strength[place] = strength;
+      s.log_decay[place] = log_decay;
     }
     wave_sync();
-    const bool real = s.path[lane] >= 0;
-    // A NaN stays: it is on the path.
-    const float own = real ? s.log_decay[lane] : 0.0f;
+    const float own = s.log_decay[lane];  // a NaN stays: it is on the path
     double sum = own < static_cast<float>(kLeastLogDecay) ? kLeastLogDecay : own;
 #pragma unroll
     for (int reach = 1; reach < 16; reach <<= 1) {
@@ -745,124 +766,121 @@ __global__ __launch_bounds__(64 * kWaves) void commit_kernel(DraftArgs a) {
     const float high = static_cast<float>(sum);
     s.sum[lane] = high;
     s.rest[lane] = static_cast<float>(sum - high);
-    if (!real) s.strength[lane] = 0.0f;
   }
   exchange();
 
-  for (int at = 0; at < kMaxNodes && s.path[at] >= 0; at += 16) {
-    const int length = __popcll(__ballot(s.path[at + r] >= 0)) / 4;  // nodes of this 16
-    const int piece = threadIdx.x & 15;
-    uint4 k_piece[kPasses];
+  const bf16_bits* const keys = a.keys + begin * a.key_stride + hk * kDim;
+  const bf16_bits* const values = a.values + begin * a.value_stride + h * kDim + first_row;
+  // Four of a lane's columns of the value of node 4 g + (r & 3) of the 16 from `at` on.
+  auto value_of = [&](int at) {
+    return *static_cast<const uint2*>(row_at(values, s.path[min(at + 4 * g + (r & 3), length - 1)],
+                                             static_cast<uint32_t>(a.value_stride), r & 12));
+  };
+  {
+    uint4 pieces[kPasses];
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
-      const int row = p * (kThreads / 16) + (threadIdx.x >> 4);
-      const uint64_t token = begin + s.path[at + min(row, length - 1)];
-      k_piece[p] = *reinterpret_cast<const uint4*>(a.keys + token * a.key_stride + hk * kDim +
-                                                   8 * piece);
-    }
-    uint2 v[kSlices];
-    {
-      const uint64_t token = begin + s.path[at + min(4 * g + (r & 3), length - 1)];
-#pragma unroll
-      for (int slice = 0; slice < kSlices; ++slice) {
-        v[slice] = *reinterpret_cast<const uint2*>(a.values + token * a.value_stride + h * kDim +
-                                                   first_row + 16 * slice + (r & 12));
+      const int first = p * (kThreads / 16) + 4 * wave;
+      pieces[p] = make_uint4(0, 0, 0, 0);
+      if (first < length) {  // the same for a wavefront; rows past the path are its last
+        pieces[p] = *static_cast<const uint4*>(
+            row_at(keys, s.path[min(first + g, length - 1)], static_cast<uint32_t>(a.key_stride),
+                   8 * r));
       }
     }
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
-      const int row = p * (kThreads / 16) + (threadIdx.x >> 4);
-      const float kk = stage_piece(s.k, row, piece, k_piece[p]);
-      if (piece == 0) s.k_unit[row] = a.normalize ? 1.0f / sqrtf(kk + kUnitEps) : 1.0f;
+      const int first = p * (kThreads / 16) + 4 * wave;
+      if (first < (length + 15) / 16 * 16) {
+        const float square = stage_piece(s.k, first + g, r, pieces[p]);
+        if (r == 0) s.k_square[first + g] = square;
+      }
     }
-    exchange();
+  }
+  uint2 v = value_of(0);
+  exchange();
 
-    const f32x4 sum = load4(&s.sum[at + 4 * g]), rest = load4(&s.rest[at + 4 * g]);
-    const f32x4 b = load4(&s.strength[at + 4 * g]), k_unit = load4(&s.k_unit[4 * g]);
-    const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (wave == 0) {
-      f32x4 kk = zero;
-#pragma unroll
-      for (int step = 0; step < 4; ++step) {
-        const uint4 k = staged(s.k, r, 4 * step + g);
-        kk = mfma(k, k, kk);
-      }
-      const float sum_c = s.sum[at + r], rest_c = s.rest[at + r], unit_c = s.k_unit[r];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float decay = decay_between(sum[c], rest[c], sum_c, rest_c);
-        const bool up = 4 * g + c > r && 4 * g + c < length;
-        s.step.at(r, 4 * g + c) = up ? -b[c] * decay * (k_unit[c] * unit_c * kk[c]) : 0.0f;
-      }
-      wave_sync();
-      invert(s.step, r, g == 0);
-    }
-    f32x4 seen[kSlices];
-#pragma unroll
-    for (int slice = 0; slice < kSlices; ++slice) seen[slice] = zero;
+  for (int at = 16 * wave; at < length; at += 16 * kWaves) {
+    f32x4 kk = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
-      const uint4 k = staged(s.k, r, 4 * step + g);
-#pragma unroll
-      for (int slice = 0; slice < kSlices; ++slice) {
-        uint4 part[3];
-        split3(cells[slice][2 * step], cells[slice][2 * step + 1], part);
-        seen[slice] = mfma3(k, part, seen[slice]);
-      }
+      const uint4 k = staged(s.k, at + r, 4 * step + g);
+      kk = mfma(k, k, kk);
     }
-    exchange();
-
-    const f32x4 inverse = s.step.run(r, 4 * g);
-    const float end_sum = s.sum[at + length - 1], end_rest = s.rest[at + length - 1];
-    const float whole = decay_between(end_sum, end_rest, 0.0f, 0.0f);
-    uint2 part[kSlices][3];  // u, weighted
+    const float unit_c = a.normalize ? 1.0f / sqrtf(s.k_square[at + r] + kUnitEps) : 1.0f;
+    if (g == 0) s.k_unit[at + r] = unit_c;
+    wave_sync();
+    const f32x4 sum = load4(&s.sum[at + 4 * g]), rest = load4(&s.rest[at + 4 * g]);
+    const f32x4 b = load4(&s.strength[at + 4 * g]), k_unit = load4(&s.k_unit[at + 4 * g]);
+    const float sum_c = s.sum[at + r], rest_c = s.rest[at + r];
+    Block& block = s.inverse[at / 16];
 #pragma unroll
-    for (int slice = 0; slice < kSlices; ++slice) {
-      const f32x4 values = value_columns(v[slice], lane);
+    for (int c = 0; c < 4; ++c) {
+      const float decay = decay_between(sum[c], rest[c], sum_c, rest_c);
+      const bool up = 4 * g + c > r && at + 4 * g + c < length;
+      block.at(r, 4 * g + c) = up ? -b[c] * decay * (k_unit[c] * unit_c * kk[c]) : 0.0f;
+    }
+    wave_sync();
+    invert(block, r, g == 0);
+  }
+  exchange();
+
+  for (int at = 0; at < length; at += 16) {
+    // Addresses by lane are formed in each round: kept over it, they take as many registers
+    // as the state.
+    asm volatile("" : "+v"(lane));
+    r = lane & 15, g = lane >> 4;
+    f32x4 seen = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int step = 0; step < 4; ++step) {
+      const uint2 low = staged_run(s.k + 16 * at, r, Row::run(step, 0, g));
+      const uint2 high = staged_run(s.k + 16 * at, r, Row::run(step, 1, g));
+      uint4 part[3];
+      split3(cells[step][0], cells[step][1], part);
+      seen = mfma3(make_uint4(low.x, low.y, high.x, high.y), part, seen);
+    }
+    const f32x4 own = value_columns(v, lane);
+    if (at + 16 < length) v = value_of(at + 16);
+
+    const int end = min(at + 15, length - 1);
+    const float end_sum = s.sum[end], end_rest = s.rest[end];
+    const float whole = decay_between(end_sum, end_rest, 0.0f, 0.0f);
+    uint2 part[3];  // u, weighted
+    {
+      const f32x4 sum = load4(&s.sum[at + 4 * g]), rest = load4(&s.rest[at + 4 * g]);
+      const f32x4 b = load4(&s.strength[at + 4 * g]), k_unit = load4(&s.k_unit[at + 4 * g]);
       f32x4 x;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const float decay = decay_between(sum[c], rest[c], 0.0f, 0.0f);
-        x[c] = b[c] * fmaf(-decay * k_unit[c], seen[slice][c], values[c]);
-        if (4 * g + c >= length) x[c] = 0.0f;
+        x[c] = at + 4 * g + c < length ? b[c] * fmaf(-decay * k_unit[c], seen[c], own[c]) : 0.0f;
       }
-      f32x4 u = block_product(inverse, x, x);
+      f32x4 u = block_product(s.inverse[at / 16].run(r, 4 * g), x, x);
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        u[c] *= decay_between(end_sum, end_rest, sum[c], rest[c]) * k_unit[c];
-        if (4 * g + c >= length) u[c] = 0.0f;
+        const float weight = decay_between(end_sum, end_rest, sum[c], rest[c]) * k_unit[c];
+        u[c] = at + 4 * g + c < length ? u[c] * weight : 0.0f;
       }
-      split3_half(u, part[slice]);
+      split3_half(u, part);
     }
-    const int token = 4 * g + (r & 3);
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
-      const uint4 keys = staged(s.k, token, 4 * step + (r >> 2));
-      const uint2 low = transpose_quad(make_uint2(keys.x, keys.y), lane);
-      const uint2 high = transpose_quad(make_uint2(keys.z, keys.w), lane);
 #pragma unroll
-      for (int slice = 0; slice < kSlices; ++slice) {
-        f32x4 x = cells[slice][2 * step] * whole, y = cells[slice][2 * step + 1] * whole;
+      for (int half = 0; half < 2; ++half) {
+        // Four keys of four nodes, a node a lane of a quad, to a key a lane.
+        const uint2 key = transpose_quad(
+            staged_run(s.k + 16 * at, 4 * g + (r & 3), Row::run(step, half, r >> 2)), lane);
+        f32x4 x = cells[step][half] * whole;
 #pragma unroll
-        for (int p = 2; p >= 0; --p) {
-          x = mfma_half(low, part[slice][p], x);
-          y = mfma_half(high, part[slice][p], y);
-        }
-        cells[slice][2 * step] = x;
-        cells[slice][2 * step + 1] = y;
+        for (int p = 2; p >= 0; --p) x = mfma_half(key, part[p], x);
+        cells[step][half] = x;
       }
     }
-    exchange();  // k and the inverse have been read
-    if (at + 16 >= kMaxNodes) break;
   }
 
 #pragma unroll
-  for (int slice = 0; slice < kSlices; ++slice) {
-#pragma unroll
-    for (int step = 0; step < 4; ++step) {
-      StateRow<Pool>::store(state + 16 * slice * kDim + 32 * step, cells[slice][2 * step],
-                            cells[slice][2 * step + 1]);
-    }
+  for (int step = 0; step < 4; ++step) {
+    Row::store(state + r * kDim, step, g, cells[step][0], cells[step][1]);
   }
 }
 
@@ -892,9 +910,9 @@ int32_t launch_tree(void* stream, const DraftArgs& args, uint64_t heads) {
 template <typename Pool>
 int32_t launch_commit(void* stream, const DraftArgs& args, uint64_t heads) {
   return heads <= kFewHeads
-             ? launch(commit_kernel<Pool, 1, 2>, dim3(static_cast<uint32_t>(4 * heads)),
-                      dim3(128), stream, args)
-             : launch(commit_kernel<Pool, 2, 4>, dim3(static_cast<uint32_t>(heads)), dim3(256),
+             ? launch(commit_kernel<Pool, 2>, dim3(static_cast<uint32_t>(4 * heads)), dim3(128),
+                      stream, args)
+             : launch(commit_kernel<Pool, 8>, dim3(static_cast<uint32_t>(heads)), dim3(512),
                       stream, args);
 }
 
