@@ -642,48 +642,85 @@ struct CommitShared {
   int path[kMaxNodes];
 };
 
-// A lane's 8 keys of a row in step `step` (of 32), as two accumulators: which keys these are
-// keeps a wavefront's loads and stores in runs of 64 bytes of a row.  Half `half` holds four
-// keys from run `place`'s on, in runs of four (place: the lane group, or a quad's number
-// where the tile's 16 keys are an operand's rows).
+// A lane's row of a slice as eight accumulators of four keys: accumulator m holds run
+// `run(m, place)` of four (place: the lane group, or a quad's number where the tile's 16 keys
+// are an operand's rows).  Loads cover 64 bytes of a row each; for the stores the quads of
+// lanes that hold neighbouring rows exchange their runs, so that each store instruction covers
+// four rows of 256 bytes: of 256 states of 32 heads that alone takes 176 us, in runs of 64
+// bytes 196, or with the nontemporal hint 226.
 template <typename Pool>
-struct StateRow;
+struct StateRows;
 
 template <>
-struct StateRow<float> {
-  static __device__ __forceinline__ int run(int step, int half, int place) {
-    return 8 * step + 4 * half + place;
+struct StateRows<float> {
+  static __device__ __forceinline__ int run(int m, int place) { return 4 * m + place; }
+  static __device__ __forceinline__ void load(const float* slice, int r, int g, f32x4 (&x)[8]) {
+#pragma unroll
+    for (int m = 0; m < 8; ++m) {
+      x[m] = __builtin_nontemporal_load(
+          reinterpret_cast<const f32x4*>(slice + r * kDim + 4 * run(m, g)));
+    }
   }
-  static __device__ __forceinline__ void load(const float* row, int step, int g, f32x4& x,
-                                              f32x4& y) {
-    x = load4(row + 4 * run(step, 0, g));
-    y = load4(row + 4 * run(step, 1, g));
-  }
-  static __device__ __forceinline__ void store(float* row, int step, int g, const f32x4& x,
-                                               const f32x4& y) {
-    store_cells(row + 4 * run(step, 0, g), x);
-    store_cells(row + 4 * run(step, 1, g), y);
+  static __device__ __forceinline__ void store(float* slice, int lane, const f32x4 (&x)[8]) {
+    const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int m = 0; m < 8; m += 4) {
+      f32x4 row[4];  // of the quad's rows, run m + its place
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const f32x4 t = transpose_quad(
+            f32x4{x[m][c], x[m + 1][c], x[m + 2][c], x[m + 3][c]}, lane);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) row[i][c] = t[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        __builtin_nontemporal_store(
+            row[i], reinterpret_cast<f32x4*>(slice + ((r & 12) + i) * kDim +
+                                             4 * run(m + (r & 3), g)));
+      }
+    }
   }
 };
 
 template <>
-struct StateRow<bf16_bits> {
-  static __device__ __forceinline__ int run(int step, int half, int place) {
-    return 8 * step + 2 * place + half;
+struct StateRows<bf16_bits> {
+  static __device__ __forceinline__ int run(int m, int place) {
+    return 8 * (m >> 1) + 2 * place + (m & 1);
   }
-  static __device__ __forceinline__ void load(const bf16_bits* row, int step, int g, f32x4& x,
-                                              f32x4& y) {
-    float w[8];
-    load8(row + 4 * run(step, 0, g), w);
-    x = f32x4{w[0], w[1], w[2], w[3]};
-    y = f32x4{w[4], w[5], w[6], w[7]};
+  static __device__ __forceinline__ void load(const bf16_bits* slice, int r, int g,
+                                              f32x4 (&x)[8]) {
+#pragma unroll
+    for (int m = 0; m < 8; m += 2) {
+      float w[8];
+      widen8(stream_load(reinterpret_cast<const uint4*>(slice + r * kDim + 4 * run(m, g))), w);
+      x[m] = f32x4{w[0], w[1], w[2], w[3]};
+      x[m + 1] = f32x4{w[4], w[5], w[6], w[7]};
+    }
   }
   // The pool's own type: one rounding a path.
-  static __device__ __forceinline__ void store(bf16_bits* row, int step, int g, const f32x4& x,
-                                               const f32x4& y) {
-    *reinterpret_cast<uint4*>(row + 4 * run(step, 0, g)) =
-        make_uint4(bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]), bf16_pair(y[0], y[1]),
-                   bf16_pair(y[2], y[3]));
+  static __device__ __forceinline__ void store(bf16_bits* slice, int lane,
+                                               const f32x4 (&x)[8]) {
+    const int r = lane & 15, g = lane >> 4;
+    u32x4_t row[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {  // a word of each of a lane's four 16-byte pieces
+      f32x4 t;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const f32x4& of = x[2 * i + (c >> 1)];
+        t[i] = __uint_as_float(c & 1 ? bf16_pair(of[2], of[3]) : bf16_pair(of[0], of[1]));
+      }
+      t = transpose_quad(t, lane);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) row[i][c] = __float_as_uint(t[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      __builtin_nontemporal_store(
+          row[i], reinterpret_cast<u32x4_t*>(slice + ((r & 12) + i) * kDim +
+                                             4 * run(2 * (r & 3), g)));
+    }
   }
 };
 
@@ -700,7 +737,7 @@ __device__ __forceinline__ uint2 staged_run(const uint4* rows, int row, int run)
 // wavefront between one 16 and the next.
 template <typename Pool, int kWaves>
 __global__ __launch_bounds__(64 * kWaves) void commit_kernel(DraftArgs a) {
-  typedef StateRow<Pool> Row;
+  typedef StateRows<Pool> Rows;
   constexpr int kThreads = 64 * kWaves;
   constexpr int kPerHead = 8 / kWaves;
   constexpr int kPasses = kMaxNodes * 16 / kThreads;
@@ -730,11 +767,8 @@ __global__ __launch_bounds__(64 * kWaves) void commit_kernel(DraftArgs a) {
   Pool* const state = static_cast<Pool*>(a.pool) +
                       (static_cast<uint64_t>(slot) * a.value_heads + h) * kTile +
                       first_row * kDim;
-  f32x4 cells[4][2];
-#pragma unroll
-  for (int step = 0; step < 4; ++step) {
-    Row::load(state + r * kDim, step, g, cells[step][0], cells[step][1]);
-  }
+  f32x4 cells[8];
+  Rows::load(state, r, g, cells);
 
   if (parent >= lane) parent = -1;
   uint64_t on_path = 0;
@@ -833,10 +867,10 @@ __global__ __launch_bounds__(64 * kWaves) void commit_kernel(DraftArgs a) {
     f32x4 seen = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
-      const uint2 low = staged_run(s.k + 16 * at, r, Row::run(step, 0, g));
-      const uint2 high = staged_run(s.k + 16 * at, r, Row::run(step, 1, g));
+      const uint2 low = staged_run(s.k + 16 * at, r, Rows::run(2 * step, g));
+      const uint2 high = staged_run(s.k + 16 * at, r, Rows::run(2 * step + 1, g));
       uint4 part[3];
-      split3(cells[step][0], cells[step][1], part);
+      split3(cells[2 * step], cells[2 * step + 1], part);
       seen = mfma3(make_uint4(low.x, low.y, high.x, high.y), part, seen);
     }
     const f32x4 own = value_columns(v, lane);
@@ -864,24 +898,17 @@ __global__ __launch_bounds__(64 * kWaves) void commit_kernel(DraftArgs a) {
       split3_half(u, part);
     }
 #pragma unroll
-    for (int step = 0; step < 4; ++step) {
+    for (int m = 0; m < 8; ++m) {
+      // Four keys of four nodes, a node a lane of a quad, to a key a lane.
+      const uint2 key = transpose_quad(
+          staged_run(s.k + 16 * at, 4 * g + (r & 3), Rows::run(m, r >> 2)), lane);
+      f32x4 x = cells[m] * whole;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        // Four keys of four nodes, a node a lane of a quad, to a key a lane.
-        const uint2 key = transpose_quad(
-            staged_run(s.k + 16 * at, 4 * g + (r & 3), Row::run(step, half, r >> 2)), lane);
-        f32x4 x = cells[step][half] * whole;
-#pragma unroll
-        for (int p = 2; p >= 0; --p) x = mfma_half(key, part[p], x);
-        cells[step][half] = x;
-      }
+      for (int p = 2; p >= 0; --p) x = mfma_half(key, part[p], x);
+      cells[m] = x;
     }
   }
-
-#pragma unroll
-  for (int step = 0; step < 4; ++step) {
-    Row::store(state + r * kDim, step, g, cells[step][0], cells[step][1]);
-  }
+  Rows::store(state, lane, cells);
 }
 
 // ---------------------------------------------------------------------- launch
