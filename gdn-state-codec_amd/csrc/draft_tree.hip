@@ -634,10 +634,12 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
 
 struct CommitShared {
   uint4 k[kMaxNodes * 16];  // the path's, like all that follows
+  uint2 columns[kMaxNodes / 16][8][64];  // of k, a key a lane, for each 16 and accumulator
   Block inverse[kMaxNodes / 16];  // of each 16: -A^T, then N
   float k_square[kMaxNodes], k_unit[kMaxNodes];
+  // Factors of a node: -b exp(G) / |k| of S k, b, and what carries u to the end of its 16.
+  float seen[kMaxNodes], strength[kMaxNodes], weight[kMaxNodes];
   float sum[kMaxNodes], rest[kMaxNodes];  // G / ln 2 from the start of each 16
-  float strength[kMaxNodes];
   float log_decay[kMaxNodes];
   int path[kMaxNodes];
 };
@@ -842,7 +844,14 @@ __global__ __launch_bounds__(64 * kWaves) void commit_kernel(DraftArgs a) {
       kk = mfma(k, k, kk);
     }
     const float unit_c = a.normalize ? 1.0f / sqrtf(s.k_square[at + r] + kUnitEps) : 1.0f;
-    if (g == 0) s.k_unit[at + r] = unit_c;
+    if (g == 0) {
+      const int node = at + r, end = min(at + 15, length - 1);
+      const float decay = decay_between(s.sum[node], s.rest[node], 0.0f, 0.0f);
+      const float carry = decay_between(s.sum[end], s.rest[end], s.sum[node], s.rest[node]);
+      s.k_unit[node] = unit_c;
+      s.seen[node] = -s.strength[node] * (decay * unit_c);
+      s.weight[node] = node < length ? carry * unit_c : 0.0f;
+    }
     wave_sync();
     const f32x4 sum = load4(&s.sum[at + 4 * g]), rest = load4(&s.rest[at + 4 * g]);
     const f32x4 b = load4(&s.strength[at + 4 * g]), k_unit = load4(&s.k_unit[at + 4 * g]);
@@ -856,6 +865,13 @@ __global__ __launch_bounds__(64 * kWaves) void commit_kernel(DraftArgs a) {
     }
     wave_sync();
     invert(block, r, g == 0);
+  }
+  for (int m = wave; m < 8; m += kWaves) {
+    for (int at = 0; at < length; at += 16) {
+      // Four keys of four nodes, a node a lane of a quad, to a key a lane.
+      s.columns[at / 16][m][lane] = transpose_quad(
+          staged_run(s.k + 16 * at, 4 * g + (r & 3), Rows::run(m, r >> 2)), lane);
+    }
   }
   exchange();
 
@@ -877,31 +893,19 @@ __global__ __launch_bounds__(64 * kWaves) void commit_kernel(DraftArgs a) {
     if (at + 16 < length) v = value_of(at + 16);
 
     const int end = min(at + 15, length - 1);
-    const float end_sum = s.sum[end], end_rest = s.rest[end];
-    const float whole = decay_between(end_sum, end_rest, 0.0f, 0.0f);
+    const float whole = decay_between(s.sum[end], s.rest[end], 0.0f, 0.0f);
     uint2 part[3];  // u, weighted
     {
-      const f32x4 sum = load4(&s.sum[at + 4 * g]), rest = load4(&s.rest[at + 4 * g]);
-      const f32x4 b = load4(&s.strength[at + 4 * g]), k_unit = load4(&s.k_unit[at + 4 * g]);
+      const f32x4 see = load4(&s.seen[at + 4 * g]), b = load4(&s.strength[at + 4 * g]);
       f32x4 x;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float decay = decay_between(sum[c], rest[c], 0.0f, 0.0f);
-        x[c] = at + 4 * g + c < length ? b[c] * fmaf(-decay * k_unit[c], seen[c], own[c]) : 0.0f;
-      }
-      f32x4 u = block_product(s.inverse[at / 16].run(r, 4 * g), x, x);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float weight = decay_between(end_sum, end_rest, sum[c], rest[c]) * k_unit[c];
-        u[c] = at + 4 * g + c < length ? u[c] * weight : 0.0f;
-      }
-      split3_half(u, part);
+      for (int c = 0; c < 4; ++c) x[c] = fmaf(see[c], seen[c], b[c] * own[c]);
+      const f32x4 u = block_product(s.inverse[at / 16].run(r, 4 * g), x, x);
+      split3_half(u * load4(&s.weight[at + 4 * g]), part);
     }
 #pragma unroll
     for (int m = 0; m < 8; ++m) {
-      // Four keys of four nodes, a node a lane of a quad, to a key a lane.
-      const uint2 key = transpose_quad(
-          staged_run(s.k + 16 * at, 4 * g + (r & 3), Rows::run(m, r >> 2)), lane);
+      const uint2 key = s.columns[at / 16][m][lane];
       f32x4 x = cells[m] * whole;
 #pragma unroll
       for (int p = 2; p >= 0; --p) x = mfma_half(key, part[p], x);
