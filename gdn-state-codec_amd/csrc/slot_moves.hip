@@ -34,12 +34,13 @@ constexpr int kSaved = GDN_STATE_CODEC_MOVE_SAVED;
 constexpr int kPlanThreads = 1024;
 constexpr int kEach = kMaxPairs / kPlanThreads;
 constexpr int kHashed = 2 * kMaxPairs;
+constexpr uint64_t kLeftOut = 1ull << 62;  // a key of a pair that is left out, at least
 
 struct Plan {
   int32_t source[kMaxPairs];
   int32_t target[kMaxPairs];
   union {
-    int32_t hashed[kHashed];   // pairs by target, -1 free
+    int32_t hashed[kHashed];   // pairs by target, then by source; -1 free
     uint64_t key[kMaxPairs];   // pairs in their order
   };
   int32_t next[kMaxPairs];     // a pair 2^i steps on
@@ -47,24 +48,42 @@ struct Plan {
   int32_t lowest[kMaxPairs];   // of the pairs passed
   uint8_t flags[kMaxPairs];
   uint8_t on_cycle[kMaxPairs];
-  int chained, cycles;
+  int chained, cycles, shared;
 };
 
-__device__ __forceinline__ uint32_t hash_of(int32_t target) {
-  return (static_cast<uint32_t>(target) * 2654435761u) >> (32 - 13);
+__device__ __forceinline__ uint32_t hash_of(int32_t slot) {
+  return (static_cast<uint32_t>(slot) * 2654435761u) >> 16;
 }
-static_assert(kHashed == 1 << 13, "the hash gives 13 bits");
 
-// The pair that writes `slot`, or -1.
-__device__ __forceinline__ int writer_of(const Plan& p, int32_t slot) {
-  uint32_t at = hash_of(slot);
-  for (int probe = 0; probe < kHashed; ++probe) {
-    const int pair = p.hashed[at];
-    if (pair < 0) return -1;
-    if (p.target[pair] == slot) return pair;
-    at = (at + 1) & (kHashed - 1);
+// The place of `slot` in the table, whose pairs name their slot in `slots`, or of the free
+// place where it would be.  At least half of the table's places stay free.
+__device__ __forceinline__ uint32_t place_of(const int32_t* hashed, const int32_t* slots,
+                                             int32_t slot, uint32_t mask) {
+  uint32_t at = hash_of(slot) & mask;
+  while (hashed[at] >= 0 && slots[hashed[at]] != slot) at = (at + 1) & mask;
+  return at;
+}
+
+// Enters pair `pair` of `slot`; of the pairs of one slot the highest stays.
+__device__ __forceinline__ void enter(int32_t* hashed, const int32_t* slots, int32_t slot,
+                                      int32_t pair, uint32_t mask) {
+  uint32_t at = hash_of(slot) & mask;
+  while (true) {
+    const int before = atomicCAS(&hashed[at], -1, pair);
+    if (before < 0) return;
+    if (slots[before] == slot) {
+      atomicMax(&hashed[at], pair);
+      return;
+    }
+    at = (at + 1) & mask;
   }
-  return -1;
+}
+
+// LDS written by other lanes of the same wavefront is read after this.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
 }
 
 // next, steps and lowest after 2^rounds >= pairs steps, from one step.
@@ -73,7 +92,7 @@ __device__ __forceinline__ void follow(Plan& p, int pairs) {
     int32_t next[kEach], steps[kEach], lowest[kEach];
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
-      const int i = threadIdx.x + e * kPlanThreads;
+      const int i = threadIdx.x + e * blockDim.x;
       if (i >= pairs) break;
       const int n = p.next[i];
       next[e] = p.next[n];
@@ -83,7 +102,7 @@ __device__ __forceinline__ void follow(Plan& p, int pairs) {
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
-      const int i = threadIdx.x + e * kPlanThreads;
+      const int i = threadIdx.x + e * blockDim.x;
       if (i >= pairs) break;
       p.next[i] = next[e];
       p.steps[i] = steps[e];
@@ -93,14 +112,16 @@ __device__ __forceinline__ void follow(Plan& p, int pairs) {
   }
 }
 
+// `table`: places of the hash table, a power of two of at least 2 x pairs.
 __global__ __launch_bounds__(kPlanThreads) void slot_moves_kernel(
     const int32_t* __restrict__ sources, const int32_t* __restrict__ targets, int pairs,
-    uint32_t slots, int4* __restrict__ steps) {
+    uint32_t slots, uint32_t table, int4* __restrict__ steps) {
   __shared__ Plan p;
-  const int t = threadIdx.x;
-  for (int i = t; i < kHashed; i += kPlanThreads) p.hashed[i] = -1;
-  if (t == 0) p.chained = p.cycles = 0;
-  for (int i = t; i < pairs; i += kPlanThreads) {
+  const int t = threadIdx.x, threads = blockDim.x;
+  const uint32_t mask = table - 1;
+  for (uint32_t i = t; i < table; i += threads) p.hashed[i] = -1;
+  if (t == 0) p.chained = p.cycles = p.shared = 0;
+  for (int i = t; i < pairs; i += threads) {
     const int32_t source = sources[i], target = targets[i];
     const bool counts = static_cast<uint32_t>(target) < slots &&
                         (source == -1 || static_cast<uint32_t>(source) < slots);
@@ -109,32 +130,23 @@ __global__ __launch_bounds__(kPlanThreads) void slot_moves_kernel(
     p.flags[i] = p.on_cycle[i] = 0;
   }
   __syncthreads();
-  for (int i = t; i < pairs; i += kPlanThreads) {
-    const int32_t target = p.target[i];
-    if (target < 0) continue;
-    uint32_t at = hash_of(target);
-    while (true) {  // at most 4096 of 8192 places are ever taken
-      const int before = atomicCAS(&p.hashed[at], -1, i);
-      if (before < 0) break;
-      if (p.target[before] == target) {  // the last pair of a target counts
-        atomicMax(&p.hashed[at], i);
-        break;
-      }
-      at = (at + 1) & (kHashed - 1);
-    }
+  for (int i = t; i < pairs; i += threads) {
+    if (p.target[i] >= 0) enter(p.hashed, p.target, p.target[i], i, mask);
   }
   __syncthreads();
   bool live[kEach];
-  int after[kEach];
+  int after[kEach], reads[kEach];
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
-    const int i = t + e * kPlanThreads;
+    const int i = t + e * threads;
     live[e] = false;
-    after[e] = -1;
+    after[e] = reads[e] = -1;
     if (i >= pairs) break;
-    live[e] = p.target[i] >= 0 && writer_of(p, p.target[i]) == i;
+    // The last pair of a target counts.
+    live[e] = p.target[i] >= 0 &&
+              p.hashed[place_of(p.hashed, p.target, p.target[i], mask)] == i;
     if (live[e] && p.source[i] >= 0) {
-      after[e] = writer_of(p, p.source[i]);
+      after[e] = p.hashed[place_of(p.hashed, p.target, p.source[i], mask)];
       if (after[e] == i) after[e] = -1;  // onto itself
     }
     p.next[i] = after[e] >= 0 ? after[e] : i;
@@ -143,10 +155,29 @@ __global__ __launch_bounds__(kPlanThreads) void slot_moves_kernel(
     if (after[e] >= 0) p.chained = 1;
   }
   __syncthreads();
-  if (!p.chained) {  // no source is overwritten: any order will do
+  // Pairs of one source, which are put side by side: its last pair's number.
+  for (uint32_t i = t; i < table; i += threads) p.hashed[i] = -1;
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = t + e * threads;
+    if (i < pairs && live[e]) enter(p.hashed, p.source, p.source[i], i, mask);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = t + e * threads;
+    if (i >= pairs) break;
+    if (live[e]) {
+      reads[e] = p.hashed[place_of(p.hashed, p.source, p.source[i], mask)];
+      if (reads[e] != i) p.shared = 1;
+    }
+  }
+  __syncthreads();
+  if (!p.chained && !p.shared) {  // any order will do
 #pragma unroll
     for (int e = 0; e < kEach; ++e) {
-      const int i = t + e * kPlanThreads;
+      const int i = t + e * threads;
       if (i >= pairs) break;
       steps[i] = live[e] ? make_int4(p.source[i], p.target[i], 0, i + 1)
                          : make_int4(-1, -1, 0, i + 1);
@@ -154,80 +185,91 @@ __global__ __launch_bounds__(kPlanThreads) void slot_moves_kernel(
     return;
   }
 
-  follow(p, pairs);
-  // Whoever has not come to an end is on a cycle now, and every pair of a cycle is
-  // reached by one of its own.
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    const int i = t + e * kPlanThreads;
-    if (i >= pairs) break;
-    // An end is its own successor; 2^rounds >= pairs real steps are taken only on cycles.
-    if (p.steps[i] >= pairs) {
-      p.on_cycle[p.next[i]] = 1;
-      p.cycles = 1;
-    }
-  }
-  __syncthreads();
-  if (p.cycles) {
-    int head[kEach];
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const int i = t + e * kPlanThreads;
-      head[e] = i < pairs && p.on_cycle[i] ? p.lowest[i] : -1;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) {
-      const int i = t + e * kPlanThreads;
-      if (i >= pairs) break;
-      if (head[e] == i) p.flags[i] |= kSaves;
-      if (head[e] >= 0 && after[e] == head[e]) {
-        p.flags[i] |= kSaved;
-        after[e] = -1;
-      }
-      p.next[i] = after[e] >= 0 ? after[e] : i;
-      p.steps[i] = after[e] >= 0 ? 1 : 0;
-    }
-    __syncthreads();
+  if (p.chained) {
     follow(p, pairs);
+    // An end is its own successor; 2^rounds >= pairs real steps are taken only on cycles,
+    // and every pair of a cycle is reached by one of its own.
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) {
+      const int i = t + e * threads;
+      if (i >= pairs) break;
+      if (p.steps[i] >= pairs) {
+        p.on_cycle[p.next[i]] = 1;
+        p.cycles = 1;
+      }
+    }
+    __syncthreads();
+    if (p.cycles) {
+      int head[kEach];
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int i = t + e * threads;
+        head[e] = i < pairs && p.on_cycle[i] ? p.lowest[i] : -1;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int i = t + e * threads;
+        if (i >= pairs) break;
+        if (head[e] == i) p.flags[i] |= kSaves;
+        if (head[e] >= 0 && after[e] == head[e]) {
+          p.flags[i] |= kSaved;
+          after[e] = -1;
+        }
+        p.next[i] = after[e] >= 0 ? after[e] : i;
+        p.steps[i] = after[e] >= 0 ? 1 : 0;
+      }
+      __syncthreads();
+      follow(p, pairs);
+    }
   }
 
-  // Order by tree (the pair at its end; what is left out last), then by falling distance.
+  // Order by what a tree's end reads, by tree (the pair at its end; what is left out last)
+  // and by falling distance.  `lowest` takes what each pair reads.
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = t + e * threads;
+    if (i < pairs) p.lowest[i] = reads[e];
+  }
+  __syncthreads();
   int size = 1;
   while (size < pairs) size <<= 1;
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
-    const int i = t + e * kPlanThreads;
+    const int i = t + e * threads;
     if (i >= size) break;
     uint64_t key = ~0ull;
     if (i < pairs) {
-      const uint64_t tree = live[e] ? p.next[i] : kMaxPairs;
-      const uint64_t away = live[e] ? kMaxPairs - p.steps[i] : 0;
-      key = tree << 32 | away << 16 | i;
+      const uint64_t end = p.next[i];
+      key = live[e] ? static_cast<uint64_t>(p.lowest[end]) << 48 | end << 32 |
+                          static_cast<uint64_t>(kMaxPairs - p.steps[i]) << 16 | i
+                    : kLeftOut | i;
     }
     p.key[i] = key;
   }
   __syncthreads();
+  // A wavefront's 64 comparisons over gaps of up to 64 are of its own 128 keys: only wider
+  // ones, and the step after them, wait for the other wavefronts.
   for (int run = 2; run <= size; run <<= 1) {
     for (int gap = run >> 1; gap > 0; gap >>= 1) {
-      for (int i = t; i < size; i += kPlanThreads) {
-        const int other = i ^ gap;
-        if (other > i) {
-          const uint64_t x = p.key[i], y = p.key[other];
-          if ((x > y) == ((i & run) == 0)) {
-            p.key[i] = y;
-            p.key[other] = x;
-          }
+      for (int pair = t; pair < size / 2; pair += threads) {
+        const int i = 2 * pair - (pair & (gap - 1)), other = i + gap;
+        const uint64_t x = p.key[i], y = p.key[other];
+        if ((x > y) == ((i & run) == 0)) {
+          p.key[i] = y;
+          p.key[other] = x;
         }
       }
-      __syncthreads();
+      if (gap > 64 || (gap == 1 && run >= 128)) __syncthreads();
+      else wave_sync();
     }
   }
-  for (int place = t; place < pairs; place += kPlanThreads) {
+  __syncthreads();
+  for (int place = t; place < pairs; place += threads) {
     const uint64_t key = p.key[place];
     const int i = static_cast<int>(key & 0xFFFF);
     const uint32_t tree = static_cast<uint32_t>(key >> 32);
-    if (tree == kMaxPairs) {
+    if (key >= kLeftOut) {
       steps[place] = make_int4(-1, -1, 0, place + 1);
       continue;
     }
@@ -312,9 +354,10 @@ __global__ __launch_bounds__(kPlanThreads) void compaction_kernel(
 // ------------------------------------------------------------------- copies
 
 constexpr int kCopyThreads = 256;
-constexpr int kBatch = 8;         // rows whose loads are all asked for before the first store
+constexpr int kBatch = 4;         // rows whose loads are all asked for before the first store
+constexpr int kFewBuffers = 9;    // of a launch with a small argument block (2 us less of a call)
 constexpr int kMostBuffers = 64;  // of one launch
-constexpr uint32_t kFill = 8 * kComputeUnits;  // workgroups that fill the card
+constexpr uint32_t kFill = 32 * kComputeUnits;  // workgroups that fill the card
 
 struct CopyBuffer {
   const char* from;
@@ -324,8 +367,9 @@ struct CopyBuffer {
   uint32_t unit;        // bytes a thread: 16, 4 or 1
 };
 
+template <int kMost>
 struct CopyArgs {
-  CopyBuffer buffers[kMostBuffers];
+  CopyBuffer buffers[kMost];
   const int4* steps;
   uint32_t count, rows, slots;
 };
@@ -350,8 +394,7 @@ __device__ __forceinline__ void copy_rows(const CopyBuffer& b, uint64_t at, cons
     for (int i = 0; i < kBatch; ++i) {
       x[i] = Unit{};
       if (row[i].y >= 0 && static_cast<uint32_t>(row[i].x) < slots && !(row[i].z & kSaved)) {
-        x[i] = __builtin_nontemporal_load(
-            reinterpret_cast<const Unit*>(from + row[i].x * b.bytes));
+        x[i] = *reinterpret_cast<const Unit*>(from + row[i].x * b.bytes);
       }
       if (row[i].y >= 0 && (row[i].z & kSaves)) {
         kept = *reinterpret_cast<const Unit*>(from + row[i].y * b.bytes);
@@ -375,7 +418,8 @@ __device__ __forceinline__ uint32_t part_begin(const int4* steps, uint32_t rows,
   return min(max(static_cast<uint32_t>(steps[at - 1].w), at), rows);
 }
 
-__global__ __launch_bounds__(kCopyThreads) void copy_slots_kernel(CopyArgs a) {
+template <int kMost>
+__global__ __launch_bounds__(kCopyThreads) void copy_slots_kernel(CopyArgs<kMost> a) {
   uint32_t i = 0;
   while (i + 1 < a.count && a.buffers[i + 1].first <= blockIdx.x) ++i;
   const CopyBuffer b = a.buffers[i];
@@ -388,6 +432,39 @@ __global__ __launch_bounds__(kCopyThreads) void copy_slots_kernel(CopyArgs a) {
   else copy_rows<uint8_t>(b, at, a.steps, begin, end, a.slots);
 }
 
+// Bytes a thread copies of a slot: what the addresses and sizes of a buffer are multiples of.
+uint32_t unit_of(const gdn_state_codec_slot_buffer& b) {
+  const uint64_t bits =
+      reinterpret_cast<uintptr_t>(b.from) | reinterpret_cast<uintptr_t>(b.to) | b.bytes;
+  return bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
+}
+uint64_t workgroups_of(const gdn_state_codec_slot_buffer& b) {
+  const uint64_t run = static_cast<uint64_t>(unit_of(b)) * kCopyThreads;
+  return (b.bytes + run - 1) / run;
+}
+
+template <int kMost>
+int32_t launch_copy(void* stream, const gdn_state_codec_slot_buffer* buffers, uint32_t count,
+                    const int32_t* steps, uint32_t rows, uint32_t slots) {
+  CopyArgs<kMost> args;
+  args.steps = reinterpret_cast<const int4*>(steps);
+  args.count = count;
+  args.rows = rows;
+  args.slots = slots;
+  uint64_t blocks = 0;
+  for (uint32_t i = 0; i < count; ++i) {
+    const gdn_state_codec_slot_buffer& b = buffers[i];
+    args.buffers[i] = {static_cast<const char*>(b.from), static_cast<char*>(b.to), b.bytes,
+                       static_cast<uint32_t>(blocks), unit_of(b)};
+    blocks += workgroups_of(b);
+  }
+  uint64_t parts = (kFill + blocks - 1) / blocks;
+  if (parts > rows) parts = rows;
+  return launch(copy_slots_kernel<kMost>,
+                dim3(static_cast<uint32_t>(blocks), static_cast<uint32_t>(parts)),
+                dim3(kCopyThreads), stream, args);
+}
+
 }  // namespace
 }  // namespace gdn
 
@@ -398,8 +475,11 @@ extern "C" int32_t statecentric_gdn_state_codec_slot_moves_launch_v1(
       slots == 0 || slots > 0x7FFFFFFFu || !gdn::aligned16(sources, targets, steps)) {
     return gdn::kStatusInvalidArgument;
   }
-  return gdn::launch(gdn::slot_moves_kernel, dim3(1), dim3(gdn::kPlanThreads), stream, sources,
-                     targets, static_cast<int>(pairs), slots, reinterpret_cast<int4*>(steps));
+  uint32_t table = 2, threads = (pairs + 63) / 64 * 64;
+  while (table < 2 * pairs) table *= 2;
+  if (threads > gdn::kPlanThreads) threads = gdn::kPlanThreads;
+  return gdn::launch(gdn::slot_moves_kernel, dim3(1), dim3(threads), stream, sources, targets,
+                     static_cast<int>(pairs), slots, table, reinterpret_cast<int4*>(steps));
 }
 
 extern "C" int32_t statecentric_gdn_state_codec_compaction_moves_launch_v1(
@@ -420,37 +500,24 @@ extern "C" int32_t statecentric_gdn_state_codec_copy_slots_launch_v1(
       slots > 0x7FFFFFFFu || !gdn::aligned16(steps)) {
     return gdn::kStatusInvalidArgument;
   }
+  // Every buffer's size fits an address, and every launch's threads its grid.
+  uint64_t blocks = 0;
   for (uint32_t i = 0; i < count; ++i) {
     const uint64_t bytes = buffers[i].bytes;
-    // A buffer's size has to fit an address.
-    if (!buffers[i].from || !buffers[i].to || bytes == 0 || bytes > (1ull << 47) / slots ||
-        (bytes + 15) / 16 / gdn::kCopyThreads + 1 > gdn::kMaxGrid / gdn::kMostBuffers / 16) {
+    if (!buffers[i].from || !buffers[i].to || bytes == 0 || bytes > (1ull << 47) / slots) {
       return gdn::kStatusInvalidArgument;
     }
+    if (i % gdn::kMostBuffers == 0) blocks = 0;
+    blocks += gdn::workgroups_of(buffers[i]);
+    if (blocks > gdn::kMaxGrid / gdn::kCopyThreads) return gdn::kStatusInvalidArgument;
   }
   for (uint32_t done = 0; done < count; done += gdn::kMostBuffers) {
-    gdn::CopyArgs args;
-    args.steps = reinterpret_cast<const int4*>(steps);
-    args.count = count - done < gdn::kMostBuffers ? count - done : gdn::kMostBuffers;
-    args.rows = rows;
-    args.slots = slots;
-    uint64_t blocks = 0;
-    for (uint32_t i = 0; i < args.count; ++i) {
-      const gdn_state_codec_slot_buffer& b = buffers[done + i];
-      const uint64_t bits = reinterpret_cast<uintptr_t>(b.from) |
-                            reinterpret_cast<uintptr_t>(b.to) | b.bytes;
-      const uint32_t unit = bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : 1;
-      args.buffers[i] = {static_cast<const char*>(b.from), static_cast<char*>(b.to), b.bytes,
-                         static_cast<uint32_t>(blocks), unit};
-      const uint64_t run = static_cast<uint64_t>(unit) * gdn::kCopyThreads;
-      blocks += (b.bytes + run - 1) / run;
-    }
-    uint64_t parts = (gdn::kFill + blocks - 1) / blocks;
-    if (parts > rows) parts = rows;
+    const uint32_t some = count - done < gdn::kMostBuffers ? count - done : gdn::kMostBuffers;
     const int32_t status =
-        gdn::launch(gdn::copy_slots_kernel,
-                    dim3(static_cast<uint32_t>(blocks), static_cast<uint32_t>(parts)),
-                    dim3(gdn::kCopyThreads), stream, args);
+        some <= gdn::kFewBuffers
+            ? gdn::launch_copy<gdn::kFewBuffers>(stream, buffers + done, some, steps, rows, slots)
+            : gdn::launch_copy<gdn::kMostBuffers>(stream, buffers + done, some, steps, rows,
+                                                  slots);
     if (status != gdn::kStatusOk) return status;
   }
   return gdn::kStatusOk;

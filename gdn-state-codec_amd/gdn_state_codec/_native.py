@@ -47,12 +47,6 @@ class DraftsStruct(ctypes.Structure):
         + [("scale", _F), ("normalize", _U32)])
 
 
-class SlotBufferStruct(ctypes.Structure):
-    """``gdn_state_codec_slot_buffer`` (include/gdn_state_codec_slots.h)."""
-
-    _fields_ = [("source", _P), ("to", _P), ("bytes", _U64)]
-
-
 # name -> argtypes (all return int32 status)
 SIGNATURES: dict[str, list] = {
     # codec, reference entry points

@@ -10,11 +10,12 @@ slots go where stays on the device, and nothing here waits for the GPU.  Checks 
 
 from __future__ import annotations
 
+import ctypes
 from typing import NamedTuple, Sequence
 
 import torch
 
-from ._native import SlotBufferStruct, native
+from ._native import native
 from .layer import _dense, _fail, _launched, _not_differentiated, _on_device, _stream
 
 MAX_MOVES = 4096
@@ -101,6 +102,7 @@ def copy_slots(buffers: torch.Tensor | Sequence[torch.Tensor], moves: SlotMoves,
         _fail("slot moves must be [rows,4]")
     _dense(steps, "slot moves", (steps.shape[0], 4), torch.int32)
     held = []
+    fields = []  # of gdn_state_codec_slot_buffer, one after another
     for i, t in enumerate(buffers):
         if t.dim() < 1 or t.shape[0] != slots or not t.is_contiguous():
             _fail(f"slot buffers must be contiguous [{slots},...], got {tuple(t.shape)} with "
@@ -110,18 +112,17 @@ def copy_slots(buffers: torch.Tensor | Sequence[torch.Tensor], moves: SlotMoves,
         if into is not None:
             to = into[i]
             _dense(to, "slot buffer to copy into", t.shape, t.dtype)
-        if t.numel():
+        size = t.numel()
+        if size:
             held.append((t, to))
+            fields += (t.data_ptr(), to.data_ptr(), size // slots * t.element_size())
     _not_differentiated("copying slots", *buffers, *(into or ()))
     if not held:
         return
-    if into is None:
-        if len(held) > 1:
-            _apart(t for t, _ in held)
-    else:
+    if into is not None:
         _apart([to for _, to in held] + list({t.data_ptr(): t for t, _ in held}.values()))
-    rows = (SlotBufferStruct * len(held))(*(
-        (t.data_ptr(), to.data_ptr(), t.numel() // slots * t.element_size())
-        for t, to in held))
+    elif len(held) > 1:
+        _apart(t for t, _ in held)
     _launched(native().copy_slots_launch_v1(
-        _stream(), rows, len(held), steps.data_ptr(), steps.shape[0], slots), "copy slots")
+        _stream(), (ctypes.c_uint64 * len(fields))(*fields), len(held), steps.data_ptr(),
+        steps.shape[0], slots), "copy slots")

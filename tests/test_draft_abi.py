@@ -11,7 +11,7 @@ import torch
 
 import gdn_state_codec as gdn
 from gdn_state_codec import _native, layer, slots
-from gdn_state_codec._native import DraftsStruct, SlotBufferStruct
+from gdn_state_codec._native import DraftsStruct
 
 P = ctypes.c_void_p(1 << 20)  # 16-byte aligned, never dereferenced
 OFF = ctypes.c_void_p((1 << 20) + 4)
@@ -52,7 +52,9 @@ def test_drafts_admission(lib, entry):
     for bad in (dict(requests=0), dict(requests=4097), dict(value_heads=3), dict(key_heads=0),
                 dict(value_heads=0), dict(normalize=2), dict(max_nodes=0), dict(max_nodes=65),
                 dict(query_stride=252), dict(key_stride=4), dict(value_stride=513),
-                dict(tokens=1 << 31), dict(value_heads=1 << 30, requests=4096, key_heads=1)):
+                dict(key_stride=(1 << 24) + 8), dict(value_stride=(1 << 24) + 8),
+                dict(query_stride=(1 << 24) + 8), dict(value_heads=(1 << 17) + 1, key_heads=1),
+                dict(tokens=1 << 31), dict(value_heads=1 << 17, requests=4096, key_heads=1)):
         assert call(drafts(**{**given, **bad})) == 1, bad
     for bad in (dict(pool=None), dict(pool=OFF), dict(slots=0), dict(slots=1 << 31),
                 dict(dtype=2), dict(last=None), dict(last=OFF)):
@@ -92,7 +94,8 @@ def test_moves_admission(lib):
 
 def test_copy_admission(lib):
     def copy(buffers=((1 << 20, 1 << 20, 64),), count=None, steps=P, rows=3, slots=9):
-        held = (SlotBufferStruct * max(1, len(buffers)))(*buffers)
+        flat = [x or 0 for buffer in buffers for x in buffer]
+        held = (ctypes.c_uint64 * max(3, len(flat)))(*flat)
         count = len(buffers) if count is None else count
         return lib.copy_slots_launch_v1(None, held, count, steps, rows, slots)
 
@@ -102,7 +105,10 @@ def test_copy_admission(lib):
                 dict(buffers=((None, 1 << 20, 64),)), dict(buffers=((1 << 20, None, 64),)),
                 dict(buffers=((1 << 20, 1 << 20, 0),)),
                 dict(buffers=((1 << 20, 1 << 20, 64), (1 << 20, 1 << 20, 0))),
-                dict(buffers=((1 << 20, 1 << 20, 1 << 46),))):
+                dict(buffers=((1 << 20, 1 << 20, 1 << 46),)),
+                dict(buffers=((1 << 20, 1 << 20, (1 << 31) + 1),), slots=1),
+                dict(buffers=((1 << 20, 1 << 20, 16),) * 64 + ((1 << 20, 1 << 20, 1 << 36),),
+                     slots=1)):
         assert copy(**bad) == 1, bad
 
 
@@ -172,12 +178,10 @@ def test_what_copies_are_launched_with(calls):
     gdn.copy_slots([a, b, torch.zeros(6, 0)], moves)
     args = calls[1][1]
     assert args[2:] == (2, moves.steps.data_ptr(), 4, 6)
-    assert [(x.source, x.to, x.bytes) for x in args[1]] == [
-        (a.data_ptr(), a.data_ptr(), 3), (b.data_ptr(), b.data_ptr(), 40)]
+    assert list(args[1]) == [a.data_ptr(), a.data_ptr(), 3, b.data_ptr(), b.data_ptr(), 40]
     into = torch.ones_like(b)
     gdn.copy_slots(b, moves, into=into)
-    assert [(x.source, x.to, x.bytes) for x in calls[2][1][1]] == [
-        (b.data_ptr(), into.data_ptr(), 40)]
+    assert list(calls[2][1][1]) == [b.data_ptr(), into.data_ptr(), 40]
     gdn.copy_slots([b, b], moves, into=[into, torch.ones_like(b)])  # one source, two copies
     for bad in (([b, b], moves), (b, moves, b), (b[:5], moves), ([], moves),
                 ([b, b], moves, [into, into]), (b, moves, into[:, :1])):
