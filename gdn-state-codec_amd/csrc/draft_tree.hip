@@ -36,6 +36,12 @@ namespace gdn {
 namespace {
 
 constexpr int kMaxNodes = GDN_STATE_CODEC_MAX_NODES;
+// A workgroup takes one head of one request, a wavefront 16 rows of its state.  (With two
+// wavefronts a workgroup, so four a head, one request's 32 heads are no faster: 6.8 us for a
+// tree of 16 nodes either way, 8 requests' 13.9 against 8.1.)
+constexpr int kWaves = 8;
+constexpr int kThreads = 64 * kWaves;
+static_assert(16 * kWaves == kDim, "a workgroup takes a whole head");
 constexpr double kInverseLn2 = 1.4426950408889634074;
 // exp of less is 0 in fp32; sums of it stay far from what fp64 cannot tell apart.
 constexpr double kLeastLogDecay = -200.0;
@@ -341,25 +347,19 @@ __device__ __forceinline__ const void* row_at(const bf16_bits* base, uint32_t ro
   return reinterpret_cast<const char*>(base) + (row * step + offset) * 2u;
 }
 
-// A workgroup takes kWaves x kSlices slices of 16 rows of one head's state.  The first
-// wavefront forms the tables and inverts, the others form the nodes' products; the
+// The first wavefront forms the tables and inverts, the others form the nodes' products; the
 // state's are between, wherever a wavefront would wait.
-template <typename Pool, int kTiles, int kSlices, int kWaves>
-__global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
-  constexpr int kThreads = 64 * kWaves;
-  constexpr int kPerHead = 8 / (kSlices * kWaves);
-  constexpr int kRows = 16 * kSlices * kWaves;  // of the state
+template <typename Pool, int kTiles>
+__global__ __launch_bounds__(kThreads) void tree_kernel(DraftArgs a) {
   constexpr int kNodes = 16 * kTiles;
   constexpr int kPasses = 2 * kNodes * 16 / kThreads;
   constexpr int kBlocks = blocks_of(kTiles);
   constexpr int kPairs = (kBlocks + kWaves - 2) / (kWaves - 1);
-  static_assert(kWaves >= 2 && 2 * kNodes * 16 % kThreads == 0, "the roles above");
   __shared__ TreeShared<kTiles> s;
 
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t item = static_cast<uint32_t>(xcd_contiguous_item(blockIdx.x, gridDim.x));
-  const uint32_t head = item / kPerHead;
+  const uint32_t head = static_cast<uint32_t>(xcd_contiguous_item(blockIdx.x, gridDim.x));
   const uint32_t n = head / a.value_heads, h = head % a.value_heads, hk = h / a.group;
   int32_t slot;
   uint64_t begin;
@@ -394,8 +394,8 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
           row_at(query ? queries : keys, row, query ? query_step : key_step, 8 * piece));
     }
   }
-  const int first_row = 16 * kSlices * static_cast<int>((item % kPerHead) * kWaves + wave);
-  uint2 v[kSlices][kTiles];
+  const int first_row = 16 * wave;
+  uint2 v[kTiles];
   {
     const bf16_bits* const values = a.values + begin * a.value_stride + h * kDim + first_row;
     const uint32_t step = static_cast<uint32_t>(a.value_stride);
@@ -403,27 +403,18 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
     for (int i = 0; i < kTiles; ++i) {
       if (i < tiles) {
         const uint32_t row = min(16 * i + 4 * g + (r & 3), nodes - 1);
-#pragma unroll
-        for (int slice = 0; slice < kSlices; ++slice) {
-          v[slice][i] = *static_cast<const uint2*>(
-              row_at(values, row, step, 16 * slice + (r & 12)));
-        }
+        v[i] = *static_cast<const uint2*>(row_at(values, row, step, r & 12));
       }
     }
   }
-  Cells<Pool> cells[kSlices][4];
+  Cells<Pool> cells[4];
   {
     const Pool* const state = static_cast<const Pool*>(a.pool) +
                               (static_cast<uint64_t>(slot) * a.value_heads + h) * kTile +
                               first_row * kDim;
     const uint32_t place = r * kDim + 8 * g;
 #pragma unroll
-    for (int slice = 0; slice < kSlices; ++slice) {
-#pragma unroll
-      for (int step = 0; step < 4; ++step) {
-        cells[slice][step].load(state + (place + 16 * slice * kDim + 32 * step));
-      }
-    }
+    for (int step = 0; step < 4; ++step) cells[step].load(state + (place + 32 * step));
   }
 
   Path path;
@@ -440,29 +431,22 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
   }
   exchange();
 
-  f32x4 seen[kSlices][kTiles], read[kSlices][kTiles];  // S0 K^T and S0 Q^T, a token a row
+  f32x4 seen[kTiles], read[kTiles];  // S0 K^T and S0 Q^T, a token a row
   auto state_products = [&]() {
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int slice = 0; slice < kSlices; ++slice) {
-#pragma unroll
-      for (int i = 0; i < kTiles; ++i) seen[slice][i] = read[slice][i] = zero;
-    }
+    for (int i = 0; i < kTiles; ++i) seen[i] = read[i] = zero;
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
-      uint4 part[kSlices][Cells<Pool>::kParts];
-#pragma unroll
-      for (int slice = 0; slice < kSlices; ++slice) cells[slice][step].parts(part[slice]);
+      uint4 part[Cells<Pool>::kParts];
+      cells[step].parts(part);
       const uint4* const k = &staged(s.k, r, 4 * step + g);
       const uint4* const q = &staged(s.q, r, 4 * step + g);
 #pragma unroll
       for (int i = 0; i < kTiles; ++i) {
         if (i < tiles) {
-#pragma unroll
-          for (int slice = 0; slice < kSlices; ++slice) {
-            seen[slice][i] = product(k[256 * i], part[slice], seen[slice][i]);
-            read[slice][i] = product(q[256 * i], part[slice], read[slice][i]);
-          }
+          seen[i] = product(k[256 * i], part, seen[i]);
+          read[i] = product(q[256 * i], part, read[i]);
         }
       }
     }
@@ -543,87 +527,73 @@ __global__ __launch_bounds__(64 * kWaves) void tree_kernel(DraftArgs a) {
   }
 
   const uint64_t bad_outputs = static_cast<uint64_t>(s.bad_output[1]) << 32 | s.bad_output[0];
-  uint64_t bad[kSlices];  // nodes that are bad, or whose r is in this column
-#pragma unroll
-  for (int slice = 0; slice < kSlices; ++slice) {
-    bad[slice] = static_cast<uint64_t>(s.bad_node[1]) << 32 | s.bad_node[0];
-  }
-  Pair u[kSlices][(kTiles + 1) / 2];
+  // Nodes that are bad, or whose r is in this column.
+  uint64_t bad = static_cast<uint64_t>(s.bad_node[1]) << 32 | s.bad_node[0];
+  Pair u[(kTiles + 1) / 2];
 #pragma unroll
   for (int i = 0; i < kTiles; ++i) {
     if (i >= tiles) break;
     const int first = 16 * i + 4 * g;
     const f32x4 see = load4(&s.seen[first]), look = load4(&s.look[first]);
     const f32x4 b = load4(&s.strength[first]);
-    f32x4 x[kSlices], out[kSlices];
+    const f32x4 values = value_columns(v[i], lane);
+    f32x4 x, out;
+    float worst = 0.0f;
 #pragma unroll
-    for (int slice = 0; slice < kSlices; ++slice) {
-      const f32x4 values = value_columns(v[slice][i], lane);
-      float worst = 0.0f;
+    for (int c = 0; c < 4; ++c) {
+      x[c] = fmaf(see[c], seen[i][c], b[c] * values[c]);
+      out[c] = look[c] * read[i][c];
+      worst = fmaf(x[c], 0.0f, worst);
+    }
+    if (__any(worst != 0.0f)) {
+      uint64_t column = 0;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        x[slice][c] = fmaf(see[c], seen[slice][i][c], b[c] * values[c]);
-        out[slice][c] = look[c] * read[slice][i][c];
-        worst = fmaf(x[slice][c], 0.0f, worst);
+        if (!finite(x[c])) column |= 1ull << (first + c), x[c] = 0.0f;
       }
-      if (__any(worst != 0.0f)) {
-        uint64_t column = 0;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          if (!finite(x[slice][c])) column |= 1ull << (first + c), x[slice][c] = 0.0f;
-        }
-        column |= __shfl_xor(column, 16);
-        column |= __shfl_xor(column, 32);
-        bad[slice] |= column;
-      }
+      column |= __shfl_xor(column, 16);
+      column |= __shfl_xor(column, 32);
+      bad |= column;
     }
-    const f32x4 inverse = s.inverse[i].run(r, 4 * g);
 #pragma unroll
-    for (int slice = 0; slice < kSlices; ++slice) {
+    for (int j = 0; j < i; j += 2) {
+      const uint2* const step = s.step + step_at(i, j);
+      x = j + 1 < i ? add_pair(step, lane, u[j / 2], x) : add_single(step, lane, u[j / 2], x);
+    }
+    uint2 part[3];
+    split3_half(block_product(s.inverse[i].run(r, 4 * g), x, x), part);
 #pragma unroll
-      for (int j = 0; j < i; j += 2) {
-        const uint2* const step = s.step + step_at(i, j);
-        x[slice] = j + 1 < i ? add_pair(step, lane, u[slice][j / 2], x[slice])
-                             : add_single(step, lane, u[slice][j / 2], x[slice]);
-      }
-      uint2 part[3];
-      split3_half(block_product(inverse, x[slice], x[slice]), part);
+    for (int p = 0; p < 3; ++p) {
+      uint4& whole = u[i / 2][p];
+      if (i % 2 == 0) whole.x = part[p].x, whole.y = part[p].y;
+      else whole.z = part[p].x, whole.w = part[p].y;
+    }
 #pragma unroll
-      for (int p = 0; p < 3; ++p) {
-        uint4& whole = u[slice][i / 2][p];
-        if (i % 2 == 0) whole.x = part[p].x, whole.y = part[p].y;
-        else whole.z = part[p].x, whole.w = part[p].y;
-      }
-      f32x4 y = out[slice];
+    for (int j = 0; j <= i; j += 2) {
+      const uint2* const looked = s.read + read_at(i, j);
+      out = j + 1 <= i ? add_pair(looked, lane, u[j / 2], out)
+                       : add_single(looked, lane, u[j / 2], out);
+    }
+    if (__any(bad != 0) || bad_outputs != 0) {
 #pragma unroll
-      for (int j = 0; j <= i; j += 2) {
-        const uint2* const looked = s.read + read_at(i, j);
-        y = j + 1 <= i ? add_pair(looked, lane, u[slice][j / 2], y)
-                       : add_single(looked, lane, u[slice][j / 2], y);
-      }
-      if (__any(bad[slice] != 0) || bad_outputs != 0) {
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint64_t self = 1ull << (first + c);
-          if ((bad[slice] & (s.above[first + c] | self)) | (bad_outputs & self)) {
-            y[c] = __uint_as_float(0x7FC00000u);
-          }
+      for (int c = 0; c < 4; ++c) {
+        const uint64_t self = 1ull << (first + c);
+        if ((bad & (s.above[first + c] | self)) | (bad_outputs & self)) {
+          out[c] = __uint_as_float(0x7FC00000u);
         }
       }
-      // A node's outputs side by side, in pieces of 16 bytes as the keys were.
-      const uint2 packed = transpose_quad(
-          make_uint2(bf16_pair(y[0], y[1]), bf16_pair(y[2], y[3])), lane);
-      const int node = first + (r & 3);
-      const int at = 2 * (kSlices * wave + slice) + (r >> 3);  // piece
-      reinterpret_cast<uint2*>(&s.out[16 * node + (at ^ (node & 15))])[r >> 2 & 1] = packed;
     }
+    // A node's outputs side by side, in pieces of 16 bytes as the keys were.
+    const uint2 packed = transpose_quad(
+        make_uint2(bf16_pair(out[0], out[1]), bf16_pair(out[2], out[3])), lane);
+    const int node = first + (r & 3);
+    const int at = 2 * wave + (r >> 3);  // piece
+    reinterpret_cast<uint2*>(&s.out[16 * node + (at ^ (node & 15))])[r >> 2 & 1] = packed;
   }
   exchange();
-  constexpr int kOutPieces = kRows / 8;
-  bf16_bits* const outputs = a.outputs + (begin * a.value_heads + h) * kDim +
-                             static_cast<int>(item % kPerHead) * kRows;
-  for (int p = threadIdx.x; p < nodes * kOutPieces; p += kThreads) {
-    const int node = p / kOutPieces, at = p % kOutPieces;
+  bf16_bits* const outputs = a.outputs + (begin * a.value_heads + h) * kDim;
+  for (int p = threadIdx.x; p < 16 * nodes; p += kThreads) {
+    const int node = p >> 4, at = p & 15;
     *reinterpret_cast<uint4*>(reinterpret_cast<char*>(outputs) +
                               (node * a.value_heads * kDim + 8 * at) * 2u) =
         s.out[16 * node + (at ^ (node & 15))];
@@ -732,23 +702,19 @@ __device__ __forceinline__ uint2 staged_run(const uint4* rows, int row, int run)
                                               (run & 1)];
 }
 
-// A workgroup takes kWaves slices of 16 rows of one head's state, which stay in registers
-// while the path's nodes are applied 16 at a time, both as the products' operand and as the
-// update's accumulators.  What depends on no state (the path, its keys in LDS, A's inverse
+// A wavefront's 16 rows of the state stay in registers while the path's nodes are applied 16
+// at a time, both as the products' operand and as the update's accumulators.  What depends on no state (the path, its keys in LDS, A's inverse
 // for each 16, by a wavefront each) comes first, so that nothing waits for another
 // wavefront between one 16 and the next.
-template <typename Pool, int kWaves>
-__global__ __launch_bounds__(64 * kWaves) void commit_kernel(DraftArgs a) {
+template <typename Pool>
+__global__ __launch_bounds__(kThreads) void commit_kernel(DraftArgs a) {
   typedef StateRows<Pool> Rows;
-  constexpr int kThreads = 64 * kWaves;
-  constexpr int kPerHead = 8 / kWaves;
   constexpr int kPasses = kMaxNodes * 16 / kThreads;
   __shared__ CommitShared s;
 
   int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t item = static_cast<uint32_t>(xcd_contiguous_item(blockIdx.x, gridDim.x));
-  const uint32_t head = item / kPerHead;
+  const uint32_t head = static_cast<uint32_t>(xcd_contiguous_item(blockIdx.x, gridDim.x));
   const uint32_t n = head / a.value_heads, h = head % a.value_heads, hk = h / a.group;
   int32_t slot;
   uint64_t begin;
@@ -765,7 +731,7 @@ __global__ __launch_bounds__(64 * kWaves) void commit_kernel(DraftArgs a) {
     log_decay = (a.log_decay + first)[lane * a.value_heads];
     strength = widen((a.beta + first)[lane * a.value_heads]);
   }
-  const int first_row = 16 * static_cast<int>((item % kPerHead) * kWaves + wave);
+  const int first_row = 16 * wave;
   Pool* const state = static_cast<Pool*>(a.pool) +
                       (static_cast<uint64_t>(slot) * a.value_heads + h) * kTile +
                       first_row * kDim;
@@ -836,7 +802,8 @@ __global__ __launch_bounds__(64 * kWaves) void commit_kernel(DraftArgs a) {
   uint2 v = value_of(0);
   exchange();
 
-  for (int at = 16 * wave; at < length; at += 16 * kWaves) {
+  if (16 * wave < length) {
+    const int at = 16 * wave;
     f32x4 kk = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
@@ -866,12 +833,10 @@ __global__ __launch_bounds__(64 * kWaves) void commit_kernel(DraftArgs a) {
     wave_sync();
     invert(block, r, g == 0);
   }
-  for (int m = wave; m < 8; m += kWaves) {
-    for (int at = 0; at < length; at += 16) {
-      // Four keys of four nodes, a node a lane of a quad, to a key a lane.
-      s.columns[at / 16][m][lane] = transpose_quad(
-          staged_run(s.k + 16 * at, 4 * g + (r & 3), Rows::run(m, r >> 2)), lane);
-    }
+  for (int at = 0; at < length; at += 16) {
+    // Four keys of four nodes, a node a lane of a quad, to a key a lane.
+    s.columns[at / 16][wave][lane] = transpose_quad(
+        staged_run(s.k + 16 * at, 4 * g + (r & 3), Rows::run(wave, r >> 2)), lane);
   }
   exchange();
 
@@ -919,32 +884,14 @@ __global__ __launch_bounds__(64 * kWaves) void commit_kernel(DraftArgs a) {
 
 // 64 rows of it are 2^31 bytes, which the kernels' 32-bit offsets hold.
 constexpr uint64_t kMaxStride = 1u << 24;  // elements between tokens
-constexpr uint32_t kFewHeads = kComputeUnits;
-
-template <typename Pool, int kTiles>
-int32_t launch_tree(void* stream, const DraftArgs& args, uint64_t heads) {
-  return heads <= kFewHeads
-             ? launch(tree_kernel<Pool, kTiles, 1, 2>, dim3(static_cast<uint32_t>(4 * heads)),
-                      dim3(128), stream, args)
-             : launch(tree_kernel<Pool, kTiles, 1, 8>, dim3(static_cast<uint32_t>(heads)),
-                      dim3(512), stream, args);
-}
 
 template <typename Pool>
-int32_t launch_tree(void* stream, const DraftArgs& args, uint64_t heads) {
+int32_t launch_tree(void* stream, const DraftArgs& args, dim3 grid) {
   const uint32_t most = args.max_nodes < args.tokens ? args.max_nodes : args.tokens;
-  return most <= 16   ? launch_tree<Pool, 1>(stream, args, heads)
-         : most <= 32 ? launch_tree<Pool, 2>(stream, args, heads)
-                      : launch_tree<Pool, 4>(stream, args, heads);
-}
-
-template <typename Pool>
-int32_t launch_commit(void* stream, const DraftArgs& args, uint64_t heads) {
-  return heads <= kFewHeads
-             ? launch(commit_kernel<Pool, 2>, dim3(static_cast<uint32_t>(4 * heads)), dim3(128),
-                      stream, args)
-             : launch(commit_kernel<Pool, 8>, dim3(static_cast<uint32_t>(heads)), dim3(512),
-                      stream, args);
+  const auto kernel = most <= 16   ? tree_kernel<Pool, 1>
+                      : most <= 32 ? tree_kernel<Pool, 2>
+                                   : tree_kernel<Pool, 4>;
+  return launch(kernel, grid, dim3(kThreads), stream, args);
 }
 
 template <bool kCommit>
@@ -967,19 +914,19 @@ int32_t launch_drafts(void* stream, const gdn_state_codec_drafts* d, const int32
     return kStatusInvalidArgument;
   }
   const uint64_t heads = static_cast<uint64_t>(d->requests) * d->value_heads;
-  if (heads > kMaxGrid / 256) return kStatusInvalidArgument;  // threads of the grid
+  if (heads > kMaxGrid / kThreads) return kStatusInvalidArgument;  // threads of the grid
   if (d->tokens == 0) return kStatusOk;  // every tree is empty
   const DraftArgs args{d->queries, d->keys, d->values, d->log_decay, d->beta, d->query_stride,
                        d->key_stride, d->value_stride, d->parents, d->offsets, d->slot_ids,
                        accepted, pool, outputs, d->tokens, slots, d->value_heads,
                        d->value_heads / d->key_heads, d->max_nodes, d->scale, d->normalize};
+  const dim3 grid(static_cast<uint32_t>(heads));
   const bool f32 = pool_dtype == kDtypeF32;
   if (kCommit) {
-    return f32 ? launch_commit<float>(stream, args, heads)
-               : launch_commit<bf16_bits>(stream, args, heads);
+    return launch(f32 ? commit_kernel<float> : commit_kernel<bf16_bits>, grid, dim3(kThreads),
+                  stream, args);
   }
-  return f32 ? launch_tree<float>(stream, args, heads)
-             : launch_tree<bf16_bits>(stream, args, heads);
+  return f32 ? launch_tree<float>(stream, args, grid) : launch_tree<bf16_bits>(stream, args, grid);
 }
 
 }  // namespace
