@@ -488,19 +488,33 @@ __global__ __launch_bounds__(kThreads) void tree_kernel(DraftArgs a) {
       if (block < kBlocks && i < tiles) {
         const int first = 16 * i + 4 * g, column = 16 * j + r;
         const float sum_c = s.sum[column], rest_c = s.rest[column], unit_c = s.k_unit[column];
-        const f32x4 sum = load4(&s.sum[first]), rest = load4(&s.rest[first]);
-        const f32x4 k_step = load4(&s.k_step[first]), q_unit = load4(&s.q_unit[first]);
+        // The rows' factors: a row at a time where registers, not LDS, decide how many
+        // workgroups share a compute unit (four then on a bf16 pool: 256 trees of 16 nodes
+        // take 68.6 us, with all rows' at once 75); else at once (the trees of up to 48 nodes
+        // 121 us, a row at a time 125).
+        constexpr bool kAtOnce = kTiles > 2;
+        f32x4 sum, rest, k_step, q_unit;
+        if (kAtOnce) {
+          sum = load4(&s.sum[first]), rest = load4(&s.rest[first]);
+          k_step = load4(&s.k_step[first]), q_unit = load4(&s.q_unit[first]);
+        }
         float worst_node = 0.0f, worst_output = 0.0f;  // NaN where a cell is no number
         f32x4 x, y;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          const bool up = (s.above[first + c] >> column & 1) != 0;
-          const bool self = first + c == column && column < nodes;
+          const int row = first + c;
+          const bool up = (s.above[row] >> column & 1) != 0;
+          const bool self = row == column && column < nodes;
+          if (!kAtOnce) {
+            sum[c] = s.sum[row], rest[c] = s.rest[row];
+            k_step[c] = s.k_step[row], q_unit[c] = s.q_unit[row];
+          }
           const float decay = decay_between(sum[c], rest[c], sum_c, rest_c) * unit_c;
           x[c] = up ? decay * k_step[c] * kk[e][c] : 0.0f;
           y[c] = up || self ? decay * q_unit[c] * qk[e][c] : 0.0f;
           worst_node = fmaf(x[c], 0.0f, worst_node);
           worst_output = fmaf(y[c], 0.0f, worst_output);
+          if (!kAtOnce) __builtin_amdgcn_sched_barrier(0);
         }
         if (__any(worst_node != 0.0f || worst_output != 0.0f)) {
           uint32_t bad_node = 0, bad_output = 0;  // a bit a row
