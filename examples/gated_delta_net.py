@@ -5,7 +5,8 @@ projection learn to repeat the token LAG positions back, on packed batches of
 ragged sequences (request_tables, gated_delta_rule and the norms, with their
 gradients).  The trained blocks are then served: a ragged batch of prompts fills
 the state pool (gated_delta_prefill), the answers are decoded token by token
-(gated_delta_step), the pool goes through the int8 codec and back (pool_encode,
+(gated_delta_step) and by trees of drafted tokens on a fork of the prompts' slots
+(slot_moves, copy_slots, gated_delta_tree, gated_delta_commit), the pool goes through the int8 codec and back (pool_encode,
 pool_decode) as a hibernated request's would, and one request is decoded by
 GdnStateCodecRuntime's windowed int8 steps from the same pool.
 
@@ -100,6 +101,16 @@ class Net(torch.nn.Module):
                 gdn.gated_delta_prefill(*inputs, tables, slots, states, resume=fresh)
                 for states in pool]
 
+    def tree_rules(self, parents, tables, slots, pool, seen: list):
+        """Each layer's rule over trees of drafted tokens, from states that stay as they are;
+        ``seen`` gets what committing an accepted path takes."""
+        def rule(states):
+            def outputs(*inputs):
+                seen.append((states, inputs[1:]))
+                return gdn.gated_delta_tree(*inputs, parents, tables, slots, states)
+            return outputs
+        return [rule(states) for states in pool]
+
     def step_rules(self, slots, pool):
         return [lambda *inputs, states=states: gdn.gated_delta_step(*inputs, states, slots)
                 for states in pool]
@@ -136,6 +147,27 @@ def train(net: Net, steps: int, device, generator, rate: float = 3e-3) -> list[f
     return torch.stack(losses).tolist()
 
 
+def decode_by_trees(net: Net, rows, lengths, answers: int, slots, pool, generator):
+    """The answers' outputs by trees of drafted tokens: each tree is a chain of the next
+    two tokens, which are accepted, and a wrong guess beside each of them."""
+    device, hidden = pool.device, rows[0].shape[1]
+    parents = torch.tensor([-1, -1, 0, 0] * len(rows), dtype=torch.int32, device=device)
+    accepted = torch.full((len(rows),), 2, dtype=torch.int32, device=device)
+    tables = gdn.request_tables(torch.full((len(rows),), 4, dtype=torch.int32, device=device),
+                                slots, 4 * len(rows))
+    outs = []
+    for i in range(0, answers, 2):
+        wrong = torch.randn((len(rows), 2, hidden), generator=generator).bfloat16().to(device)
+        tokens = torch.cat([torch.stack([row[n + i], guess[0], row[n + i + 1], guess[1]])
+                            for row, n, guess in zip(rows, lengths, wrong)])
+        seen = []
+        out = net(tokens, net.tree_rules(parents, tables, slots, pool, seen))
+        outs.append(out.view(len(rows), 4, hidden)[:, ::2])
+        for states, inputs in seen:
+            gdn.gated_delta_commit(*inputs, parents, accepted, tables, slots, states)
+    return torch.cat(outs, 1)  # [requests,answers,hidden]
+
+
 def apart(x: torch.Tensor, y: torch.Tensor) -> float:
     x, y = x.double(), y.double()
     return float((x - y).norm() / y.norm())
@@ -169,7 +201,13 @@ def serve(net: Net, lengths, answers: int, device, generator) -> dict[str, float
         return torch.stack(outs, 1)  # [requests,answers,hidden]
 
     expected = torch.stack(expected)
-    off = {"decoded": apart(decode(pool), expected)}
+    # The same by trees, on slots that the prompts' states were forked to.
+    forked = pool.clone()
+    ends = (slots + 1).contiguous()
+    gdn.copy_slots(list(forked), gdn.slot_moves(slots, ends, pool.shape[1]))
+    off = {"decoded": apart(decode(pool), expected),
+           "decoded by trees": apart(decode_by_trees(net, rows, lengths, answers, ends, forked,
+                                                     generator), expected)}
 
     codes = gdn.pool_encode(after_prompts, slots, gdn.LAYOUT_VALUE_KEY)
     restored = torch.zeros_like(after_prompts)
