@@ -78,13 +78,6 @@ struct Staged {
 };
 static_assert(workgroups_by_lds(sizeof(Staged)) == 3, "three workgroups share a compute unit");
 
-// LDS written by other lanes of the same wavefront is read after this.
-__device__ __forceinline__ void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-}
-
 // c + a b for 16 x 16 fp32 blocks: lane l has row l & 15, columns 4 g.. of a, and
 // rows 4 g.. of b's column l & 15 (an accumulator).
 __device__ __forceinline__ f32x4 block_product(const f32x4& a, const f32x4& b, f32x4 c) {

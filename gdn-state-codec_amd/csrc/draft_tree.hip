@@ -125,13 +125,6 @@ struct Block {
   }
 };
 
-// LDS written by other lanes of the same wavefront is read after this.
-__device__ __forceinline__ void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-}
-
 // N = (I + A)^-1 - I of a diagonal block that holds -A^T (row m: column m of -A), column
 // `column` by each lane that stores it:  N_i = -A_i - sum_(m<i) A_im N_m, one m after
 // another, so that each step waits for one fma alone.  The other lanes compute whatever
@@ -717,9 +710,11 @@ __device__ __forceinline__ uint2 staged_run(const uint4* rows, int row, int run)
 }
 
 // A wavefront's 16 rows of the state stay in registers while the path's nodes are applied 16
-// at a time, both as the products' operand and as the update's accumulators.  What depends on no state (the path, its keys in LDS, A's inverse
-// for each 16, by a wavefront each) comes first, so that nothing waits for another
-// wavefront between one 16 and the next.
+// at a time, both as the products' operand and as the update's accumulators.  What depends
+// on no state (the path, its keys in LDS, A's inverse for each 16, by a wavefront each) comes
+// first, so that nothing waits for another wavefront between one 16 and the next.
+//
+// @COMMIT@
 template <typename Pool>
 __global__ __launch_bounds__(kThreads) void commit_kernel(DraftArgs a) {
   typedef StateRows<Pool> Rows;
@@ -917,7 +912,8 @@ int32_t launch_drafts(void* stream, const gdn_state_codec_drafts* d, const int32
       d->value_heads % d->key_heads != 0 || d->max_nodes == 0 || d->max_nodes > kMaxNodes ||
       d->normalize > 1 || d->query_stride % 8 != 0 || d->key_stride % 8 != 0 ||
       d->value_stride % 8 != 0 || d->query_stride > kMaxStride || d->key_stride > kMaxStride ||
-      d->value_stride > kMaxStride || d->value_heads > kMaxStride / kDim || !d->offsets || !d->slot_ids ||
+      d->value_stride > kMaxStride || d->value_heads > kMaxStride / kDim || !d->offsets ||
+      !d->slot_ids ||
       !token_rows(d->tokens, d->keys, d->values, d->log_decay, d->beta, d->parents) ||
       (kCommit ? !accepted || d->queries != nullptr
                : !token_rows(d->tokens, d->queries, outputs)) ||

@@ -18,6 +18,7 @@
 #include <stdint.h>
 
 #include "gdn_state_codec_slots.h"
+#include "lane_exchange.h"
 #include "launch.h"
 #include "stream_memory.h"
 
@@ -77,13 +78,6 @@ __device__ __forceinline__ void enter(int32_t* hashed, const int32_t* slots, int
     }
     at = (at + 1) & mask;
   }
-}
-
-// LDS written by other lanes of the same wavefront is read after this.
-__device__ __forceinline__ void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
 }
 
 // next, steps and lowest after 2^rounds >= pairs steps, from one step.

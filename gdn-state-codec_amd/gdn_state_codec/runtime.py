@@ -379,6 +379,9 @@ class GdnStateCodecRuntime:
         if slot is None:
             raise RuntimeError(f"GDN State Codec: cache index {cache_index} has no slot to fork")
         targets = [target for target in dict.fromkeys(targets) if target != cache_index]
+        if any(target < 0 for target in targets):
+            raise RuntimeError(f"GDN State Codec: cache indices to fork to must not be negative, "
+                               f"got {targets}")
         forks = [slot.blank() for _ in targets]
         if forks:
             live = slot.window.slot_rows(slot.heads)

@@ -76,13 +76,19 @@ def compaction_moves(live: torch.Tensor) -> Compaction:
     return Compaction(SlotMoves(steps.view(rows, 4), slots), placed, count)
 
 
-def _apart(tensors) -> None:
-    """Refuses tensors that share memory, which the copies would race on."""
-    ranges = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
-                    for t in tensors)
-    for (_, end), (begin, _) in zip(ranges, ranges[1:]):
-        if begin < end:
+def _apart(written, read=()) -> None:
+    """Refuses tensors that are written and share memory with another, which the copies
+    would race on."""
+    ranges = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), writes)
+                    for tensors, writes in ((written, True), (read, False)) for t in tensors)
+    written_to = read_to = 0
+    for begin, end, writes in ranges:
+        if begin < written_to or (writes and begin < read_to):
             _fail("slot buffers must not share memory")
+        if writes:
+            written_to = max(written_to, end)
+        else:
+            read_to = max(read_to, end)
 
 
 def copy_slots(buffers: torch.Tensor | Sequence[torch.Tensor], moves: SlotMoves,
@@ -90,7 +96,7 @@ def copy_slots(buffers: torch.Tensor | Sequence[torch.Tensor], moves: SlotMoves,
     """Carries ``moves`` out on every tensor of a cache: each contiguous
     [moves.slots, ...], of any types and sizes, sharing no memory.  With ``into``, tensors
     of the same shapes and types, the rows go there from ``buffers``, which stay as they
-    are.  One launch for every 64 tensors."""
+    are (one may be read into several).  One launch for every 64 tensors."""
     if isinstance(buffers, torch.Tensor):
         buffers = (buffers,)
     if isinstance(into, torch.Tensor):
@@ -120,9 +126,9 @@ def copy_slots(buffers: torch.Tensor | Sequence[torch.Tensor], moves: SlotMoves,
     if not held:
         return
     if into is not None:
-        _apart([to for _, to in held] + list({t.data_ptr(): t for t, _ in held}.values()))
+        _apart([to for _, to in held], [t for t, _ in held])
     elif len(held) > 1:
-        _apart(t for t, _ in held)
+        _apart([t for t, _ in held])
     _launched(native().copy_slots_launch_v1(
         _stream(), (ctypes.c_uint64 * len(fields))(*fields), len(held), steps.data_ptr(),
         steps.shape[0], slots), "copy slots")

@@ -155,7 +155,7 @@ typedef struct gdn_state_codec_drafts {
   const uint16_t* values;       /* bf16 [tokens][value_heads][128] */
   const float* log_decay;       /* [tokens][value_heads] */
   const uint16_t* beta;         /* bf16 [tokens][value_heads] */
-  uint64_t query_stride;        /* elements between tokens, multiples of 8 */
+  uint64_t query_stride;        /* elements between tokens, multiples of 8 up to 2^24 */
   uint64_t key_stride;
   uint64_t value_stride;
   const int32_t* parents;       /* [tokens], 4-byte aligned: the parent's place in its
@@ -165,7 +165,7 @@ typedef struct gdn_state_codec_drafts {
   const int32_t* slot_ids;      /* [requests] */
   uint32_t requests;            /* 1..4096 */
   uint32_t tokens;
-  uint32_t value_heads;
+  uint32_t value_heads;         /* 1..2^17 */
   uint32_t key_heads;
   uint32_t max_nodes;           /* 1..64 */
   float scale;

@@ -47,7 +47,7 @@ int32_t statecentric_gdn_state_codec_compaction_moves_launch_v1(
     int32_t* count);
 
 /* One tensor of a cache: `bytes` a slot, slots side by side.  `to` is `from` itself, or
- * memory that overlaps no buffer of the call. */
+ * other memory; what one buffer writes overlaps nothing that another reads or writes. */
 typedef struct gdn_state_codec_slot_buffer {
   const void* from;
   void* to;
@@ -56,7 +56,7 @@ typedef struct gdn_state_codec_slot_buffer {
 
 /* to[target] <- from[source] for every row of `steps` (of slot_moves or compaction_moves
  * for the same number of slots) and every one of `count` buffers (host memory, read before
- * the call returns), which are different memory. */
+ * the call returns). */
 int32_t statecentric_gdn_state_codec_copy_slots_launch_v1(
     void* stream, const gdn_state_codec_slot_buffer* buffers, uint32_t count,
     const int32_t* steps, uint32_t rows, uint32_t slots);

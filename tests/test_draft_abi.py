@@ -183,6 +183,8 @@ def test_what_copies_are_launched_with(calls):
     gdn.copy_slots(b, moves, into=into)
     assert list(calls[2][1][1]) == [b.data_ptr(), into.data_ptr(), 40]
     gdn.copy_slots([b, b], moves, into=[into, torch.ones_like(b)])  # one source, two copies
+    rows = torch.zeros(7, 4)  # what is only read may overlap
+    gdn.copy_slots([rows[:6], rows[1:]], moves, into=[torch.ones(6, 4), torch.ones(6, 4)])
     for bad in (([b, b], moves), (b, moves, b), (b[:5], moves), ([], moves),
                 ([b, b], moves, [into, into]), (b, moves, into[:, :1])):
         with pytest.raises(RuntimeError, match="GDN State Codec"):

@@ -283,6 +283,11 @@ def test_runtime_fork(device):
 
     with pytest.raises(RuntimeError, match="no slot"):
         runtime.fork(1, [2])
+    step(1, tokens[0])
+    with pytest.raises(RuntimeError, match="negative"):
+        runtime.fork(1, [2, -1])
+    assert list(runtime._slots) == [1]
+    runtime.invalidate([1])
     for token in tokens[:9]:
         step(1, token)
     step(4, tokens[0])  # a slot of its own, forgotten by the fork
@@ -333,7 +338,11 @@ def test_refusals(device):
                 (x, moves, x.clone().bfloat16()), (x, moves, x.cpu()),
                 ([x, wide], moves, [long[:4], long[3:].repeat(1, 2)[:, :16].clone()[:3]]),
                 ([x, x], moves, [wide.view(8, 8)[:4], wide.view(8, 8)[2:6]]),
-                (long[:4], moves, long[3:])):
+                (long[:4], moves, long[3:]),
+                # read from one address: the longer of the two overlaps what is written
+                ([wide.view(-1)[:64].view(4, 16), wide.view(-1)[:16].view(4, 4)], moves,
+                 [wide.clone(), wide.view(-1)[48:].view(4, 4)]),
+                ([wide, wide], moves, [wide.clone(), wide])):
         with pytest.raises(RuntimeError, match="GDN State Codec"):
             gdn.copy_slots(*bad)
     assert torch.equal(x, before)
