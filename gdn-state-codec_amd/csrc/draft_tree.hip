@@ -342,6 +342,15 @@ __device__ __forceinline__ const void* row_at(const bf16_bits* base, uint32_t ro
 
 // The first wavefront forms the tables and inverts, the others form the nodes' products; the
 // state's are between, wherever a wavefront would wait.
+//
+// What bounds it (32 heads): few nodes, HBM: 64 trees of 16 on an fp32 pool take 35 us, of
+// which the bytes are 25.  Many nodes, one workgroup's phases, of which two (four of 16
+// nodes) share a compute unit: 256 trees of up to 48 nodes on a bf16 pool take 118 us (bytes
+// 68), 128 chains of 64 on an fp32 pool 135 (bytes 77).  The matrix units are busy for 20 and
+// 36% of that, wavefronts wait for 54 and 42% of their lives; the loads and stores without
+// the rest take about 100 us, the rest without them as much.  A persistent workgroup that asks
+// for the next head's nodes, 32 nodes at a time with less LDS, two heads a workgroup and
+// launches of their own for the smaller trees of a batch are no faster.
 template <typename Pool, int kTiles>
 __global__ __launch_bounds__(kThreads) void tree_kernel(DraftArgs a) {
   constexpr int kNodes = 16 * kTiles;
@@ -714,7 +723,10 @@ __device__ __forceinline__ uint2 staged_run(const uint4* rows, int row, int run)
 // on no state (the path, its keys in LDS, A's inverse for each 16, by a wavefront each) comes
 // first, so that nothing waits for another wavefront between one 16 and the next.
 //
-// @COMMIT@
+// What bounds it (32 heads): 256 paths of up to 16 nodes on an fp32 pool take 179 us, HBM
+// (the state's reads and writes alone 176, 5.6 TB/s); 128 paths of up to 64 on a bf16 pool
+// 115, where the bytes are 56: the chain of four rounds, whose splits and products wait for
+// each other with two workgroups a compute unit (the matrix units are busy for 28% of it).
 template <typename Pool>
 __global__ __launch_bounds__(kThreads) void commit_kernel(DraftArgs a) {
   typedef StateRows<Pool> Rows;
@@ -894,6 +906,11 @@ __global__ __launch_bounds__(kThreads) void commit_kernel(DraftArgs a) {
 // 64 rows of it are 2^31 bytes, which the kernels' 32-bit offsets hold.
 constexpr uint64_t kMaxStride = 1u << 24;  // elements between tokens
 
+// By the most nodes that a tree may have, since lengths stay on the device: LDS and registers
+// of the smaller forms let more workgroups share a compute unit.  Trees of 16 nodes, 32 heads,
+// by the forms of 16, 32 and 64: 256 on an fp32 pool 122, 125 and 129 us, on a bf16 pool 71,
+// 71.5 and 88; 64 of them 33.3, 34.8 and 36.3, and 21.4, 21.9 and 26.0.  256 trees of up to
+// 32 nodes on a bf16 pool by those of 32 and 64: 81 and 96.
 template <typename Pool>
 int32_t launch_tree(void* stream, const DraftArgs& args, dim3 grid) {
   const uint32_t most = args.max_nodes < args.tokens ? args.max_nodes : args.tokens;
