@@ -11,9 +11,9 @@
 // ends read one slot stand side by side, so that a fork's reads after the first come from
 // the caches: 300 slots of 32 encoded heads (330 MB, each source once) take 55 us, unsorted 75.
 //
-// One workgroup finds the order in LDS (hash tables, pointer doubling, a bitonic sort): 3.9
-// us for 4 pairs, 13.5 for a beam step's 96 and 14 for 300, barriers and LDS latency; the
-// moves of a compaction of 256 slots 4.8.
+// One workgroup finds the order (hash tables and pointer doubling in LDS, a sort): 3.8 us for
+// 4 pairs, 9 for a beam step's 96 and 8.5 for 300, barriers and LDS latency; the moves of a
+// compaction of 256 slots 4.8.
 //
 // copy_slots needs no order between threads: a thread owns a run of 16 bytes of every
 // slot and carries the rows out in turn, kBatch loads at a time.  A load may come before any
@@ -49,7 +49,7 @@ struct Plan {
   int32_t target[kMaxPairs];
   union {
     int32_t hashed[kHashed];   // pairs by target, then by source; -1 free
-    uint64_t key[kMaxPairs];   // pairs in their order
+    uint64_t key[kMaxPairs];   // to sort pairs by
   };
   int32_t next[kMaxPairs];     // a pair 2^i steps on
   int32_t steps[kMaxPairs];    // how many of them are real
@@ -110,6 +110,67 @@ __device__ __forceinline__ void follow(Plan& p, int pairs) {
       p.lowest[i] = lowest[e];
     }
     __syncthreads();
+  }
+}
+
+// x of lane ^ kMask.
+template <int kMask>
+__device__ __forceinline__ uint64_t partner(uint64_t x, int lane) {
+  if constexpr (kMask == 16 || kMask == 32) {
+    const bool up = (lane & kMask) != 0;
+    const auto low = kMask == 32 ? __builtin_amdgcn_permlane32_swap(x, x, false, false)
+                                 : __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    const auto high = kMask == 32
+        ? __builtin_amdgcn_permlane32_swap(x >> 32, x >> 32, false, false)
+        : __builtin_amdgcn_permlane16_swap(x >> 32, x >> 32, false, false);
+    const uint32_t low_up = low[0], low_down = low[1], high_up = high[0], high_down = high[1];
+    return static_cast<uint64_t>(up ? high_up : high_down) << 32 | (up ? low_up : low_down);
+  } else {
+    return dpp_xor<kMask>(x);
+  }
+}
+
+// One step of sorting key[e] of place threadIdx.x + e x blockDim.x, with the keys of the
+// places `gap` on.
+__device__ __forceinline__ uint64_t sorted(uint64_t key, uint64_t other, int place, int gap,
+                                           int run) {
+  const bool least = ((place & gap) == 0) == ((place & run) == 0);
+  return (key < other) == least ? key : other;
+}
+template <int kGap>
+__device__ __forceinline__ void sort_lanes(uint64_t (&key)[kEach], int run, int size) {
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    if (e * static_cast<int>(blockDim.x) >= size) break;
+    key[e] = sorted(key[e], partner<kGap>(key[e], threadIdx.x), threadIdx.x + e * blockDim.x,
+                    kGap, run);
+  }
+}
+// Sorts the first `size` places (a power of two).  Bitonic: keys of one wavefront's places
+// are exchanged between lanes, others through `shared` (all through it: 96 pairs' order
+// takes 12.5 us, 300 pairs' 13.8).
+__device__ __forceinline__ void sort(uint64_t (&key)[kEach], uint64_t* shared, int size) {
+  const int t = threadIdx.x, threads = blockDim.x;
+  for (int run = 2; run <= size; run <<= 1) {
+    for (int gap = run >> 1; gap >= 64; gap >>= 1) {
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        if (e * threads < size) shared[t + e * threads] = key[e];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int place = t + e * threads;
+        if (e * threads < size) key[e] = sorted(key[e], shared[place ^ gap], place, gap, run);
+      }
+      __syncthreads();
+    }
+    if (run >= 64) sort_lanes<32>(key, run, size);
+    if (run >= 32) sort_lanes<16>(key, run, size);
+    if (run >= 16) sort_lanes<8>(key, run, size);
+    if (run >= 8) sort_lanes<4>(key, run, size);
+    if (run >= 4) sort_lanes<2>(key, run, size);
+    sort_lanes<1>(key, run, size);
   }
 }
 
@@ -235,52 +296,36 @@ __global__ __launch_bounds__(kPlanThreads) void slot_moves_kernel(
   __syncthreads();
   int size = 1;
   while (size < pairs) size <<= 1;
+  uint64_t key[kEach];
 #pragma unroll
   for (int e = 0; e < kEach; ++e) {
     const int i = t + e * threads;
-    if (i >= size) break;
-    uint64_t key = ~0ull;
+    key[e] = ~0ull;
     if (i < pairs) {
       const uint64_t end = p.next[i];
-      key = live[e] ? static_cast<uint64_t>(p.lowest[end]) << 48 | end << 32 |
-                          static_cast<uint64_t>(kMaxPairs - p.steps[i]) << 16 | i
-                    : kLeftOut | i;
-    }
-    p.key[i] = key;
-  }
-  __syncthreads();
-  // A wavefront's 64 comparisons over gaps of up to 64 are of its own 128 keys: only wider
-  // ones, and the step after them, wait for the other wavefronts.
-  for (int run = 2; run <= size; run <<= 1) {
-    for (int gap = run >> 1; gap > 0; gap >>= 1) {
-      for (int pair = t; pair < size / 2; pair += threads) {
-        const int i = 2 * pair - (pair & (gap - 1)), other = i + gap;
-        const uint64_t x = p.key[i], y = p.key[other];
-        if ((x > y) == ((i & run) == 0)) {
-          p.key[i] = y;
-          p.key[other] = x;
-        }
-      }
-      if (gap > 64 || (gap == 1 && run >= 128)) __syncthreads();
-      else wave_sync();
+      key[e] = live[e] ? static_cast<uint64_t>(p.lowest[end]) << 48 | end << 32 |
+                             static_cast<uint64_t>(kMaxPairs - p.steps[i]) << 16 | i
+                       : kLeftOut | i;
     }
   }
   __syncthreads();
-  for (int place = t; place < pairs; place += threads) {
-    const uint64_t key = p.key[place];
-    const int i = static_cast<int>(key & 0xFFFF);
-    const uint32_t tree = static_cast<uint32_t>(key >> 32);
-    if (key >= kLeftOut) {
-      steps[place] = make_int4(-1, -1, 0, place + 1);
-      continue;
-    }
-    int low = place + 1, high = pairs;  // the first place of another tree
-    while (low < high) {
-      const int middle = (low + high) / 2;
-      if (static_cast<uint32_t>(p.key[middle] >> 32) == tree) low = middle + 1;
-      else high = middle;
-    }
-    steps[place] = make_int4(p.source[i], p.target[i], p.flags[i], low);
+  sort(key, p.key, size);
+  // A tree's last pair, the one at its end, says where it ends.
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int end = static_cast<int>(key[e] >> 32 & 0xFFFF);
+    if (key[e] < kLeftOut && (key[e] & 0xFFFF) == end) p.steps[end] = t + e * threads + 1;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int place = t + e * threads;
+    if (place >= pairs) break;
+    const int i = static_cast<int>(key[e] & 0xFFFF);
+    const int end = static_cast<int>(key[e] >> 32 & 0xFFFF);
+    steps[place] = key[e] < kLeftOut
+                       ? make_int4(p.source[i], p.target[i], p.flags[i], p.steps[end])
+                       : make_int4(-1, -1, 0, place + 1);
   }
 }
 
@@ -482,9 +527,9 @@ extern "C" int32_t statecentric_gdn_state_codec_slot_moves_launch_v1(
       slots == 0 || slots > 0x7FFFFFFFu || !gdn::aligned16(sources, targets, steps)) {
     return gdn::kStatusInvalidArgument;
   }
-  uint32_t table = 2, threads = (pairs + 63) / 64 * 64;
+  uint32_t table = 2, threads = 64;
   while (table < 2 * pairs) table *= 2;
-  if (threads > gdn::kPlanThreads) threads = gdn::kPlanThreads;
+  while (threads < pairs && threads < gdn::kPlanThreads) threads *= 2;
   return gdn::launch(gdn::slot_moves_kernel, dim3(1), dim3(threads), stream, sources, targets,
                      static_cast<int>(pairs), slots, table, reinterpret_cast<int4*>(steps));
 }
