@@ -620,15 +620,21 @@ __global__ __launch_bounds__(kThreads) void tree_kernel(DraftArgs a) {
 
 struct CommitShared {
   uint4 k[kMaxNodes * 16];  // the path's, like all that follows
-  uint2 columns[kMaxNodes / 16][8][64];  // of k, a key a lane, for each 16 and accumulator
+  uint4 columns[kMaxNodes / 32][8][64];  // of k, a key a lane, for each 32 and accumulator
   Block inverse[kMaxNodes / 16];  // of each 16: -A^T, then N
+  alignas(16) uint2 step[kMaxNodes / 32][kBlockPlaces];  // -A of each 32's second 16 and first
   float k_square[kMaxNodes], k_unit[kMaxNodes];
-  // Factors of a node: -b exp(G) / |k| of S k, b, and what carries u to the end of its 16.
+  // Factors of a node: -b exp(G) / |k| of S k, b, and what carries u to the end of its 32.
   float seen[kMaxNodes], strength[kMaxNodes], weight[kMaxNodes];
-  float sum[kMaxNodes], rest[kMaxNodes];  // G / ln 2 from the start of each 16
+  float sum[kMaxNodes], rest[kMaxNodes];  // G / ln 2 from the start of each 32
   float log_decay[kMaxNodes];
   int path[kMaxNodes];
 };
+
+// Two bf16 values held in fp32.
+__device__ __forceinline__ uint32_t held_pair(float low, float high) {
+  return upper_halves(__float_as_uint(low), __float_as_uint(high));
+}
 
 // A lane's row of a slice as eight accumulators of four keys: accumulator m holds run
 // `run(m, place)` of four (place: the lane group, or a quad's number where the tile's 16 keys
@@ -718,15 +724,17 @@ __device__ __forceinline__ uint2 staged_run(const uint4* rows, int row, int run)
                                               (run & 1)];
 }
 
-// A wavefront's 16 rows of the state stay in registers while the path's nodes are applied 16
+// A wavefront's 16 rows of the state stay in registers while the path's nodes are applied 32
 // at a time, both as the products' operand and as the update's accumulators.  What depends
-// on no state (the path, its keys in LDS, A's inverse for each 16, by a wavefront each) comes
-// first, so that nothing waits for another wavefront between one 16 and the next.
+// on no state comes first (the path, its keys in LDS, for each 32 the inverses of A's two
+// diagonal blocks and the block below them, by a wavefront each), so that nothing waits for
+// another wavefront between one 32 and the next.
 //
-// What bounds it (32 heads): 256 paths of up to 16 nodes on an fp32 pool take 179 us, HBM
+// What bounds it (32 heads): 256 paths of up to 16 nodes on an fp32 pool take 180 us, HBM
 // (the state's reads and writes alone 176, 5.6 TB/s); 128 paths of up to 64 on a bf16 pool
-// 115, where the bytes are 56: the chain of four rounds, whose splits and products wait for
-// each other with two workgroups a compute unit (the matrix units are busy for 28% of it).
+// 99, where the bytes are 56: vector instructions and the waits of one chain, with three
+// workgroups a compute unit.  16 nodes at a time, with no block below the diagonal but twice
+// as many splits of the state, they take 114.
 template <typename Pool>
 __global__ __launch_bounds__(kThreads) void commit_kernel(DraftArgs a) {
   typedef StateRows<Pool> Rows;
@@ -781,9 +789,9 @@ __global__ __launch_bounds__(kThreads) void commit_kernel(DraftArgs a) {
     const float own = s.log_decay[lane];  // a NaN stays: it is on the path
     double sum = own < static_cast<float>(kLeastLogDecay) ? kLeastLogDecay : own;
 #pragma unroll
-    for (int reach = 1; reach < 16; reach <<= 1) {
+    for (int reach = 1; reach < 32; reach <<= 1) {
       const double before = __shfl_up(sum, reach);
-      if (r >= reach) sum += before;
+      if ((lane & 31) >= reach) sum += before;
     }
     sum *= kInverseLn2;
     const float high = static_cast<float>(sum);
@@ -820,9 +828,10 @@ __global__ __launch_bounds__(kThreads) void commit_kernel(DraftArgs a) {
       }
     }
   }
-  uint2 v = value_of(0);
+  uint2 v[2] = {value_of(0), value_of(16)};
   exchange();
 
+  auto unit_of = [&](float square) { return a.normalize ? 1.0f / sqrtf(square + kUnitEps) : 1.0f; };
   if (16 * wave < length) {
     const int at = 16 * wave;
     f32x4 kk = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -831,9 +840,9 @@ __global__ __launch_bounds__(kThreads) void commit_kernel(DraftArgs a) {
       const uint4 k = staged(s.k, at + r, 4 * step + g);
       kk = mfma(k, k, kk);
     }
-    const float unit_c = a.normalize ? 1.0f / sqrtf(s.k_square[at + r] + kUnitEps) : 1.0f;
+    const float unit_c = unit_of(s.k_square[at + r]);
     if (g == 0) {
-      const int node = at + r, end = min(at + 15, length - 1);
+      const int node = at + r, end = min(node | 31, length - 1);
       const float decay = decay_between(s.sum[node], s.rest[node], 0.0f, 0.0f);
       const float carry = decay_between(s.sum[end], s.rest[end], s.sum[node], s.rest[node]);
       s.k_unit[node] = unit_c;
@@ -853,48 +862,102 @@ __global__ __launch_bounds__(kThreads) void commit_kernel(DraftArgs a) {
     }
     wave_sync();
     invert(block, r, g == 0);
+  } else if (wave >= kWaves - 2 && 32 * (kWaves - 1 - wave) + 16 < length) {
+    const int column = 32 * (kWaves - 1 - wave), row = column + 16;
+    f32x4 kk = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int step = 0; step < 4; ++step) {
+      kk = mfma(staged(s.k, row + r, 4 * step + g), staged(s.k, column + r, 4 * step + g), kk);
+    }
+    const f32x4 sum = load4(&s.sum[row + 4 * g]), rest = load4(&s.rest[row + 4 * g]);
+    const f32x4 b = load4(&s.strength[row + 4 * g]), square = load4(&s.k_square[row + 4 * g]);
+    const float sum_c = s.sum[column + r], rest_c = s.rest[column + r];
+    const float unit_c = unit_of(s.k_square[column + r]);
+    f32x4 x;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const float decay = decay_between(sum[c], rest[c], sum_c, rest_c);
+      const float k_unit = unit_of(square[c]);
+      x[c] = row + 4 * g + c < length ? -b[c] * decay * (k_unit * unit_c * kk[c]) : 0.0f;
+    }
+    store_operand(s.step[kWaves - 1 - wave], false, false, lane, x);
   }
-  for (int at = 0; at < length; at += 16) {
+  for (int at = 0; at < length; at += 32) {
     // Four keys of four nodes, a node a lane of a quad, to a key a lane.
-    s.columns[at / 16][wave][lane] = transpose_quad(
-        staged_run(s.k + 16 * at, 4 * g + (r & 3), Rows::run(wave, r >> 2)), lane);
+    const int run = Rows::run(wave, r >> 2), row = 4 * g + (r & 3);
+    const uint2 x = transpose_quad(staged_run(s.k + 16 * at, row, run), lane);
+    uint2 y = make_uint2(0, 0);
+    if (at + 16 < length) y = transpose_quad(staged_run(s.k + 16 * (at + 16), row, run), lane);
+    s.columns[at / 32][wave][lane] = make_uint4(x.x, x.y, y.x, y.y);
   }
   exchange();
 
-  for (int at = 0; at < length; at += 16) {
+  for (int at = 0; at < length; at += 32) {
     // Addresses by lane are formed in each round: kept over it, they take as many registers
     // as the state.
     asm volatile("" : "+v"(lane));
     r = lane & 15, g = lane >> 4;
-    f32x4 seen = {0.0f, 0.0f, 0.0f, 0.0f};
+    const bool two = at + 16 < length;
+    f32x4 seen[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+    auto see = [&](const auto& part, int step) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        if (i == 1 && !two) break;
+        const uint4* const rows = s.k + 16 * (at + 16 * i);
+        const uint2 low = staged_run(rows, r, Rows::run(2 * step, g));
+        const uint2 high = staged_run(rows, r, Rows::run(2 * step + 1, g));
+        seen[i] = product(make_uint4(low.x, low.y, high.x, high.y), part, seen[i]);
+      }
+    };
 #pragma unroll
     for (int step = 0; step < 4; ++step) {
-      const uint2 low = staged_run(s.k + 16 * at, r, Rows::run(2 * step, g));
-      const uint2 high = staged_run(s.k + 16 * at, r, Rows::run(2 * step + 1, g));
-      uint4 part[3];
-      split3(cells[2 * step], cells[2 * step + 1], part);
-      seen = mfma3(make_uint4(low.x, low.y, high.x, high.y), part, seen);
+      const f32x4 x = cells[2 * step], y = cells[2 * step + 1];
+      if (sizeof(Pool) == 2 && at == 0) {  // what was read has one part
+        const uint4 part[1] = {make_uint4(held_pair(x[0], x[1]), held_pair(x[2], x[3]),
+                                          held_pair(y[0], y[1]), held_pair(y[2], y[3]))};
+        see(part, step);
+      } else {
+        uint4 part[3];
+        split3(x, y, part);
+        see(part, step);
+      }
     }
-    const f32x4 own = value_columns(v, lane);
-    if (at + 16 < length) v = value_of(at + 16);
-
-    const int end = min(at + 15, length - 1);
+    const int end = min(at + 31, length - 1);
     const float whole = decay_between(s.sum[end], s.rest[end], 0.0f, 0.0f);
-    uint2 part[3];  // u, weighted
-    {
-      const f32x4 see = load4(&s.seen[at + 4 * g]), b = load4(&s.strength[at + 4 * g]);
+    // Zeros where there is no second 16.
+    uint4 part[3] = {};  // u, weighted: the first 16's and the second's side by side
+    Pair first = {};     // u of the first 16
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (i == 1 && !two) break;
+      const int node = at + 16 * i + 4 * g;
+      const f32x4 own = value_columns(v[i], lane);
+      if (at + 32 + 16 * i < length) v[i] = value_of(at + 32 + 16 * i);
+      const f32x4 factor = load4(&s.seen[node]), b = load4(&s.strength[node]);
       f32x4 x;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) x[c] = fmaf(see[c], seen[c], b[c] * own[c]);
-      const f32x4 u = block_product(s.inverse[at / 16].run(r, 4 * g), x, x);
-      split3_half(u * load4(&s.weight[at + 4 * g]), part);
+      for (int c = 0; c < 4; ++c) x[c] = fmaf(factor[c], seen[i][c], b[c] * own[c]);
+      if (i == 1) x = add_single(s.step[at / 32], lane, first, x);
+      const f32x4 u = block_product(s.inverse[at / 16 + i].run(r, 4 * g), x, x);
+      uint2 half[3];
+      if (i == 0 && two) {
+        split3_half(u, half);
+#pragma unroll
+        for (int p = 0; p < 3; ++p) first[p].x = half[p].x, first[p].y = half[p].y;
+      }
+      split3_half(u * load4(&s.weight[node]), half);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) {
+        if (i == 0) part[p].x = half[p].x, part[p].y = half[p].y;
+        else part[p].z = half[p].x, part[p].w = half[p].y;
+      }
     }
 #pragma unroll
     for (int m = 0; m < 8; ++m) {
-      const uint2 key = s.columns[at / 16][m][lane];
+      const uint4 key = s.columns[at / 32][m][lane];
       f32x4 x = cells[m] * whole;
 #pragma unroll
-      for (int p = 2; p >= 0; --p) x = mfma_half(key, part[p], x);
+      for (int p = 2; p >= 0; --p) x = mfma(key, part[p], x);
       cells[m] = x;
     }
   }
