@@ -224,6 +224,19 @@ def test_log_decays_of_minus_infinity_forget(device, shape):
     batch.check_commit([63, 19, 0])
 
 
+@pytest.mark.parametrize("pool_dtype", [torch.float32, torch.bfloat16])
+def test_log_decays_above_zero(device, pool_dtype):
+    """States that grow, by up to e^32: the terms grow alike, so the bounds stay."""
+    batch = Batch(device, [ref.parents_of(s, n, 9) for s, n in
+                           (("chain", 64), ("any", 50), ("branches", 33), ("chain", 17))],
+                  4, 2, pool_dtype, 47, padded=False)
+    batch.g.uniform_(-0.3, 0.5, generator=torch.Generator().manual_seed(47))
+    batch.g[:64, 0] = 0.5
+    batch.dev_g.copy_(batch.g)
+    batch.check_tree()
+    batch.check_commit([63, 49, 32, 16])
+
+
 def test_keys_that_are_all_alike(device):
     """Every write is over the same key: the solve's worst case, as in prefill's test."""
     batch = Batch(device, [ref.parents_of(s, 64, 8) for s in SHAPES], 2, 1, torch.float32, 45,
