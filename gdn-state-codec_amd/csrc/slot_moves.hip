@@ -16,11 +16,12 @@
 // compaction of 256 slots 4.8.
 //
 // copy_slots needs no order between threads: a thread owns a run of 16 bytes of every
-// slot and carries the rows out in turn, kBatch loads at a time.  A load may come before any
+// slot and carries the rows out in turn, some loads at a time.  A load may come before any
 // store (each reads what its slot held before the call), a store never before the loads
 // of the rows before it.  Trees are dealt over the grid's second dimension, so that many
 // small slots fill the card too.  HBM bounds it: 96 slots of 8 layers' 32 heads (2.7 GB, each
-// source once) take 510 us, 5.3 TB/s; 90 moves of a compaction (512 MB) 88 us, 5.8 TB/s.
+// source once) take 523 us, 5.2 TB/s; 90 moves of a compaction (512 MB) 85 us, 6.0 TB/s.  One
+// cycle over many small slots is bound by its own order: 500 slots of 32 KiB take 42 us.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -400,9 +401,14 @@ __global__ __launch_bounds__(kPlanThreads) void compaction_kernel(
 // ------------------------------------------------------------------- copies
 
 constexpr int kCopyThreads = 256;
-// Rows whose loads are all asked for before the first store.  With 2, 4, 8 and 16 the 96 slots
-// take 511, 511, 514 and 745 us, the 300 encoded ones 55.1, 55.8, 56.5 and 62.7.
-constexpr int kBatch = 4;
+// Rows whose loads are all asked for before the first store.  The few workgroups of small slots
+// wait for latency: one cycle of 500 slots of 32 KiB (8 workgroups) takes 42 us with 8 rows, 53
+// with 4 and 126 with loads that wait for each other, of 512 KiB (128) 89, 114 and 290; 16 are
+// no faster.  Where workgroups fill the card, several reads at a time of slots that lie a power
+// of two apart cost more than they hide: a cycle of 500 slots of 4 MiB (1,024) takes 805 us with
+// 1, 968 with 4 and 953 with 8, 96 slots of 8 layers 523, 520 and 528.
+constexpr int kBatchOfFew = 8, kBatchOfMany = 1;
+constexpr uint64_t kManyWorkgroups = 4 * kComputeUnits;
 constexpr int kFewBuffers = 9;    // of a launch with a small argument block (2 us less of a call)
 constexpr int kMostBuffers = 64;  // of one launch
 // Workgroups that fill the card: 8, 16, 32 and 64 a compute unit copy the 300 encoded slots in
@@ -424,40 +430,76 @@ struct CopyArgs {
   uint32_t count, rows, slots;
 };
 
-// A thread's run of `sizeof(Unit)` bytes of every slot, for rows begin .. end - 1.  Loads are
-// plain: with the nontemporal hint the 96 slots above take 557 us and not 519, since rows that
-// read one slot do not share it.
-template <typename Unit>
-__device__ __forceinline__ void copy_rows(const CopyBuffer& b, uint64_t at, const int4* steps,
+// x of one lane.
+__device__ __forceinline__ uint64_t lane_value(uint64_t x, int lane) {
+  const uint32_t low = __builtin_amdgcn_readlane(static_cast<uint32_t>(x), lane);
+  const uint32_t high = __builtin_amdgcn_readlane(static_cast<uint32_t>(x >> 32), lane);
+  return static_cast<uint64_t>(high) << 32 | low;
+}
+
+// Rows begin .. end - 1 for the threads' runs of `sizeof(Unit)` bytes from byte `start` of
+// every slot on.  A wavefront's lanes hold a row of the plan each, 64 at a time, and kBatch of
+// them are carried out together: all loads, then all stores, up to a row that writes what was
+// kept (so that one value is kept at a time).  A row that reads nothing loads from the first
+// slot, so that no load depends on a branch.  Loads are plain: with the nontemporal hint the
+// 96 slots above take 557 us and not 519, since rows that read one slot do not share it.
+template <typename Unit, int kBatch>
+__device__ __forceinline__ void copy_rows(const CopyBuffer& b, uint64_t start, const int4* steps,
                                           uint32_t begin, uint32_t end, uint32_t slots) {
-  if (at >= b.bytes) return;
-  const char* const from = b.from + at;
-  char* const to = b.to + at;
+  constexpr uint32_t kAll = (1u << kBatch) - 1;
+  const uint32_t offset = threadIdx.x * sizeof(Unit);
+  const bool active = start + offset < b.bytes;
+  const char* const from = b.from + start;
+  char* const to = b.to + start;
+  const int lane = threadIdx.x & 63;
   Unit kept = {};
-  for (uint32_t first = begin; first < end; first += kBatch) {
-    int4 row[kBatch];
-    Unit x[kBatch];
+  for (uint32_t chunk = begin; chunk < end; chunk += 64) {
+    const bool in = chunk + lane < end;
+    const int4 row = steps[in ? chunk + lane : begin];
+    const bool writes = in && static_cast<uint32_t>(row.y) < slots;
+    const bool reads = writes && static_cast<uint32_t>(row.x) < slots && !(row.z & kSaved);
+    const uint64_t target = writes ? row.y * b.bytes : 0, source = reads ? row.x * b.bytes : 0;
+    const uint64_t all_write = __ballot(writes), all_read = __ballot(reads);
+    const uint64_t all_save = __ballot(writes && (row.z & kSaves));
+    const uint64_t all_saved = __ballot(writes && (row.z & kSaved));
+    int first = 0;
+    while (first < 64 && all_write >> first != 0) {
+      const uint32_t saved = static_cast<uint32_t>(all_saved >> first) & kAll;
+      const uint32_t some = saved ? (saved ^ (saved - 1)) : kAll;  // up to the lowest
+      const uint32_t write = static_cast<uint32_t>(all_write >> first) & some;
+      const uint32_t read = static_cast<uint32_t>(all_read >> first) & some;
+      const uint32_t save = static_cast<uint32_t>(all_save >> first) & some;
+      const char* at[kBatch];
+      char* out[kBatch];
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      row[i] = first + i < end ? steps[first + i] : make_int4(-1, -1, 0, 0);
-      if (static_cast<uint32_t>(row[i].y) >= slots) row[i].y = -1;
-    }
+      for (int i = 0; i < kBatch; ++i) {
+        at[i] = from + lane_value(source, first + i);
+        out[i] = to + lane_value(target, first + i);
+      }
+      const char* const keep = from + lane_value(target, first + __builtin_ctz(save | 1u << 31));
+      if (active) {
+        Unit x[kBatch];
+        if (read) {
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      x[i] = Unit{};
-      if (row[i].y >= 0 && static_cast<uint32_t>(row[i].x) < slots && !(row[i].z & kSaved)) {
-        x[i] = *reinterpret_cast<const Unit*>(from + row[i].x * b.bytes);
-      }
-      if (row[i].y >= 0 && (row[i].z & kSaves)) {
-        kept = *reinterpret_cast<const Unit*>(from + row[i].y * b.bytes);
-      }
-      if (row[i].z & kSaved) x[i] = kept;
-    }
+          for (int i = 0; i < kBatch; ++i) x[i] = *reinterpret_cast<const Unit*>(at[i] + offset);
+        }
+        if (save) kept = *reinterpret_cast<const Unit*>(keep + offset);
+        if ((read & write) == kAll) {
 #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      if (row[i].y >= 0) {
-        __builtin_nontemporal_store(x[i], reinterpret_cast<Unit*>(to + row[i].y * b.bytes));
+          for (int i = 0; i < kBatch; ++i) {
+            __builtin_nontemporal_store(x[i], reinterpret_cast<Unit*>(out[i] + offset));
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            if (write >> i & 1) {
+              const Unit value = read >> i & 1 ? x[i] : saved >> i & 1 ? kept : Unit{};
+              __builtin_nontemporal_store(value, reinterpret_cast<Unit*>(out[i] + offset));
+            }
+          }
+        }
       }
+      first += saved ? __builtin_ctz(saved) + 1 : kBatch;
     }
   }
 }
@@ -470,18 +512,17 @@ __device__ __forceinline__ uint32_t part_begin(const int4* steps, uint32_t rows,
   return min(max(static_cast<uint32_t>(steps[at - 1].w), at), rows);
 }
 
-template <int kMost>
+template <int kMost, int kBatch>
 __global__ __launch_bounds__(kCopyThreads) void copy_slots_kernel(CopyArgs<kMost> a) {
   uint32_t i = 0;
   while (i + 1 < a.count && a.buffers[i + 1].first <= blockIdx.x) ++i;
   const CopyBuffer b = a.buffers[i];
   const uint32_t begin = part_begin(a.steps, a.rows, blockIdx.y, gridDim.y);
   const uint32_t end = part_begin(a.steps, a.rows, blockIdx.y + 1, gridDim.y);
-  const uint64_t at =
-      (static_cast<uint64_t>(blockIdx.x - b.first) * kCopyThreads + threadIdx.x) * b.unit;
-  if (b.unit == 16) copy_rows<u32x4_t>(b, at, a.steps, begin, end, a.slots);
-  else if (b.unit == 4) copy_rows<uint32_t>(b, at, a.steps, begin, end, a.slots);
-  else copy_rows<uint8_t>(b, at, a.steps, begin, end, a.slots);
+  const uint64_t at = static_cast<uint64_t>(blockIdx.x - b.first) * kCopyThreads * b.unit;
+  if (b.unit == 16) copy_rows<u32x4_t, kBatch>(b, at, a.steps, begin, end, a.slots);
+  else if (b.unit == 4) copy_rows<uint32_t, kBatch>(b, at, a.steps, begin, end, a.slots);
+  else copy_rows<uint8_t, kBatch>(b, at, a.steps, begin, end, a.slots);
 }
 
 // Bytes a thread copies of a slot: what the addresses and sizes of a buffer are multiples of.
@@ -512,7 +553,8 @@ int32_t launch_copy(void* stream, const gdn_state_codec_slot_buffer* buffers, ui
   }
   uint64_t parts = (kFill + blocks - 1) / blocks;
   if (parts > rows) parts = rows;
-  return launch(copy_slots_kernel<kMost>,
+  return launch(blocks < kManyWorkgroups ? copy_slots_kernel<kMost, kBatchOfFew>
+                                         : copy_slots_kernel<kMost, kBatchOfMany>,
                 dim3(static_cast<uint32_t>(blocks), static_cast<uint32_t>(parts)),
                 dim3(kCopyThreads), stream, args);
 }

@@ -122,6 +122,19 @@ def test_rows_of_any_size(device, shape, dtype):
         gdn.copy_slots(buffer, gdn.slot_moves(ints(sources, device), ints(targets, device), 23))
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size,dtype,more", [(270001, torch.int8, 0), (275001, torch.float32, 0),
+                                             (1050004, torch.float32, 0),
+                                             (5000, torch.float32, 70)])
+def test_many_workgroups(device, kind, size, dtype, more):
+    """Rows of 1,024 and more workgroups, in units of 1, 4 and 16 bytes, alone and in many
+    buffers; cleared slots beside the moved ones, more rows than are carried out together."""
+    sources, targets = _pairs(kind, 30, 25, random.Random(size))
+    sources[3] = sources[20] = -1
+    check(device, sources, targets, 30,
+          [filled((30, size), dtype, device, i) for i in range(1 + more)])
+
+
 def test_rows_that_start_at_any_byte(device):
     """A buffer that is a slice: 4-byte and 1-byte aligned, the bytes around it untouched."""
     for dtype, skip in ((torch.float32, 1), (torch.int8, 3), (torch.int8, 4)):
