@@ -412,7 +412,7 @@ constexpr uint64_t kManyWorkgroups = 4 * kComputeUnits;
 constexpr int kFewBuffers = 9;    // of a launch with a small argument block (2 us less of a call)
 constexpr int kMostBuffers = 64;  // of one launch
 // Workgroups that fill the card: 8, 16, 32 and 64 a compute unit copy the 300 encoded slots in
-// 59.2, 57.5, 55.8 and 56.3 us, the 96 in 515, 515, 511 and 510.
+// 56.9, 56.8, 55.6 and 57.1 us, the 90 of 4 layers in 107, 106, 102 and 105.
 constexpr uint32_t kFill = 32 * kComputeUnits;
 
 struct CopyBuffer {
