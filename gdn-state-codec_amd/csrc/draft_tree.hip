@@ -19,8 +19,11 @@
 // on the diagonal is formed by substitution, which is stable for any keys.
 //
 // Bad values.  A product takes every cell, also those that are zero, so a NaN or an
-// infinity in r or A would reach every node.  Those cells are set to zero, and the nodes
-// that they belong to noted, for their outputs and those below them.
+// infinity in A, M, r or u would reach every node.  Those cells are set to zero, and the
+// nodes that they belong to noted, for their outputs and those below them.  u is looked at
+// too: finite inputs may sum up to more than fp32 holds, and the parts of a value above the
+// largest bf16 are no numbers.  Where the inverse of a block passes that range, which the
+// writes themselves need not, the block is solved node by node.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -46,6 +49,7 @@ constexpr double kInverseLn2 = 1.4426950408889634074;
 // exp of less is 0 in fp32; sums of it stay far from what fp64 cannot tell apart.
 constexpr double kLeastLogDecay = -200.0;
 constexpr float kLargest = 0x1.fffffep127f;
+constexpr float kLargestPart = 0x1.fep127f;  // of what is cut into bf16 parts
 
 struct DraftArgs {
   const bf16_bits* queries;
@@ -128,11 +132,22 @@ struct Block {
   }
 };
 
-// N = (I + A)^-1 - I of a diagonal block that holds -A^T (row m: column m of -A), column
-// `column` by each lane that stores it:  N_i = -A_i - sum_(m<i) A_im N_m, one m after
-// another, so that each step waits for one fma alone.  The other lanes compute whatever
-// is there.
-__device__ __forceinline__ void invert(Block& block, int column, bool stores) {
+// Whether all parts of x, and with them every product with 0, are numbers.
+__device__ __forceinline__ bool in_range(float x) { return fabsf(x) <= kLargestPart; }
+__device__ __forceinline__ float largest(float x, float y, float z) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_maximum(x, y), z);
+}
+__device__ __forceinline__ float largest(const f32x4& x) {  // NaN where a cell is
+  return largest(largest(fabsf(x[0]), fabsf(x[1]), fabsf(x[2])), fabsf(x[3]), 0.0f);
+}
+__device__ __forceinline__ bool in_range(const f32x4& x) { return in_range(largest(x)); }
+
+// N = (I + A)^-1 - I of a diagonal block, from -A^T (row m of `block`: column m of -A),
+// column `column` by each lane that stores it:  N_i = -A_i - sum_(m<i) A_im N_m, one m
+// after another, so that each step waits for one fma alone.  The other lanes compute
+// whatever is there.  Returns whether the lane's column is in range.
+__device__ __forceinline__ bool invert(const Block& block, Block& inverse, int column,
+                                       bool stores) {
   f32x4 n[4];
 #pragma unroll
   for (int c = 0; c < 4; ++c) n[c] = block.run(column, 4 * c);
@@ -151,11 +166,12 @@ __device__ __forceinline__ void invert(Block& block, int column, bool stores) {
   // Formed here, not where it is stored: all rows would wait in registers.
 #pragma unroll
   for (int c = 0; c < 4; ++c) asm volatile("" : "+v"(n[c]));
-  wave_sync();  // -A^T has been read
+  wave_sync();  // `inverse` may be `block`
   if (stores) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) block.at(i, column) = n[i / 4][i % 4];
+    for (int i = 0; i < 16; ++i) inverse.at(i, column) = n[i / 4][i % 4];
   }
+  return in_range(f32x4{largest(n[0]), largest(n[1]), largest(n[2]), largest(n[3])});
 }
 
 // A value that all lanes share, known to be one.
@@ -193,7 +209,57 @@ __device__ __forceinline__ f32x4 value_columns(const uint2& w, int lane) {
   return f32x4{widen_low(t.x), widen_high(t.x), widen_low(t.y), widen_high(t.y)};
 }
 
-__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= kLargest; }
+// Sets the cells of a lane's column that are out of range to 0, and gives their nodes, a bit
+// each, in all lanes of that column.
+__device__ __forceinline__ uint32_t set_apart(f32x4& x, int lane) {
+  uint32_t column = 0;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    if (!in_range(x[c])) column |= 1u << (4 * (lane >> 4) + c), x[c] = 0.0f;
+  }
+  column |= __shfl_xor(column, 16);
+  return column | __shfl_xor(column, 32);
+}
+
+// The same, after x <- (I + A)^-1 x of one block from -A^T, node after node: what an inverse
+// past fp32's range cannot give.
+__device__ __forceinline__ uint32_t solve_by_steps(const Block& block, f32x4& x, int lane) {
+#pragma unroll 1
+  for (int from = 0; from < 4; ++from) {  // the lane group that has the node
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      float u = __shfl(x[c], 16 * from + (lane & 15));
+      if (!in_range(u)) u = 0.0f;
+      const f32x4 below = block.run(4 * from + c, 4 * (lane >> 4));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = fmaf(below[i], u, x[i]);
+    }
+  }
+  return set_apart(x, lane);
+}
+
+// u = x + N x of 16 nodes, and the nodes that are not in range (then 0), a bit each.  A cell
+// of x or u that is out of range would reach every node through the zeros of the products
+// it enters, so both are looked at, but u first: it is out of range wherever x or a cell of
+// N is.
+__device__ __forceinline__ uint32_t solve(const Block& inverse, const Block& block, int lane,
+                                          f32x4& x) {
+  const f32x4 n = inverse.run(lane & 15, 4 * (lane >> 4));
+  const f32x4 u = block_product(n, x, x);
+  uint32_t bad = 0;
+  if (__any(!in_range(u))) {
+    if (__any(!in_range(n))) {
+      bad = solve_by_steps(block, x, lane);
+    } else {
+      bad = set_apart(x, lane);
+      x = block_product(n, x, x);
+      bad |= set_apart(x, lane);
+    }
+  } else {
+    x = u;
+  }
+  return bad;
+}
 
 // -------------------------------------------------------------------- the tree
 
@@ -265,7 +331,8 @@ struct TreeShared {
     };
     uint4 out[kNodes * 16];       // once all products of k and q are formed
   };
-  Block inverse[kTiles];          // on the diagonal: -A^T, then N
+  Block own[kTiles];              // on the diagonal: -A^T
+  Block inverse[kTiles];          // and N
   alignas(16) uint2 step[step_places(kTiles)];  // -A below it
   alignas(16) uint2 read[read_places(kTiles)];  // M
   alignas(16) float k_square[kNodes], q_square[kNodes];
@@ -354,8 +421,13 @@ __device__ __forceinline__ const void* row_at(const bf16_bits* base, uint32_t ro
 // the rest take about 100 us, the rest without them as much.  A persistent workgroup that asks
 // for the next head's nodes, 32 nodes at a time with less LDS, two heads a workgroup and
 // launches of their own for the smaller trees of a batch are no faster.
+//
+// Four workgroups a compute unit for a bf16 pool's trees of up to 32 nodes: 64 registers, which
+// the compiler is held to (it takes 66 otherwise: 256 trees 95 us, 91 so).
 template <typename Pool, int kTiles>
-__global__ __launch_bounds__(kThreads) void tree_kernel(DraftArgs a) {
+__global__ __launch_bounds__(kThreads)
+__attribute__((amdgpu_waves_per_eu(sizeof(Pool) == 2 && kTiles <= 2 ? 8 : 2)))
+void tree_kernel(DraftArgs a) {
   constexpr int kNodes = 16 * kTiles;
   constexpr int kPasses = 2 * kNodes * 16 / kThreads;
   constexpr int kBlocks = blocks_of(kTiles);
@@ -463,7 +535,7 @@ __global__ __launch_bounds__(kThreads) void tree_kernel(DraftArgs a) {
     state_products();
     exchange();
     const int diagonal = min(g, kTiles - 1);
-    invert(s.inverse[diagonal], r, g < tiles);
+    invert(s.own[diagonal], s.inverse[diagonal], r, g < tiles);
     exchange();
   } else {
     f32x4 kk[kPairs], qk[kPairs];
@@ -503,7 +575,7 @@ __global__ __launch_bounds__(kThreads) void tree_kernel(DraftArgs a) {
           sum = load4(&s.sum[first]), rest = load4(&s.rest[first]);
           k_step = load4(&s.k_step[first]), q_unit = load4(&s.q_unit[first]);
         }
-        float worst_node = 0.0f, worst_output = 0.0f;  // NaN where a cell is no number
+        float worst = 0.0f;
         f32x4 x, y;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -517,23 +589,22 @@ __global__ __launch_bounds__(kThreads) void tree_kernel(DraftArgs a) {
           const float decay = decay_between(sum[c], rest[c], sum_c, rest_c) * unit_c;
           x[c] = up ? decay * k_step[c] * kk[e][c] : 0.0f;
           y[c] = up || self ? decay * q_unit[c] * qk[e][c] : 0.0f;
-          worst_node = fmaf(x[c], 0.0f, worst_node);
-          worst_output = fmaf(y[c], 0.0f, worst_output);
+          worst = largest(worst, fabsf(x[c]), fabsf(y[c]));
           if (!kAtOnce) __builtin_amdgcn_sched_barrier(0);
         }
-        if (__any(worst_node != 0.0f || worst_output != 0.0f)) {
+        if (__any(!in_range(worst))) {
           uint32_t bad_node = 0, bad_output = 0;  // a bit a row
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            if (!finite(x[c])) bad_node |= 1u << c, x[c] = 0.0f;
-            if (!finite(y[c])) bad_output |= 1u << c, y[c] = 0.0f;
+            if (!in_range(x[c])) bad_node |= 1u << c, x[c] = 0.0f;
+            if (!in_range(y[c])) bad_output |= 1u << c, y[c] = 0.0f;
           }
           if (bad_node) atomicOr(&s.bad_node[first >> 5], bad_node << (first & 31));
           if (bad_output) atomicOr(&s.bad_output[first >> 5], bad_output << (first & 31));
         }
         if (i == j) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) s.inverse[i].at(r, 4 * g + c) = x[c];
+          for (int c = 0; c < 4; ++c) s.own[i].at(r, 4 * g + c) = x[c];
         } else {
           store_operand(s.step + step_at(i, j), (j | 1) < i, (j & 1) != 0, lane, x);
         }
@@ -546,7 +617,7 @@ __global__ __launch_bounds__(kThreads) void tree_kernel(DraftArgs a) {
   }
 
   const uint64_t bad_outputs = static_cast<uint64_t>(s.bad_output[1]) << 32 | s.bad_output[0];
-  // Nodes that are bad, or whose r is in this column.
+  // Nodes that are bad, or whose u is in this column.
   uint64_t bad = static_cast<uint64_t>(s.bad_node[1]) << 32 | s.bad_node[0];
   const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
   Pair u[(kTiles + 1) / 2];
@@ -558,22 +629,10 @@ __global__ __launch_bounds__(kThreads) void tree_kernel(DraftArgs a) {
     const f32x4 b = load4(&s.strength[first]);
     const f32x4 values = value_columns(v[i], lane);
     f32x4 x, out;
-    float worst = 0.0f;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       x[c] = fmaf(see[c], seen[i][c], b[c] * values[c]);
       out[c] = look[c] * read[i][c];
-      worst = fmaf(x[c], 0.0f, worst);
-    }
-    if (__any(worst != 0.0f)) {
-      uint64_t column = 0;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if (!finite(x[c])) column |= 1ull << (first + c), x[c] = 0.0f;
-      }
-      column |= __shfl_xor(column, 16);
-      column |= __shfl_xor(column, 32);
-      bad |= column;
     }
 #pragma unroll
     for (int j = 0; j < i; j += 2) {
@@ -582,8 +641,9 @@ __global__ __launch_bounds__(kThreads) void tree_kernel(DraftArgs a) {
           : i < 2   ? add_single(step, lane, u[j / 2], x)
                     : x + add_single(step, lane, u[j / 2], zero);
     }
+    bad |= static_cast<uint64_t>(solve(s.inverse[i], s.own[i], lane, x)) << (16 * i);
     uint2 part[3];
-    split3_half(block_product(s.inverse[i].run(r, 4 * g), x, x), part);
+    split3_half(x, part);
 #pragma unroll
     for (int p = 0; p < 3; ++p) {
       uint4& whole = u[i / 2][p];
@@ -629,6 +689,8 @@ struct CommitShared {
   uint4 k[kMaxNodes * 16];  // the path's, like all that follows
   uint4 columns[kMaxNodes / 32][8][64];  // of k, a key a lane, for each 32 and accumulator
   Block inverse[kMaxNodes / 16];  // of each 16: -A^T, then N
+  alignas(16) int32_t steep[kWaves];  // whether a cell of what each wavefront forms of A
+                                      // and N is out of range
   alignas(16) uint2 step[kMaxNodes / 32][kBlockPlaces];  // -A of each 32's second 16 and first
   float k_square[kMaxNodes], k_unit[kMaxNodes];
   // Factors of a node: -b exp(G) / |k| of S k, b, and what carries u to the end of its 32.
@@ -731,6 +793,46 @@ __device__ __forceinline__ uint2 staged_run(const uint4* rows, int row, int run)
                                               (run & 1)];
 }
 
+// A wavefront's 16 rows after the path, token by token: S <- e^g S + b (v - e^g S k) k^T.
+// For paths whose inverses pass fp32's range, which their writes need not.  Its keys are read
+// where they are used, a run at a time, so that it takes no more registers than the other form.
+template <typename Pool>
+__device__ __forceinline__ void commit_by_steps(const CommitShared& s, const DraftArgs& a,
+                                                const bf16_bits* values, int length, int lane,
+                                                f32x4 (&x)[8]) {
+  const int r = lane & 15, g = lane >> 4;
+#pragma unroll 1
+  for (int node = 0; node < length; ++node) {
+    const float log_decay = s.log_decay[node], unit = s.k_unit[node], b = s.strength[node];
+    const float value = widen(values[s.path[node] * a.value_stride + r]);
+    const float decay =
+        decay_between(log_decay * static_cast<float>(kInverseLn2), 0.0f, 0.0f, 0.0f);
+    auto key = [&](int m) {
+      __builtin_amdgcn_sched_barrier(0);
+      asm volatile("" ::: "memory");
+      const uint2 w = staged_run(s.k, node, StateRows<Pool>::run(m, g));
+      return f32x4{widen_low(w.x), widen_high(w.x), widen_low(w.y), widen_high(w.y)};
+    };
+    float seen = 0.0f;
+#pragma unroll
+    for (int m = 0; m < 8; ++m) {
+      const f32x4 k = key(m);
+      x[m] *= decay;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) seen = fmaf(x[m][c], k[c], seen);
+    }
+    seen += __shfl_xor(seen, 16);
+    seen += __shfl_xor(seen, 32);
+    const float write = b * (value - unit * seen) * unit;
+#pragma unroll
+    for (int m = 0; m < 8; ++m) {
+      const f32x4 k = key(m);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) x[m][c] = fmaf(write, k[c], x[m][c]);
+    }
+  }
+}
+
 // A wavefront's 16 rows of the state stay in registers while the path's nodes are applied 32
 // at a time, both as the products' operand and as the update's accumulators.  What depends
 // on no state comes first (the path, its keys in LDS, for each 32 the inverses of A's two
@@ -742,8 +844,14 @@ __device__ __forceinline__ uint2 staged_run(const uint4* rows, int row, int run)
 // 99, where the bytes are 56: vector instructions and the waits of one chain, with three
 // workgroups a compute unit.  16 nodes at a time, with no block below the diagonal but twice
 // as many splits of the state, they take 114.
+//
+// Three workgroups a compute unit: 80 registers, which the compiler is held to for a bf16 pool
+// (it takes 82 otherwise: 115 us).  An fp32 pool's form has 80 by itself; held to them it is
+// ordered otherwise, and 256 paths take 186 us.
 template <typename Pool>
-__global__ __launch_bounds__(kThreads) void commit_kernel(DraftArgs a) {
+__global__ __launch_bounds__(kThreads)
+__attribute__((amdgpu_waves_per_eu(sizeof(Pool) == 2 ? 6 : 2)))
+void commit_kernel(DraftArgs a) {
   typedef StateRows<Pool> Rows;
   constexpr int kPasses = kMaxNodes * 16 / kThreads;
   __shared__ CommitShared s;
@@ -779,7 +887,7 @@ __global__ __launch_bounds__(kThreads) void commit_kernel(DraftArgs a) {
   for (int node = last; node >= 0; node = __builtin_amdgcn_readlane(parent, node)) {
     on_path |= 1ull << node;
   }
-  const int length = __popcll(on_path);
+  int length = __popcll(on_path);
   if (wave == 0) {
     if (lane >= length) {
       s.path[lane] = -1;
@@ -839,6 +947,7 @@ __global__ __launch_bounds__(kThreads) void commit_kernel(DraftArgs a) {
   exchange();
 
   auto unit_of = [&](float square) { return a.normalize ? 1.0f / sqrtf(square + kUnitEps) : 1.0f; };
+  int32_t steep = 0;
   if (16 * wave < length) {
     const int at = 16 * wave;
     f32x4 kk = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -868,7 +977,7 @@ __global__ __launch_bounds__(kThreads) void commit_kernel(DraftArgs a) {
       block.at(r, 4 * g + c) = up ? -b[c] * decay * (k_unit[c] * unit_c * kk[c]) : 0.0f;
     }
     wave_sync();
-    invert(block, r, g == 0);
+    steep = __any(!invert(block, block, r, g == 0));
   } else if (wave >= kWaves - 2 && 32 * (kWaves - 1 - wave) + 16 < length) {
     const int column = 32 * (kWaves - 1 - wave), row = column + 16;
     f32x4 kk = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -887,8 +996,10 @@ __global__ __launch_bounds__(kThreads) void commit_kernel(DraftArgs a) {
       const float k_unit = unit_of(square[c]);
       x[c] = row + 4 * g + c < length ? -b[c] * decay * (k_unit * unit_c * kk[c]) : 0.0f;
     }
+    steep = __any(!in_range(x));
     store_operand(s.step[kWaves - 1 - wave], false, false, lane, x);
   }
+  if (lane == 0) s.steep[wave] = steep;
   for (int at = 0; at < length; at += 32) {
     // Four keys of four nodes, a node a lane of a quad, to a key a lane.
     const int run = Rows::run(wave, r >> 2), row = 4 * g + (r & 3);
@@ -899,6 +1010,11 @@ __global__ __launch_bounds__(kThreads) void commit_kernel(DraftArgs a) {
   }
   exchange();
 
+  if (__any(s.steep[lane % kWaves])) {
+    asm volatile("" : "+v"(lane));
+    commit_by_steps<Pool>(s, a, values, length, lane, cells);
+    length = 0;
+  }
   for (int at = 0; at < length; at += 32) {
     // Addresses by lane are formed in each round: kept over it, they take as many registers
     // as the state.

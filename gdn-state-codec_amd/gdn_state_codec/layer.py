@@ -383,9 +383,9 @@ def gated_delta_tree(queries: torch.Tensor, keys: torch.Tensor, values: torch.Te
     where all trees are smaller, saying so saves time.
 
     Returns bf16 [T,H,128]; rows of no request, of padding and of nodes past ``max_nodes``
-    stay as they were (zeros without ``out``).  A NaN or an infinity in a node's token
-    reaches outputs of that node and those below it only.  Not differentiable, as
-    :func:`gated_delta_step`."""
+    stay as they were (zeros without ``out``).  A NaN or an infinity in a node's token, or a
+    write that passes fp32's range (3.39e38, of finite tokens), reaches outputs of that node
+    and those below it only.  Not differentiable, as :func:`gated_delta_step`."""
     drafts = _drafts(queries, keys, values, log_decay, beta, parents, tables, slot_ids,
                      normalize, max_nodes, scale)
     pool_dtype = _pool(pool, drafts.value_heads)

@@ -182,7 +182,8 @@ typedef struct gdn_state_codec_drafts {
  * A NaN or an infinity in a node's token leaves the outputs that it reaches in that node
  * and in those below it without a finite value, and no other node's: of a value its own
  * column's, of a key, a log decay or a write strength the head's, of a query the node's
- * alone.  A log decay of -inf is no such value: it forgets. */
+ * alone.  A log decay of -inf is no such value: it forgets.  So with finite tokens whose
+ * node writes more than the largest bf16 value, 3.39e38, to a column: that column's. */
 int32_t statecentric_gdn_state_codec_gated_delta_tree_launch_v1(
     void* stream, const gdn_state_codec_drafts* drafts, const void* pool, uint32_t slots,
     uint32_t pool_dtype, uint16_t* outputs);
