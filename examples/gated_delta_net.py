@@ -6,9 +6,10 @@ ragged sequences (request_tables, gated_delta_rule and the norms, with their
 gradients).  The trained blocks are then served: a ragged batch of prompts fills
 the state pool (gated_delta_prefill), the answers are decoded token by token
 (gated_delta_step) and by trees of drafted tokens on a fork of the prompts' slots
-(slot_moves, copy_slots, gated_delta_tree, gated_delta_commit), the pool goes through the int8 codec and back (pool_encode,
-pool_decode) as a hibernated request's would, and one request is decoded by
-GdnStateCodecRuntime's windowed int8 steps from the same pool.
+(slot_moves, copy_slots, gated_delta_tree, gated_delta_commit), the pool goes
+through the int8 codec and back (pool_encode, pool_decode) as a hibernated request's
+would, and one request is decoded by GdnStateCodecRuntime's windowed int8 steps from
+the same pool.
 
     python examples/gated_delta_net.py [--steps N]
 
@@ -149,20 +150,25 @@ def train(net: Net, steps: int, device, generator, rate: float = 3e-3) -> list[f
 
 def decode_by_trees(net: Net, rows, lengths, answers: int, slots, pool, generator):
     """The answers' outputs by trees of drafted tokens: each tree is a chain of the next
-    two tokens, which are accepted, and a wrong guess beside each of them."""
+    two tokens (the last answer's, where their number is odd, of it alone), which are
+    accepted, and a wrong guess beside each of them."""
     device, hidden = pool.device, rows[0].shape[1]
-    parents = torch.tensor([-1, -1, 0, 0] * len(rows), dtype=torch.int32, device=device)
-    accepted = torch.full((len(rows),), 2, dtype=torch.int32, device=device)
-    tables = gdn.request_tables(torch.full((len(rows),), 4, dtype=torch.int32, device=device),
-                                slots, 4 * len(rows))
+
+    def ints(x):
+        return torch.tensor(x * len(rows), dtype=torch.int32, device=device)
+
     outs = []
     for i in range(0, answers, 2):
-        wrong = torch.randn((len(rows), 2, hidden), generator=generator).bfloat16().to(device)
-        tokens = torch.cat([torch.stack([row[n + i], guess[0], row[n + i + 1], guess[1]])
+        depth = min(2, answers - i)
+        nodes = 2 * depth
+        wrong = torch.randn((len(rows), depth, hidden), generator=generator).bfloat16().to(device)
+        tokens = torch.cat([torch.stack([row[n + i:n + i + depth], guess], 1).flatten(0, 1)
                             for row, n, guess in zip(rows, lengths, wrong)])
+        parents, accepted = ints([-1, -1, 0, 0][:nodes]), ints([nodes - 2])
+        tables = gdn.request_tables(ints([nodes]), slots, nodes * len(rows))
         seen = []
         out = net(tokens, net.tree_rules(parents, tables, slots, pool, seen))
-        outs.append(out.view(len(rows), 4, hidden)[:, ::2])
+        outs.append(out.view(len(rows), nodes, hidden)[:, ::2])
         for states, inputs in seen:
             gdn.gated_delta_commit(*inputs, parents, accepted, tables, slots, states)
     return torch.cat(outs, 1)  # [requests,answers,hidden]
