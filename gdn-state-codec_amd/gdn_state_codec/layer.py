@@ -404,14 +404,15 @@ def gated_delta_tree(queries: torch.Tensor, keys: torch.Tensor, values: torch.Te
 def gated_delta_commit(keys: torch.Tensor, values: torch.Tensor, log_decay: torch.Tensor,
                        beta: torch.Tensor, parents: torch.Tensor, accepted: torch.Tensor,
                        tables: RequestTables, slot_ids: torch.Tensor, pool: torch.Tensor,
-                       normalize: bool = True) -> None:
+                       normalize: bool = True, max_nodes: int = MAX_NODES) -> None:
     """Advances the states ``pool`` at ``slot_ids`` (distinct) in place by the accepted
     nodes of :func:`gated_delta_tree`'s trees: those on the path from the cached state
-    down to ``accepted[r]`` (int32 [N], a node's place in its request, among its first 64).
-    A request that accepts nothing (-1, or no node's place) keeps its state.  The other
-    arguments are that call's.  A bf16 state is rounded once, however long the path."""
+    down to ``accepted[r]`` (int32 [N], a node's place in its request, among its first
+    ``max_nodes``).  A request that accepts nothing (-1, or no such place) keeps its state.
+    The other arguments are that call's, ``max_nodes`` too: what it left out is not accepted.
+    A bf16 state is rounded once, however long the path."""
     drafts = _drafts(None, keys, values, log_decay, beta, parents, tables, slot_ids, normalize,
-                     MAX_NODES, 1.0)
+                     max_nodes, 1.0)
     pool_dtype = _pool(pool, drafts.value_heads)
     _not_differentiated("gated delta commit", keys, values, log_decay, beta, pool)
     _dense(accepted, "accepted nodes", (drafts.requests,), torch.int32)
