@@ -115,3 +115,49 @@ def test_growth_that_no_write_meets(device, nodes, places, last, pool_dtype):
     exact = pool_dtype == torch.float32
     close(batch.dev_pool[int(batch.slots[0])], states[chain[-1]], FP32 if exact else BF16,
           "state")
+
+
+@pytest.mark.parametrize("pool_dtype", [torch.float32, torch.bfloat16])
+def test_growth_with_decays(device, pool_dtype):
+    """The same on a path with decays, one of them -inf before the writes."""
+    chain = list(range(20))
+    batch = _steep(device, 20, chain, pool_dtype, 16)
+    batch.g.uniform_(-0.5, 0.0, generator=torch.Generator().manual_seed(69))
+    batch.g[2] = float("-inf")
+    batch.pool.normal_(generator=torch.Generator().manual_seed(70)).mul_(1e-30)
+    batch.dev_g.copy_(batch.g)
+    batch.dev_pool.copy_(batch.pool)
+    want, states = batch.reference(0)
+    got = batch.tree().cpu()
+    for node in range(3, 20):
+        for head in range(2):
+            close(got[node, head], want[node, head], 2.0 ** -7, f"node {node}")
+    batch.commit([19])
+    close(batch.dev_pool[int(batch.slots[0])], states[19],
+          FP32 if pool_dtype == torch.float32 else BF16, "state")
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("what", ["value", "strength", "key"])
+@pytest.mark.parametrize("nodes,chain", [(16, range(0, 14)), (64, range(16, 31))])
+def test_bad_values_beside_steep_keys(device, nodes, chain, what, bad):
+    """A bad node beside a chain whose inverse is past the range: neither reaches the other."""
+    chain = list(chain)
+    batch = _steep(device, nodes, chain, torch.float32, chain[-3])
+    node = chain[-1] + 1
+    want, _ = batch.reference(0)
+    if what == "value":
+        batch.dev_mixed[node, 256 + 128 + 9] = bad  # head 1's column 9
+    elif what == "strength":
+        batch.dev_b[node, 1] = bad
+    else:
+        batch.dev_mixed[node, 128 + 3] = bad
+    got = batch.tree().cpu()
+    for i in range(nodes):
+        reached = node in ref.path(batch.parents[0], i)
+        for head in range(2):
+            if not reached or (what != "key" and head == 0):
+                close(got[i, head], want[i, head], 2.0 ** -7, f"node {i}")
+            else:
+                columns = [9] if what == "value" else range(128)
+                assert not torch.isfinite(got[i, head, list(columns)]).any()
