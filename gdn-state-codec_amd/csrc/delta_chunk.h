@@ -283,6 +283,14 @@ __device__ __forceinline__ f32x4 mfma3(const uint4 (&a)[3], const uint4& b, f32x
   return mfma(a[0], b, c);
 }
 
+// c + a b for 16 x 16 fp32 blocks: lane l has row l & 15, columns 4 g.. of a, and
+// rows 4 g.. of b's column l & 15 (an accumulator).
+__device__ __forceinline__ f32x4 block_product(const f32x4& a, const f32x4& b, f32x4 c) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+  return c;
+}
+
 __device__ __forceinline__ f32x4 load4(const float* p) {
   return *reinterpret_cast<const f32x4*>(p);
 }

@@ -78,14 +78,6 @@ struct Staged {
 };
 static_assert(workgroups_by_lds(sizeof(Staged)) == 3, "three workgroups share a compute unit");
 
-// c + a b for 16 x 16 fp32 blocks: lane l has row l & 15, columns 4 g.. of a, and
-// rows 4 g.. of b's column l & 15 (an accumulator).
-__device__ __forceinline__ f32x4 block_product(const f32x4& a, const f32x4& b, f32x4 c) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
-  return c;
-}
-
 __device__ __forceinline__ f32x4 times(const f32x4& a, const f32x4& b) {
   return f32x4{a[0] * b[0], a[1] * b[1], a[2] * b[2], a[3] * b[3]};
 }

@@ -14,9 +14,12 @@
 //
 // Products with the state are on the bf16 matrix cores: k and q are exact as they are
 // (their norms are factors of the results), an fp32 state is three parts (delta_chunk.h),
-// a bf16 one itself.  What follows, A, M and u, is fp32 on the fp32 matrix cores, whose
-// accumulators are the next product's operand as they are.  (I + A)^-1 of 16 x 16 blocks
-// on the diagonal is formed by substitution, which is stable for any keys.
+// a bf16 one itself.  So are those of A's blocks below the diagonal and of M with u, and a
+// commit's of u with k: A, M and u are fp32 in three parts each, and of the nine products
+// of two such the six that fp32 has room for are summed, in fp32.  A's blocks on the
+// diagonal alone are on the fp32 matrix cores, whose accumulators are the next product's
+// operand as they are: their (I + A)^-1, 16 x 16, is formed by substitution, which is stable
+// for any keys.
 //
 // Bad values.  A product takes every cell, also those that are zero, so a NaN or an
 // infinity in A, M, r or u would reach every node.  Those cells are set to zero, and the
@@ -99,14 +102,6 @@ __device__ __forceinline__ f32x4 product(const uint4& a, const uint4 (&b)[3], f3
 }
 __device__ __forceinline__ f32x4 product(const uint4& a, const uint4 (&b)[1], f32x4 c) {
   return mfma(a, b[0], c);
-}
-
-// c + a b for 16 x 16 fp32 blocks: lane l has row l & 15, columns 4 g.. of a, and
-// rows 4 g.. of b's column l & 15 (an accumulator).
-__device__ __forceinline__ f32x4 block_product(const f32x4& a, const f32x4& b, f32x4 c) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
-  return c;
 }
 
 // c + a b of 16 places of a contraction.  c is no sum of mfma's: right behind an instruction
