@@ -408,14 +408,15 @@ __device__ __forceinline__ const void* row_at(const bf16_bits* base, uint32_t ro
 // The first wavefront forms the tables and inverts, the others form the nodes' products; the
 // state's are between, wherever a wavefront would wait.
 //
-// What bounds it (32 heads): few nodes, HBM: 64 trees of 16 on an fp32 pool take 35 us, of
-// which the bytes are 25.  Many nodes, one workgroup's phases, of which two (four of 16
-// nodes) share a compute unit: 256 trees of up to 48 nodes on a bf16 pool take 118 us (bytes
-// 68), 128 chains of 64 on an fp32 pool 135 (bytes 77).  The matrix units are busy for 20 and
-// 36% of that, wavefronts wait for 54 and 42% of their lives; the loads and stores without
-// the rest take about 100 us, the rest without them as much.  A persistent workgroup that asks
-// for the next head's nodes, 32 nodes at a time with less LDS, two heads a workgroup and
-// launches of their own for the smaller trees of a batch are no faster.
+// What bounds it (32 heads): few nodes, latency around the bytes: 64 trees of 16 on an fp32
+// pool take 32 us by the form of 16 nodes (three workgroups a compute unit), 35 by that of 64
+// (two, so four rounds of the card), of which the bytes are 25.  Many nodes, a workgroup's
+// phases, of which two share a compute unit: 256 trees of up to 48 nodes on a bf16 pool take
+// 122 us (bytes 68), 128 chains of 64 on an fp32 pool 131 (bytes 77).  The matrix units are busy
+// for 20 and 36% of that, wavefronts wait for 54 and 41% of their lives; the loads and stores
+// without the rest take about 100 us, the rest without them as much.  A persistent workgroup
+// that asks for the next head's nodes, 32 nodes at a time with less LDS, two heads a workgroup
+// and launches of their own for the smaller trees of a batch are no faster.
 //
 // Four workgroups a compute unit for a bf16 pool's trees of up to 32 nodes: 64 registers, which
 // the compiler is held to (it takes 66 otherwise: 256 trees 95 us, 91 so).
@@ -1088,10 +1089,11 @@ void commit_kernel(DraftArgs a) {
 constexpr uint64_t kMaxStride = 1u << 24;  // elements between tokens
 
 // By the most nodes that a tree may have, since lengths stay on the device: LDS and registers
-// of the smaller forms let more workgroups share a compute unit.  Trees of 16 nodes, 32 heads,
-// by the forms of 16, 32 and 64: 256 on an fp32 pool 122, 125 and 129 us, on a bf16 pool 71,
-// 71.5 and 88; 64 of them 33.3, 34.8 and 36.3, and 21.4, 21.9 and 26.0.  256 trees of up to
-// 32 nodes on a bf16 pool by those of 32 and 64: 81 and 96.
+// of the smaller forms let more workgroups share a compute unit (three, two and two on an fp32
+// pool, four, four and two on a bf16 one).  Trees of 16 nodes, 32 heads, by the forms of 16, 32
+// and 64: 256 on an fp32 pool 127, 129 and 134 us, on a bf16 pool 74, 74 and 92; 64 of them 31.8,
+// 33.9 and 35.5, and 21.3, 21.4 and 26.2.  256 trees of up to 32 nodes by those of 32 and 64: 139
+// and 142, and 81 and 102.
 template <typename Pool>
 int32_t launch_tree(void* stream, const DraftArgs& args, dim3 grid) {
   const uint32_t most = args.max_nodes < args.tokens ? args.max_nodes : args.tokens;

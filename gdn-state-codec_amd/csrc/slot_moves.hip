@@ -401,12 +401,16 @@ __global__ __launch_bounds__(kPlanThreads) void compaction_kernel(
 // ------------------------------------------------------------------- copies
 
 constexpr int kCopyThreads = 256;
-// Rows whose loads are all asked for before the first store.  The few workgroups of small slots
-// wait for latency: one cycle of 500 slots of 32 KiB (8 workgroups) takes 42 us with 8 rows, 53
-// with 4 and 126 with loads that wait for each other, of 512 KiB (128) 89, 114 and 290; 16 are
-// no faster.  Where workgroups fill the card, several reads at a time of slots that lie a power
-// of two apart cost more than they hide: a cycle of 500 slots of 4 MiB (1,024) takes 805 us with
-// 1, 968 with 4 and 953 with 8, 96 slots of 8 layers 523, 520 and 528.
+// Rows whose loads are all asked for before the first store, by the workgroups that one slot
+// takes.  Chains and cycles are one part of the grid each, and their few workgroups wait for
+// latency: a cycle of 500 slots takes, with 8 rows and with 1, 45 and 124 us on 8 workgroups
+// (32 KiB), 117 and 344 on 128, 212 and 402 on 256, 424 and 467 on 512, 640 and 633 on 768, 856
+// and 812 on 1,024 (4 MiB: reads of slots that lie a power of two apart cost more than they
+// hide), 300 encoded slots of 32 heads (218) permuted 129 and 214, 96 beams of 2 MiB (512) 60
+// and 79.  Forks, whose pairs spread over the grid's second dimension, have less to wait for and
+// pay: those encoded slots 52 and 49, 96 slots of 512 KiB (128) 16 and 12, of 2 MiB 38 and 36.
+// The rule is the chains', which gain more than forks lose; 96 beams of 8 layers (4,096) take
+// 527 and 508.  4 rows are between the two, 16 no faster than 8.
 constexpr int kBatchOfFew = 8, kBatchOfMany = 1;
 constexpr uint64_t kManyWorkgroups = 4 * kComputeUnits;
 constexpr int kFewBuffers = 9;    // of a launch with a small argument block (2 us less of a call)
